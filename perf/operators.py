@@ -228,14 +228,14 @@ def _dither(place, step):
 
 
 def _encode(m, v, place, step):
-    """8-bit states: per block of 128 the exponent of the largest magnitude (rounded up where three bits of
-    mantissa would carry), per element three bits of mantissa and four (m, signed) or five (v) of exponent,
-    rounded by a dither; a v above zero never becomes zero."""
+    """8-bit states: per block of 128 the exponent of the largest magnitude (rounded up where the element's own
+    code would pass the largest one), per element three bits of mantissa and four (m: the codes of float8_e4m3fn) or
+    five (v, unsigned) of exponent, rounded by a dither; a v above zero never becomes zero."""
     out = []
-    for x, top, dither in zip((m, v), (15, 31), _dither(place, step)):
+    for x, top, carry, dither in zip((m, v), (15, 31), (0x1FFFFF, 0xFFFFF), _dither(place, step)):
         x = x.view(-1, BLOCK)
         most = x.abs().amax(1, keepdim=True).view(torch.int32)
-        e = (most + 0xFFFFF) >> 23
+        e = (most + carry) >> 23
         code = (torch.ldexp(x.abs(), top - e).view(torch.int32) + dither) >> 20
         code = code | ((x.view(torch.int32) >> 24) & 0x80) if top == 15 else torch.where(x > 0, code.clamp(min=1), code)
         out += [code.to(torch.uint8).view(-1), e.to(torch.uint8).view(-1)]
@@ -355,7 +355,7 @@ def _exact_state(x, top, a, b, step):
     blocks = torch.cat([x, pad]).view(-1, BLOCK)
     most = blocks.abs().amax(1, keepdim=True)
     mantissa, exponent = torch.frexp(most)                        # most = mantissa * 2^exponent, mantissa in [1/2, 1)
-    exponent = torch.where(mantissa > 15 / 16, exponent, exponent - 1)
+    exponent = torch.where(mantissa > (14 / 16 if top == 15 else 15 / 16), exponent, exponent - 1)
     own_power = torch.frexp(blocks.abs())[1] - 1
     power = torch.maximum(own_power, exponent - (top - 1))
     step_size = torch.pow(2.0, (power - 3).double())
