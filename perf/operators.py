@@ -217,14 +217,28 @@ def _plain_coefficient(grad, max_norm):
     return norm, (max_norm / (norm + 1e-6)).clamp(max=1.0)
 
 
-def _dither(place, step):
-    """20 bits for each element and moment, evenly spread over an element's steps and over a step's elements."""
-    def wrap(c):                 # as a signed 32-bit factor
-        return c - (1 << 32) if c >= 1 << 31 else c
+def _wrap(c):                    # as a signed 32-bit factor
+    return c - (1 << 32) if c >= 1 << 31 else c
 
-    at = place[:, None] + torch.arange(BLOCK, dtype=torch.int32, device=place.device)
-    for a, b in ((0x9E3779B9, 0xC13FA9A9), (0x6A09E667, 0x91E10DA5)):
-        yield ((at * wrap(a) + wrap(step * b & 0xFFFFFFFF)) >> 12) & 0xFFFFF
+
+def _mix(step):
+    """32 bits that go by the step alone: multiplications by odd numbers and exclusive ors with what is shifted down."""
+    x = step * 0x9E3779B9 & 0xFFFFFFFF
+    x = (x ^ x >> 16) * 0xC13FA9A9 & 0xFFFFFFFF
+    x = (x ^ x >> 15) * 0x91E10DA5 & 0xFFFFFFFF
+    return x ^ x >> 16
+
+
+def _dither(place, step):
+    """20 bits for each element and moment, by the element's place in its tensor and the step."""
+    h = (place[:, None] + torch.arange(BLOCK, dtype=torch.int32, device=place.device)) * _wrap(0x9E3779B9) + _wrap(_mix(step))
+    x = (h ^ (h >> 15 & 0x1FFFF)) & 0xFFFFFF
+    return x * 0xC13FA9 >> 12 & 0xFFFFF, x * 0x91E10D >> 12 & 0xFFFFF
+
+
+def _scaled(x, n):
+    """x * 2^n, exactly (torch.ldexp goes through pow, which is a unit off for some n on the GPU)."""
+    return x * (n + 127 << 23).view(torch.float32)
 
 
 def _encode(m, v, place, step):
@@ -236,7 +250,7 @@ def _encode(m, v, place, step):
         x = x.view(-1, BLOCK)
         most = x.abs().amax(1, keepdim=True).view(torch.int32)
         e = (most + carry) >> 23
-        code = (torch.ldexp(x.abs(), top - e).view(torch.int32) + dither) >> 20
+        code = (_scaled(x.abs(), top - e).view(torch.int32) + dither) >> 20
         code = code | ((x.view(torch.int32) >> 24) & 0x80) if top == 15 else torch.where(x > 0, code.clamp(min=1), code)
         out += [code.to(torch.uint8).view(-1), e.to(torch.uint8).view(-1)]
     return out
@@ -245,9 +259,9 @@ def _encode(m, v, place, step):
 def _decode(code, e, top):
     c, e = code.view(-1, BLOCK).to(torch.int32), e.view(-1, 1).to(torch.int32)
     if top == 15:
-        x = torch.ldexp(((c & 0x7F) << 20).view(torch.float32), e - top)
+        x = _scaled(((c & 0x7F) << 20).view(torch.float32), e - top)
         return torch.where(c > 0x7F, -x, x).view(-1)
-    return torch.ldexp((c << 20).view(torch.float32), e - top).view(-1)
+    return _scaled((c << 20).view(torch.float32), e - top).view(-1)
 
 
 def _adamw(s):
@@ -347,7 +361,7 @@ def _route(s):
 
 
 # ---- the definitions in 64 bits ------------------------------------------------------------------------------
-def _exact_state(x, top, a, b, step):
+def _exact_state(x, top, factor, step):
     """x (one tensor's moment) as its 8-bit codes' values: to a multiple of 2^-3 of its own power of two (of the
     lowest one below that), up with the chance that the dither's 20 bits give."""
     n = x.numel()
@@ -360,7 +374,8 @@ def _exact_state(x, top, a, b, step):
     power = torch.maximum(own_power, exponent - (top - 1))
     step_size = torch.pow(2.0, (power - 3).double())
     i = torch.arange(blocks.numel(), device=x.device, dtype=torch.int64).view(-1, BLOCK)
-    u = ((i * a + step * b & 0xFFFFFFFF) >> 12).double() / (1 << 20)
+    h = (i * 0x9E3779B9 + _mix(step)) % (1 << 32)
+    u = ((h ^ h >> 15) % (1 << 24) * factor % (1 << 32) >> 12).double() / (1 << 20)
     q = torch.floor(blocks.abs() / step_size + u)
     if top == 31:
         q = torch.where(blocks > 0, q.clamp(min=1), q)
@@ -387,8 +402,8 @@ def _exact_optimizer(case, seed):
         mq, vq = torch.zeros_like(m), torch.zeros_like(v)
         for o, shape in zip(s["starts"], s["shapes"]):
             at = slice(o, o + _numel(shape))
-            mq[at] = _exact_state(m[at], 15, 0x9E3779B9, 0xC13FA9A9, t)
-            vq[at] = _exact_state(v[at], 31, 0x6A09E667, 0x91E10DA5, t)
+            mq[at] = _exact_state(m[at], 15, 0xC13FA9, t)
+            vq[at] = _exact_state(v[at], 31, 0x91E10D, t)
         m, v = mq, vq
     return {"param": param, "m": m, "v": v, "norm": total if case["clip"] else None}
 
