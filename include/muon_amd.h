@@ -158,6 +158,42 @@ typedef struct MuonAdamDesc {
     int32_t reserved;    /* 0                                                                 */
 } MuonAdamDesc;
 
+/* One tensor of an AdamW group.  States in 32 bits: exp_avg and exp_avg_sq are numel floats.  In 8 bits: numel codes of
+ * one byte each, and one shared exponent for every muon_amd_adamw_shared_elems() consecutive elements:
+ *   exp_avg     code s eeee fff : (-1)^s 2^(E - 127) (1 + f/8) 2^(e - 15)     (e = 0: f/8 2^-14)
+ *   exp_avg_sq  code   eeeee fff:        2^(E - 127) (1 + f/8) 2^(e - 31)     (e = 0: f/8 2^-30)
+ * E = 255: every element of the block is not a number; zeroed memory is a state of zeros.    */
+typedef struct MuonAdamWDesc {
+    void* param;                 /* numel of dtype                                            */
+    const void* grad;            /* numel of dtype                                            */
+    void* exp_avg;
+    void* exp_avg_sq;
+    uint8_t* exp_avg_exponent;   /* 8-bit states: one byte for each block of a tensor, else NULL */
+    uint8_t* exp_avg_sq_exponent;
+    int64_t numel;
+    int32_t dtype;               /* MUON_AMD_SRC_*: storage type of param and grad            */
+    int32_t reserved;            /* 0                                                         */
+} MuonAdamWDesc;
+
+/* One tensor's 8-bit states and where their values go. */
+typedef struct MuonAdamWValuesDesc {
+    const uint8_t* exp_avg;
+    const uint8_t* exp_avg_sq;
+    const uint8_t* exp_avg_exponent;
+    const uint8_t* exp_avg_sq_exponent;
+    uint16_t* exp_avg_out;       /* numel bf16                                                */
+    uint16_t* exp_avg_sq_out;    /* numel bf16                                                */
+    int64_t numel;
+} MuonAdamWValuesDesc;
+
+/* One gradient. */
+typedef struct MuonGradDesc {
+    void* grad;                  /* numel of dtype                                            */
+    int64_t numel;
+    int32_t dtype;               /* MUON_AMD_SRC_*                                            */
+    int32_t reserved;            /* 0                                                         */
+} MuonGradDesc;
+
 /* One matrix of the AOL rescaling step of the 4-iteration variant (muon.py:776-785), in the
  * wide orientation: X is m_p x n_p with m_p <= n_p (zero padded).                           */
 typedef struct MuonAolDesc {
@@ -234,6 +270,9 @@ size_t muon_amd_sizeof_tile_job(void);
 size_t muon_amd_sizeof_adam_desc(void);
 size_t muon_amd_sizeof_aol_desc(void);
 size_t muon_amd_sizeof_chunk_run(void);
+size_t muon_amd_sizeof_adamw_desc(void);
+size_t muon_amd_sizeof_adamw_values_desc(void);
+size_t muon_amd_sizeof_grad_desc(void);
 
 /* Elements each block of the flat elementwise launches covers (momentum, apply, adam), and
  * the edge of the square tile of the normalise/transposing launch. */
@@ -392,6 +431,33 @@ int muon_amd_adam(const MuonAdamDesc* descs_dev, const int32_t* block_prefix_dev
                   float bias1, float bias2,
                   const float* scalars_dev /* {lr, wd_factor, w1, w2, eps, bias1, bias2} */,
                   void* stream);
+
+/* ---- AdamW over many tensors, states in 32 or 8 bits ---------------------------------------- */
+/* g' = c g;  m <- lerp(m, g', w1);  v <- lerp(v, g'^2, w2);
+ * param <- param*wd_factor - lr*(m/bias1) / (sqrt(v/bias2) + eps)
+ * in fp32, with c = *grad_scale_dev (NULL: 1).  8-bit states are rounded by a dither that goes by the element's place in
+ * its tensor and by `step`.  block_prefix_dev: blocks of muon_amd_elementwise_block_elems() elements.
+ * scalars_dev: NULL, or {lr, wd_factor, w1, w2, eps, bias1, bias2, step} as floats in device memory.  */
+int muon_amd_adamw_shared_elems(void);
+int muon_amd_validate_adamw(const MuonAdamWDesc* descs_host, int ntensors, const int32_t* block_prefix_host, int state_bits);
+int muon_amd_adamw(const MuonAdamWDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks, int state_bits,
+                   float lr, float wd_factor, float w1, float w2, float eps, float bias1, float bias2, uint32_t step,
+                   const float* grad_scale_dev, const float* scalars_dev, void* stream);
+/* The values that 8-bit states stand for. */
+int muon_amd_validate_adamw_values(const MuonAdamWValuesDesc* descs_host, int ntensors, const int32_t* block_prefix_host);
+int muon_amd_adamw_values(const MuonAdamWValuesDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks,
+                          void* stream);
+
+/* ---- the norm of all gradients, and clipping by it ------------------------------------------- */
+/* out_dev[0] = sqrt(sum of squares of all elements), out_dev[1] = min(1, max_norm / (out_dev[0] + 1e-6));
+ * muon_amd_grad_clip also multiplies every gradient by out_dev[1] in place.  partials_dev: workspace of
+ * muon_amd_grad_norm_partials() doubles.  Blocks as in muon_amd_adamw.                          */
+int muon_amd_grad_norm_partials(void);
+int muon_amd_validate_grads(const MuonGradDesc* descs_host, int ntensors, const int32_t* block_prefix_host);
+int muon_amd_grad_norm(const MuonGradDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks,
+                       double* partials_dev, float max_norm, float* out_dev, void* stream);
+int muon_amd_grad_clip(const MuonGradDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks,
+                       double* partials_dev, float max_norm, float* out_dev, void* stream);
 
 #ifdef __cplusplus
 }

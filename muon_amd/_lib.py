@@ -62,6 +62,16 @@ CHUNK_RUN = np.dtype(
      ("aol_seg_blocks", "<i4"), ("norm_in_normalize", "<i4")],
     align=True)
 
+ADAMW_DESC = np.dtype(
+    [("param", "<u8"), ("grad", "<u8"), ("exp_avg", "<u8"), ("exp_avg_sq", "<u8"), ("exp_avg_exponent", "<u8"),
+     ("exp_avg_sq_exponent", "<u8"), ("numel", "<i8"), ("dtype", "<i4"), ("reserved", "<i4")],
+    align=True)
+ADAMW_VALUES_DESC = np.dtype(
+    [("exp_avg", "<u8"), ("exp_avg_sq", "<u8"), ("exp_avg_exponent", "<u8"), ("exp_avg_sq_exponent", "<u8"),
+     ("exp_avg_out", "<u8"), ("exp_avg_sq_out", "<u8"), ("numel", "<i8")],
+    align=True)
+GRAD_DESC = np.dtype([("grad", "<u8"), ("numel", "<i8"), ("dtype", "<i4"), ("reserved", "<i4")], align=True)
+
 _c_int = ctypes.c_int
 _c_float = ctypes.c_float
 _vp = ctypes.c_void_p
@@ -103,6 +113,19 @@ SIGNATURES = {
     "muon_amd_apply": (_c_int, [_vp, _vp, _c_int, _c_int, _c_float, _c_float, _vp, _vp]),
     "muon_amd_adam": (_c_int, [_vp, _vp, _c_int, _c_int, _c_float, _c_float, _c_float, _c_float,
                                _c_float, _c_float, _c_float, _vp, _vp]),
+    "muon_amd_sizeof_adamw_desc": (ctypes.c_size_t, []),
+    "muon_amd_sizeof_adamw_values_desc": (ctypes.c_size_t, []),
+    "muon_amd_sizeof_grad_desc": (ctypes.c_size_t, []),
+    "muon_amd_adamw_shared_elems": (_c_int, []),
+    "muon_amd_validate_adamw": (_c_int, [_vp, _c_int, _vp, _c_int]),
+    "muon_amd_adamw": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_float, _c_float, _c_float, _c_float, _c_float, _c_float,
+                                _c_float, ctypes.c_uint32, _vp, _vp, _vp]),
+    "muon_amd_validate_adamw_values": (_c_int, [_vp, _c_int, _vp]),
+    "muon_amd_adamw_values": (_c_int, [_vp, _vp, _c_int, _c_int, _vp]),
+    "muon_amd_grad_norm_partials": (_c_int, []),
+    "muon_amd_validate_grads": (_c_int, [_vp, _c_int, _vp]),
+    "muon_amd_grad_norm": (_c_int, [_vp, _vp, _c_int, _c_int, _vp, _c_float, _vp, _vp]),
+    "muon_amd_grad_clip": (_c_int, [_vp, _vp, _c_int, _c_int, _vp, _c_float, _vp, _vp]),
 }
 
 
@@ -131,7 +154,9 @@ def load():
         raise MuonAmdError(f"ABI mismatch: library {lib.muon_amd_abi_version()}, binding {ABI_VERSION}")
     for dt, fn in ((MAT_DESC, lib.muon_amd_sizeof_mat_desc), (GEMM_DESC, lib.muon_amd_sizeof_gemm_desc),
                    (TILE_JOB, lib.muon_amd_sizeof_tile_job), (ADAM_DESC, lib.muon_amd_sizeof_adam_desc),
-                   (AOL_DESC, lib.muon_amd_sizeof_aol_desc), (CHUNK_RUN, lib.muon_amd_sizeof_chunk_run)):
+                   (AOL_DESC, lib.muon_amd_sizeof_aol_desc), (CHUNK_RUN, lib.muon_amd_sizeof_chunk_run),
+                   (ADAMW_DESC, lib.muon_amd_sizeof_adamw_desc), (ADAMW_VALUES_DESC, lib.muon_amd_sizeof_adamw_values_desc),
+                   (GRAD_DESC, lib.muon_amd_sizeof_grad_desc)):
         if dt.itemsize != fn():
             raise MuonAmdError(f"struct layout mismatch: binding {dt.itemsize} bytes, library {fn()}")
     _lib = lib

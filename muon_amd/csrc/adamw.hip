@@ -1,0 +1,411 @@
+// AdamW over many tensors in one launch, with states in 32 or in 8 bits, and the values that 8-bit states stand for.
+//
+//   g' = c g;  m <- m + w1 (g' - m);  v <- v + w2 (g'^2 - v);  p <- p wd_factor - (lr / bias1) m / (sqrt(v / bias2) + eps)
+//
+// with c read from device memory (the coefficient of a clipped gradient) or 1.  Arithmetic is fp32 whatever p is stored
+// in; p rounds once.
+//
+// States of 8 bits.  128 consecutive elements of a tensor (a block) share a power of two 2^(E - 127), E one byte, for
+// each moment; an element keeps three bits of mantissa and its exponent below the shared one:
+//   m: sign, four bits of exponent, 2^(E - 127) (1 + f/8) 2^(e - 15): the codes of OCP's e4m3, whose largest is 1.75 x 2^8
+//   v: five bits of exponent, 2^(E - 127) (1 + f/8) 2^(e - 31), no sign
+// (e = 0: f/8 of the lowest power, as in IEEE 754).  A power of two as the shared factor makes scaling exact, and E the
+// exponent field of the largest magnitude of the block, one more where that element itself could round past the
+// largest code.  E = 255 says that the block holds a value that is not finite: all of it reads as NaN, so an overflow
+// shows in the next step as it would in 32 bits.
+// Rounding to three bits is dithered: to the 20 bits that are dropped, 20 bits are added that go by the element's place
+// in its tensor and by the step, as good as independent from step to step and between the moments, so that a moment is
+// right on average.  To nearest, one that moves by less than half a step of its code (6 % of it; a step moves v by at
+// most 1 - beta2 of itself) would never move; and a sequence that fills the unit interval evenly over the steps (multiples
+// of an irrational number) leaves moments 2 % off, since what is rounded goes by the steps before.
+// v above zero never rounds to the code zero, whose update would divide by eps alone.
+#include <type_traits>
+
+#include "vector.h"
+
+namespace muon_amd {
+
+constexpr int AW_THREADS = 256;
+constexpr int AW_GROUPS = 4;                                    // groups of eight per thread: all their loads go out first
+constexpr int AW_BLOCK_ELEMS = AW_THREADS * 8 * AW_GROUPS;      // elements per workgroup
+constexpr int AW_SHARED = 128;                                  // elements that share an exponent: 16 lanes of a wave
+
+struct AdamWArgs {
+    float neg_lr;        // -lr / bias1
+    float wd_factor, w1, w2, eps;
+    float rsqrt_bias2;   // 1 / sqrt(bias2)
+    uint32_t dither;     // of the step
+};
+
+// The dither of element i at step t: h = i D + mix(t) mod 2^32, x the low 24 bits of h ^ (h >> 15), and of the products
+// of x with a constant for each moment (24-bit factors: the target's fast integer product) bits 12 to 31.
+constexpr uint32_t DITHER_I = 0x9E3779B9u, DITHER_M = 0xC13FA9u, DITHER_V = 0x91E10Du;
+__host__ __device__ __forceinline__ uint32_t mix_step(uint32_t t) {
+    uint32_t x = t * 0x9E3779B9u;
+    x = (x ^ (x >> 16)) * 0xC13FA9A9u;
+    x = (x ^ (x >> 15)) * 0x91E10DA5u;
+    return x ^ (x >> 16);
+}
+
+typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2v_byte __attribute__((ext_vector_type(2), aligned(1)));
+
+__device__ __forceinline__ AdamWArgs read_args(AdamWArgs a, const float* sc) {
+    if (sc) {   // {lr, wd_factor, w1, w2, eps, bias1, bias2, step} read at run time instead of the arguments
+        a.neg_lr = -sc[0] / sc[5];
+        a.wd_factor = sc[1];
+        a.w1 = sc[2];
+        a.w2 = sc[3];
+        a.eps = sc[4];
+        a.rsqrt_bias2 = 1.f / sqrtf(sc[6]);
+        a.dither = mix_step(static_cast<uint32_t>(sc[7]));
+    }
+    return a;
+}
+
+// The two moments; the square is rounded before it is subtracted from, as for tensors of fp32.
+__device__ __forceinline__ void moments(float& m, float& v, float g, const AdamWArgs& a) {
+#pragma clang fp contract(off)
+    const float gg = g * g;
+    m = lerp_torch(m, g, a.w1);
+    v = lerp_torch(v, gg, a.w2);
+}
+
+// ---- states in 32 bits -------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void adamw32_group(Group8<T>& p, const Group8<T>& g, Group8<float>& m, Group8<float>& v,
+                                              float c, const AdamWArgs& a) {
+    float pn[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float gk = g[k] * c;
+        float mk = m[k], vk = v[k];
+        moments(mk, vk, gk, a);
+        m.set(k, mk);
+        v.set(k, vk);
+        pn[k] = fmaf(a.neg_lr, mk / fmaf(sqrtf(vk), a.rsqrt_bias2, a.eps), p[k] * a.wd_factor);
+    }
+    p = Group8<T>::of(pn);
+}
+
+template <typename T>
+__device__ __forceinline__ void adamw32_block(const MuonAdamWDesc& d, int64_t base, float c, const AdamWArgs& a) {
+    const int64_t numel = d.numel;
+    T* __restrict__ const p = static_cast<T*>(d.param);
+    const T* __restrict__ const g = static_cast<const T*>(d.grad);
+    float* __restrict__ const m = static_cast<float*>(d.exp_avg);
+    float* __restrict__ const v = static_cast<float*>(d.exp_avg_sq);
+    if (base + AW_BLOCK_ELEMS <= numel) {
+        Group8<T> pv[AW_GROUPS], gv[AW_GROUPS];
+        Group8<float> mv[AW_GROUPS], vv[AW_GROUPS];
+#pragma unroll
+        for (int i = 0; i < AW_GROUPS; ++i) {
+            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
+            gv[i] = Group8<T>::template load<true>(g + e);
+            mv[i] = Group8<float>::load<true>(m + e);
+            vv[i] = Group8<float>::load<true>(v + e);
+            pv[i] = Group8<T>::template load<true>(p + e);
+        }
+#pragma unroll
+        for (int i = 0; i < AW_GROUPS; ++i) {
+            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
+            adamw32_group<T>(pv[i], gv[i], mv[i], vv[i], c, a);
+            mv[i].template store<true>(m + e);
+            vv[i].template store<true>(v + e);
+            pv[i].template store<true>(p + e);
+        }
+        return;
+    }
+#pragma unroll 1
+    for (int64_t e = base + threadIdx.x * 8; e < numel; e += AW_THREADS * 8) {
+        Group8<T> pv = load_group<T, true>(p, e, numel);
+        const Group8<T> gv = load_group<T, true>(g, e, numel);
+        Group8<float> mv = load_group<float, true>(m, e, numel), vv = load_group<float, true>(v, e, numel);
+        adamw32_group<T>(pv, gv, mv, vv, c, a);
+        store_group<float, true>(m, e, numel, mv);
+        store_group<float, true>(v, e, numel, vv);
+        store_group<T, true>(p, e, numel, pv);
+    }
+}
+
+__global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(const MuonAdamWDesc* __restrict__ descs,
+                                                            const int32_t* __restrict__ prefix, int ntensors, AdamWArgs args,
+                                                            const float* __restrict__ grad_scale, const float* __restrict__ sc) {
+    const AdamWArgs a = read_args(args, sc);
+    const float c = grad_scale ? *grad_scale : 1.f;
+    const int b = blockIdx.x, ti = find_segment(prefix, ntensors, b);
+    const MuonAdamWDesc d = descs[ti];
+    const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS;
+    if (d.dtype == MUON_AMD_SRC_BF16) adamw32_block<uint16_t>(d, base, c, a);
+    else adamw32_block<float>(d, base, c, a);
+}
+
+// ---- states in 8 bits --------------------------------------------------------------------------------------
+// The larger of two pairs of 16-bit numbers over the 16 lanes of a row, in every lane.
+__device__ __forceinline__ uint32_t row_max2(uint32_t x) {
+    const auto step = [&](uint32_t other) {
+        x = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, x), __builtin_bit_cast(u16x2_t, other)));
+    };
+    step(__builtin_amdgcn_mov_dpp(x, 0xB1, 0xf, 0xf, true));       // quad_perm 1,0,3,2
+    step(__builtin_amdgcn_mov_dpp(x, 0x4E, 0xf, 0xf, true));       // quad_perm 2,3,0,1
+    step(__builtin_amdgcn_mov_dpp(x, 0x141, 0xf, 0xf, true));      // row_half_mirror
+    step(__builtin_amdgcn_mov_dpp(x, 0x140, 0xf, 0xf, true));      // row_mirror
+    return x;
+}
+
+__device__ __forceinline__ uint32_t max3u(uint32_t a, uint32_t b, uint32_t c) { return max(max(a, b), c); }
+
+// The values of eight codes, as they are held (m) or (v), whose block has the shared exponent E.
+__device__ __forceinline__ void decode_m(u32x2v code, int E, float (&m)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(code[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(code[h], true);
+        m[4 * h] = ldexpf(lo[0], E - 135);            // (e4m3 itself: 2^(e - 7))
+        m[4 * h + 1] = ldexpf(lo[1], E - 135);
+        m[4 * h + 2] = ldexpf(hi[0], E - 135);
+        m[4 * h + 3] = ldexpf(hi[1], E - 135);
+    }
+}
+__device__ __forceinline__ void decode_v(u32x2v code, int E, float (&v)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const uint32_t c = (code[k >> 2] >> (8 * (k & 3))) & 0xffu;
+        v[k] = ldexpf(__uint_as_float(c << 20), E - 31);
+    }
+}
+
+// One group: parameters and moments after the step, the new codes, and the new shared exponents of the block (whose 16
+// groups are those of a row of lanes: every lane of the wave calls this; what is beyond the tensor is zero).
+template <typename T>
+__device__ __forceinline__ void adamw8_group(Group8<T>& p, const Group8<T>& g, u32x2v& mc, u32x2v& vc, int& Em, int& Ev,
+                                             uint32_t i0, float c, const AdamWArgs& a) {
+    float m[8], v[8], pn[8];
+    decode_m(mc, Em, m);
+    decode_v(vc, Ev, v);
+    const float poison = max(Em, Ev) == 255 ? __builtin_nanf("") : 0.f;
+    uint32_t most_m = 0, most_v = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float gk = fmaf(g[k], c, poison);
+        moments(m[k], v[k], gk, a);
+        most_m = max(most_m, __float_as_uint(m[k]) & 0x7fffffffu);
+        most_v = max(most_v, __float_as_uint(v[k]) & 0x7fffffffu);
+        const float denominator = fmaf(__builtin_amdgcn_sqrtf(v[k]), a.rsqrt_bias2, a.eps);
+        pn[k] = fmaf(a.neg_lr, m[k] * __builtin_amdgcn_rcpf(denominator), p[k] * a.wd_factor);
+    }
+    p = Group8<T>::of(pn);
+    // exponent fields, one more where three bits of mantissa are not enough below the next power (m: 1.75 is the last)
+    const uint32_t both = row_max2(((most_m + 0x1fffffu) >> 23) | ((most_v + 0xfffffu) >> 23 << 16));
+    Em = static_cast<int>(both & 0xffffu);
+    Ev = static_cast<int>(both >> 16);
+    if (max(Em, Ev) >= 255) Em = Ev = 255;
+    uint32_t h32 = i0 * DITHER_I + a.dither;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t cm = 0, cv = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float mk = m[4 * h + k], vk = v[4 * h + k];
+            const uint32_t ym = __float_as_uint(ldexpf(fabsf(mk), 15 - Em));
+            const uint32_t yv = __float_as_uint(ldexpf(vk, 31 - Ev));
+            const uint32_t x = (h32 ^ (h32 >> 15)) & 0xffffffu;
+            const uint32_t qm = ((ym + (x * DITHER_M >> 12)) >> 20) | ((__float_as_uint(mk) >> 24) & 0x80u);
+            const uint32_t qv = max((yv + (x * DITHER_V >> 12)) >> 20, min(__float_as_uint(vk), 1u));
+            cm |= qm << (8 * k);
+            cv |= qv << (8 * k);
+            h32 += DITHER_I;
+        }
+        mc[h] = cm;
+        vc[h] = cv;
+    }
+}
+
+__device__ __forceinline__ u32x2v load_codes(const uint8_t* p, int64_t e, int64_t n) {
+    if (e + 8 <= n) return load_as<true, u32x2v_byte>(p + e);
+    u32x2v c = {0u, 0u};
+#pragma unroll
+    for (int k = 0; k < 7; ++k)
+        if (e + k < n) c[k >> 2] |= static_cast<uint32_t>(p[e + k]) << (8 * (k & 3));
+    return c;
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, int64_t e, int64_t n, u32x2v c) {
+    if (e + 8 <= n) {
+        store_as<true, u32x2v_byte>(p + e, c);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 7; ++k)
+        if (e + k < n) p[e + k] = static_cast<uint8_t>(c[k >> 2] >> (8 * (k & 3)));
+}
+
+template <typename T>
+__device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t base, float c, const AdamWArgs& a) {
+    const int64_t numel = d.numel;
+    T* __restrict__ const p = static_cast<T*>(d.param);
+    const T* __restrict__ const g = static_cast<const T*>(d.grad);
+    uint8_t* __restrict__ const m = static_cast<uint8_t*>(d.exp_avg);
+    uint8_t* __restrict__ const v = static_cast<uint8_t*>(d.exp_avg_sq);
+    uint8_t* __restrict__ const me = d.exp_avg_exponent;
+    uint8_t* __restrict__ const ve = d.exp_avg_sq_exponent;
+    if (base + AW_BLOCK_ELEMS <= numel) {
+        Group8<T> pv[AW_GROUPS], gv[AW_GROUPS];
+        u32x2v mv[AW_GROUPS], vv[AW_GROUPS];
+        int Em[AW_GROUPS], Ev[AW_GROUPS];
+#pragma unroll
+        for (int i = 0; i < AW_GROUPS; ++i) {
+            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
+            Em[i] = me[e / AW_SHARED];
+            Ev[i] = ve[e / AW_SHARED];
+            mv[i] = load_as<true, u32x2v_byte>(m + e);
+            vv[i] = load_as<true, u32x2v_byte>(v + e);
+            gv[i] = Group8<T>::template load<true>(g + e);
+            pv[i] = Group8<T>::template load<true>(p + e);
+        }
+#pragma unroll
+        for (int i = 0; i < AW_GROUPS; ++i) {
+            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
+            adamw8_group<T>(pv[i], gv[i], mv[i], vv[i], Em[i], Ev[i], static_cast<uint32_t>(e), c, a);
+            store_as<true, u32x2v_byte>(m + e, mv[i]);
+            store_as<true, u32x2v_byte>(v + e, vv[i]);
+            pv[i].template store<true>(p + e);
+            if ((threadIdx.x & 15) == 0) {
+                me[e / AW_SHARED] = static_cast<uint8_t>(Em[i]);
+                ve[e / AW_SHARED] = static_cast<uint8_t>(Ev[i]);
+            }
+        }
+        return;
+    }
+#pragma unroll 1
+    for (int64_t at = base; at < numel; at += AW_THREADS * 8) {      // (the wave stays whole: its lanes exchange maxima)
+        const int64_t e = at + threadIdx.x * 8;
+        const bool any = e < numel;
+        int Em = any ? me[e / AW_SHARED] : 0, Ev = any ? ve[e / AW_SHARED] : 0;
+        u32x2v mv = load_codes(m, e, numel), vv = load_codes(v, e, numel);
+        Group8<T> pv = load_group<T, true>(p, e, numel);
+        const Group8<T> gv = load_group<T, true>(g, e, numel);
+        adamw8_group<T>(pv, gv, mv, vv, Em, Ev, static_cast<uint32_t>(e), c, a);
+        store_codes(m, e, numel, mv);
+        store_codes(v, e, numel, vv);
+        store_group<T, true>(p, e, numel, pv);
+        if (any && (threadIdx.x & 15) == 0) {
+            me[e / AW_SHARED] = static_cast<uint8_t>(Em);
+            ve[e / AW_SHARED] = static_cast<uint8_t>(Ev);
+        }
+    }
+}
+
+__global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(const MuonAdamWDesc* __restrict__ descs,
+                                                           const int32_t* __restrict__ prefix, int ntensors, AdamWArgs args,
+                                                           const float* __restrict__ grad_scale, const float* __restrict__ sc) {
+    const AdamWArgs a = read_args(args, sc);
+    const float c = grad_scale ? *grad_scale : 1.f;
+    const int b = blockIdx.x, ti = find_segment(prefix, ntensors, b);
+    const MuonAdamWDesc d = descs[ti];
+    const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS;
+    if (d.dtype == MUON_AMD_SRC_BF16) adamw8_block<uint16_t>(d, base, c, a);
+    else adamw8_block<float>(d, base, c, a);
+}
+
+// The values of 8-bit states in bf16, which holds each of them exactly down to the least one that it has (three bits of
+// mantissa; only blocks below 2^-100 reach bf16's own subnormal numbers).
+__global__ __launch_bounds__(AW_THREADS) void adamw_values_kernel(const MuonAdamWValuesDesc* __restrict__ descs,
+                                                                 const int32_t* __restrict__ prefix, int ntensors) {
+    const int b = blockIdx.x, ti = find_segment(prefix, ntensors, b);
+    const MuonAdamWValuesDesc d = descs[ti];
+    const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS, numel = d.numel;
+#pragma unroll
+    for (int i = 0; i < AW_GROUPS; ++i) {
+        const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
+        if (e >= numel) return;
+        const int Em = d.exp_avg_exponent[e / AW_SHARED], Ev = d.exp_avg_sq_exponent[e / AW_SHARED];
+        float m[8], v[8];
+        decode_m(load_codes(d.exp_avg, e, numel), Em, m);
+        decode_v(load_codes(d.exp_avg_sq, e, numel), Ev, v);
+        if (Em == 255)
+            for (float& x : m) x = __builtin_nanf("");
+        if (Ev == 255)
+            for (float& x : v) x = __builtin_nanf("");
+        store_group<uint16_t, true>(d.exp_avg_out, e, numel, Group8<uint16_t>::of(m));
+        store_group<uint16_t, true>(d.exp_avg_sq_out, e, numel, Group8<uint16_t>::of(v));
+    }
+}
+
+// Checks a table's block prefix against its tensors' sizes.
+template <typename D>
+static int check_prefix(const char* what, const D* descs, int n, const int32_t* prefix) {
+    MUON_REQUIRE(descs && prefix, "%s: null table", what);
+    MUON_REQUIRE(n > 0, "%s: ntensors=%d", what, n);
+    MUON_REQUIRE(prefix[0] == 0, "%s: prefix must start at 0", what);
+    for (int i = 0; i < n; ++i) {
+        MUON_REQUIRE(descs[i].numel > 0, "%s: tensor %d: numel=%lld", what, i, static_cast<long long>(descs[i].numel));
+        const int64_t nblk = (descs[i].numel + AW_BLOCK_ELEMS - 1) / AW_BLOCK_ELEMS;
+        MUON_REQUIRE(static_cast<int64_t>(prefix[i + 1]) - prefix[i] == nblk, "%s: tensor %d: prefix gives %d blocks, need %lld", what,
+                     i, prefix[i + 1] - prefix[i], static_cast<long long>(nblk));
+    }
+    return MUON_AMD_OK;
+}
+
+}  // namespace muon_amd
+
+using namespace muon_amd;
+
+extern "C" {
+
+size_t muon_amd_sizeof_adamw_desc(void) { return sizeof(MuonAdamWDesc); }
+size_t muon_amd_sizeof_adamw_values_desc(void) { return sizeof(MuonAdamWValuesDesc); }
+int muon_amd_adamw_shared_elems(void) { return AW_SHARED; }
+
+int muon_amd_validate_adamw(const MuonAdamWDesc* descs, int ntensors, const int32_t* prefix, int state_bits) {
+    MUON_REQUIRE(state_bits == 8 || state_bits == 32, "validate_adamw: state_bits=%d", state_bits);
+    if (const int rc = check_prefix("validate_adamw", descs, ntensors, prefix)) return rc;
+    for (int i = 0; i < ntensors; ++i) {
+        const MuonAdamWDesc& d = descs[i];
+        MUON_REQUIRE(d.param && d.grad && d.exp_avg && d.exp_avg_sq, "validate_adamw: tensor %d: null pointer", i);
+        MUON_REQUIRE(state_bits == 32 || (d.exp_avg_exponent && d.exp_avg_sq_exponent),
+                     "validate_adamw: tensor %d: states in 8 bits need their exponents", i);
+        MUON_REQUIRE(d.dtype == MUON_AMD_SRC_F32 || d.dtype == MUON_AMD_SRC_BF16, "validate_adamw: tensor %d: dtype=%d", i, d.dtype);
+        const uintptr_t elem = d.dtype == MUON_AMD_SRC_BF16 ? 2 : 4;
+        MUON_REQUIRE(reinterpret_cast<uintptr_t>(d.param) % elem == 0 && reinterpret_cast<uintptr_t>(d.grad) % elem == 0 &&
+                         (state_bits == 8 || (reinterpret_cast<uintptr_t>(d.exp_avg) % 4 == 0 &&
+                                              reinterpret_cast<uintptr_t>(d.exp_avg_sq) % 4 == 0)),
+                     "validate_adamw: tensor %d: address not a multiple of the element's size", i);
+    }
+    return MUON_AMD_OK;
+}
+
+int muon_amd_validate_adamw_values(const MuonAdamWValuesDesc* descs, int ntensors, const int32_t* prefix) {
+    if (const int rc = check_prefix("validate_adamw_values", descs, ntensors, prefix)) return rc;
+    for (int i = 0; i < ntensors; ++i) {
+        const MuonAdamWValuesDesc& d = descs[i];
+        MUON_REQUIRE(d.exp_avg && d.exp_avg_sq && d.exp_avg_exponent && d.exp_avg_sq_exponent && d.exp_avg_out && d.exp_avg_sq_out,
+                     "validate_adamw_values: tensor %d: null pointer", i);
+        MUON_REQUIRE(reinterpret_cast<uintptr_t>(d.exp_avg_out) % 2 == 0 && reinterpret_cast<uintptr_t>(d.exp_avg_sq_out) % 2 == 0,
+                     "validate_adamw_values: tensor %d: address not a multiple of the element's size", i);
+    }
+    return MUON_AMD_OK;
+}
+
+int muon_amd_adamw(const MuonAdamWDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks, int state_bits,
+                   float lr, float wd_factor, float w1, float w2, float eps, float bias1, float bias2, uint32_t step,
+                   const float* grad_scale_dev, const float* scalars_dev, void* stream) {
+    MUON_REQUIRE(descs_dev && block_prefix_dev, "adamw: null table");
+    MUON_REQUIRE(ntensors > 0 && nblocks > 0, "adamw: ntensors=%d nblocks=%d", ntensors, nblocks);
+    MUON_REQUIRE(state_bits == 8 || state_bits == 32, "adamw: state_bits=%d", state_bits);
+    MUON_REQUIRE(scalars_dev || (bias1 != 0.f && bias2 > 0.f), "adamw: zero bias correction");
+    const AdamWArgs a{-lr / bias1, wd_factor, w1, w2, eps, 1.f / sqrtf(bias2), mix_step(step)};
+    const auto kernel = state_bits == 8 ? adamw8_kernel : adamw32_kernel;
+    hipLaunchKernelGGL(kernel, dim3(nblocks), dim3(AW_THREADS), 0, static_cast<hipStream_t>(stream), descs_dev, block_prefix_dev,
+                       ntensors, a, grad_scale_dev, scalars_dev);
+    return check_launch("adamw");
+}
+
+int muon_amd_adamw_values(const MuonAdamWValuesDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks,
+                          void* stream) {
+    MUON_REQUIRE(descs_dev && block_prefix_dev, "adamw_values: null table");
+    MUON_REQUIRE(ntensors > 0 && nblocks > 0, "adamw_values: ntensors=%d nblocks=%d", ntensors, nblocks);
+    hipLaunchKernelGGL(adamw_values_kernel, dim3(nblocks), dim3(AW_THREADS), 0, static_cast<hipStream_t>(stream), descs_dev,
+                       block_prefix_dev, ntensors);
+    return check_launch("adamw_values");
+}
+
+}  // extern "C"

@@ -1,0 +1,176 @@
+// The 2-norm of many gradients together, the coefficient that clips it, and the gradients scaled in place:
+//   norm = sqrt(sum_i g_i^2),  coefficient = min(1, max_norm / (norm + 1e-6))
+// Squares and sums are formed in 64 bits (the target adds and multiplies them as fast as 32), so no gradient that is
+// finite in its own type overflows and none is lost below the sum.  The order of the sum is fixed: a workgroup strides
+// over the blocks of the table, its threads' sums join in a tree, and the workgroups' sums are added by index.
+#include "vector.h"
+
+namespace muon_amd {
+
+constexpr int GN_THREADS = 256;
+constexpr int GN_GROUPS = 4;
+constexpr int GN_BLOCK_ELEMS = GN_THREADS * 8 * GN_GROUPS;      // as the blocks of the optimizer's launches
+constexpr int GN_PARTIALS = 2048;                               // workgroups: eight for each CU
+
+__device__ __forceinline__ double block_sum_256(double v, double* smem4) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    if ((threadIdx.x & 63) == 0) smem4[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (smem4[0] + smem4[1]) + (smem4[2] + smem4[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ double squares_of_block(const MuonGradDesc& d, int64_t base) {
+    const T* __restrict__ const g = static_cast<const T*>(d.grad);
+    Group8<T> gv[GN_GROUPS];
+#pragma unroll
+    for (int i = 0; i < GN_GROUPS; ++i) {
+        const int64_t e = base + (i * GN_THREADS + threadIdx.x) * 8;
+        gv[i] = load_group<T, false>(g, e, d.numel);
+    }
+    double s[2] = {0., 0.};
+#pragma unroll
+    for (int i = 0; i < GN_GROUPS; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const double x = gv[i][k];
+            s[k & 1] = fma(x, x, s[k & 1]);
+        }
+    return s[0] + s[1];
+}
+
+__global__ __launch_bounds__(GN_THREADS) void grad_squares_kernel(const MuonGradDesc* __restrict__ descs,
+                                                                 const int32_t* __restrict__ prefix, int ntensors, int nblocks,
+                                                                 double* __restrict__ partials) {
+    __shared__ double red[4];
+    double s = 0.;
+    for (int b = blockIdx.x; b < nblocks; b += gridDim.x) {
+        const int ti = find_segment(prefix, ntensors, b);
+        const MuonGradDesc d = descs[ti];
+        const int64_t base = static_cast<int64_t>(b - prefix[ti]) * GN_BLOCK_ELEMS;
+        s += d.dtype == MUON_AMD_SRC_BF16 ? squares_of_block<uint16_t>(d, base) : squares_of_block<float>(d, base);
+    }
+    const double total = block_sum_256(s, red);
+    if (threadIdx.x == 0) partials[blockIdx.x] = total;
+}
+
+// The norm from the partial sums, in every thread.
+__device__ __forceinline__ float norm_of(const double* __restrict__ partials, int n, double* smem4) {
+    double s = 0.;
+    for (int i = threadIdx.x; i < n; i += GN_THREADS) s += partials[i];
+    return static_cast<float>(sqrt(block_sum_256(s, smem4)));
+}
+// A norm that is not a number gives a coefficient that is not one either.
+__device__ __forceinline__ float coefficient_of(float norm, float max_norm) {
+    const float c = max_norm / (norm + 1e-6f);
+    return c > 1.f ? 1.f : c;
+}
+
+__global__ __launch_bounds__(GN_THREADS) void grad_norm_kernel(const double* __restrict__ partials, int n, float max_norm,
+                                                              float* __restrict__ out) {
+    __shared__ double red[4];
+    const float norm = norm_of(partials, n, red);
+    if (threadIdx.x == 0) {
+        out[0] = norm;
+        out[1] = coefficient_of(norm, max_norm);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_block(const MuonGradDesc& d, int64_t base, float c) {
+    T* __restrict__ const g = static_cast<T*>(d.grad);
+    Group8<T> gv[GN_GROUPS];
+#pragma unroll
+    for (int i = 0; i < GN_GROUPS; ++i) {
+        const int64_t e = base + (i * GN_THREADS + threadIdx.x) * 8;
+        gv[i] = load_group<T, true>(g, e, d.numel);
+    }
+#pragma unroll
+    for (int i = 0; i < GN_GROUPS; ++i) {
+        const int64_t e = base + (i * GN_THREADS + threadIdx.x) * 8;
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = gv[i][k] * c;
+        store_group<T, true>(g, e, d.numel, Group8<T>::of(x));
+    }
+}
+
+// Every workgroup forms the coefficient from the partial sums (16 KB, from the L2), which saves a launch between the
+// two passes; it leaves at once where nothing is to be scaled.
+__global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const MuonGradDesc* __restrict__ descs,
+                                                               const int32_t* __restrict__ prefix, int ntensors, int nblocks,
+                                                               const double* __restrict__ partials, int n, float max_norm,
+                                                               float* __restrict__ out) {
+    __shared__ double red[4];
+    const float norm = norm_of(partials, n, red), c = coefficient_of(norm, max_norm);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        out[0] = norm;
+        out[1] = c;
+    }
+    if (c == 1.f) return;
+    for (int b = blockIdx.x; b < nblocks; b += gridDim.x) {
+        const int ti = find_segment(prefix, ntensors, b);
+        const MuonGradDesc d = descs[ti];
+        const int64_t base = static_cast<int64_t>(b - prefix[ti]) * GN_BLOCK_ELEMS;
+        if (d.dtype == MUON_AMD_SRC_BF16) scale_block<uint16_t>(d, base, c);
+        else scale_block<float>(d, base, c);
+    }
+}
+
+}  // namespace muon_amd
+
+using namespace muon_amd;
+
+extern "C" {
+
+size_t muon_amd_sizeof_grad_desc(void) { return sizeof(MuonGradDesc); }
+int muon_amd_grad_norm_partials(void) { return GN_PARTIALS; }
+
+int muon_amd_validate_grads(const MuonGradDesc* descs, int ntensors, const int32_t* prefix) {
+    MUON_REQUIRE(descs && prefix, "validate_grads: null table");
+    MUON_REQUIRE(ntensors > 0, "validate_grads: ntensors=%d", ntensors);
+    MUON_REQUIRE(prefix[0] == 0, "validate_grads: prefix must start at 0");
+    for (int i = 0; i < ntensors; ++i) {
+        const MuonGradDesc& d = descs[i];
+        MUON_REQUIRE(d.grad && d.numel > 0, "validate_grads: tensor %d: null pointer or numel=%lld", i, static_cast<long long>(d.numel));
+        MUON_REQUIRE(d.dtype == MUON_AMD_SRC_F32 || d.dtype == MUON_AMD_SRC_BF16, "validate_grads: tensor %d: dtype=%d", i, d.dtype);
+        MUON_REQUIRE(reinterpret_cast<uintptr_t>(d.grad) % (d.dtype == MUON_AMD_SRC_BF16 ? 2 : 4) == 0,
+                     "validate_grads: tensor %d: address not a multiple of the element's size", i);
+        const int64_t nblk = (d.numel + GN_BLOCK_ELEMS - 1) / GN_BLOCK_ELEMS;
+        MUON_REQUIRE(static_cast<int64_t>(prefix[i + 1]) - prefix[i] == nblk, "validate_grads: tensor %d: prefix gives %d blocks, need %lld",
+                     i, prefix[i + 1] - prefix[i], static_cast<long long>(nblk));
+    }
+    return MUON_AMD_OK;
+}
+
+static int grad_squares(const MuonGradDesc* descs_dev, const int32_t* prefix_dev, int ntensors, int nblocks, double* partials_dev,
+                        float max_norm, const float* out_dev, hipStream_t stream) {
+    MUON_REQUIRE(descs_dev && prefix_dev && partials_dev && out_dev, "grad_norm: null table, workspace or output");
+    MUON_REQUIRE(ntensors > 0 && nblocks > 0, "grad_norm: ntensors=%d nblocks=%d", ntensors, nblocks);
+    MUON_REQUIRE(max_norm >= 0.f, "grad_norm: max_norm=%g", max_norm);
+    hipLaunchKernelGGL(grad_squares_kernel, dim3(nblocks < GN_PARTIALS ? nblocks : GN_PARTIALS), dim3(GN_THREADS), 0, stream,
+                       descs_dev, prefix_dev, ntensors, nblocks, partials_dev);
+    return check_launch("grad_norm");
+}
+
+int muon_amd_grad_norm(const MuonGradDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks, double* partials_dev,
+                       float max_norm, float* out_dev, void* stream) {
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (const int rc = grad_squares(descs_dev, block_prefix_dev, ntensors, nblocks, partials_dev, max_norm, out_dev, s)) return rc;
+    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(GN_THREADS), 0, s, partials_dev, nblocks < GN_PARTIALS ? nblocks : GN_PARTIALS,
+                       max_norm, out_dev);
+    return check_launch("grad_norm");
+}
+
+int muon_amd_grad_clip(const MuonGradDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks, double* partials_dev,
+                       float max_norm, float* out_dev, void* stream) {
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (const int rc = grad_squares(descs_dev, block_prefix_dev, ntensors, nblocks, partials_dev, max_norm, out_dev, s)) return rc;
+    const int n = nblocks < GN_PARTIALS ? nblocks : GN_PARTIALS;
+    hipLaunchKernelGGL(grad_scale_kernel, dim3(n), dim3(GN_THREADS), 0, s, descs_dev, block_prefix_dev, ntensors, nblocks, partials_dev,
+                       n, max_norm, out_dev);
+    return check_launch("grad_clip");
+}
+
+}  // extern "C"

@@ -549,6 +549,61 @@ class AdamGroupEngine:
         self.enqueue()
 
 
+class AdamWGroupEngine:
+    """One AdamW launch over a fixed list of tensors with states in 32 or 8 bits (prepare / enqueue as above)."""
+
+    N_SCALARS = 8          # {lr, 1 - lr * weight_decay, 1 - beta1, 1 - beta2, eps, 1 - beta1**t, 1 - beta2**t, t}
+    POINTERS = ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_exponent", "exp_avg_sq_exponent")
+    STEP_MODULUS = 1 << 24     # the dither goes by the step modulo this: fp32 scalars hold it exactly
+
+    def __init__(self, numels, dtypes, state_bits, device):
+        _lib.load()
+        self.device = torch.device(device)
+        self.state_bits = int(state_bits)
+        self.descs = np.zeros(len(numels), dtype=_lib.ADAMW_DESC)
+        self.descs["numel"], self.descs["dtype"] = numels, dtypes
+        self.prefix = _plan.adam_block_prefix(numels)
+        self.nblocks = int(self.prefix[-1])
+        self.prefix_dev = _upload(self.prefix, self.device)
+        self.desc_dev = torch.empty(self.descs.nbytes, dtype=torch.uint8, device=self.device)
+        self.staging = _Staging(self.device)
+        self.nbytes = sum(int(n) * ((6 if t == _lib.SRC_BF16 else 12) + (4 if self.state_bits == 8 else 16)) for n, t in zip(numels, dtypes))
+        self.key = None
+        self._hyper = None
+        self._grad_scale = None
+
+    def prepare(self, pointers, *, lr, weight_decay, betas, eps, step, grad_scale=None):
+        """pointers: for each name of POINTERS the tensors' addresses (the last two only with 8 bits).
+        grad_scale: a one-element fp32 tensor on the device, or None."""
+        if pointers != self.key:
+            for name, column in zip(self.POINTERS, pointers):
+                self.descs[name] = column
+            _lib.check(_lib.load().muon_amd_validate_adamw(_lib.host_ptr(self.descs), len(self.descs), _lib.host_ptr(self.prefix),
+                                                           self.state_bits), "validate_adamw")
+            self.staging.upload(self.descs, self.desc_dev)
+            self.key = pointers
+        # python doubles, rounded to float by the call
+        self._hyper = [lr, 1 - lr * weight_decay, 1 - betas[0], 1 - betas[1], eps,
+                       1 - betas[0] ** step, 1 - betas[1] ** step, step % self.STEP_MODULUS]
+        self._grad_scale = grad_scale
+
+    def scalars(self):
+        return [float(x) for x in self._hyper]
+
+    def structure_key(self):
+        return (id(self), None if self._grad_scale is None else self._grad_scale.data_ptr())
+
+    def join(self):
+        pass
+
+    def enqueue(self, scalars_ptr: int = 0, join: bool = True):
+        lib = _lib.load()
+        scale = None if self._grad_scale is None else self._grad_scale.data_ptr()
+        _launch("adamw", self.nbytes, lambda: _lib.check(lib.muon_amd_adamw(
+            self.desc_dev.data_ptr(), self.prefix_dev.data_ptr(), len(self.descs), self.nblocks, self.state_bits, *self._hyper,
+            scale, scalars_ptr or None, _stream_ptr(self.device)), "adamw"))
+
+
 class StepGraph:
     """A whole optimizer step on one device as one HIP graph: the launches of every engine of the
     step are recorded once and replayed afterwards.  What changes between steps is read by the

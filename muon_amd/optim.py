@@ -10,10 +10,11 @@ from __future__ import annotations
 
 import weakref
 
+import numpy as np
 import torch
 
-from . import engine as _engine
-from .engine import AdamGroupEngine, MuonGroupEngine, StepGraph, require_gpu_tensor
+from . import _lib, engine as _engine, plan as _plan
+from .engine import AdamGroupEngine, AdamWGroupEngine, MuonGroupEngine, StepGraph, _launch, _Staging, _stream_ptr, _upload, require_gpu_tensor
 from .functional import _rounding_flag, _src_dtype
 
 NS_STEPS = 5          # the reference classes never pass a step count: muon_update's default rules
@@ -310,6 +311,75 @@ class _MuonBase(torch.optim.Optimizer):
             self._keepalive.append(items)
         self._writebacks += writebacks
 
+    # ---- AdamW with states in 32 or 8 bits (AdamW itself, and the auxiliary groups on request) ----
+    def _adamw_state(self, p, state, bits):
+        """A parameter's state tensors in the engine's order, made on its first step and checked on every one."""
+        if len(state) == 0:
+            if bits == 32:
+                state["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                state["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            else:                                 # zeroed codes and exponents are zero moments
+                shared = -(-p.numel() // _lib.load().muon_amd_adamw_shared_elems())
+                for key in ("exp_avg", "exp_avg_sq"):
+                    state[key] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+                    state[key + "_exponent"] = torch.zeros(shared, dtype=torch.uint8, device=p.device)
+            state["step"] = 0
+        kind = torch.float32 if bits == 32 else torch.uint8
+        tensors = [state.get("exp_avg"), state.get("exp_avg_sq")]
+        for t in tensors:
+            if t is None or t.dtype != kind or t.shape != p.shape or t.device != p.device or not t.is_contiguous():
+                raise NotImplementedError(f"a state of {bits} bits is a contiguous {kind} tensor of the parameter's shape on its device")
+        if bits == 8:
+            shared = -(-p.numel() // _lib.load().muon_amd_adamw_shared_elems())
+            for key in ("exp_avg_exponent", "exp_avg_sq_exponent"):
+                t = state.get(key)
+                if t is None or t.dtype != torch.uint8 or t.shape != (shared,) or t.device != p.device or not t.is_contiguous():
+                    raise NotImplementedError(f"{key} of a state of 8 bits is a contiguous uint8 tensor of {shared} elements")
+                tensors.append(t)
+        return tensors
+
+    def _adamw_group_step(self, gi, group, bits, grad_scale=None, missing_grad_is_zero=True):
+        by_step, writebacks = {}, []
+        for p in group["params"]:
+            if p.grad is None and not missing_grad_is_zero:
+                continue
+            self._check_param(p)
+            g = self._grad_of(p)
+            state = self.state[p]
+            tensors = self._adamw_state(p, state, bits)
+            step_now = int(state["step"]) + 1
+            self._step_bumps.append((state, step_now))
+            if p.numel() > 0:
+                by_step.setdefault((step_now, p.device), []).append(
+                    (p, (self._dense(p, writebacks), self._dense(g, writebacks, written=False), *tensors)))
+        for (step, device), items in by_step.items():
+            if grad_scale is not None and grad_scale.device != device:
+                raise _lib.MuonAmdError(f"grad_scale is on {grad_scale.device}, parameters are on {device}")
+            key = (gi, device, tuple(id(p) for p, _ in items))
+            eng = self._adam_engines.get(key)
+            if eng is None:
+                with torch.cuda.device(device):
+                    eng = AdamWGroupEngine([p.numel() for p, _ in items], [_src_dtype(p) for p, _ in items], bits, device)
+                self._adam_engines[key] = eng
+            eng.prepare([[t[j].data_ptr() for _, t in items] for j in range(4 if bits == 32 else 6)],
+                        lr=float(group["lr"]), weight_decay=float(group["weight_decay"]),
+                        betas=(float(group["betas"][0]), float(group["betas"][1])), eps=float(group["eps"]), step=step,
+                        grad_scale=grad_scale)
+            self._pending.append(eng)
+            self._keepalive.append((items, grad_scale))
+        self._writebacks += writebacks
+
+    def _load_adamw_state(self, state_dict, params):
+        """After torch's load_state_dict, which converts every state tensor to its parameter's type: the tensors of
+        `params` as they were saved."""
+        mine = {id(p) for p in params}
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
+            if id(p) in mine:
+                for key, value in state_dict["state"].get(i, {}).items():
+                    if isinstance(value, torch.Tensor) and key != "step":
+                        self.state[p][key] = value.detach().to(p.device, copy=True)
+
     def _launch_pending(self):
         """Enqueue what the group loop prepared: eagerly, or (use_graph=True) as one recorded graph
         per device that is replayed every step; then copy back tensors that went through a
@@ -411,6 +481,115 @@ class Muon(SingleDeviceMuon):
         return super().step(closure)
 
 
+class AdamW(_MuonBase):
+    """AdamW over many tensors as one launch, with states in 32 bits (whatever the parameters are stored in) or in 8.
+
+        m = lerp(m, g, 1 - beta1);  v = lerp(v, g^2, 1 - beta2)
+        p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
+
+    fp32 or bf16 parameters with gradients of the same type; fp32 arithmetic, one rounding of p.  A parameter without a
+    gradient is left alone, as torch.optim.AdamW leaves it.
+
+    state_bits=32: `exp_avg` and `exp_avg_sq` in fp32.  state_bits=8: codes of 8 bits (uint8 tensors of the parameter's
+    shape) with one shared power of two for every 128 consecutive elements (`exp_avg_exponent`, `exp_avg_sq_exponent`):
+    `exp_avg` in the codes of float8_e4m3fn, `exp_avg_sq` with five bits of exponent, three of mantissa and no sign.  An
+    element's code is within 1/16 (on average over the steps: equal) of its moment from 2^-14 (2^-30) of the largest of
+    its 128 upwards, and a multiple of 2^-17 (2^-33) of that power below.  Rounding is by a fixed dither of the element's
+    place and the step, so a run repeats bit for bit.  A moment that is not finite makes its 128 elements NaN.
+
+    grad_scale of step(): a one-element fp32 tensor on the device that multiplies the gradients on the way, as
+    clip_coefficient returns it (or the inverse of a loss scale).  use_graph records the launch into a HIP graph and
+    replays it (see SingleDeviceMuon).  state_values() gives the moments as tensors of numbers."""
+
+    _RUNTIME_OPTIONS = _MuonBase._RUNTIME_OPTIONS + ("_state_bits",)
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, use_graph=False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"betas must be in [0, 1), got {betas!r}")
+        if not (lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0):
+            raise ValueError(f"lr, eps and weight_decay must not be negative, got {lr!r}, {eps!r}, {weight_decay!r}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self._init_runtime("reference", False, None, use_graph=use_graph)
+        self._state_bits = state_bits
+        self._value_tables = {}
+
+    def _hook_group(self, group):                 # no matrix of this optimizer has an early stage
+        pass
+
+    def __setstate__(self, state):
+        bits = state.get("muon_amd_options", {}).get("_state_bits", getattr(self, "_state_bits", 32))
+        super().__setstate__(state)
+        self._state_bits, self._value_tables = bits, {}
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        self._load_adamw_state(state_dict, [p for g in self.param_groups for p in g["params"]])
+
+    @torch.no_grad()
+    def step(self, closure=None, *, grad_scale=None):
+        loss = self._run_closure(closure)
+        if grad_scale is not None:
+            require_gpu_tensor(grad_scale, "grad_scale")
+            if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
+                raise TypeError(f"grad_scale must be one fp32 number, got {grad_scale.dtype} of shape {tuple(grad_scale.shape)}")
+        for gi, group in enumerate(self.param_groups):
+            self._adamw_group_step(gi, group, self._state_bits, grad_scale, missing_grad_is_zero=False)
+        self._launch_pending()
+        return loss
+
+    @torch.no_grad()
+    def state_values(self, out=None):
+        """The moments of the parameters that have a state, in the order of the groups, as a list of pairs (exp_avg,
+        exp_avg_sq).  32 bits: the state tensors.  8 bits: bf16 tensors, which hold every value exactly while the
+        largest of its 128 is at least 2^-100; `out`: a list of pairs of contiguous bf16 tensors that take them."""
+        params = [p for g in self.param_groups for p in g["params"] if len(self.state[p])]
+        if self._state_bits == 32:
+            if out is not None:
+                raise ValueError("states of 32 bits are returned as they are: out is for 8 bits")
+            return [(self.state[p]["exp_avg"], self.state[p]["exp_avg_sq"]) for p in params]
+        if out is None:
+            out = [tuple(torch.empty(p.shape, dtype=torch.bfloat16, device=p.device) for _ in range(2)) for p in params]
+        elif len(out) != len(params):
+            raise ValueError(f"out has {len(out)} pairs for {len(params)} parameters with a state")
+        rows = {}
+        for p, pair in zip(params, out):
+            tensors = self._adamw_state(p, self.state[p], 8)
+            for t in pair:
+                if t.dtype != torch.bfloat16 or t.numel() != p.numel() or t.device != p.device or not t.is_contiguous():
+                    raise ValueError("out takes contiguous bf16 tensors of the parameters' sizes on their devices")
+            if p.numel():
+                rows.setdefault(p.device, []).append((*tensors, *pair, p.numel()))
+        for device, items in rows.items():
+            table = self._value_tables.get(device)
+            if table is None:
+                table = self._value_tables[device] = _ValueTable(device)
+            with torch.cuda.device(device):
+                table.run([(*(t.data_ptr() for t in row[:6]), row[6]) for row in items])
+        return list(out)
+
+
+class _ValueTable:
+    """The table of the launch that turns 8-bit states into numbers."""
+
+    def __init__(self, device):
+        self.device, self.staging, self.key = device, _Staging(device), None
+
+    def run(self, rows):
+        lib = _lib.load()
+        if rows != self.key:
+            d = np.array(rows, dtype=_lib.ADAMW_VALUES_DESC)
+            prefix = _plan.adam_block_prefix([r[6] for r in rows])
+            _lib.check(lib.muon_amd_validate_adamw_values(_lib.host_ptr(d), len(d), _lib.host_ptr(prefix)), "validate_adamw_values")
+            self.desc_dev = self.staging.upload(d, torch.empty(d.nbytes, dtype=torch.uint8, device=self.device))
+            self.prefix_dev = _upload(prefix, self.device)
+            self.nblocks, self.elems = int(prefix[-1]), int(d["numel"].sum())
+            self.key = rows
+        _launch("adamw_values", 6 * self.elems, lambda: _lib.check(lib.muon_amd_adamw_values(
+            self.desc_dev.data_ptr(), self.prefix_dev.data_ptr(), len(rows), self.nblocks, _stream_ptr(self.device)), "adamw_values"))
+
+
 def _fill_aux_adam_groups(param_groups, sort_muon: bool):
     for group in param_groups:
         assert "use_muon" in group
@@ -430,15 +609,32 @@ def _fill_aux_adam_groups(param_groups, sort_muon: bool):
 
 
 class SingleDeviceMuonWithAuxAdam(_MuonBase):
-    """Reference muon.py:202-260: Muon for `use_muon=True` groups, Adam for the others."""
+    """Reference muon.py:202-260: Muon for `use_muon=True` groups, Adam for the others.
+
+    adam_state_bits (keyword-only, not in the reference): None keeps the Adam states in the parameters' type, as the
+    reference does; 32 or 8 runs those groups as AdamW does, with states in fp32 or in 8 bits."""
 
     _SORT_MUON = False
+    _RUNTIME_OPTIONS = _MuonBase._RUNTIME_OPTIONS + ("_adam_state_bits",)
 
     def __init__(self, param_groups, *, ns_rounding="reference", mutate_grad=False, workspace_bytes=None,
-                 ns_variant="ns5", use_graph=False, overlap_backward=False):
+                 ns_variant="ns5", use_graph=False, overlap_backward=False, adam_state_bits=None):
+        if adam_state_bits not in (None, 8, 32):
+            raise ValueError(f"adam_state_bits must be None, 8 or 32, got {adam_state_bits!r}")
         _fill_aux_adam_groups(param_groups, self._SORT_MUON)
         super().__init__(param_groups, dict())
         self._init_runtime(ns_rounding, mutate_grad, workspace_bytes, ns_variant, use_graph, overlap_backward)
+        self._adam_state_bits = adam_state_bits
+
+    def __setstate__(self, state):
+        bits = state.get("muon_amd_options", {}).get("_adam_state_bits", getattr(self, "_adam_state_bits", None))
+        super().__setstate__(state)
+        self._adam_state_bits = bits
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        if self._adam_state_bits is not None:
+            self._load_adamw_state(state_dict, [p for g in self.param_groups if not g["use_muon"] for p in g["params"]])
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -446,8 +642,10 @@ class SingleDeviceMuonWithAuxAdam(_MuonBase):
         for gi, group in enumerate(self.param_groups):
             if group["use_muon"]:
                 self._muon_group_step(gi, group)
-            else:
+            elif self._adam_state_bits is None:
                 self._adam_group_step(gi, group)
+            else:
+                self._adamw_group_step(gi, group, self._adam_state_bits)
         self._launch_pending()
         return loss
 
