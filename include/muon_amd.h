@@ -194,6 +194,30 @@ typedef struct MuonGradDesc {
     int32_t reserved;            /* 0                                                         */
 } MuonGradDesc;
 
+/* The residual step between two blocks and its gradients (one struct for both directions; a host struct that is read
+ * during the call).  Rows of `width` elements; the ld_* are distances between rows in elements, outputs are contiguous.
+ * The residual stream (x, h, dh, dx) is stored as stream_dtype; b, y, gate and their gradients as block_dtype (bf16 if the
+ * stream is bf16); the vectors and their gradients as weight_dtype.                            */
+#define MUON_AMD_GATE_NONE    0
+#define MUON_AMD_GATE_TOKEN   1
+#define MUON_AMD_GATE_CHANNEL 2
+typedef struct MuonResidualNorm {
+    const void* x;  const void* b;
+    const void* gate;            /* logits, rows x width or (gate_is_token) rows; NULL: no gate */
+    const void* post_weight;  const void* pre_weight;    /* width                             */
+    const void* scale;           /* width or (scale_is_one) one element; NULL: 1              */
+    void* h;  void* y;           /* forward                                                   */
+    float* rstd;                 /* rows x 2: written by forward (NULL: not), read by backward */
+    const void* dh;  const void* dy;                     /* backward: NULL stands for zeros   */
+    void* dx;  void* db;  void* dgate;                   /* backward: NULL is not written     */
+    void* dpost_weight;  void* dpre_weight;  void* dscale;
+    float* partials;             /* backward: muon_amd_residual_norm_partials() floats if one of those three is asked for */
+    int64_t rows, ld_x, ld_b, ld_gate, ld_dh, ld_dy;
+    int32_t width, stream_dtype, block_dtype, weight_dtype, gate_is_token, scale_is_one;
+    float eps;
+    int32_t reserved;
+} MuonResidualNorm;
+
 /* One matrix of the AOL rescaling step of the 4-iteration variant (muon.py:776-785), in the
  * wide orientation: X is m_p x n_p with m_p <= n_p (zero padded).                           */
 typedef struct MuonAolDesc {
@@ -458,6 +482,16 @@ int muon_amd_grad_norm(const MuonGradDesc* descs_dev, const int32_t* block_prefi
                        double* partials_dev, float max_norm, float* out_dev, void* stream);
 int muon_amd_grad_clip(const MuonGradDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks,
                        double* partials_dev, float max_norm, float* out_dev, void* stream);
+
+/* ---- norms on both sides of a block with its gate and residual scale ------------------------- */
+/* h = x + scale * sigmoid(gate) * (b * rsqrt(mean(b^2) + eps)) * post_weight
+ * y = h * rsqrt(mean(h^2) + eps) * pre_weight                  (h unrounded)
+ * and from dh, dy the gradients of every input.  fp32 arithmetic and sums; the sums over rows in a fixed order. */
+size_t  muon_amd_sizeof_residual_norm(void);
+int     muon_amd_residual_norm_max_width(void);
+int64_t muon_amd_residual_norm_partials(int64_t rows, int width);
+int     muon_amd_residual_norm(const MuonResidualNorm* args_host, void* stream);
+int     muon_amd_residual_norm_backward(const MuonResidualNorm* args_host, void* stream);
 
 #ifdef __cplusplus
 }

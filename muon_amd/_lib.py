@@ -72,6 +72,15 @@ ADAMW_VALUES_DESC = np.dtype(
     align=True)
 GRAD_DESC = np.dtype([("grad", "<u8"), ("numel", "<i8"), ("dtype", "<i4"), ("reserved", "<i4")], align=True)
 
+
+class ResidualNormArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "b", "gate", "post_weight", "pre_weight", "scale", "h", "y", "rstd", "dh", "dy",
+                                                "dx", "db", "dgate", "dpost_weight", "dpre_weight", "dscale", "partials")] +
+                [(n, ctypes.c_int64) for n in ("rows", "ld_x", "ld_b", "ld_gate", "ld_dh", "ld_dy")] +
+                [(n, ctypes.c_int32) for n in ("width", "stream_dtype", "block_dtype", "weight_dtype", "gate_is_token", "scale_is_one")] +
+                [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)])
+
+
 _c_int = ctypes.c_int
 _c_float = ctypes.c_float
 _vp = ctypes.c_void_p
@@ -125,6 +134,11 @@ SIGNATURES = {
     "muon_amd_grad_norm_partials": (_c_int, []),
     "muon_amd_validate_grads": (_c_int, [_vp, _c_int, _vp]),
     "muon_amd_grad_norm": (_c_int, [_vp, _vp, _c_int, _c_int, _vp, _c_float, _vp, _vp]),
+    "muon_amd_sizeof_residual_norm": (ctypes.c_size_t, []),
+    "muon_amd_residual_norm_max_width": (_c_int, []),
+    "muon_amd_residual_norm_partials": (ctypes.c_int64, [ctypes.c_int64, _c_int]),
+    "muon_amd_residual_norm": (_c_int, [ctypes.POINTER(ResidualNormArgs), _vp]),
+    "muon_amd_residual_norm_backward": (_c_int, [ctypes.POINTER(ResidualNormArgs), _vp]),
     "muon_amd_grad_clip": (_c_int, [_vp, _vp, _c_int, _c_int, _vp, _c_float, _vp, _vp]),
 }
 
@@ -159,6 +173,9 @@ def load():
                    (GRAD_DESC, lib.muon_amd_sizeof_grad_desc)):
         if dt.itemsize != fn():
             raise MuonAmdError(f"struct layout mismatch: binding {dt.itemsize} bytes, library {fn()}")
+    for struct, fn in ((ResidualNormArgs, lib.muon_amd_sizeof_residual_norm),):
+        if ctypes.sizeof(struct) != fn():
+            raise MuonAmdError(f"struct layout mismatch: binding {ctypes.sizeof(struct)} bytes, library {fn()}")
     _lib = lib
     return lib
 

@@ -1,0 +1,438 @@
+// The step between two blocks of a transformer, with its gradients: the norm after a block, its gate and residual
+// scale, the addition to the residual stream, and the norm before the next block.  Per row (token) of D channels:
+//   nb = b rb,  rb = (mean(b^2) + eps)^-1/2;   h = x + s sig(z) nb wpost
+//   nh = h rh,  rh = (mean(h^2) + eps)^-1/2;   y = nh wpre
+// and backward, from the gradients dh and dy of both results, with k = s wpost:
+//   e  = dh + rh dy wpre,  c1 = mean(dy wpre nh),  dx = e - rh c1 nh
+//   c2 = mean(dx k sig nb),  db = rb (dx k sig - c2 nb),  dz = dx k nb sig (1 - sig)
+//   q  = sum over rows of dx sig nb:  dwpost = s q,  ds = wpost q;   dwpre = sum over rows of dy nh
+// All sums are fp32 whatever the tensors are stored in; h enters the second norm and the gradients unrounded (the
+// backward pass forms it again from x and b, which costs what reading it would), so that the gradients of the vectors are
+// as exact as the inputs.  c2 follows from sums that do not wait for c1 (dx is linear in it):
+//   D c2 = sum(e k sig nb) - rh c1 sum(nh k sig nb)
+// so that a row takes one reduction; the gradient of a gate for the whole row is (1 - sig) D c2.
+//
+// Memory bounds both passes.  A row stays in the registers of TPR threads (one wave up to 1024 channels forward, 512
+// backward: no barrier), 8 elements per access; a workgroup takes row after row with the weights of its channels, and
+// backward their sums, held in registers, and the workgroups' sums are joined in a fixed order by a second launch.
+#include <type_traits>
+
+#include "vector.h"
+
+namespace muon_amd {
+
+enum { GATE_NONE = MUON_AMD_GATE_NONE, GATE_TOKEN = MUON_AMD_GATE_TOKEN, GATE_CHANNEL = MUON_AMD_GATE_CHANNEL };
+constexpr int RN_MAX_WIDTH = 16384;
+constexpr int RN_THREADS = 256;            // of a workgroup, more where a row needs them
+
+// The sum over the 64 lanes, in every lane.
+__device__ __forceinline__ float lanes_sum(float v) {
+    const auto other = [](float x, auto ctrl) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    v += other(v, std::integral_constant<int, 0xB1>{});      // quad_perm 1,0,3,2
+    v += other(v, std::integral_constant<int, 0x4E>{});      // quad_perm 2,3,0,1
+    v += other(v, std::integral_constant<int, 0x141>{});     // row_half_mirror
+    v += other(v, std::integral_constant<int, 0x140>{});     // row_mirror
+    const auto row = [&](int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); };
+    return (row(0) + row(16)) + (row(32) + row(48));
+}
+
+// Sums over the threads of a row.  Rows of one wave need no barrier; else every wave leaves its sums in one of two sets of
+// slots, which the caller alternates between (one barrier a sum: who writes a set again has passed the barrier after
+// which the others read it).
+template <int TPR, int N>
+__device__ __forceinline__ void row_sums(float (&s)[N], float (*slots)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] = lanes_sum(s[k]);
+    if constexpr (TPR > 64) {
+        constexpr int WAVES = TPR / 64;
+        const int wave = threadIdx.x >> 6, first = wave & ~(WAVES - 1);
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < N; ++k) slots[wave][k] = s[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            float t = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) t += slots[first + w][k];
+            s[k] = t;
+        }
+    }
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+
+// Eight elements of a vector of weights in fp32 (zero beyond the row).
+__device__ __forceinline__ void load_weights(const void* p, int dtype, int c, int width, float (&w)[8]) {
+    if (dtype == MUON_AMD_SRC_BF16) {
+        const Group8<uint16_t> g = load_group<uint16_t, false>(static_cast<const uint16_t*>(p), c, width);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = g[k];
+    } else {
+        const Group8<float> g = load_group<float, false>(static_cast<const float*>(p), c, width);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = g[k];
+    }
+}
+__device__ __forceinline__ float load_one(const void* p, int dtype, int64_t i) {
+    return dtype == MUON_AMD_SRC_BF16 ? bf2f(static_cast<const uint16_t*>(p)[i]) : static_cast<const float*>(p)[i];
+}
+// The scale of eight channels: one per channel, one for all, or none.
+__device__ __forceinline__ void load_scale(const MuonResidualNorm& a, int c, float (&s)[8]) {
+    if (a.scale && !a.scale_is_one) {
+        load_weights(a.scale, a.weight_dtype, c, a.width, s);
+        return;
+    }
+    const float one = a.scale ? load_one(a.scale, a.weight_dtype, 0) : 1.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] = one;
+}
+
+template <typename X, typename B, int GATE, int TPR, int V>
+__global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_forward_kernel(const MuonResidualNorm a) {
+    constexpr int THREADS = TPR > RN_THREADS ? TPR : RN_THREADS, ROWS = THREADS / TPR;
+    __shared__ float slots[2][THREADS / 64][1];
+    const int t = threadIdx.x % TPR, width = a.width;
+    float k[V][8], wpre[V][8];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = (j * TPR + t) * 8;
+        float s[8];
+        load_scale(a, c, s);
+        load_weights(a.post_weight, a.weight_dtype, c, width, k[j]);
+        load_weights(a.pre_weight, a.weight_dtype, c, width, wpre[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[j][i] *= s[i];
+    }
+    const float per = 1.f / static_cast<float>(width);
+    for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS; first < a.rows; first += static_cast<int64_t>(gridDim.x) * ROWS) {
+        const int64_t row = first + threadIdx.x / TPR;
+        const bool in = row < a.rows;                             // (rows of several waves meet at barriers)
+        const int n = in ? width : 0;
+        const X* const x = static_cast<const X*>(a.x) + row * a.ld_x;
+        const B* const b = static_cast<const B*>(a.b) + row * a.ld_b;
+        const B* const z = static_cast<const B*>(a.gate) + row * a.ld_gate;
+        Group8<X> xv[V];
+        Group8<B> bv[V], zv[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (j * TPR + t) * 8;
+            bv[j] = load_group<B, true>(b, c, n);
+            xv[j] = load_group<X, true>(x, c, n);
+            if constexpr (GATE == GATE_CHANNEL) zv[j] = load_group<B, true>(z, c, n);
+        }
+        float whole = 1.f;
+        if constexpr (GATE == GATE_TOKEN) whole = in ? sigmoid(Group8<B>::load_first(z, 1)[0]) : 0.f;
+        float sum[1] = {0.f};
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[0] = fmaf(bv[j][i], bv[j][i], sum[0]);
+        row_sums<TPR, 1>(sum, slots[0]);
+        const float rb = 1.f / sqrtf(fmaf(sum[0], per, a.eps));
+        float h[V][8];
+        sum[0] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (j * TPR + t) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float sig = GATE == GATE_CHANNEL ? sigmoid(zv[j][i]) : whole;
+                h[j][i] = fmaf(bv[j][i] * rb, k[j][i] * sig, xv[j][i]);
+                if (c + i < n) sum[0] = fmaf(h[j][i], h[j][i], sum[0]);
+            }
+            store_group<X, false>(static_cast<X*>(a.h) + row * width, c, n, Group8<X>::of(h[j]));
+        }
+        row_sums<TPR, 1>(sum, slots[1]);
+        const float rh = 1.f / sqrtf(fmaf(sum[0], per, a.eps));
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (j * TPR + t) * 8;
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = h[j][i] * rh * wpre[j][i];
+            store_group<B, false>(static_cast<B*>(a.y) + row * width, c, n, Group8<B>::of(y));
+        }
+        if (in && t == 0 && a.rstd) {
+            a.rstd[2 * row] = rb;
+            a.rstd[2 * row + 1] = rh;
+        }
+    }
+}
+
+template <typename X, typename B, int GATE, int TPR, int V>
+__global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_backward_kernel(const MuonResidualNorm a) {
+    constexpr int THREADS = TPR > RN_THREADS ? TPR : RN_THREADS, ROWS = THREADS / TPR;
+    __shared__ float slots[2][THREADS / 64][3];
+    const int t = threadIdx.x % TPR, width = a.width;
+    float k[V][8], wpre[V][8], q[V][8], r[V][8];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = (j * TPR + t) * 8;
+        float s[8];
+        load_scale(a, c, s);
+        load_weights(a.post_weight, a.weight_dtype, c, width, k[j]);
+        load_weights(a.pre_weight, a.weight_dtype, c, width, wpre[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            k[j][i] *= s[i];
+            q[j][i] = r[j][i] = 0.f;
+        }
+    }
+    const float per = 1.f / static_cast<float>(width);
+    int set = 0;
+    for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS; first < a.rows; first += static_cast<int64_t>(gridDim.x) * ROWS) {
+        const int64_t row = first + threadIdx.x / TPR;
+        const bool in = row < a.rows;
+        const int n = in ? width : 0;
+        const X* const x = static_cast<const X*>(a.x) + row * a.ld_x;
+        const B* const b = static_cast<const B*>(a.b) + row * a.ld_b;
+        const B* const z = static_cast<const B*>(a.gate) + row * a.ld_gate;
+        Group8<X> xv[V], dhv[V];
+        Group8<B> bv[V], zv[V], dyv[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (j * TPR + t) * 8;
+            bv[j] = load_group<B, true>(b, c, n);
+            xv[j] = load_group<X, true>(x, c, n);
+            if constexpr (GATE == GATE_CHANNEL) zv[j] = load_group<B, true>(z, c, n);
+            dyv[j] = a.dy ? load_group<B, true>(static_cast<const B*>(a.dy) + row * a.ld_dy, c, n) : Group8<B>::zero();
+            dhv[j] = a.dh ? load_group<X, true>(static_cast<const X*>(a.dh) + row * a.ld_dh, c, n) : Group8<X>::zero();
+        }
+        const float rb = in ? a.rstd[2 * row] : 0.f, rh = in ? a.rstd[2 * row + 1] : 0.f;
+        float whole = 1.f;
+        if constexpr (GATE == GATE_TOKEN) whole = in ? sigmoid(Group8<B>::load_first(z, 1)[0]) : 0.f;
+        float sums[3] = {0.f, 0.f, 0.f};
+        float nh[V][8], e[V][8], sig[V][8];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sig[j][i] = GATE == GATE_CHANNEL ? sigmoid(zv[j][i]) : whole;
+                const float kk = k[j][i] * sig[j][i], nb = bv[j][i] * rb;
+                nh[j][i] = fmaf(nb, kk, xv[j][i]) * rh;
+                const float dn = dyv[j][i] * wpre[j][i];
+                e[j][i] = fmaf(rh, dn, dhv[j][i]);
+                sums[0] = fmaf(dn, nh[j][i], sums[0]);
+                sums[1] = fmaf(e[j][i] * kk, nb, sums[1]);
+                sums[2] = fmaf(nh[j][i] * kk, nb, sums[2]);
+                r[j][i] = fmaf(dyv[j][i], nh[j][i], r[j][i]);
+            }
+        row_sums<TPR, 3>(sums, slots[set]);
+        set ^= 1;
+        const float c1 = sums[0] * per * rh, dc2 = fmaf(-c1, sums[2], sums[1]), c2 = dc2 * per;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (j * TPR + t) * 8;
+            float dx[8], db[8], dz[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float nb = bv[j][i] * rb, kk = k[j][i] * sig[j][i];
+                dx[i] = fmaf(-c1, nh[j][i], e[j][i]);
+                db[i] = rb * fmaf(dx[i], kk, -c2 * nb);
+                const float g = dx[i] * nb;
+                q[j][i] = fmaf(g, sig[j][i], q[j][i]);
+                dz[i] = g * kk * (1.f - sig[j][i]);
+            }
+            if (a.dx) store_group<X, false>(static_cast<X*>(a.dx) + row * width, c, n, Group8<X>::of(dx));
+            if (a.db) store_group<B, false>(static_cast<B*>(a.db) + row * width, c, n, Group8<B>::of(db));
+            if constexpr (GATE == GATE_CHANNEL)
+                if (a.dgate) store_group<B, false>(static_cast<B*>(a.dgate) + row * width, c, n, Group8<B>::of(dz));
+        }
+        if constexpr (GATE == GATE_TOKEN)
+            if (in && t == 0 && a.dgate) {
+                const float one[8] = {(1.f - whole) * dc2};
+                Group8<B>::of(one).store_first(static_cast<B*>(a.dgate) + row, 1);
+            }
+    }
+    // sums of this workgroup: its rows' threads one after the other, through LDS where there is more than one
+    if (!a.partials) return;
+    float* const out = a.partials + static_cast<int64_t>(blockIdx.x) * 2 * width;
+    if constexpr (ROWS > 1) {
+        __shared__ float joined[ROWS - 1][2][V][8][TPR];
+        const int sub = threadIdx.x / TPR;
+        if (sub > 0)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    joined[sub - 1][0][j][i][t] = q[j][i];
+                    joined[sub - 1][1][j][i][t] = r[j][i];
+                }
+        __syncthreads();
+        if (sub > 0) return;
+        for (int o = 0; o < ROWS - 1; ++o)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    q[j][i] += joined[o][0][j][i][t];
+                    r[j][i] += joined[o][1][j][i][t];
+                }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = (j * TPR + t) * 8;
+        store_group<float, false>(out, c, width, Group8<float>::of(q[j]));
+        store_group<float, false>(out + width, c, width, Group8<float>::of(r[j]));
+    }
+}
+
+// The sums over the workgroups: 64 columns of q or r per workgroup, 16 shares of the partial rows joined in order.
+constexpr int RS_SHARES = 16;
+__device__ __forceinline__ void store_one(void* p, int dtype, int64_t i, float v) {
+    if (dtype == MUON_AMD_SRC_BF16) static_cast<uint16_t*>(p)[i] = f2bf(v);
+    else static_cast<float*>(p)[i] = v;
+}
+__global__ __launch_bounds__(64 * RS_SHARES) void residual_columns_kernel(const MuonResidualNorm a, int npartials, float* __restrict__ one) {
+    __shared__ float part[RS_SHARES][64];
+    const int lane = threadIdx.x & 63, share = threadIdx.x >> 6, width = a.width;
+    const int c = blockIdx.x * 64 + lane, which = blockIdx.y;            // 0: q, 1: r
+    float s = 0.f;
+    if (c < width)
+        for (int g = share; g < npartials; g += RS_SHARES) s += a.partials[(static_cast<int64_t>(g) * 2 + which) * width + c];
+    part[share][lane] = s;
+    __syncthreads();
+    if (share > 0 || c >= width) return;
+    for (int o = 1; o < RS_SHARES; ++o) s += part[o][lane];
+    if (which) {
+        if (a.dpre_weight) store_one(a.dpre_weight, a.weight_dtype, c, s);
+        return;
+    }
+    if (a.dpost_weight)
+        store_one(a.dpost_weight, a.weight_dtype, c, a.scale ? s * load_one(a.scale, a.weight_dtype, a.scale_is_one ? 0 : c) : s);
+    const float ds = s * load_one(a.post_weight, a.weight_dtype, c);
+    if (one) one[c] = ds;
+    else if (a.dscale) store_one(a.dscale, a.weight_dtype, c, ds);
+}
+
+// The gradient of a scale that all channels share.
+__global__ __launch_bounds__(256) void residual_scale_kernel(const float* __restrict__ one, int width, void* dscale, int dtype) {
+    __shared__ float part[4];
+    float s = 0.f;
+    for (int c = threadIdx.x; c < width; c += 256) s += one[c];
+    s = lanes_sum(s);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) store_one(dscale, dtype, 0, (part[0] + part[1]) + (part[2] + part[3]));
+}
+
+// How a width is shared among threads: threads per row (a power of two) and groups of eight per thread.
+template <int T, int G>
+struct Shape {
+    static constexpr int TPR = T, V = G;
+};
+template <typename F>
+static void with_forward_shape(int width, F&& f) {
+    if (width <= 512) f(Shape<64, 1>{});
+    else if (width <= 1024) f(Shape<64, 2>{});
+    else if (width <= 2048) f(Shape<128, 2>{});
+    else if (width <= 4096) f(Shape<256, 2>{});
+    else if (width <= 8192) f(Shape<512, 2>{});
+    else f(Shape<1024, 2>{});
+}
+template <typename F>
+static void with_backward_shape(int width, F&& f) {
+    if (width <= 512) f(Shape<64, 1>{});
+    else if (width <= 1024) f(Shape<128, 1>{});
+    else if (width <= 2048) f(Shape<256, 1>{});
+    else if (width <= 4096) f(Shape<512, 1>{});
+    else if (width <= 8192) f(Shape<1024, 1>{});
+    else f(Shape<1024, 2>{});
+}
+template <typename F>
+static void with_types(const MuonResidualNorm& a, F&& f) {
+    const auto gates = [&](auto x, auto b) {
+        if (!a.gate) f(x, b, std::integral_constant<int, GATE_NONE>{});
+        else if (a.gate_is_token) f(x, b, std::integral_constant<int, GATE_TOKEN>{});
+        else f(x, b, std::integral_constant<int, GATE_CHANNEL>{});
+    };
+    if (a.stream_dtype == MUON_AMD_SRC_BF16) gates(uint16_t{}, uint16_t{});
+    else if (a.block_dtype == MUON_AMD_SRC_BF16) gates(float{}, uint16_t{});
+    else gates(float{}, float{});
+}
+
+// Workgroups of a launch over `rows` rows: all of them, up to `per_cu` for each of the 256 CUs.
+static int workgroups(int64_t rows, int rows_each, int per_cu) {
+    const int64_t n = (rows + rows_each - 1) / rows_each;
+    return static_cast<int>(n < 256 * per_cu ? n : 256 * per_cu);
+}
+static int backward_workgroups(int64_t rows, int width) {
+    int n = 0;
+    with_backward_shape(width, [&](auto s) {
+        constexpr int TPR = decltype(s)::TPR, THREADS = TPR > RN_THREADS ? TPR : RN_THREADS;
+        n = workgroups(rows, THREADS / TPR, 1024 / THREADS);
+    });
+    return n;
+}
+
+static int check_residual(const MuonResidualNorm* a, const char* what) {
+    MUON_REQUIRE(a, "%s: null arguments", what);
+    MUON_REQUIRE(a->rows > 0 && a->width > 0 && a->width <= RN_MAX_WIDTH, "%s: rows=%lld width=%d (at most %d)", what,
+                 static_cast<long long>(a->rows), a->width, RN_MAX_WIDTH);
+    MUON_REQUIRE(a->x && a->b && a->post_weight && a->pre_weight, "%s: null input", what);
+    for (const int32_t t : {a->stream_dtype, a->block_dtype, a->weight_dtype})
+        MUON_REQUIRE(t == MUON_AMD_SRC_F32 || t == MUON_AMD_SRC_BF16, "%s: dtype=%d", what, t);
+    MUON_REQUIRE(a->stream_dtype == MUON_AMD_SRC_F32 || a->block_dtype == MUON_AMD_SRC_BF16,
+                 "%s: a bf16 residual stream takes a bf16 block", what);
+    MUON_REQUIRE(a->eps >= 0.f, "%s: eps=%g", what, a->eps);
+    return MUON_AMD_OK;
+}
+
+}  // namespace muon_amd
+
+using namespace muon_amd;
+
+extern "C" {
+
+size_t muon_amd_sizeof_residual_norm(void) { return sizeof(MuonResidualNorm); }
+int muon_amd_residual_norm_max_width(void) { return RN_MAX_WIDTH; }
+
+int64_t muon_amd_residual_norm_partials(int64_t rows, int width) {
+    if (rows <= 0 || width <= 0 || width > RN_MAX_WIDTH) return 0;
+    return (static_cast<int64_t>(backward_workgroups(rows, width)) * 2 + 1) * width;
+}
+
+int muon_amd_residual_norm(const MuonResidualNorm* args, void* stream) {
+    if (const int rc = check_residual(args, "residual_norm")) return rc;
+    MUON_REQUIRE(args->h && args->y, "residual_norm: null output");
+    const MuonResidualNorm a = *args;
+    with_types(a, [&](auto x, auto b, auto gate) {
+        with_forward_shape(a.width, [&](auto s) {
+            constexpr int TPR = decltype(s)::TPR, V = decltype(s)::V, THREADS = TPR > RN_THREADS ? TPR : RN_THREADS;
+            hipLaunchKernelGGL((residual_forward_kernel<decltype(x), decltype(b), decltype(gate)::value, TPR, V>),
+                               dim3(workgroups(a.rows, THREADS / TPR, 2048 / THREADS)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a);
+        });
+    });
+    return check_launch("residual_norm");
+}
+
+int muon_amd_residual_norm_backward(const MuonResidualNorm* args, void* stream) {
+    if (const int rc = check_residual(args, "residual_norm_backward")) return rc;
+    const MuonResidualNorm a = *args;
+    MUON_REQUIRE(a.rstd && (a.dy || a.dh), "residual_norm_backward: null input");
+    const bool columns = a.dpost_weight || a.dpre_weight || a.dscale;
+    MUON_REQUIRE(!columns || a.partials, "residual_norm_backward: null workspace");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const int n = backward_workgroups(a.rows, a.width);
+    MuonResidualNorm b = a;
+    if (!columns) b.partials = nullptr;
+    with_types(a, [&](auto x, auto y, auto gate) {
+        with_backward_shape(a.width, [&](auto s) {
+            constexpr int TPR = decltype(s)::TPR, V = decltype(s)::V, THREADS = TPR > RN_THREADS ? TPR : RN_THREADS;
+            hipLaunchKernelGGL((residual_backward_kernel<decltype(x), decltype(y), decltype(gate)::value, TPR, V>), dim3(n), dim3(THREADS),
+                               0, st, b);
+        });
+    });
+    if (const int rc = check_launch("residual_norm_backward")) return rc;
+    if (!columns) return MUON_AMD_OK;
+    float* const one = a.dscale && a.scale_is_one ? a.partials + static_cast<int64_t>(n) * 2 * a.width : nullptr;
+    hipLaunchKernelGGL(residual_columns_kernel, dim3((a.width + 63) / 64, 2), dim3(64 * RS_SHARES), 0, st, a, n, one);
+    if (const int rc = check_launch("residual_norm_backward")) return rc;
+    if (one) hipLaunchKernelGGL(residual_scale_kernel, dim3(1), dim3(256), 0, st, one, a.width, a.dscale, a.weight_dtype);
+    return check_launch("residual_norm_backward");
+}
+
+}  // extern "C"
