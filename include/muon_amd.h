@@ -218,6 +218,24 @@ typedef struct MuonResidualNorm {
     int32_t reserved;
 } MuonResidualNorm;
 
+/* Routing of tokens to experts, forward and backward (a host struct that is read during the call). */
+typedef struct MuonRoute {
+    const void* logits;          /* tokens x experts of dtype, ld_logits elements from row to row */
+    const uint8_t* mask;         /* tokens bytes, zero: the token takes no part; NULL: all do     */
+    float* weights;              /* tokens x k                                                    */
+    int32_t* indices;            /* tokens x k, -1 where a choice is not there                    */
+    int32_t* counts;             /* experts                                                       */
+    float* balance;  float* z;   /* one float each                                                */
+    float* part;                 /* one float: tokens that take part, at least 1                  */
+    float* lse;                  /* tokens: log sum exp; -infinity for a token that takes no part */
+    float* partials;             /* forward: muon_amd_route_partials() floats                     */
+    const float* dweights;       /* backward: tokens x k, ld_dweights from row to row; NULL: zeros */
+    const float* dbalance;  const float* dz;             /* backward: one float each; NULL: zero  */
+    void* dlogits;               /* backward: tokens x experts of dtype                           */
+    int64_t tokens, ld_logits, ld_dweights;
+    int32_t experts, k, dtype, normalize;
+} MuonRoute;
+
 /* One matrix of the AOL rescaling step of the 4-iteration variant (muon.py:776-785), in the
  * wide orientation: X is m_p x n_p with m_p <= n_p (zero padded).                           */
 typedef struct MuonAolDesc {
@@ -492,6 +510,18 @@ int     muon_amd_residual_norm_max_width(void);
 int64_t muon_amd_residual_norm_partials(int64_t rows, int width);
 int     muon_amd_residual_norm(const MuonResidualNorm* args_host, void* stream);
 int     muon_amd_residual_norm_backward(const MuonResidualNorm* args_host, void* stream);
+
+/* ---- routing of tokens to experts with its losses --------------------------------------------- */
+/* Per token: p = softmax(logits), the k largest logits (ties: the lowest index), their probabilities as weights
+ * (normalize: divided by their sum).  A logit of -infinity is never chosen.  Over the N tokens that take part (not masked
+ * out, with a logit above -infinity): counts, balance = experts * sum_e counts_e / (N k) * mean p_e, z = mean of
+ * lse^2.  Backward reads what forward wrote.                                                        */
+size_t  muon_amd_sizeof_route(void);
+int     muon_amd_route_max_experts(void);
+int     muon_amd_route_max_k(void);
+int64_t muon_amd_route_partials(int64_t tokens, int experts);
+int     muon_amd_route(const MuonRoute* args_host, void* stream);
+int     muon_amd_route_backward(const MuonRoute* args_host, void* stream);
 
 #ifdef __cplusplus
 }

@@ -7,7 +7,7 @@ hand-written HIP kernels in libmuon_amd.so (see include/muon_amd.h for its C ABI
 from .functional import (adam_update, clear_engine_cache, muon_update, zeropower_via_aol4,
                          zeropower_via_newtonschulz5)
 from .gradients import clip_coefficient, clip_grad_norm_
-from .layers import residual_norm
+from .layers import Routing, residual_norm, route_topk
 from .ops import ns_line_1, ns_line_2, ns_line_3
 from .optim import AdamW, Muon, MuonWithAuxAdam, SingleDeviceMuon, SingleDeviceMuonWithAuxAdam
 from ._lib import MuonAmdError
@@ -16,6 +16,6 @@ __all__ = [
     "Muon", "SingleDeviceMuon", "MuonWithAuxAdam", "SingleDeviceMuonWithAuxAdam",
     "zeropower_via_newtonschulz5", "zeropower_via_aol4", "muon_update", "adam_update", "clear_engine_cache",
     "ns_line_1", "ns_line_2", "ns_line_3",
-    "AdamW", "clip_grad_norm_", "clip_coefficient", "residual_norm",
+    "AdamW", "clip_grad_norm_", "clip_coefficient", "residual_norm", "route_topk", "Routing",
     "MuonAmdError",
 ]

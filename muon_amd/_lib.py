@@ -81,6 +81,13 @@ class ResidualNormArgs(ctypes.Structure):
                 [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)])
 
 
+class RouteArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "mask", "weights", "indices", "counts", "balance", "z", "part", "lse", "partials",
+                                                "dweights", "dbalance", "dz", "dlogits")] +
+                [(n, ctypes.c_int64) for n in ("tokens", "ld_logits", "ld_dweights")] +
+                [(n, ctypes.c_int32) for n in ("experts", "k", "dtype", "normalize")])
+
+
 _c_int = ctypes.c_int
 _c_float = ctypes.c_float
 _vp = ctypes.c_void_p
@@ -139,6 +146,12 @@ SIGNATURES = {
     "muon_amd_residual_norm_partials": (ctypes.c_int64, [ctypes.c_int64, _c_int]),
     "muon_amd_residual_norm": (_c_int, [ctypes.POINTER(ResidualNormArgs), _vp]),
     "muon_amd_residual_norm_backward": (_c_int, [ctypes.POINTER(ResidualNormArgs), _vp]),
+    "muon_amd_sizeof_route": (ctypes.c_size_t, []),
+    "muon_amd_route_max_experts": (_c_int, []),
+    "muon_amd_route_max_k": (_c_int, []),
+    "muon_amd_route_partials": (ctypes.c_int64, [ctypes.c_int64, _c_int]),
+    "muon_amd_route": (_c_int, [ctypes.POINTER(RouteArgs), _vp]),
+    "muon_amd_route_backward": (_c_int, [ctypes.POINTER(RouteArgs), _vp]),
     "muon_amd_grad_clip": (_c_int, [_vp, _vp, _c_int, _c_int, _vp, _c_float, _vp, _vp]),
 }
 
@@ -173,7 +186,7 @@ def load():
                    (GRAD_DESC, lib.muon_amd_sizeof_grad_desc)):
         if dt.itemsize != fn():
             raise MuonAmdError(f"struct layout mismatch: binding {dt.itemsize} bytes, library {fn()}")
-    for struct, fn in ((ResidualNormArgs, lib.muon_amd_sizeof_residual_norm),):
+    for struct, fn in ((ResidualNormArgs, lib.muon_amd_sizeof_residual_norm), (RouteArgs, lib.muon_amd_sizeof_route)):
         if ctypes.sizeof(struct) != fn():
             raise MuonAmdError(f"struct layout mismatch: binding {ctypes.sizeof(struct)} bytes, library {fn()}")
     _lib = lib

@@ -20,7 +20,8 @@ import tempfile
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmuon_amd.so")
-SOURCES = ["capi.hip", "elementwise.hip", "aol.hip", "ns_gemm.hip", "small.hip", "step.hip", "adamw.hip", "grad_norm.hip", "residual.hip"]
+SOURCES = ["capi.hip", "elementwise.hip", "aol.hip", "ns_gemm.hip", "small.hip", "step.hip", "adamw.hip", "grad_norm.hip",
+           "residual.hip", "route.hip"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # hipcc -O3 must not form packed-fp32 instructions on this target

@@ -4,10 +4,13 @@ functions with gradients.
     residual_norm(x, block, post_weight, pre_weight, gate=..., scale=...)  -> h, y
         the norm after a block, its gate and residual scale, the addition to the residual stream, and the norm before
         the next block, in one pass
+    route_topk(logits, k)  -> weights, indices, counts, balance_loss, z_loss
+        the experts of each token, tokens per expert, and the losses that keep them balanced
 """
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -142,3 +145,96 @@ def residual_norm(x: torch.Tensor, block: torch.Tensor, post_weight: torch.Tenso
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
     return _ResidualNorm.apply(x, block, post_weight, pre_weight, gate, scale, float(eps))
+
+
+class Routing(NamedTuple):
+    """What route_topk returns."""
+    weights: torch.Tensor        # (..., k) fp32
+    indices: torch.Tensor        # (..., k) int32, -1 where a choice is not there
+    counts: torch.Tensor         # (experts,) int32
+    balance_loss: torch.Tensor   # 0-dim fp32
+    z_loss: torch.Tensor         # 0-dim fp32
+
+
+class _RouteTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, mask, normalize):
+        experts = logits.size(-1)
+        tokens = logits.numel() // experts
+        f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)
+        weights, indices = f32(*logits.shape[:-1], k), torch.empty(*logits.shape[:-1], k, dtype=torch.int32, device=logits.device)
+        ctx.set_materialize_grads(False)
+        ctx.normalize = normalize
+        if tokens == 0:
+            counts, balance, z = torch.zeros(experts, dtype=torch.int32, device=logits.device), f32().zero_(), f32().zero_()
+            ctx.save_for_backward(logits, None, None, None, None, None, None)
+        else:
+            counts, balance, z = torch.empty(experts, dtype=torch.int32, device=logits.device), f32(), f32()
+            part, lse = f32(), f32(tokens)
+            lib = _lib.load()
+            partials = f32(lib.muon_amd_route_partials(tokens, experts))
+            a, keep = _route_args(logits, mask, weights, indices, counts, part, lse, normalize)
+            a.balance, a.z, a.partials = balance.data_ptr(), z.data_ptr(), partials.data_ptr()
+            with torch.cuda.device(logits.device):
+                _launch("route", logits.numel() * logits.element_size() + 8 * indices.numel(), lambda: _lib.check(
+                    lib.muon_amd_route(ctypes.byref(a), _stream_ptr(logits.device)), "route"))
+            if ctx.needs_input_grad[0]:
+                ctx.save_for_backward(logits, mask, weights, indices, counts, part, lse)
+        ctx.mark_non_differentiable(indices, counts)
+        return weights, indices, counts, balance, z
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dweights, _, __, dbalance, dz):
+        logits, mask, weights, indices, counts, part, lse = ctx.saved_tensors
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if lse is None:
+            return dlogits, None, None, None
+        a, keep = _route_args(logits, mask, weights, indices, counts, part, lse, ctx.normalize)
+        a.dlogits = dlogits.data_ptr()
+        if dweights is not None:
+            dweights = _rows(dweights, a.k)
+            a.dweights, a.ld_dweights = dweights.data_ptr(), dweights.stride(0)
+        a.dbalance, a.dz = (None if t is None else t.data_ptr() for t in (dbalance, dz))
+        with torch.cuda.device(logits.device):
+            _launch("route_backward", 2 * logits.numel() * logits.element_size() + 12 * indices.numel(), lambda: _lib.check(
+                _lib.load().muon_amd_route_backward(ctypes.byref(a), _stream_ptr(logits.device)), "route_backward"))
+        return dlogits, None, None, None
+
+
+def _route_args(logits, mask, weights, indices, counts, part, lse, normalize):
+    """The arguments of both directions, and the tensors behind the addresses in them."""
+    rows = _rows(logits, logits.size(-1))
+    flags = None if mask is None else mask.contiguous()
+    a = _lib.RouteArgs(logits=rows.data_ptr(), mask=None if flags is None else flags.data_ptr(), weights=weights.data_ptr(),
+                       indices=indices.data_ptr(), counts=counts.data_ptr(), part=part.data_ptr(), lse=lse.data_ptr(), tokens=rows.size(0),
+                       ld_logits=rows.stride(0), experts=rows.size(1), k=weights.size(-1), dtype=_DTYPES[logits.dtype],
+                       normalize=int(normalize))
+    return a, (rows, flags)
+
+
+def route_topk(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = None, normalize: bool = True) -> Routing:
+    """The k experts of each token from its logits (..., experts), fp32 or bf16, with the losses of a balanced router:
+
+        p = softmax(logits);  indices: the k largest logits, of equal ones the lowest index first
+        weights = p at indices, divided by their sum (normalize=False: as they are)
+        counts[e] = tokens that have e among their k
+        balance_loss = E sum_e (counts[e] / (N k)) (mean of p[:, e]);  z_loss = mean of logsumexp(logits)^2
+
+    over the N tokens that take part: those whose `mask` (bool, the shape of logits without its last dimension) is true and
+    that have an expert available at all.  An expert whose logit is -infinity is not available to that token; a
+    choice that is not there has index -1 and weight 0.  A token that takes no part has indices -1, weights 0 and no
+    gradient.  Gradients flow to the logits from weights, balance_loss (through p; counts are constants) and z_loss.
+    NaN counts as the largest logit.  At most 1024 experts and 32 choices.  Sums are fp32 in a fixed order."""
+    require_gpu_tensor(logits, "logits")
+    _dtype(logits, "logits")
+    lib = _lib.load()
+    if logits.ndim < 1 or not 1 <= logits.size(-1) <= lib.muon_amd_route_max_experts():
+        raise ValueError(f"logits must have 1 to {lib.muon_amd_route_max_experts()} experts as their last dimension, got {tuple(logits.shape)}")
+    if isinstance(k, bool) or int(k) != k or not 1 <= k <= min(logits.size(-1), lib.muon_amd_route_max_k()):
+        raise ValueError(f"k must be 1 to {min(logits.size(-1), lib.muon_amd_route_max_k())}, got {k!r}")
+    if mask is not None:
+        require_gpu_tensor(mask, "mask")
+        if mask.dtype != torch.bool or mask.shape != logits.shape[:-1] or mask.device != logits.device:
+            raise ValueError(f"mask must be a bool tensor of shape {tuple(logits.shape[:-1])} on {logits.device}, got {mask.dtype} {tuple(mask.shape)}")
+    return Routing(*_RouteTopk.apply(logits, int(k), mask, bool(normalize)))
