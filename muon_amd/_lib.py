@@ -193,6 +193,28 @@ def load():
     return lib
 
 
+_native = None
+
+
+def native():
+    """The host side of the operators (muon_amd._native, built with the library), bound to this library's entry points."""
+    global _native
+    if _native is not None:
+        return _native
+    lib = load()
+    import torch                                  # noqa: F401  (the module links against torch's libraries)
+    try:
+        from . import _native as module
+    except ImportError as e:
+        raise MuonAmdError(f"muon_amd/_native.so is missing or does not load ({e}): build it with `python -m muon_amd.build`. "
+                           "There is no fallback implementation.") from None
+    if module.abi_version() != ABI_VERSION:
+        raise MuonAmdError(f"ABI mismatch: muon_amd._native {module.abi_version()}, binding {ABI_VERSION}")
+    module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in SIGNATURES}, MuonAmdError)
+    _native = module
+    return module
+
+
 def check(rc: int, what: str = "") -> None:
     if rc != 0:
         msg = load().muon_amd_last_error().decode("utf-8", "replace")

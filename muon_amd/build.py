@@ -2,6 +2,8 @@
 
     python -m muon_amd.build
 
+and muon_amd/_native.so, the host side of the operators (csrc/host.cpp), with g++ against torch's C++ interface.
+
 After the library is built, the GEMM kernels are compiled once more to assembly and checked
 (`check_fragment_waits`): their main loop requests its LDS fragments through inline assembly and
 waits for them by hand, which is only correct while the compiler does not touch a requested
@@ -20,6 +22,7 @@ import tempfile
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmuon_amd.so")
+NATIVE_OUT = os.path.join(HERE, "_native.so")
 SOURCES = ["capi.hip", "elementwise.hip", "aol.hip", "ns_gemm.hip", "small.hip", "step.hip", "adamw.hip", "grad_norm.hip",
            "residual.hip", "route.hip"]
 FLAGS = [
@@ -134,6 +137,21 @@ def check_store_data(asm_text: str) -> int:
     return nstores
 
 
+def native_command(out: str) -> list:
+    """The g++ line that builds muon_amd._native."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), sysconfig.get_paths()["include"]]
+    lib = os.path.join(root, "lib")
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[a for d in includes for a in ("-isystem", d)], os.path.join(CSRC, "host.cpp"), "-o", out,
+            "-L" + lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-Wl,-rpath," + lib]
+
+
 def build(verbose: bool = True, check: bool = True) -> str:
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     tmp = OUT + ".tmp"
@@ -142,6 +160,8 @@ def build(verbose: bool = True, check: bool = True) -> str:
         compile_flags = [f for f in FLAGS if f != "-shared"]
         cmds = [[hipcc, *compile_flags, *SOURCE_FLAGS.get(src, []), "-c", os.path.join(CSRC, src), "-o", obj]
                 for src, obj in zip(SOURCES, objects)]
+        native_tmp = NATIVE_OUT + ".tmp"
+        cmds.append(native_command(native_tmp))
         if verbose:
             print("\n".join(" ".join(c) for c in cmds), flush=True)
         procs = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for c in cmds]
@@ -151,7 +171,7 @@ def build(verbose: bool = True, check: bool = True) -> str:
             procs, outputs = [link], [link.stdout + link.stderr]
         if any(p.returncode for p in procs):
             sys.stderr.write("".join(outputs))
-            raise RuntimeError("hipcc failed building libmuon_amd.so")
+            raise RuntimeError("building libmuon_amd.so and _native.so failed")
     if check:
         with tempfile.TemporaryDirectory() as d:
             listing = os.path.join(d, "ns_gemm.s")
@@ -167,6 +187,7 @@ def build(verbose: bool = True, check: bool = True) -> str:
             if verbose:
                 print(f"ns_gemm.hip: {n} hand-waited fragment reads followed through the listing, none touched early", flush=True)
     os.replace(tmp, OUT)
+    os.replace(native_tmp, NATIVE_OUT)
     return OUT
 
 

@@ -572,16 +572,19 @@ class AdamWGroupEngine:
         self._hyper = None
         self._grad_scale = None
 
-    def prepare(self, pointers, *, lr, weight_decay, betas, eps, step, grad_scale=None):
-        """pointers: for each name of POINTERS the tensors' addresses (the last two only with 8 bits).
-        grad_scale: a one-element fp32 tensor on the device, or None."""
-        if pointers != self.key:
-            for name, column in zip(self.POINTERS, pointers):
+    def bind(self, key, columns):
+        """Rewrites the table if `key`, which stands for the addresses, is another than at the last call.  columns(): for
+        each name of POINTERS the tensors' addresses (the last two only with 8 bits)."""
+        if key != self.key:
+            for name, column in zip(self.POINTERS, columns()):
                 self.descs[name] = column
             _lib.check(_lib.load().muon_amd_validate_adamw(_lib.host_ptr(self.descs), len(self.descs), _lib.host_ptr(self.prefix),
                                                            self.state_bits), "validate_adamw")
             self.staging.upload(self.descs, self.desc_dev)
-            self.key = pointers
+            self.key = key
+
+    def prepare(self, *, lr, weight_decay, betas, eps, step, grad_scale=None):
+        """grad_scale: a one-element fp32 tensor on the device, or None."""
         # python doubles, rounded to float by the call
         self._hyper = [lr, 1 - lr * weight_decay, 1 - betas[0], 1 - betas[1], eps,
                        1 - betas[0] ** step, 1 - betas[1] ** step, step % self.STEP_MODULUS]

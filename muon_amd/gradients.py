@@ -31,7 +31,7 @@ class _GradList:
         self.descs["numel"], self.descs["dtype"] = numels, dtypes
         self.prefix = _plan.adam_block_prefix(numels)
         self.nblocks = int(self.prefix[-1])
-        self.nbytes = sum(n * (2 if t == _lib.SRC_BF16 else 4) for n, t in zip(numels, dtypes))
+        self.nbytes = int(sum(n * (2 if t == _lib.SRC_BF16 else 4) for n, t in zip(numels, dtypes)))
         self.prefix_dev = _upload(self.prefix, device)
         self.desc_dev = torch.empty(self.descs.nbytes, dtype=torch.uint8, device=device)
         self.partials = torch.empty(_lib.load().muon_amd_grad_norm_partials(), dtype=torch.float64, device=device)
@@ -39,9 +39,10 @@ class _GradList:
         self.key = None
 
     def run(self, pointers, max_norm, in_place):
+        """pointers: the gradients' addresses as the bytes of 64-bit numbers."""
         lib = _lib.load()
         if pointers != self.key:
-            self.descs["grad"] = pointers
+            self.descs["grad"] = np.frombuffer(pointers, dtype=np.uint64)
             _lib.check(lib.muon_amd_validate_grads(_lib.host_ptr(self.descs), len(self.descs), _lib.host_ptr(self.prefix)), "validate_grads")
             self.staging.upload(self.descs, self.desc_dev)
             self.key = pointers
@@ -53,12 +54,10 @@ class _GradList:
         return out[0], out[1]
 
 
-def _clip(parameters, max_norm, in_place):
-    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    max_norm = float(max_norm)
-    if not max_norm >= 0.0:
-        raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    grads, writebacks, seen = [], [], set()
+def _general_rows(parameters, writebacks):
+    """What _native.gradient_rows gives for plain gradients: (device index, sizes and types, addresses, the tensors behind
+    them); other strides go through contiguous copies."""
+    grads, seen = [], set()
     for p in parameters:
         g = p.grad
         if g is None:
@@ -66,26 +65,44 @@ def _clip(parameters, max_norm, in_place):
         require_gpu_tensor(g, "gradient")
         if g.is_sparse or g.dtype not in (torch.float32, torch.bfloat16):
             raise NotImplementedError(f"muon_amd clips dense fp32 and bf16 gradients; got {g.dtype}{' (sparse)' if g.is_sparse else ''}")
+        if id(p) in seen:
+            raise ValueError("the same parameter is in the list twice")
+        seen.add(id(p))
         if not g.is_contiguous():                 # the kernels address row-major memory
             c = g.contiguous()
             writebacks.append((g, c))
             g = c
         if g.numel():
-            if id(p) in seen:
-                raise ValueError("the same parameter is in the list twice")
-            seen.add(id(p))
             grads.append(g)
     if not grads:
+        return None
+    if any(g.device != grads[0].device for g in grads):
+        raise _lib.MuonAmdError("the gradients must be on one device")
+    kinds = np.array([(g.numel(), _src_dtype(g)) for g in grads], dtype=np.int64)
+    return grads[0].device.index, kinds.tobytes(), np.array([g.data_ptr() for g in grads], dtype=np.uint64).tobytes(), grads
+
+
+def _clip(parameters, max_norm, in_place):
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    writebacks = []
+    rows = _lib.native().gradient_rows(parameters) or _general_rows(parameters, writebacks)
+    if rows is None:
         device = parameters[0].device if parameters else "cpu"
         return torch.zeros((), device=device), torch.ones((), device=device)
-    device = grads[0].device
-    if any(g.device != device for g in grads):
-        raise _lib.MuonAmdError("the gradients must be on one device")
-    numels, dtypes = tuple(g.numel() for g in grads), tuple(_src_dtype(g) for g in grads)
+    index, kinds, pointers = rows[:3]
+    device = torch.device("cuda", index)
+
+    def make():
+        sizes = np.frombuffer(kinds, dtype=np.int64).reshape(-1, 2)
+        return _GradList(sizes[:, 0], sizes[:, 1], device)
+
     with torch.cuda.device(device):
-        table = _cached(("grads", device, numels, dtypes), lambda: _GradList(numels, dtypes, device), _GRAD_CACHE, _GRAD_CACHE_MAX)
+        table = _cached(("grads", index, kinds), make, _GRAD_CACHE, _GRAD_CACHE_MAX)
         with _exclusive(table, device):
-            result = table.run([g.data_ptr() for g in grads], max_norm, in_place)
+            result = table.run(pointers, max_norm, in_place)
     if in_place:
         for dst, src in writebacks:
             dst.copy_(src)

@@ -50,6 +50,8 @@ class _MuonBase(torch.optim.Optimizer):
         self._writebacks = []         # (destination, contiguous copy) pairs to copy back after the launches
         self._keepalive = []          # temporaries whose addresses the pending launches use
         self._step_bumps = []         # (Adam state, new step count) written when the launches go out
+        self._adamw_tables = {}       # group index -> (_native.AdamWTable, engine, device): the addresses of a plain group
+        self._table_bumps = []        # (table, new step count), likewise
 
     _RUNTIME_OPTIONS = ("_ns_rounding", "_mutate_grad", "_workspace_bytes", "_ns_variant", "_use_graph",
                         "_overlap_backward")
@@ -339,6 +341,19 @@ class _MuonBase(torch.optim.Optimizer):
         return tensors
 
     def _adamw_group_step(self, gi, group, bits, grad_scale=None, missing_grad_is_zero=True):
+        hyper = dict(lr=float(group["lr"]), weight_decay=float(group["weight_decay"]),
+                     betas=(float(group["betas"][0]), float(group["betas"][1])), eps=float(group["eps"]), grad_scale=grad_scale)
+        # a group whose tensors were all plain at the last step: their addresses, read again, are all there is to do
+        table, eng, device = self._adamw_tables.get(gi, (None, None, None))
+        if table is not None and (grad_scale is None or grad_scale.device == device):
+            step = table.collect(group["params"], self.state)
+            if step > 0:
+                eng.bind((id(table), table.version), table.columns)
+                eng.prepare(step=step, **hyper)
+                self._pending.append(eng)
+                self._table_bumps.append((table, step))
+                self._keepalive.append(grad_scale)
+                return
         by_step, writebacks = {}, []
         for p in group["params"]:
             if p.grad is None and not missing_grad_is_zero:
@@ -352,21 +367,24 @@ class _MuonBase(torch.optim.Optimizer):
             if p.numel() > 0:
                 by_step.setdefault((step_now, p.device), []).append(
                     (p, (self._dense(p, writebacks), self._dense(g, writebacks, written=False), *tensors)))
+        self._adamw_tables.pop(gi, None)
         for (step, device), items in by_step.items():
             if grad_scale is not None and grad_scale.device != device:
                 raise _lib.MuonAmdError(f"grad_scale is on {grad_scale.device}, parameters are on {device}")
             key = (gi, device, tuple(id(p) for p, _ in items))
+            numels, dtypes = [p.numel() for p, _ in items], [_src_dtype(p) for p, _ in items]
             eng = self._adam_engines.get(key)
             if eng is None:
                 with torch.cuda.device(device):
-                    eng = AdamWGroupEngine([p.numel() for p, _ in items], [_src_dtype(p) for p, _ in items], bits, device)
+                    eng = AdamWGroupEngine(numels, dtypes, bits, device)
                 self._adam_engines[key] = eng
-            eng.prepare([[t[j].data_ptr() for _, t in items] for j in range(4 if bits == 32 else 6)],
-                        lr=float(group["lr"]), weight_decay=float(group["weight_decay"]),
-                        betas=(float(group["betas"][0]), float(group["betas"][1])), eps=float(group["eps"]), step=step,
-                        grad_scale=grad_scale)
+            columns = [[t[j].data_ptr() for _, t in items] for j in range(4 if bits == 32 else 6)]
+            eng.bind(columns, lambda: columns)
+            eng.prepare(step=step, **hyper)
             self._pending.append(eng)
             self._keepalive.append((items, grad_scale))
+            if not writebacks and len(items) == len(group["params"]):
+                self._adamw_tables[gi] = (_lib.native().AdamWTable(numels, dtypes, bits), eng, device)
         self._writebacks += writebacks
 
     def _load_adamw_state(self, state_dict, params):
@@ -387,6 +405,8 @@ class _MuonBase(torch.optim.Optimizer):
         try:
             for state, step_now in self._step_bumps:
                 state["step"] = step_now
+            for table, step_now in self._table_bumps:
+                table.bump(step_now)
             by_device = {}
             for eng in self._pending:
                 by_device.setdefault(eng.device, []).append(eng)
@@ -409,11 +429,13 @@ class _MuonBase(torch.optim.Optimizer):
             for dst, src in self._writebacks:
                 dst.copy_(src)
         finally:
-            self._pending, self._writebacks, self._keepalive, self._step_bumps = [], [], [], []
+            self._forget_pending()
+
+    def _forget_pending(self):
+        self._pending, self._writebacks, self._keepalive, self._step_bumps, self._table_bumps = [], [], [], [], []
 
     def _run_closure(self, closure):
-        # nothing left over from a step that raised
-        self._pending, self._writebacks, self._keepalive, self._step_bumps = [], [], [], []
+        self._forget_pending()        # nothing left over from a step that raised
         loss = None
         if closure is not None:
             with torch.enable_grad():

@@ -268,3 +268,12 @@ def test_refusals():
     for bad in (dict(), dict(rstd=4096), dict(rstd=4096, dy=4096, dpre_weight=4096)):
         assert lib.muon_amd_residual_norm_backward(ctypes.byref(_lib.ResidualNormArgs(**{**good, **bad})), None) == -1
     assert lib.muon_amd_residual_norm_partials(0, 8) == 0 and lib.muon_amd_residual_norm_partials(100, 8) > 0
+
+
+@gpu
+def test_no_second_derivatives():
+    t, dh, dy = make((4, 16), F32, F32, F32)
+    h, y = muon_amd.residual_norm(t["x"], t["block"], t["post_weight"], t["pre_weight"], gate=t["gate"], scale=t["scale"])
+    g, = torch.autograd.grad((h.sum() + y.sum()), t["x"], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), t["x"])

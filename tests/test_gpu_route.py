@@ -254,3 +254,11 @@ def test_refusals():
     assert lib.muon_amd_route_backward(ctypes.byref(_lib.RouteArgs(**{**good, "dlogits": None})), None) == -1
     assert lib.muon_amd_route(None, None) == -1 and lib.muon_amd_route_backward(None, None) == -1
     assert lib.muon_amd_route_partials(0, 8) == 0 and lib.muon_amd_route_partials(100, 8) > 0
+
+
+@gpu
+def test_no_second_derivatives():
+    leaf = torch.randn(4, 8, device=DEV, requires_grad=True)
+    g, = torch.autograd.grad(muon_amd.route_topk(leaf, 2).balance_loss, leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), leaf)
