@@ -482,8 +482,9 @@ int muon_amd_adam(const MuonAdamDesc* descs_dev, const int32_t* block_prefix_dev
  * scalars_dev: NULL, or {lr, wd_factor, w1, w2, eps, bias1, bias2, step} as floats in device memory.  */
 int muon_amd_adamw_shared_elems(void);
 int muon_amd_validate_adamw(const MuonAdamWDesc* descs_host, int ntensors, const int32_t* block_prefix_host, int state_bits);
-int muon_amd_adamw(const MuonAdamWDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks, int state_bits,
-                   float lr, float wd_factor, float w1, float w2, float eps, float bias1, float bias2, uint32_t step,
+int muon_amd_adamw(const MuonAdamWDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks,
+                   int dtype /* MUON_AMD_SRC_* of all tensors, or -1: not all of one */, int state_bits, float lr,
+                   float wd_factor, float w1, float w2, float eps, float bias1, float bias2, uint32_t step,
                    const float* grad_scale_dev, const float* scalars_dev, void* stream);
 /* The values that 8-bit states stand for. */
 int muon_amd_validate_adamw_values(const MuonAdamWValuesDesc* descs_host, int ntensors, const int32_t* block_prefix_host);

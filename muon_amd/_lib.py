@@ -134,7 +134,7 @@ SIGNATURES = {
     "muon_amd_sizeof_grad_desc": (ctypes.c_size_t, []),
     "muon_amd_adamw_shared_elems": (_c_int, []),
     "muon_amd_validate_adamw": (_c_int, [_vp, _c_int, _vp, _c_int]),
-    "muon_amd_adamw": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_float, _c_float, _c_float, _c_float, _c_float, _c_float,
+    "muon_amd_adamw": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_float, _c_float, _c_float, _c_float, _c_float, _c_float,
                                 _c_float, ctypes.c_uint32, _vp, _vp, _vp]),
     "muon_amd_validate_adamw_values": (_c_int, [_vp, _c_int, _vp]),
     "muon_amd_adamw_values": (_c_int, [_vp, _vp, _c_int, _c_int, _vp]),

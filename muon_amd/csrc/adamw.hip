@@ -26,9 +26,9 @@
 namespace muon_amd {
 
 constexpr int AW_THREADS = 256;
-constexpr int AW_GROUPS = 4;                                    // groups of eight per thread: all their loads go out first
-constexpr int AW_BLOCK_ELEMS = AW_THREADS * 8 * AW_GROUPS;      // elements per workgroup
-constexpr int AW_SHARED = 128;                                  // elements that share an exponent: 16 lanes of a wave
+constexpr int AW_EACH = 32;                                     // elements per thread: all their loads go out first
+constexpr int AW_BLOCK_ELEMS = AW_THREADS * AW_EACH;            // elements per workgroup
+constexpr int AW_SHARED = 128;                                  // elements that share an exponent
 
 struct AdamWArgs {
     float neg_lr;        // -lr / bias1
@@ -47,9 +47,6 @@ __host__ __device__ __forceinline__ uint32_t mix_step(uint32_t t) {
     return x ^ (x >> 16);
 }
 
-typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x2v_byte __attribute__((ext_vector_type(2), aligned(1)));
-
 __device__ __forceinline__ AdamWArgs read_args(AdamWArgs a, const float* sc) {
     if (sc) {   // {lr, wd_factor, w1, w2, eps, bias1, bias2, step} read at run time instead of the arguments
         a.neg_lr = -sc[0] / sc[5];
@@ -63,129 +60,174 @@ __device__ __forceinline__ AdamWArgs read_args(AdamWArgs a, const float* sc) {
     return a;
 }
 
-// The two moments; the square is rounded before it is subtracted from, as for tensors of fp32.
+// The two moments; the square is rounded before it is subtracted from, as for tensors of fp32.  A weight of a half and
+// more is taken from the other end, new + (w - 1)(new - old), which is `new` itself for w = 1; which end is the same for
+// the whole launch.
+__device__ __forceinline__ float lerp_from(float old, float now, float w) {
+    const bool far = fabsf(w) >= 0.5f;
+    return fmaf(far ? w - 1.f : w, now - old, far ? now : old);
+}
 __device__ __forceinline__ void moments(float& m, float& v, float g, const AdamWArgs& a) {
 #pragma clang fp contract(off)
     const float gg = g * g;
-    m = lerp_torch(m, g, a.w1);
-    v = lerp_torch(v, gg, a.w2);
+    m = lerp_from(m, g, a.w1);
+    v = lerp_from(v, gg, a.w2);
 }
 
 // ---- states in 32 bits -------------------------------------------------------------------------------------
 template <typename T>
-__device__ __forceinline__ void adamw32_group(Group8<T>& p, const Group8<T>& g, Group8<float>& m, Group8<float>& v,
-                                              float c, const AdamWArgs& a) {
-    float pn[8];
+__device__ __forceinline__ void adamw32_pack(Pack<T, 4>& p, const Pack<T, 4>& g, Pack<float, 4>& m, Pack<float, 4>& v, float c,
+                                             const AdamWArgs& a) {
+    float pn[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float gk = g[k] * c;
+    for (int k = 0; k < 4; ++k) {
         float mk = m[k], vk = v[k];
-        moments(mk, vk, gk, a);
-        m.set(k, mk);
-        v.set(k, vk);
+        moments(mk, vk, g[k] * c, a);
+        m.v[k] = mk;
+        v.v[k] = vk;
         pn[k] = fmaf(a.neg_lr, mk / fmaf(sqrtf(vk), a.rsqrt_bias2, a.eps), p[k] * a.wd_factor);
     }
-    p = Group8<T>::of(pn);
+    p = Pack<T, 4>::of(pn);
 }
 
 template <typename T>
 __device__ __forceinline__ void adamw32_block(const MuonAdamWDesc& d, int64_t base, float c, const AdamWArgs& a) {
+    constexpr int PACKS = AW_EACH / 4;
     const int64_t numel = d.numel;
     T* __restrict__ const p = static_cast<T*>(d.param);
     const T* __restrict__ const g = static_cast<const T*>(d.grad);
     float* __restrict__ const m = static_cast<float*>(d.exp_avg);
     float* __restrict__ const v = static_cast<float*>(d.exp_avg_sq);
     if (base + AW_BLOCK_ELEMS <= numel) {
-        Group8<T> pv[AW_GROUPS], gv[AW_GROUPS];
-        Group8<float> mv[AW_GROUPS], vv[AW_GROUPS];
+        Pack<T, 4> pv[PACKS], gv[PACKS];
+        Pack<float, 4> mv[PACKS], vv[PACKS];
 #pragma unroll
-        for (int i = 0; i < AW_GROUPS; ++i) {
-            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
-            gv[i] = Group8<T>::template load<true>(g + e);
-            mv[i] = Group8<float>::load<true>(m + e);
-            vv[i] = Group8<float>::load<true>(v + e);
-            pv[i] = Group8<T>::template load<true>(p + e);
+        for (int i = 0; i < PACKS; ++i) {
+            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 4;
+            gv[i] = Pack<T, 4>::template load<true>(g + e);
+            mv[i] = Pack<float, 4>::load<true>(m + e);
+            vv[i] = Pack<float, 4>::load<true>(v + e);
+            pv[i] = Pack<T, 4>::template load<true>(p + e);
         }
 #pragma unroll
-        for (int i = 0; i < AW_GROUPS; ++i) {
-            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
-            adamw32_group<T>(pv[i], gv[i], mv[i], vv[i], c, a);
-            mv[i].template store<true>(m + e);
-            vv[i].template store<true>(v + e);
+        for (int i = 0; i < PACKS; ++i) {
+            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 4;
+            adamw32_pack<T>(pv[i], gv[i], mv[i], vv[i], c, a);
+            mv[i].store<true>(m + e);
+            vv[i].store<true>(v + e);
             pv[i].template store<true>(p + e);
         }
         return;
     }
 #pragma unroll 1
-    for (int64_t e = base + threadIdx.x * 8; e < numel; e += AW_THREADS * 8) {
-        Group8<T> pv = load_group<T, true>(p, e, numel);
-        const Group8<T> gv = load_group<T, true>(g, e, numel);
-        Group8<float> mv = load_group<float, true>(m, e, numel), vv = load_group<float, true>(v, e, numel);
-        adamw32_group<T>(pv, gv, mv, vv, c, a);
-        store_group<float, true>(m, e, numel, mv);
-        store_group<float, true>(v, e, numel, vv);
-        store_group<T, true>(p, e, numel, pv);
+    for (int64_t e = base + threadIdx.x * 4; e < numel; e += AW_THREADS * 4) {
+        Pack<T, 4> pv = load_pack<T, 4, true>(p, e, numel);
+        const Pack<T, 4> gv = load_pack<T, 4, true>(g, e, numel);
+        Pack<float, 4> mv = load_pack<float, 4, true>(m, e, numel), vv = load_pack<float, 4, true>(v, e, numel);
+        adamw32_pack<T>(pv, gv, mv, vv, c, a);
+        store_pack<float, 4, true>(m, e, numel, mv);
+        store_pack<float, 4, true>(v, e, numel, vv);
+        store_pack<T, 4, true>(p, e, numel, pv);
     }
 }
 
+// DTYPE: the type of every parameter of the launch, or AW_MIXED.  A kernel for both types takes the registers of the
+// larger half (fp32 in packs of four: 187 instead of 153 with 8-bit states, and 80 instead of 69 us over 50257 x 768 bf16).
+constexpr int AW_MIXED = -1;
+template <int DTYPE, typename F>
+__device__ __forceinline__ void with_type(const MuonAdamWDesc& d, F&& f) {
+    if (DTYPE == MUON_AMD_SRC_BF16 || (DTYPE == AW_MIXED && d.dtype == MUON_AMD_SRC_BF16)) f(uint16_t{});
+    else f(float{});
+}
+
+template <int DTYPE>
 __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(const MuonAdamWDesc* __restrict__ descs,
                                                             const int32_t* __restrict__ prefix, int ntensors, AdamWArgs args,
                                                             const float* __restrict__ grad_scale, const float* __restrict__ sc) {
     const AdamWArgs a = read_args(args, sc);
     const float c = grad_scale ? *grad_scale : 1.f;
-    const int b = blockIdx.x, ti = find_segment(prefix, ntensors, b);
+    const int b = blockIdx.x, ti = find_segment_wave(prefix, ntensors, b);
     const MuonAdamWDesc d = descs[ti];
     const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS;
-    if (d.dtype == MUON_AMD_SRC_BF16) adamw32_block<uint16_t>(d, base, c, a);
-    else adamw32_block<float>(d, base, c, a);
+    with_type<DTYPE>(d, [&](auto t) { adamw32_block<decltype(t)>(d, base, c, a); });
 }
 
 // ---- states in 8 bits --------------------------------------------------------------------------------------
-// The larger of two pairs of 16-bit numbers over the 16 lanes of a row, in every lane.
-__device__ __forceinline__ uint32_t row_max2(uint32_t x) {
-    const auto step = [&](uint32_t other) {
-        x = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, x), __builtin_bit_cast(u16x2_t, other)));
+// The larger of two pairs of 16-bit numbers over LANES (16 or 32) lanes next to each other, in every lane.
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_max2(uint32_t x) {
+    const auto larger = [](uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
     };
-    step(__builtin_amdgcn_mov_dpp(x, 0xB1, 0xf, 0xf, true));       // quad_perm 1,0,3,2
-    step(__builtin_amdgcn_mov_dpp(x, 0x4E, 0xf, 0xf, true));       // quad_perm 2,3,0,1
-    step(__builtin_amdgcn_mov_dpp(x, 0x141, 0xf, 0xf, true));      // row_half_mirror
-    step(__builtin_amdgcn_mov_dpp(x, 0x140, 0xf, 0xf, true));      // row_mirror
+    x = larger(x, __builtin_amdgcn_mov_dpp(x, 0xB1, 0xf, 0xf, true));       // quad_perm 1,0,3,2
+    x = larger(x, __builtin_amdgcn_mov_dpp(x, 0x4E, 0xf, 0xf, true));       // quad_perm 2,3,0,1
+    x = larger(x, __builtin_amdgcn_mov_dpp(x, 0x141, 0xf, 0xf, true));      // row_half_mirror
+    x = larger(x, __builtin_amdgcn_mov_dpp(x, 0x140, 0xf, 0xf, true));      // row_mirror
+    if constexpr (LANES == 32) {
+        const auto rows = __builtin_amdgcn_permlane16_swap(x, x, false, false);       // even rows twice, odd rows twice
+        x = larger(rows[0], rows[1]);
+    }
     return x;
 }
 
-__device__ __forceinline__ uint32_t max3u(uint32_t a, uint32_t b, uint32_t c) { return max(max(a, b), c); }
-
-// The values of eight codes, as they are held (m) or (v), whose block has the shared exponent E.
-__device__ __forceinline__ void decode_m(u32x2v code, int E, float (&m)[8]) {
+// G codes of one byte each, as words.
+template <int G>
+struct Codes {
+    typedef uint32_t words __attribute__((ext_vector_type(G / 4)));
+    typedef uint32_t words_any __attribute__((ext_vector_type(G / 4), aligned(1)));
+    words w;
+    static __device__ __forceinline__ Codes load(const uint8_t* p) { return {load_as<true, words_any>(p)}; }
+    __device__ __forceinline__ void store(uint8_t* p) const { store_as<true, words_any>(p, w); }
+    static __device__ __forceinline__ Codes load(const uint8_t* p, int64_t e, int64_t n) {
+        if (e + G <= n) return load(p + e);
+        Codes c{words(0u)};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(code[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(code[h], true);
+        for (int k = 0; k < G - 1; ++k)
+            if (e + k < n) c.w[k >> 2] |= static_cast<uint32_t>(p[e + k]) << (8 * (k & 3));
+        return c;
+    }
+    __device__ __forceinline__ void store(uint8_t* p, int64_t e, int64_t n) const {
+        if (e + G <= n) {
+            store(p + e);
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < G - 1; ++k)
+            if (e + k < n) p[e + k] = static_cast<uint8_t>(w[k >> 2] >> (8 * (k & 3)));
+    }
+};
+
+// The values of codes, as they are held (m) or (v), whose block has the shared exponent E.
+template <int G>
+__device__ __forceinline__ void decode_m(const Codes<G>& c, int E, float (&m)[G]) {
+#pragma unroll
+    for (int h = 0; h < G / 4; ++h) {
+        const uint32_t w = c.w[h];
+        const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
         m[4 * h] = ldexpf(lo[0], E - 135);            // (e4m3 itself: 2^(e - 7))
         m[4 * h + 1] = ldexpf(lo[1], E - 135);
         m[4 * h + 2] = ldexpf(hi[0], E - 135);
         m[4 * h + 3] = ldexpf(hi[1], E - 135);
     }
 }
-__device__ __forceinline__ void decode_v(u32x2v code, int E, float (&v)[8]) {
+template <int G>
+__device__ __forceinline__ void decode_v(const Codes<G>& c, int E, float (&v)[G]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const uint32_t c = (code[k >> 2] >> (8 * (k & 3))) & 0xffu;
-        v[k] = ldexpf(__uint_as_float(c << 20), E - 31);
-    }
+    for (int k = 0; k < G; ++k) v[k] = ldexpf(__uint_as_float(((c.w[k >> 2] >> (8 * (k & 3))) & 0xffu) << 20), E - 31);
 }
 
-// One group: parameters and moments after the step, the new codes, and the new shared exponents of the block (whose 16
-// groups are those of a row of lanes: every lane of the wave calls this; what is beyond the tensor is zero).
-template <typename T>
-__device__ __forceinline__ void adamw8_group(Group8<T>& p, const Group8<T>& g, u32x2v& mc, u32x2v& vc, int& Em, int& Ev,
-                                             uint32_t i0, float c, const AdamWArgs& a) {
-    float m[8], v[8], pn[8];
-    decode_m(mc, Em, m);
-    decode_v(vc, Ev, v);
+// One pack: parameters and moments after the step, the new codes, and the new shared exponents of its block, which is
+// that of 128 / G lanes (every lane of the wave calls this; what is beyond the tensor is zero).
+template <typename T, int G>
+__device__ __forceinline__ void adamw8_pack(Pack<T, G>& p, const Pack<T, G>& g, Codes<G>& mc, Codes<G>& vc, int& Em, int& Ev,
+                                            uint32_t i0, float c, const AdamWArgs& a) {
+    float m[G], v[G], pn[G];
+    decode_m<G>(mc, Em, m);
+    decode_v<G>(vc, Ev, v);
     const float poison = max(Em, Ev) == 255 ? __builtin_nanf("") : 0.f;
     uint32_t most_m = 0, most_v = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < G; ++k) {
         const float gk = fmaf(g[k], c, poison);
         moments(m[k], v[k], gk, a);
         most_m = max(most_m, __float_as_uint(m[k]) & 0x7fffffffu);
@@ -193,15 +235,15 @@ __device__ __forceinline__ void adamw8_group(Group8<T>& p, const Group8<T>& g, u
         const float denominator = fmaf(__builtin_amdgcn_sqrtf(v[k]), a.rsqrt_bias2, a.eps);
         pn[k] = fmaf(a.neg_lr, m[k] * __builtin_amdgcn_rcpf(denominator), p[k] * a.wd_factor);
     }
-    p = Group8<T>::of(pn);
+    p = Pack<T, G>::of(pn);
     // exponent fields, one more where three bits of mantissa are not enough below the next power (m: 1.75 is the last)
-    const uint32_t both = row_max2(((most_m + 0x1fffffu) >> 23) | ((most_v + 0xfffffu) >> 23 << 16));
+    const uint32_t both = lanes_max2<AW_SHARED / G>(((most_m + 0x1fffffu) >> 23) | ((most_v + 0xfffffu) >> 23 << 16));
     Em = static_cast<int>(both & 0xffffu);
     Ev = static_cast<int>(both >> 16);
     if (max(Em, Ev) >= 255) Em = Ev = 255;
     uint32_t h32 = i0 * DITHER_I + a.dither;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < G / 4; ++h) {
         uint32_t cm = 0, cv = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -215,31 +257,14 @@ __device__ __forceinline__ void adamw8_group(Group8<T>& p, const Group8<T>& g, u
             cv |= qv << (8 * k);
             h32 += DITHER_I;
         }
-        mc[h] = cm;
-        vc[h] = cv;
+        mc.w[h] = cm;
+        vc.w[h] = cv;
     }
-}
-
-__device__ __forceinline__ u32x2v load_codes(const uint8_t* p, int64_t e, int64_t n) {
-    if (e + 8 <= n) return load_as<true, u32x2v_byte>(p + e);
-    u32x2v c = {0u, 0u};
-#pragma unroll
-    for (int k = 0; k < 7; ++k)
-        if (e + k < n) c[k >> 2] |= static_cast<uint32_t>(p[e + k]) << (8 * (k & 3));
-    return c;
-}
-__device__ __forceinline__ void store_codes(uint8_t* p, int64_t e, int64_t n, u32x2v c) {
-    if (e + 8 <= n) {
-        store_as<true, u32x2v_byte>(p + e, c);
-        return;
-    }
-#pragma unroll
-    for (int k = 0; k < 7; ++k)
-        if (e + k < n) p[e + k] = static_cast<uint8_t>(c[k >> 2] >> (8 * (k & 3)));
 }
 
 template <typename T>
 __device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t base, float c, const AdamWArgs& a) {
+    constexpr int G = pack_of<T>, PACKS = AW_EACH / G, LANES = AW_SHARED / G;
     const int64_t numel = d.numel;
     T* __restrict__ const p = static_cast<T*>(d.param);
     const T* __restrict__ const g = static_cast<const T*>(d.grad);
@@ -248,85 +273,85 @@ __device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t bas
     uint8_t* __restrict__ const me = d.exp_avg_exponent;
     uint8_t* __restrict__ const ve = d.exp_avg_sq_exponent;
     if (base + AW_BLOCK_ELEMS <= numel) {
-        Group8<T> pv[AW_GROUPS], gv[AW_GROUPS];
-        u32x2v mv[AW_GROUPS], vv[AW_GROUPS];
-        int Em[AW_GROUPS], Ev[AW_GROUPS];
+        Pack<T, G> pv[PACKS], gv[PACKS];
+        Codes<G> mv[PACKS], vv[PACKS];
+        int Em[PACKS], Ev[PACKS];
 #pragma unroll
-        for (int i = 0; i < AW_GROUPS; ++i) {
-            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
-            Em[i] = me[e / AW_SHARED];
-            Ev[i] = ve[e / AW_SHARED];
-            mv[i] = load_as<true, u32x2v_byte>(m + e);
-            vv[i] = load_as<true, u32x2v_byte>(v + e);
-            gv[i] = Group8<T>::template load<true>(g + e);
-            pv[i] = Group8<T>::template load<true>(p + e);
+        for (int i = 0; i < PACKS; ++i) {
+            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * G;
+            Em[i] = load_as<false, uint8_t>(me + e / AW_SHARED);
+            Ev[i] = load_as<false, uint8_t>(ve + e / AW_SHARED);
+            mv[i] = Codes<G>::load(m + e);
+            vv[i] = Codes<G>::load(v + e);
+            gv[i] = Pack<T, G>::template load<true>(g + e);
+            pv[i] = Pack<T, G>::template load<true>(p + e);
         }
 #pragma unroll
-        for (int i = 0; i < AW_GROUPS; ++i) {
-            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
-            adamw8_group<T>(pv[i], gv[i], mv[i], vv[i], Em[i], Ev[i], static_cast<uint32_t>(e), c, a);
-            store_as<true, u32x2v_byte>(m + e, mv[i]);
-            store_as<true, u32x2v_byte>(v + e, vv[i]);
+        for (int i = 0; i < PACKS; ++i) {
+            const int64_t e = base + (i * AW_THREADS + threadIdx.x) * G;
+            adamw8_pack<T, G>(pv[i], gv[i], mv[i], vv[i], Em[i], Ev[i], static_cast<uint32_t>(e), c, a);
+            mv[i].store(m + e);
+            vv[i].store(v + e);
             pv[i].template store<true>(p + e);
-            if ((threadIdx.x & 15) == 0) {
-                me[e / AW_SHARED] = static_cast<uint8_t>(Em[i]);
-                ve[e / AW_SHARED] = static_cast<uint8_t>(Ev[i]);
+            if ((threadIdx.x & (LANES - 1)) == 0) {
+                store_as<false, uint8_t>(me + e / AW_SHARED, static_cast<uint8_t>(Em[i]));
+                store_as<false, uint8_t>(ve + e / AW_SHARED, static_cast<uint8_t>(Ev[i]));
             }
         }
         return;
     }
 #pragma unroll 1
-    for (int64_t at = base; at < numel; at += AW_THREADS * 8) {      // (the wave stays whole: its lanes exchange maxima)
-        const int64_t e = at + threadIdx.x * 8;
+    for (int64_t at = base; at < numel; at += AW_THREADS * G) {      // (the wave stays whole: its lanes exchange maxima)
+        const int64_t e = at + threadIdx.x * G;
         const bool any = e < numel;
         int Em = any ? me[e / AW_SHARED] : 0, Ev = any ? ve[e / AW_SHARED] : 0;
-        u32x2v mv = load_codes(m, e, numel), vv = load_codes(v, e, numel);
-        Group8<T> pv = load_group<T, true>(p, e, numel);
-        const Group8<T> gv = load_group<T, true>(g, e, numel);
-        adamw8_group<T>(pv, gv, mv, vv, Em, Ev, static_cast<uint32_t>(e), c, a);
-        store_codes(m, e, numel, mv);
-        store_codes(v, e, numel, vv);
-        store_group<T, true>(p, e, numel, pv);
-        if (any && (threadIdx.x & 15) == 0) {
+        Codes<G> mv = Codes<G>::load(m, e, numel), vv = Codes<G>::load(v, e, numel);
+        Pack<T, G> pv = load_pack<T, G, true>(p, e, numel);
+        const Pack<T, G> gv = load_pack<T, G, true>(g, e, numel);
+        adamw8_pack<T, G>(pv, gv, mv, vv, Em, Ev, static_cast<uint32_t>(e), c, a);
+        mv.store(m, e, numel);
+        vv.store(v, e, numel);
+        store_pack<T, G, true>(p, e, numel, pv);
+        if (any && (threadIdx.x & (LANES - 1)) == 0) {
             me[e / AW_SHARED] = static_cast<uint8_t>(Em);
             ve[e / AW_SHARED] = static_cast<uint8_t>(Ev);
         }
     }
 }
 
+template <int DTYPE>
 __global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(const MuonAdamWDesc* __restrict__ descs,
                                                            const int32_t* __restrict__ prefix, int ntensors, AdamWArgs args,
                                                            const float* __restrict__ grad_scale, const float* __restrict__ sc) {
     const AdamWArgs a = read_args(args, sc);
     const float c = grad_scale ? *grad_scale : 1.f;
-    const int b = blockIdx.x, ti = find_segment(prefix, ntensors, b);
+    const int b = blockIdx.x, ti = find_segment_wave(prefix, ntensors, b);
     const MuonAdamWDesc d = descs[ti];
     const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS;
-    if (d.dtype == MUON_AMD_SRC_BF16) adamw8_block<uint16_t>(d, base, c, a);
-    else adamw8_block<float>(d, base, c, a);
+    with_type<DTYPE>(d, [&](auto t) { adamw8_block<decltype(t)>(d, base, c, a); });
 }
 
 // The values of 8-bit states in bf16, which holds each of them exactly down to the least one that it has (three bits of
 // mantissa; only blocks below 2^-100 reach bf16's own subnormal numbers).
 __global__ __launch_bounds__(AW_THREADS) void adamw_values_kernel(const MuonAdamWValuesDesc* __restrict__ descs,
                                                                  const int32_t* __restrict__ prefix, int ntensors) {
-    const int b = blockIdx.x, ti = find_segment(prefix, ntensors, b);
+    const int b = blockIdx.x, ti = find_segment_wave(prefix, ntensors, b);
     const MuonAdamWValuesDesc d = descs[ti];
     const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS, numel = d.numel;
 #pragma unroll
-    for (int i = 0; i < AW_GROUPS; ++i) {
+    for (int i = 0; i < AW_EACH / 8; ++i) {
         const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
         if (e >= numel) return;
-        const int Em = d.exp_avg_exponent[e / AW_SHARED], Ev = d.exp_avg_sq_exponent[e / AW_SHARED];
+        const int Em = load_as<false, uint8_t>(d.exp_avg_exponent + e / AW_SHARED), Ev = load_as<false, uint8_t>(d.exp_avg_sq_exponent + e / AW_SHARED);
         float m[8], v[8];
-        decode_m(load_codes(d.exp_avg, e, numel), Em, m);
-        decode_v(load_codes(d.exp_avg_sq, e, numel), Ev, v);
+        decode_m<8>(Codes<8>::load(d.exp_avg, e, numel), Em, m);
+        decode_v<8>(Codes<8>::load(d.exp_avg_sq, e, numel), Ev, v);
         if (Em == 255)
             for (float& x : m) x = __builtin_nanf("");
         if (Ev == 255)
             for (float& x : v) x = __builtin_nanf("");
-        store_group<uint16_t, true>(d.exp_avg_out, e, numel, Group8<uint16_t>::of(m));
-        store_group<uint16_t, true>(d.exp_avg_sq_out, e, numel, Group8<uint16_t>::of(v));
+        store_pack<uint16_t, 8, false>(d.exp_avg_out, e, numel, Pack<uint16_t, 8>::of(m));
+        store_pack<uint16_t, 8, false>(d.exp_avg_sq_out, e, numel, Pack<uint16_t, 8>::of(v));
     }
 }
 
@@ -385,15 +410,19 @@ int muon_amd_validate_adamw_values(const MuonAdamWValuesDesc* descs, int ntensor
     return MUON_AMD_OK;
 }
 
-int muon_amd_adamw(const MuonAdamWDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks, int state_bits,
+int muon_amd_adamw(const MuonAdamWDesc* descs_dev, const int32_t* block_prefix_dev, int ntensors, int nblocks, int dtype, int state_bits,
                    float lr, float wd_factor, float w1, float w2, float eps, float bias1, float bias2, uint32_t step,
                    const float* grad_scale_dev, const float* scalars_dev, void* stream) {
     MUON_REQUIRE(descs_dev && block_prefix_dev, "adamw: null table");
     MUON_REQUIRE(ntensors > 0 && nblocks > 0, "adamw: ntensors=%d nblocks=%d", ntensors, nblocks);
     MUON_REQUIRE(state_bits == 8 || state_bits == 32, "adamw: state_bits=%d", state_bits);
+    MUON_REQUIRE(dtype == MUON_AMD_SRC_F32 || dtype == MUON_AMD_SRC_BF16 || dtype == AW_MIXED, "adamw: dtype=%d", dtype);
     MUON_REQUIRE(scalars_dev || (bias1 != 0.f && bias2 > 0.f), "adamw: zero bias correction");
     const AdamWArgs a{-lr / bias1, wd_factor, w1, w2, eps, 1.f / sqrtf(bias2), mix_step(step)};
-    const auto kernel = state_bits == 8 ? adamw8_kernel : adamw32_kernel;
+    const auto pick = [&](auto f32, auto bf16, auto mixed) { return dtype == MUON_AMD_SRC_F32 ? f32 : dtype == MUON_AMD_SRC_BF16 ? bf16 : mixed; };
+    const auto kernel = state_bits == 8
+                            ? pick(adamw8_kernel<MUON_AMD_SRC_F32>, adamw8_kernel<MUON_AMD_SRC_BF16>, adamw8_kernel<AW_MIXED>)
+                            : pick(adamw32_kernel<MUON_AMD_SRC_F32>, adamw32_kernel<MUON_AMD_SRC_BF16>, adamw32_kernel<AW_MIXED>);
     hipLaunchKernelGGL(kernel, dim3(nblocks), dim3(AW_THREADS), 0, static_cast<hipStream_t>(stream), descs_dev, block_prefix_dev,
                        ntensors, a, grad_scale_dev, scalars_dev);
     return check_launch("adamw");

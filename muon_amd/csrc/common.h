@@ -106,6 +106,20 @@ __device__ __forceinline__ int find_segment(const int32_t* __restrict__ prefix, 
     return lo;
 }
 
+// The same by a whole wave (every lane calls it, with the same arguments): 64 entries at a time instead of one after the
+// other, so a launch over up to 64 tensors waits for one load before its descriptor's.
+__device__ __forceinline__ int find_segment_wave(const int32_t* __restrict__ prefix, int n, int b) {
+    int lo = 0;
+    const int lane = static_cast<int>(threadIdx.x & 63);
+    for (int stride = n > 4096 ? 4096 : n > 64 ? 64 : 1; ; stride >>= 6) {
+        // entries lo + stride, lo + 2 stride, ..: how many are at or below b
+        const int i = lo + (lane + 1) * stride;
+        const uint64_t below = __ballot(i < n && prefix[i < n ? i : n] <= b);
+        lo += __builtin_popcountll(below) * stride;
+        if (stride == 1) return __builtin_amdgcn_readfirstlane(lo);
+    }
+}
+
 // Sum over the 64 lanes of a wavefront; every lane gets the total.
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

@@ -12,9 +12,14 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/Event.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <cstring>
+#include <list>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -36,7 +41,12 @@ struct Api {
     decltype(&muon_amd_route) route;
     decltype(&muon_amd_route_backward) route_backward;
     decltype(&muon_amd_route_partials) route_partials;
-    int max_width, max_experts, max_k, shared_elems;
+    decltype(&muon_amd_validate_grads) validate_grads;
+    decltype(&muon_amd_grad_norm) grad_norm;
+    decltype(&muon_amd_grad_clip) grad_clip;
+    decltype(&muon_amd_validate_adamw_values) validate_adamw_values;
+    decltype(&muon_amd_adamw_values) adamw_values;
+    int max_width, max_experts, max_k, shared_elems, block_elems, norm_partials;
 } api{};
 
 struct LibraryError : std::runtime_error {
@@ -50,6 +60,9 @@ void check(int rc, const char* what) {
 void* current_stream(const c10::Device& device) {
     return c10::hip::getCurrentHIPStream(device.index()).stream();
 }
+
+// The current stream as torch's device-independent interface names it.
+c10::Stream stream_of(const c10::Device& device) { return c10::impl::VirtualGuardImpl(device.type()).getStream(device); }
 
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? MUON_AMD_SRC_BF16 : MUON_AMD_SRC_F32; }
 bool taken(const Tensor& t) { return t.is_cuda() && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16); }
@@ -438,31 +451,154 @@ class AdamWTable {
     const py::str step_{"step"};
 };
 
-// The gradients of a list of parameters: {device, sizes and types as bytes, addresses as bytes}, or None: not the common
-// case (other strides, types or devices, a parameter that is in the list twice, no gradient at all).
-py::object gradient_rows(const py::list& params) {
-    std::vector<int64_t> kinds, pointers;
+// A table of descriptors and its block prefix on the device.  A table is never rewritten: other contents get memory of
+// their own, so a launch on one stream cannot see what a call on another stream uploads.
+class Table {
+   public:
+    template <typename D>
+    void upload(const std::vector<D>& descs, const c10::Device& device) {
+        std::vector<int32_t> prefix(descs.size() + 1, 0);
+        for (size_t i = 0; i < descs.size(); ++i)
+            prefix[i + 1] = prefix[i] + static_cast<int32_t>((descs[i].numel + api.block_elems - 1) / api.block_elems);
+        check(validator<D>()(descs.data(), static_cast<int>(descs.size()), prefix.data()), "validate");
+        const size_t first = descs.size() * sizeof(D), size = first + prefix.size() * sizeof(int32_t);
+        Tensor host = at::empty({static_cast<int64_t>(size)}, at::TensorOptions().dtype(at::kByte).pinned_memory(true));
+        std::memcpy(host.data_ptr(), descs.data(), first);
+        std::memcpy(static_cast<char*>(host.data_ptr()) + first, prefix.data(), prefix.size() * sizeof(int32_t));
+        memory_ = host.to(device, /*non_blocking=*/true);
+        prefix_ = first;
+        n_ = static_cast<int>(descs.size());
+        blocks_ = prefix.back();
+        uploaded_ = c10::Event(device.type());
+        uploaded_.record(stream_of(device));
+    }
+    // Before a launch on the current stream: its table is there, and stays while it runs.
+    // (What a HIP graph records cannot wait for an event from outside of it: a caller that captures has made the call before.)
+    void use(const c10::Device& device) {
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) return;
+        const c10::Stream stream = stream_of(device);
+        uploaded_.block(stream);
+        memory_.record_stream(stream);
+    }
+    template <typename D>
+    const D* descs() const { return static_cast<const D*>(memory_.data_ptr()); }
+    const int32_t* prefix() const { return reinterpret_cast<const int32_t*>(static_cast<const char*>(memory_.data_ptr()) + prefix_); }
+    int size() const { return n_; }
+    int blocks() const { return blocks_; }
+
+   private:
+    template <typename D>
+    static auto validator() {
+        if constexpr (std::is_same_v<D, MuonGradDesc>) return api.validate_grads;
+        else return api.validate_adamw_values;
+    }
+    Tensor memory_;
+    size_t prefix_ = 0;
+    int n_ = 0, blocks_ = 0;
+    c10::Event uploaded_{c10::DeviceType::CUDA};
+};
+
+struct GradTable {
+    c10::Device device;
+    std::vector<MuonGradDesc> descs;
+    Table table;
+};
+// The tables of the last gradient lists, newest first (calls hold the interpreter's lock).
+std::list<GradTable>& grad_tables() {
+    static std::list<GradTable> tables;
+    return tables;
+}
+constexpr size_t GRAD_TABLES = 16;
+
+// (norm, coefficient) of these gradients (dense fp32 or bf16 tensors of one device, row-major, not empty).
+std::tuple<Tensor, Tensor> clip_tensors(const std::vector<const Tensor*>& grads, double max_norm, bool in_place) {
+    const c10::Device device = grads[0]->device();
+    std::vector<MuonGradDesc> descs(grads.size());
+    for (size_t i = 0; i < grads.size(); ++i) descs[i] = {grads[i]->data_ptr(), grads[i]->numel(), dtype_of(*grads[i]), 0};
+    const c10::DeviceGuard guard(device);
+    auto& tables = grad_tables();
+    const auto same = [&](const GradTable& t) {
+        return t.device == device && t.descs.size() == descs.size() &&
+               std::memcmp(t.descs.data(), descs.data(), descs.size() * sizeof(MuonGradDesc)) == 0;
+    };
+    const auto found = std::find_if(tables.begin(), tables.end(), same);
+    if (found != tables.end()) {
+        tables.splice(tables.begin(), tables, found);
+    } else {
+        GradTable fresh{device, std::move(descs), {}};
+        fresh.table.upload(fresh.descs, device);
+        tables.push_front(std::move(fresh));
+        if (tables.size() > GRAD_TABLES) tables.pop_back();
+    }
+    Table& table = tables.front().table;
+    const auto options = at::TensorOptions().device(device);
+    const Tensor out = at::empty({2}, options.dtype(at::kFloat));
+    const Tensor partials = at::empty({std::min(table.blocks(), api.norm_partials)}, options.dtype(at::kDouble));
+    table.use(device);
+    check((in_place ? api.grad_clip : api.grad_norm)(table.descs<MuonGradDesc>(), table.prefix(), table.size(), table.blocks(),
+                                                     partials.data_ptr<double>(), static_cast<float>(max_norm), out.data_ptr<float>(),
+                                                     current_stream(device)),
+          in_place ? "grad_clip" : "grad_norm");
+    return {out.select(0, 0), out.select(0, 1)};
+}
+
+// The same for the gradients of a list of parameters; None: not the common case (other strides, types or devices, a
+// parameter that is in the list twice, no gradient at all).
+std::optional<std::tuple<Tensor, Tensor>> clip(const py::list& params, double max_norm, bool in_place) {
+    std::vector<const Tensor*> grads;
     std::vector<const void*> seen;
-    std::optional<c10::Device> device;
     const Py_ssize_t n = PyList_GET_SIZE(params.ptr());
     for (Py_ssize_t i = 0; i < n; ++i) {
         PyObject* const p = PyList_GET_ITEM(params.ptr(), i);
-        if (!THPVariable_Check(p)) return py::none();
+        if (!THPVariable_Check(p)) return std::nullopt;
         const Tensor& g = THPVariable_Unpack(p).grad();
         if (!g.defined()) continue;
-        if (!taken(g) || g.layout() != at::kStrided || !g.is_contiguous() || g.numel() == 0) return py::none();
-        if (!device) device = g.device();
-        if (g.device() != *device) return py::none();
-        kinds.push_back(g.numel());
-        kinds.push_back(dtype_of(g));
-        pointers.push_back(reinterpret_cast<int64_t>(g.data_ptr()));
+        if (!taken(g) || g.layout() != at::kStrided || !g.is_contiguous() || g.numel() == 0 ||
+            (!grads.empty() && g.device() != grads[0]->device()))
+            return std::nullopt;
+        grads.push_back(&g);
         seen.push_back(p);
     }
     std::sort(seen.begin(), seen.end());
-    if (pointers.empty() || std::adjacent_find(seen.begin(), seen.end()) != seen.end()) return py::none();
-    const auto bytes = [](const std::vector<int64_t>& v) { return py::bytes(reinterpret_cast<const char*>(v.data()), v.size() * sizeof(int64_t)); };
-    return py::make_tuple(static_cast<int>(device->index()), bytes(kinds), bytes(pointers));
+    if (grads.empty() || std::adjacent_find(seen.begin(), seen.end()) != seen.end()) return std::nullopt;
+    return clip_tensors(grads, max_norm, in_place);
 }
+std::tuple<Tensor, Tensor> clip_list(const std::vector<Tensor>& grads, double max_norm, bool in_place) {
+    std::vector<const Tensor*> pointers;
+    for (const Tensor& g : grads) {
+        TORCH_CHECK(taken(g) && g.is_contiguous() && g.numel() > 0 && g.device() == grads[0].device(), "not a plain gradient");
+        pointers.push_back(&g);
+    }
+    return clip_tensors(pointers, max_norm, in_place);
+}
+
+// The launch that turns 8-bit states into numbers, for tensors of one device: rows of {exp_avg, exp_avg_sq, their
+// exponents, the two bf16 tensors that take the values}, whose sizes and types the caller has checked.
+class ValueTable {
+   public:
+    void run(const std::vector<std::vector<Tensor>>& rows) {
+        std::vector<MuonAdamWValuesDesc> descs(rows.size());
+        const auto bytes = [](const Tensor& t) { return static_cast<const uint8_t*>(t.data_ptr()); };
+        for (size_t i = 0; i < rows.size(); ++i) {
+            const auto& r = rows[i];
+            descs[i] = {bytes(r[0]), bytes(r[1]), bytes(r[2]), bytes(r[3]), static_cast<uint16_t*>(r[4].data_ptr()),
+                        static_cast<uint16_t*>(r[5].data_ptr()), r[0].numel()};
+        }
+        const c10::Device device = rows[0][0].device();
+        const c10::DeviceGuard guard(device);
+        if (descs.size() != descs_.size() || std::memcmp(descs.data(), descs_.data(), descs.size() * sizeof(descs[0])) != 0) {
+            table_.upload(descs, device);
+            descs_ = std::move(descs);
+        }
+        table_.use(device);
+        check(api.adamw_values(table_.descs<MuonAdamWValuesDesc>(), table_.prefix(), table_.size(), table_.blocks(), current_stream(device)),
+              "adamw_values");
+    }
+
+   private:
+    std::vector<MuonAdamWValuesDesc> descs_;
+    Table table_;
+};
 
 void bind(const py::dict& addresses, const py::object& error) {
     const auto get = [&](auto& f, const char* name) {
@@ -475,6 +611,11 @@ void bind(const py::dict& addresses, const py::object& error) {
     get(api.route, "muon_amd_route");
     get(api.route_backward, "muon_amd_route_backward");
     get(api.route_partials, "muon_amd_route_partials");
+    get(api.validate_grads, "muon_amd_validate_grads");
+    get(api.grad_norm, "muon_amd_grad_norm");
+    get(api.grad_clip, "muon_amd_grad_clip");
+    get(api.validate_adamw_values, "muon_amd_validate_adamw_values");
+    get(api.adamw_values, "muon_amd_adamw_values");
     const auto number = [&](const char* name) {
         int (*f)(void);
         get(f, name);
@@ -484,6 +625,8 @@ void bind(const py::dict& addresses, const py::object& error) {
     api.max_experts = number("muon_amd_route_max_experts");
     api.max_k = number("muon_amd_route_max_k");
     api.shared_elems = number("muon_amd_adamw_shared_elems");
+    api.block_elems = number("muon_amd_elementwise_block_elems");
+    api.norm_partials = number("muon_amd_grad_norm_partials");
     const auto same = [&](const char* name, size_t size) {
         size_t (*f)(void);
         get(f, name);
@@ -491,6 +634,8 @@ void bind(const py::dict& addresses, const py::object& error) {
     };
     same("muon_amd_sizeof_residual_norm", sizeof(MuonResidualNorm));
     same("muon_amd_sizeof_route", sizeof(MuonRoute));
+    same("muon_amd_sizeof_grad_desc", sizeof(MuonGradDesc));
+    same("muon_amd_sizeof_adamw_values_desc", sizeof(MuonAdamWValuesDesc));
     static PyObject* raised;
     raised = error.inc_ref().ptr();
     py::register_exception_translator([](std::exception_ptr p) {
@@ -509,7 +654,10 @@ PYBIND11_MODULE(_native, m) {
     m.def("abi_version", [] { return MUON_AMD_ABI_VERSION; });
     m.def("residual_norm", &residual_norm);
     m.def("route_topk", &route_topk);
-    m.def("gradient_rows", &gradient_rows);
+    m.def("clip", &clip);
+    m.def("clip_list", &clip_list);
+    m.def("clear_tables", [] { grad_tables().clear(); });
+    py::class_<ValueTable>(m, "ValueTable").def(py::init<>()).def("run", &ValueTable::run);
     py::class_<AdamWTable>(m, "AdamWTable")
         .def(py::init<std::vector<int64_t>, std::vector<int>, int>())
         .def("collect", &AdamWTable::collect)

@@ -13,7 +13,7 @@
 // so that a row takes one reduction; the gradient of a gate for the whole row is (1 - sig) D c2.
 //
 // Memory bounds both passes.  A row stays in the registers of TPR threads (one wave up to 1024 channels forward, 512
-// backward: no barrier), 8 elements per access; a workgroup takes row after row with the weights of its channels, and
+// backward: no barrier), 16 bytes of the residual stream per access; a workgroup takes row after row with the weights of its channels, and
 // backward their sums, held in registers, and the workgroups' sums are joined in a fixed order by a second launch.
 #include <type_traits>
 
@@ -64,47 +64,56 @@ __device__ __forceinline__ void row_sums(float (&s)[N], float (*slots)[N]) {
 
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
-// Eight elements of a vector of weights in fp32 (zero beyond the row).
-__device__ __forceinline__ void load_weights(const void* p, int dtype, int c, int width, float (&w)[8]) {
+// A pack's elements of a vector of weights in fp32 (zero beyond the row).
+template <int G>
+__device__ __forceinline__ void load_weights(const void* p, int dtype, int c, int width, float (&w)[G]) {
     if (dtype == MUON_AMD_SRC_BF16) {
-        const Group8<uint16_t> g = load_group<uint16_t, false>(static_cast<const uint16_t*>(p), c, width);
+        const Pack<uint16_t, G> g = load_pack<uint16_t, G, false>(static_cast<const uint16_t*>(p), c, width);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = g[k];
+        for (int k = 0; k < G; ++k) w[k] = g[k];
     } else {
-        const Group8<float> g = load_group<float, false>(static_cast<const float*>(p), c, width);
+        #pragma unroll
+        for (int h = 0; h < G; h += 4) {
+            const Pack<float, 4> g = load_pack<float, 4, false>(static_cast<const float*>(p), c + h, width);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = g[k];
+            for (int k = 0; k < 4; ++k) w[h + k] = g[k];
+        }
     }
 }
 __device__ __forceinline__ float load_one(const void* p, int dtype, int64_t i) {
     return dtype == MUON_AMD_SRC_BF16 ? bf2f(static_cast<const uint16_t*>(p)[i]) : static_cast<const float*>(p)[i];
 }
-// The scale of eight channels: one per channel, one for all, or none.
-__device__ __forceinline__ void load_scale(const MuonResidualNorm& a, int c, float (&s)[8]) {
+__device__ __forceinline__ void store_one(void* p, int dtype, int64_t i, float v) {
+    if (dtype == MUON_AMD_SRC_BF16) static_cast<uint16_t*>(p)[i] = f2bf(v);
+    else static_cast<float*>(p)[i] = v;
+}
+// The scale of a pack's channels: one per channel, one for all, or none.
+template <int G>
+__device__ __forceinline__ void load_scale(const MuonResidualNorm& a, int c, float (&s)[G]) {
     if (a.scale && !a.scale_is_one) {
         load_weights(a.scale, a.weight_dtype, c, a.width, s);
         return;
     }
     const float one = a.scale ? load_one(a.scale, a.weight_dtype, 0) : 1.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s[k] = one;
+    for (int k = 0; k < G; ++k) s[k] = one;
 }
 
-template <typename X, typename B, int GATE, int TPR, int V>
+template <typename X, typename B, int GATE, int TPR, int V, int G>
 __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_forward_kernel(const MuonResidualNorm a) {
     constexpr int THREADS = TPR > RN_THREADS ? TPR : RN_THREADS, ROWS = THREADS / TPR;
     __shared__ float slots[2][THREADS / 64][1];
     const int t = threadIdx.x % TPR, width = a.width;
-    float k[V][8], wpre[V][8];
+    float k[V][G], wpre[V][G];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = (j * TPR + t) * 8;
-        float s[8];
+        const int c = (j * TPR + t) * G;
+        float s[G];
         load_scale(a, c, s);
         load_weights(a.post_weight, a.weight_dtype, c, width, k[j]);
         load_weights(a.pre_weight, a.weight_dtype, c, width, wpre[j]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) k[j][i] *= s[i];
+        for (int i = 0; i < G; ++i) k[j][i] *= s[i];
     }
     const float per = 1.f / static_cast<float>(width);
     for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS; first < a.rows; first += static_cast<int64_t>(gridDim.x) * ROWS) {
@@ -114,46 +123,46 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
         const X* const x = static_cast<const X*>(a.x) + row * a.ld_x;
         const B* const b = static_cast<const B*>(a.b) + row * a.ld_b;
         const B* const z = static_cast<const B*>(a.gate) + row * a.ld_gate;
-        Group8<X> xv[V];
-        Group8<B> bv[V], zv[V];
+        Pack<X, G> xv[V];
+        Pack<B, G> bv[V], zv[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (j * TPR + t) * 8;
-            bv[j] = load_group<B, true>(b, c, n);
-            xv[j] = load_group<X, true>(x, c, n);
-            if constexpr (GATE == GATE_CHANNEL) zv[j] = load_group<B, true>(z, c, n);
+            const int c = (j * TPR + t) * G;
+            bv[j] = load_pack<B, G, true>(b, c, n);
+            xv[j] = load_pack<X, G, true>(x, c, n);
+            if constexpr (GATE == GATE_CHANNEL) zv[j] = load_pack<B, G, true>(z, c, n);
         }
         float whole = 1.f;
-        if constexpr (GATE == GATE_TOKEN) whole = in ? sigmoid(Group8<B>::load_first(z, 1)[0]) : 0.f;
+        if constexpr (GATE == GATE_TOKEN) whole = in ? sigmoid(load_one(a.gate, a.block_dtype, row * a.ld_gate)) : 0.f;
         float sum[1] = {0.f};
 #pragma unroll
         for (int j = 0; j < V; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[0] = fmaf(bv[j][i], bv[j][i], sum[0]);
+            for (int i = 0; i < G; ++i) sum[0] = fmaf(bv[j][i], bv[j][i], sum[0]);
         row_sums<TPR, 1>(sum, slots[0]);
         const float rb = 1.f / sqrtf(fmaf(sum[0], per, a.eps));
-        float h[V][8];
+        float h[V][G];
         sum[0] = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (j * TPR + t) * 8;
+            const int c = (j * TPR + t) * G;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < G; ++i) {
                 const float sig = GATE == GATE_CHANNEL ? sigmoid(zv[j][i]) : whole;
                 h[j][i] = fmaf(bv[j][i] * rb, k[j][i] * sig, xv[j][i]);
                 if (c + i < n) sum[0] = fmaf(h[j][i], h[j][i], sum[0]);
             }
-            store_group<X, false>(static_cast<X*>(a.h) + row * width, c, n, Group8<X>::of(h[j]));
+            store_pack<X, G, false>(static_cast<X*>(a.h) + row * width, c, n, Pack<X, G>::of(h[j]));
         }
         row_sums<TPR, 1>(sum, slots[1]);
         const float rh = 1.f / sqrtf(fmaf(sum[0], per, a.eps));
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (j * TPR + t) * 8;
-            float y[8];
+            const int c = (j * TPR + t) * G;
+            float y[G];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = h[j][i] * rh * wpre[j][i];
-            store_group<B, false>(static_cast<B*>(a.y) + row * width, c, n, Group8<B>::of(y));
+            for (int i = 0; i < G; ++i) y[i] = h[j][i] * rh * wpre[j][i];
+            store_pack<B, G, false>(static_cast<B*>(a.y) + row * width, c, n, Pack<B, G>::of(y));
         }
         if (in && t == 0 && a.rstd) {
             a.rstd[2 * row] = rb;
@@ -162,21 +171,21 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
     }
 }
 
-template <typename X, typename B, int GATE, int TPR, int V>
+template <typename X, typename B, int GATE, int TPR, int V, int G>
 __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_backward_kernel(const MuonResidualNorm a) {
     constexpr int THREADS = TPR > RN_THREADS ? TPR : RN_THREADS, ROWS = THREADS / TPR;
     __shared__ float slots[2][THREADS / 64][3];
     const int t = threadIdx.x % TPR, width = a.width;
-    float k[V][8], wpre[V][8], q[V][8], r[V][8];
+    float k[V][G], wpre[V][G], q[V][G], r[V][G];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = (j * TPR + t) * 8;
-        float s[8];
+        const int c = (j * TPR + t) * G;
+        float s[G];
         load_scale(a, c, s);
         load_weights(a.post_weight, a.weight_dtype, c, width, k[j]);
         load_weights(a.pre_weight, a.weight_dtype, c, width, wpre[j]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < G; ++i) {
             k[j][i] *= s[i];
             q[j][i] = r[j][i] = 0.f;
         }
@@ -190,26 +199,26 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
         const X* const x = static_cast<const X*>(a.x) + row * a.ld_x;
         const B* const b = static_cast<const B*>(a.b) + row * a.ld_b;
         const B* const z = static_cast<const B*>(a.gate) + row * a.ld_gate;
-        Group8<X> xv[V], dhv[V];
-        Group8<B> bv[V], zv[V], dyv[V];
+        Pack<X, G> xv[V], dhv[V];
+        Pack<B, G> bv[V], zv[V], dyv[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (j * TPR + t) * 8;
-            bv[j] = load_group<B, true>(b, c, n);
-            xv[j] = load_group<X, true>(x, c, n);
-            if constexpr (GATE == GATE_CHANNEL) zv[j] = load_group<B, true>(z, c, n);
-            dyv[j] = a.dy ? load_group<B, true>(static_cast<const B*>(a.dy) + row * a.ld_dy, c, n) : Group8<B>::zero();
-            dhv[j] = a.dh ? load_group<X, true>(static_cast<const X*>(a.dh) + row * a.ld_dh, c, n) : Group8<X>::zero();
+            const int c = (j * TPR + t) * G;
+            bv[j] = load_pack<B, G, true>(b, c, n);
+            xv[j] = load_pack<X, G, true>(x, c, n);
+            if constexpr (GATE == GATE_CHANNEL) zv[j] = load_pack<B, G, true>(z, c, n);
+            dyv[j] = a.dy ? load_pack<B, G, true>(static_cast<const B*>(a.dy) + row * a.ld_dy, c, n) : Pack<B, G>::zero();
+            dhv[j] = a.dh ? load_pack<X, G, true>(static_cast<const X*>(a.dh) + row * a.ld_dh, c, n) : Pack<X, G>::zero();
         }
         const float rb = in ? a.rstd[2 * row] : 0.f, rh = in ? a.rstd[2 * row + 1] : 0.f;
         float whole = 1.f;
-        if constexpr (GATE == GATE_TOKEN) whole = in ? sigmoid(Group8<B>::load_first(z, 1)[0]) : 0.f;
+        if constexpr (GATE == GATE_TOKEN) whole = in ? sigmoid(load_one(a.gate, a.block_dtype, row * a.ld_gate)) : 0.f;
         float sums[3] = {0.f, 0.f, 0.f};
-        float nh[V][8], e[V][8], sig[V][8];
+        float nh[V][G], e[V][G], sig[V][G];
 #pragma unroll
         for (int j = 0; j < V; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < G; ++i) {
                 sig[j][i] = GATE == GATE_CHANNEL ? sigmoid(zv[j][i]) : whole;
                 const float kk = k[j][i] * sig[j][i], nb = bv[j][i] * rb;
                 nh[j][i] = fmaf(nb, kk, xv[j][i]) * rh;
@@ -225,10 +234,10 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
         const float c1 = sums[0] * per * rh, dc2 = fmaf(-c1, sums[2], sums[1]), c2 = dc2 * per;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (j * TPR + t) * 8;
-            float dx[8], db[8], dz[8];
+            const int c = (j * TPR + t) * G;
+            float dx[G], db[G], dz[G];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < G; ++i) {
                 const float nb = bv[j][i] * rb, kk = k[j][i] * sig[j][i];
                 dx[i] = fmaf(-c1, nh[j][i], e[j][i]);
                 db[i] = rb * fmaf(dx[i], kk, -c2 * nb);
@@ -236,28 +245,25 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
                 q[j][i] = fmaf(g, sig[j][i], q[j][i]);
                 dz[i] = g * kk * (1.f - sig[j][i]);
             }
-            if (a.dx) store_group<X, false>(static_cast<X*>(a.dx) + row * width, c, n, Group8<X>::of(dx));
-            if (a.db) store_group<B, false>(static_cast<B*>(a.db) + row * width, c, n, Group8<B>::of(db));
+            if (a.dx) store_pack<X, G, false>(static_cast<X*>(a.dx) + row * width, c, n, Pack<X, G>::of(dx));
+            if (a.db) store_pack<B, G, false>(static_cast<B*>(a.db) + row * width, c, n, Pack<B, G>::of(db));
             if constexpr (GATE == GATE_CHANNEL)
-                if (a.dgate) store_group<B, false>(static_cast<B*>(a.dgate) + row * width, c, n, Group8<B>::of(dz));
+                if (a.dgate) store_pack<B, G, false>(static_cast<B*>(a.dgate) + row * width, c, n, Pack<B, G>::of(dz));
         }
         if constexpr (GATE == GATE_TOKEN)
-            if (in && t == 0 && a.dgate) {
-                const float one[8] = {(1.f - whole) * dc2};
-                Group8<B>::of(one).store_first(static_cast<B*>(a.dgate) + row, 1);
-            }
+            if (in && t == 0 && a.dgate) store_one(a.dgate, a.block_dtype, row, (1.f - whole) * dc2);
     }
     // sums of this workgroup: its rows' threads one after the other, through LDS where there is more than one
     if (!a.partials) return;
     float* const out = a.partials + static_cast<int64_t>(blockIdx.x) * 2 * width;
     if constexpr (ROWS > 1) {
-        __shared__ float joined[ROWS - 1][2][V][8][TPR];
+        __shared__ float joined[ROWS - 1][2][V][G][TPR];
         const int sub = threadIdx.x / TPR;
         if (sub > 0)
 #pragma unroll
             for (int j = 0; j < V; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < G; ++i) {
                     joined[sub - 1][0][j][i][t] = q[j][i];
                     joined[sub - 1][1][j][i][t] = r[j][i];
                 }
@@ -267,36 +273,52 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
 #pragma unroll
             for (int j = 0; j < V; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < G; ++i) {
                     q[j][i] += joined[o][0][j][i][t];
                     r[j][i] += joined[o][1][j][i][t];
                 }
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = (j * TPR + t) * 8;
-        store_group<float, false>(out, c, width, Group8<float>::of(q[j]));
-        store_group<float, false>(out + width, c, width, Group8<float>::of(r[j]));
+        const int c = (j * TPR + t) * G;
+#pragma unroll
+        for (int h = 0; h < G; h += 4) {
+            store_pack<float, 4, false>(out, c + h, width, Pack<float, 4>{f32x4v{q[j][h], q[j][h + 1], q[j][h + 2], q[j][h + 3]}});
+            store_pack<float, 4, false>(out + width, c + h, width, Pack<float, 4>{f32x4v{r[j][h], r[j][h + 1], r[j][h + 2], r[j][h + 3]}});
+        }
     }
 }
 
-// The sums over the workgroups: 64 columns of q or r per workgroup, 16 shares of the partial rows joined in order.
-constexpr int RS_SHARES = 16;
-__device__ __forceinline__ void store_one(void* p, int dtype, int64_t i, float v) {
-    if (dtype == MUON_AMD_SRC_BF16) static_cast<uint16_t*>(p)[i] = f2bf(v);
-    else static_cast<float*>(p)[i] = v;
-}
-__global__ __launch_bounds__(64 * RS_SHARES) void residual_columns_kernel(const MuonResidualNorm a, int npartials, float* __restrict__ one) {
-    __shared__ float part[RS_SHARES][64];
-    const int lane = threadIdx.x & 63, share = threadIdx.x >> 6, width = a.width;
-    const int c = blockIdx.x * 64 + lane, which = blockIdx.y;            // 0: q, 1: r
+// The sums over the workgroups: RS_COLUMNS columns of q or r per workgroup, RS_SHARES shares of the partial rows, each
+// of which reads four rows at a time, joined in order.  What bounds it is latency: 64 columns and 16 shares (few
+// workgroups with long shares) took 18 us for 1024 partial rows of 2048.
+constexpr int RS_COLUMNS = 16, RS_SHARES = 64;
+__global__ __launch_bounds__(RS_COLUMNS * RS_SHARES) void residual_columns_kernel(const MuonResidualNorm a, int npartials,
+                                                                                  float* __restrict__ one) {
+    __shared__ float part[RS_SHARES][RS_COLUMNS];
+    const int lane = threadIdx.x % RS_COLUMNS, share = threadIdx.x / RS_COLUMNS, width = a.width;
+    const int c = blockIdx.x * RS_COLUMNS + lane, which = blockIdx.y;            // 0: q, 1: r
     float s = 0.f;
-    if (c < width)
-        for (int g = share; g < npartials; g += RS_SHARES) s += a.partials[(static_cast<int64_t>(g) * 2 + which) * width + c];
+    if (c < width) {
+        const float* const from = a.partials + static_cast<int64_t>(which) * width + c;
+        const int64_t step = 2 * static_cast<int64_t>(width);
+        int g = share;
+        for (; g + 3 * RS_SHARES < npartials; g += 4 * RS_SHARES) {
+            const float p0 = from[g * step], p1 = from[(g + RS_SHARES) * step], p2 = from[(g + 2 * RS_SHARES) * step],
+                        p3 = from[(g + 3 * RS_SHARES) * step];
+            s += (p0 + p1) + (p2 + p3);
+        }
+        for (; g < npartials; g += RS_SHARES) s += from[g * step];
+    }
     part[share][lane] = s;
     __syncthreads();
+    for (int half = RS_SHARES / 2; half >= 64 / RS_COLUMNS; half >>= 1) {
+        if (share < half) part[share][lane] += part[share + half][lane];
+        __syncthreads();
+    }
     if (share > 0 || c >= width) return;
-    for (int o = 1; o < RS_SHARES; ++o) s += part[o][lane];
+    s = part[0][lane];
+    for (int o = 1; o < 64 / RS_COLUMNS; ++o) s += part[o][lane];
     if (which) {
         if (a.dpre_weight) store_one(a.dpre_weight, a.weight_dtype, c, s);
         return;
@@ -319,10 +341,10 @@ __global__ __launch_bounds__(256) void residual_scale_kernel(const float* __rest
     if (threadIdx.x == 0) store_one(dscale, dtype, 0, (part[0] + part[1]) + (part[2] + part[3]));
 }
 
-// How a width is shared among threads: threads per row (a power of two) and groups of eight per thread.
-template <int T, int G>
+// How a width is shared among threads: threads per row (a power of two) and times eight elements per thread.
+template <int T, int E>
 struct Shape {
-    static constexpr int TPR = T, V = G;
+    static constexpr int TPR = T, EIGHTS = E;
 };
 template <typename F>
 static void with_forward_shape(int width, F&& f) {
@@ -401,8 +423,8 @@ int muon_amd_residual_norm(const MuonResidualNorm* args, void* stream) {
     const MuonResidualNorm a = *args;
     with_types(a, [&](auto x, auto b, auto gate) {
         with_forward_shape(a.width, [&](auto s) {
-            constexpr int TPR = decltype(s)::TPR, V = decltype(s)::V, THREADS = TPR > RN_THREADS ? TPR : RN_THREADS;
-            hipLaunchKernelGGL((residual_forward_kernel<decltype(x), decltype(b), decltype(gate)::value, TPR, V>),
+            constexpr int TPR = decltype(s)::TPR, G = pack_of<decltype(x)>, V = 8 / G * decltype(s)::EIGHTS, THREADS = TPR > RN_THREADS ? TPR : RN_THREADS;
+            hipLaunchKernelGGL((residual_forward_kernel<decltype(x), decltype(b), decltype(gate)::value, TPR, V, G>),
                                dim3(workgroups(a.rows, THREADS / TPR, 2048 / THREADS)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a);
         });
     });
@@ -421,15 +443,15 @@ int muon_amd_residual_norm_backward(const MuonResidualNorm* args, void* stream) 
     if (!columns) b.partials = nullptr;
     with_types(a, [&](auto x, auto y, auto gate) {
         with_backward_shape(a.width, [&](auto s) {
-            constexpr int TPR = decltype(s)::TPR, V = decltype(s)::V, THREADS = TPR > RN_THREADS ? TPR : RN_THREADS;
-            hipLaunchKernelGGL((residual_backward_kernel<decltype(x), decltype(y), decltype(gate)::value, TPR, V>), dim3(n), dim3(THREADS),
+            constexpr int TPR = decltype(s)::TPR, G = pack_of<decltype(x)>, V = 8 / G * decltype(s)::EIGHTS, THREADS = TPR > RN_THREADS ? TPR : RN_THREADS;
+            hipLaunchKernelGGL((residual_backward_kernel<decltype(x), decltype(y), decltype(gate)::value, TPR, V, G>), dim3(n), dim3(THREADS),
                                0, st, b);
         });
     });
     if (const int rc = check_launch("residual_norm_backward")) return rc;
     if (!columns) return MUON_AMD_OK;
     float* const one = a.dscale && a.scale_is_one ? a.partials + static_cast<int64_t>(n) * 2 * a.width : nullptr;
-    hipLaunchKernelGGL(residual_columns_kernel, dim3((a.width + 63) / 64, 2), dim3(64 * RS_SHARES), 0, st, a, n, one);
+    hipLaunchKernelGGL(residual_columns_kernel, dim3((a.width + RS_COLUMNS - 1) / RS_COLUMNS, 2), dim3(RS_COLUMNS * RS_SHARES), 0, st, a, n, one);
     if (const int rc = check_launch("residual_norm_backward")) return rc;
     if (one) hipLaunchKernelGGL(residual_scale_kernel, dim3(1), dim3(256), 0, st, one, a.width, a.dscale, a.weight_dtype);
     return check_launch("residual_norm_backward");

@@ -1,5 +1,9 @@
-// Groups of eight elements in their storage type (fp32, or bf16 as uint16_t) at any element address, as the streaming
-// kernels move them: 16 bytes of bf16, twice 16 bytes of fp32.  The target's vector accesses take any address.
+// Packs of four or eight elements in their storage type (fp32, or bf16 as uint16_t) at any element address, as the
+// streaming kernels move them.  The target's vector accesses take any address.
+//
+// A pack is 16 bytes or less (eight fp32 elements are two packs of four): lanes then lie next to each other in every
+// access.  Eight fp32 elements per lane as two accesses 32 bytes apart touch each line twice, with the non-temporal hint
+// once too early: AdamW with 32-bit states over 32000 x 2048 bf16 took 341 us that way.
 #pragma once
 
 #include "common.h"
@@ -8,8 +12,10 @@ namespace muon_amd {
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
 typedef float f32x4v_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4v_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2v_any __attribute__((ext_vector_type(2), aligned(2)));
 
 #define MUON_GLOBAL __attribute__((address_space(1)))
 
@@ -26,86 +32,76 @@ __device__ __forceinline__ void store_as(P* p, V v) {
     else *q = v;
 }
 
-template <typename T>
-struct Group8;
+// G elements of T.
+template <typename T, int G>
+struct Pack;
 
 template <>
-struct Group8<float> {
-    f32x4v a, b;
-    __device__ __forceinline__ float operator[](int k) const { return k < 4 ? a[k] : b[k - 4]; }
-    __device__ __forceinline__ void set(int k, float v) {
-        if (k < 4) a[k] = v;
-        else b[k - 4] = v;
-    }
-    static __device__ __forceinline__ Group8 zero() { return {f32x4v{0.f, 0.f, 0.f, 0.f}, f32x4v{0.f, 0.f, 0.f, 0.f}}; }
+struct Pack<float, 4> {
+    f32x4v v;
+    __device__ __forceinline__ float operator[](int k) const { return v[k]; }
+    static __device__ __forceinline__ Pack zero() { return {f32x4v{0.f, 0.f, 0.f, 0.f}}; }
     template <bool NT>
-    static __device__ __forceinline__ Group8 load(const float* p) {
-        return {load_as<NT, f32x4v_any>(p), load_as<NT, f32x4v_any>(p + 4)};
-    }
-    // the first n of the eight (the others zero)
-    static __device__ __forceinline__ Group8 load_first(const float* p, int n) {
-        Group8 g = zero();
-#pragma unroll
-        for (int k = 0; k < 7; ++k)
-            if (k < n) g.set(k, p[k]);
-        return g;
+    static __device__ __forceinline__ Pack load(const float* p) {
+        return {load_as<NT, f32x4v_any>(p)};
     }
     template <bool NT>
     __device__ __forceinline__ void store(float* p) const {
-        store_as<NT, f32x4v_any>(p, a);
-        store_as<NT, f32x4v_any>(p + 4, b);
+        store_as<NT, f32x4v_any>(p, v);
     }
-    __device__ __forceinline__ void store_first(float* p, int n) const {
-#pragma unroll
-        for (int k = 0; k < 7; ++k)
-            if (k < n) p[k] = (*this)[k];
-    }
-    // eight values in this storage type
-    static __device__ __forceinline__ Group8 of(const float (&v)[8]) {
-        return {f32x4v{v[0], v[1], v[2], v[3]}, f32x4v{v[4], v[5], v[6], v[7]}};
-    }
+    __device__ __forceinline__ void put(int k, float x) { v[k] = x; }         // an element in storage, as it is loaded
+    __device__ __forceinline__ float get(int k) const { return v[k]; }
+    static __device__ __forceinline__ Pack of(const float (&x)[4]) { return {f32x4v{x[0], x[1], x[2], x[3]}}; }
 };
 
-template <>
-struct Group8<uint16_t> {
-    u32x4v v;
+template <int G>
+struct Pack<uint16_t, G> {
+    typedef uint32_t words __attribute__((ext_vector_type(G / 2)));
+    typedef uint32_t words_any __attribute__((ext_vector_type(G / 2), aligned(2)));
+    words v;
     __device__ __forceinline__ float operator[](int k) const { return k & 1 ? bf_hi(v[k >> 1]) : bf_lo(v[k >> 1]); }
-    static __device__ __forceinline__ Group8 zero() { return {u32x4v{0u, 0u, 0u, 0u}}; }
+    static __device__ __forceinline__ Pack zero() { return {words(0u)}; }
     template <bool NT>
-    static __device__ __forceinline__ Group8 load(const uint16_t* p) {
-        return {load_as<NT, u32x4v_any>(p)};
-    }
-    static __device__ __forceinline__ Group8 load_first(const uint16_t* p, int n) {
-        Group8 g = zero();
-#pragma unroll
-        for (int k = 0; k < 7; ++k)
-            if (k < n) g.v[k >> 1] |= static_cast<uint32_t>(p[k]) << (16 * (k & 1));
-        return g;
+    static __device__ __forceinline__ Pack load(const uint16_t* p) {
+        return {load_as<NT, words_any>(p)};
     }
     template <bool NT>
     __device__ __forceinline__ void store(uint16_t* p) const {
-        store_as<NT, u32x4v_any>(p, v);
+        store_as<NT, words_any>(p, v);
     }
-    __device__ __forceinline__ void store_first(uint16_t* p, int n) const {
+    __device__ __forceinline__ void put(int k, uint16_t x) { v[k >> 1] |= static_cast<uint32_t>(x) << (16 * (k & 1)); }
+    __device__ __forceinline__ uint16_t get(int k) const { return static_cast<uint16_t>(v[k >> 1] >> (16 * (k & 1))); }
+    static __device__ __forceinline__ Pack of(const float (&x)[G]) {
+        Pack p;
 #pragma unroll
-        for (int k = 0; k < 7; ++k)
-            if (k < n) p[k] = static_cast<uint16_t>(v[k >> 1] >> (16 * (k & 1)));
-    }
-    static __device__ __forceinline__ Group8 of(const float (&x)[8]) {
-        return {u32x4v{pack2bf(x[0], x[1]), pack2bf(x[2], x[3]), pack2bf(x[4], x[5]), pack2bf(x[6], x[7])}};
+        for (int k = 0; k < G / 2; ++k) p.v[k] = pack2bf(x[2 * k], x[2 * k + 1]);
+        return p;
     }
 };
 
-// The group at element e of a row (tensor) of n elements: whole, its first n - e elements, or nothing.
-template <typename T, bool NT>
-__device__ __forceinline__ Group8<T> load_group(const T* p, int64_t e, int64_t n) {
-    if (e + 8 <= n) return Group8<T>::template load<NT>(p + e);
-    return Group8<T>::load_first(p + e, e < n ? static_cast<int>(n - e) : 0);
+// The pack at element e of a row (tensor) of n elements: whole, its first n - e elements and zeros, or zeros.
+template <typename T, int G, bool NT, typename I>
+__device__ __forceinline__ Pack<T, G> load_pack(const T* p, I e, I n) {
+    if (e + G <= n) return Pack<T, G>::template load<NT>(p + e);
+    Pack<T, G> g = Pack<T, G>::zero();
+#pragma unroll
+    for (int k = 0; k < G - 1; ++k)
+        if (e + k < n) g.put(k, p[e + k]);
+    return g;
 }
-template <typename T, bool NT>
-__device__ __forceinline__ void store_group(T* p, int64_t e, int64_t n, const Group8<T>& g) {
-    if (e + 8 <= n) g.template store<NT>(p + e);
-    else if (e < n) g.store_first(p + e, static_cast<int>(n - e));
+template <typename T, int G, bool NT, typename I>
+__device__ __forceinline__ void store_pack(T* p, I e, I n, const Pack<T, G>& g) {
+    if (e + G <= n) {
+        g.template store<NT>(p + e);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < G - 1; ++k)
+        if (e + k < n) p[e + k] = g.get(k);
 }
+
+// Elements of a pack where T decides alone: 16 bytes.
+template <typename T>
+constexpr int pack_of = 16 / sizeof(T);
 
 }  // namespace muon_amd

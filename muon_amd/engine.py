@@ -560,6 +560,7 @@ class AdamWGroupEngine:
         _lib.load()
         self.device = torch.device(device)
         self.state_bits = int(state_bits)
+        self.dtype = dtypes[0] if len(set(dtypes)) == 1 else -1
         self.descs = np.zeros(len(numels), dtype=_lib.ADAMW_DESC)
         self.descs["numel"], self.descs["dtype"] = numels, dtypes
         self.prefix = _plan.adam_block_prefix(numels)
@@ -603,7 +604,7 @@ class AdamWGroupEngine:
         lib = _lib.load()
         scale = None if self._grad_scale is None else self._grad_scale.data_ptr()
         _launch("adamw", self.nbytes, lambda: _lib.check(lib.muon_amd_adamw(
-            self.desc_dev.data_ptr(), self.prefix_dev.data_ptr(), len(self.descs), self.nblocks, self.state_bits, *self._hyper,
+            self.desc_dev.data_ptr(), self.prefix_dev.data_ptr(), len(self.descs), self.nblocks, self.dtype, self.state_bits, *self._hyper,
             scale, scalars_ptr or None, _stream_ptr(self.device)), "adamw"))
 
 

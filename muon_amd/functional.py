@@ -66,6 +66,8 @@ def clear_engine_cache() -> None:
     with _CACHE_LOCK:
         _ENGINE_CACHE.clear()
         _PRODUCT_CACHE.clear()
+    if _lib._native is not None:
+        _lib._native.clear_tables()               # of the gradient lists
 
 
 def _rounding_flag(rounding: str) -> bool:

@@ -10,11 +10,10 @@ from __future__ import annotations
 
 import weakref
 
-import numpy as np
 import torch
 
-from . import _lib, engine as _engine, plan as _plan
-from .engine import AdamGroupEngine, AdamWGroupEngine, MuonGroupEngine, StepGraph, _launch, _Staging, _stream_ptr, _upload, require_gpu_tensor
+from . import _lib, engine as _engine
+from .engine import AdamGroupEngine, AdamWGroupEngine, MuonGroupEngine, StepGraph, _launch, require_gpu_tensor
 from .functional import _rounding_flag, _src_dtype
 
 NS_STEPS = 5          # the reference classes never pass a step count: muon_update's default rules
@@ -566,7 +565,7 @@ class AdamW(_MuonBase):
         """The moments of the parameters that have a state, in the order of the groups, as a list of pairs (exp_avg,
         exp_avg_sq).  32 bits: the state tensors.  8 bits: bf16 tensors, which hold every value exactly while the
         largest of its 128 is at least 2^-100; `out`: a list of pairs of contiguous bf16 tensors that take them."""
-        params = [p for g in self.param_groups for p in g["params"] if len(self.state[p])]
+        params = [p for g in self.param_groups for p in g["params"] if self.state.get(p)]
         if self._state_bits == 32:
             if out is not None:
                 raise ValueError("states of 32 bits are returned as they are: out is for 8 bits")
@@ -582,34 +581,14 @@ class AdamW(_MuonBase):
                 if t.dtype != torch.bfloat16 or t.numel() != p.numel() or t.device != p.device or not t.is_contiguous():
                     raise ValueError("out takes contiguous bf16 tensors of the parameters' sizes on their devices")
             if p.numel():
-                rows.setdefault(p.device, []).append((*tensors, *pair, p.numel()))
+                rows.setdefault(p.device, []).append((*tensors, *pair))
         for device, items in rows.items():
             table = self._value_tables.get(device)
             if table is None:
-                table = self._value_tables[device] = _ValueTable(device)
+                table = self._value_tables[device] = _lib.native().ValueTable()
             with torch.cuda.device(device):
-                table.run([(*(t.data_ptr() for t in row[:6]), row[6]) for row in items])
+                _launch("adamw_values", 6 * sum(r[0].numel() for r in items), lambda: table.run(items))
         return list(out)
-
-
-class _ValueTable:
-    """The table of the launch that turns 8-bit states into numbers."""
-
-    def __init__(self, device):
-        self.device, self.staging, self.key = device, _Staging(device), None
-
-    def run(self, rows):
-        lib = _lib.load()
-        if rows != self.key:
-            d = np.array(rows, dtype=_lib.ADAMW_VALUES_DESC)
-            prefix = _plan.adam_block_prefix([r[6] for r in rows])
-            _lib.check(lib.muon_amd_validate_adamw_values(_lib.host_ptr(d), len(d), _lib.host_ptr(prefix)), "validate_adamw_values")
-            self.desc_dev = self.staging.upload(d, torch.empty(d.nbytes, dtype=torch.uint8, device=self.device))
-            self.prefix_dev = _upload(prefix, self.device)
-            self.nblocks, self.elems = int(prefix[-1]), int(d["numel"].sum())
-            self.key = rows
-        _launch("adamw_values", 6 * self.elems, lambda: _lib.check(lib.muon_amd_adamw_values(
-            self.desc_dev.data_ptr(), self.prefix_dev.data_ptr(), len(rows), self.nblocks, _stream_ptr(self.device)), "adamw_values"))
 
 
 def _fill_aux_adam_groups(param_groups, sort_muon: bool):

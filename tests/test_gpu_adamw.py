@@ -162,6 +162,15 @@ def test_other_betas(betas, bits):
 
 
 @gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_types_mixed_in_one_launch(bits):
+    params = [p for ps in (make([300, 9000], torch.bfloat16), make([8193, 40], torch.float32)) for p in ps]
+    opt = muon_amd.AdamW(params, lr=LR, betas=BETAS, eps=EPS, weight_decay=WD, state_bits=bits)
+    for k in range(2):
+        step_and_check(opt, params, bits)
+
+
+@gpu
 def test_gradients_over_many_powers_and_zeros():
     # from 2^-60 to 2^40 within one block of 128, blocks of zeros, and a block whose largest is far below the others
     params = make([128 * 6 + 50], torch.float32)
@@ -406,5 +415,5 @@ def test_tables_are_checked():
         bad = d.copy()
         bad[name] = value
         assert check(bad, prefix, 32) == -1
-    assert lib.muon_amd_adamw(None, None, 1, 1, 8, 0.1, 1.0, 0.1, 0.1, 1e-8, 0.5, 0.5, 1, None, None, None) == -1
+    assert lib.muon_amd_adamw(None, None, 1, 1, -1, 8, 0.1, 1.0, 0.1, 0.1, 1e-8, 0.5, 0.5, 1, None, None, None) == -1
     assert lib.muon_amd_adamw_values(None, None, 1, 1, None) == -1
