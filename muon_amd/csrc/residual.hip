@@ -46,8 +46,8 @@ __device__ __forceinline__ void row_sums(float (&s)[N], float (*slots)[N]) {
 #pragma unroll
     for (int k = 0; k < N; ++k) s[k] = lanes_sum(s[k]);
     if constexpr (TPR > 64) {
-        constexpr int WAVES = TPR / 64;
-        const int wave = threadIdx.x >> 6, first = wave & ~(WAVES - 1);
+        constexpr int WAVES = TPR / 64;                  // (a power of two where rows share a workgroup)
+        const int wave = threadIdx.x >> 6, first = TPR < RN_THREADS ? wave & ~(WAVES - 1) : 0;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int k = 0; k < N; ++k) slots[wave][k] = s[k];
@@ -99,26 +99,93 @@ __device__ __forceinline__ void load_scale(const MuonResidualNorm& a, int c, flo
     for (int k = 0; k < G; ++k) s[k] = one;
 }
 
+// The weights of a workgroup's channels, which it uses for row after row: k = scale * post_weight, and pre_weight.  They
+// wait in LDS (128 KB for the widest row; 32 bytes of reads per 8 elements and row, far below what LDS gives;
+// conflict-free: four channels of a thread next to those of the next), which leaves room for more waves in the registers:
+// with the weights there 8192 x 8192 bf16 took 254 us backward instead of 205.
+template <int TPR, int V, int G>
+struct Weights {
+    static constexpr int QUADS = V * G / 4;
+    f32x4v* shared;                        // [2][QUADS][TPR]
+
+    __device__ __forceinline__ void load(const MuonResidualNorm& a, f32x4v* space) {
+        shared = space;
+        const int t = threadIdx.x % TPR;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (j * TPR + t) * G;
+            float s[G], post[G], pre[G];
+            load_scale<G>(a, c, s);
+            load_weights<G>(a.post_weight, a.weight_dtype, c, a.width, post);
+            load_weights<G>(a.pre_weight, a.weight_dtype, c, a.width, pre);
+#pragma unroll
+            for (int i = 0; i < G; ++i) post[i] *= s[i];
+            if (threadIdx.x < TPR)
+#pragma unroll
+                for (int h = 0; h < G / 4; ++h) {
+                    shared[(j * (G / 4) + h) * TPR + t] = f32x4v{post[4 * h], post[4 * h + 1], post[4 * h + 2], post[4 * h + 3]};
+                    shared[(QUADS + j * (G / 4) + h) * TPR + t] = f32x4v{pre[4 * h], pre[4 * h + 1], pre[4 * h + 2], pre[4 * h + 3]};
+                }
+        }
+        __syncthreads();
+    }
+    template <int WHICH>
+    __device__ __forceinline__ void get(int j, float (&out)[G]) const {
+#pragma unroll
+        for (int h = 0; h < G / 4; ++h) {
+            const f32x4v v = shared[(WHICH * QUADS + j * (G / 4) + h) * TPR + threadIdx.x % TPR];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[4 * h + i] = v[i];
+        }
+    }
+};
+
+// A result that is larger than what the memory-side cache keeps of a launch goes out with the non-temporal hint, so that it
+// does not push out what is still to be read: 16384 x 4096 bf16 128 -> 121 us forward and 205 -> 197 backward; with everything
+// in the cache the hint costs (8192 x 2048: 26.2 -> 28.6 and 39.9 -> 42.5 us).
+constexpr int64_t RN_CACHE = 256ll << 20;
+template <typename T, int G>
+__device__ __forceinline__ void store_row(T* p, int c, int n, const Pack<T, G>& g, bool nt) {
+    if (nt) store_pack<T, G, true>(p, c, n, g);
+    else store_pack<T, G, false>(p, c, n, g);
+}
+
+// The pack at channel c of a row of `width`.  It is requested whole and without a branch, from where it lies in the row
+// (the last one of a row that ends within it: from its last G elements), so that all loads of a row go out
+// together; settle() then moves what a lane at the end of the row got to its place, with zeros beyond the row.  (With a
+// branch at each load 5003 x 1600 took 46 us backward, and 38 without.)
+template <typename T, int G>
+__device__ __forceinline__ Pack<T, G> request(const T* row, int c, int width) {
+    if (width < G) return load_pack<T, G, true>(row, c, width);
+    return Pack<T, G>::template load<true>(row + min(c, width - G));
+}
+template <typename T, int G>
+__device__ __forceinline__ void settle(Pack<T, G>& v, int c, int width) {
+    if (width < G || c + G <= width) return;
+    const int shift = min(c - (width - G), G);
+#pragma unroll
+    for (int by = 1; by <= G; by <<= 1) {
+        Pack<T, G> moved = Pack<T, G>::zero();
+#pragma unroll
+        for (int k = 0; k + by < G; ++k) moved.put(k, v.get(k + by));
+        if (shift & by) v = moved;
+    }
+}
+
 template <typename X, typename B, int GATE, int TPR, int V, int G>
-__global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_forward_kernel(const MuonResidualNorm a) {
+__global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_forward_kernel(const MuonResidualNorm a, const bool nt) {
     constexpr int THREADS = TPR > RN_THREADS ? TPR : RN_THREADS, ROWS = THREADS / TPR;
     __shared__ float slots[2][THREADS / 64][1];
     const int t = threadIdx.x % TPR, width = a.width;
-    float k[V][G], wpre[V][G];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = (j * TPR + t) * G;
-        float s[G];
-        load_scale(a, c, s);
-        load_weights(a.post_weight, a.weight_dtype, c, width, k[j]);
-        load_weights(a.pre_weight, a.weight_dtype, c, width, wpre[j]);
-#pragma unroll
-        for (int i = 0; i < G; ++i) k[j][i] *= s[i];
-    }
+    typedef Weights<TPR, V, G> W;
+    __shared__ f32x4v weights[2 * W::QUADS * TPR];
+    W w;
+    w.load(a, weights);
     const float per = 1.f / static_cast<float>(width);
     for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS; first < a.rows; first += static_cast<int64_t>(gridDim.x) * ROWS) {
-        const int64_t row = first + threadIdx.x / TPR;
-        const bool in = row < a.rows;                             // (rows of several waves meet at barriers)
+        const int64_t place = first + (ROWS > 1 ? threadIdx.x / TPR : 0);
+        const bool in = ROWS == 1 || place < a.rows;              // (rows of several waves meet at barriers)
+        const int64_t row = in ? place : a.rows - 1;
         const int n = in ? width : 0;
         const X* const x = static_cast<const X*>(a.x) + row * a.ld_x;
         const B* const b = static_cast<const B*>(a.b) + row * a.ld_b;
@@ -128,12 +195,19 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * TPR + t) * G;
-            bv[j] = load_pack<B, G, true>(b, c, n);
-            xv[j] = load_pack<X, G, true>(x, c, n);
-            if constexpr (GATE == GATE_CHANNEL) zv[j] = load_pack<B, G, true>(z, c, n);
+            bv[j] = request<B, G>(b, c, width);
+            xv[j] = request<X, G>(x, c, width);
+            if constexpr (GATE == GATE_CHANNEL) zv[j] = request<B, G>(z, c, width);
         }
         float whole = 1.f;
-        if constexpr (GATE == GATE_TOKEN) whole = in ? sigmoid(load_one(a.gate, a.block_dtype, row * a.ld_gate)) : 0.f;
+        if constexpr (GATE == GATE_TOKEN) whole = sigmoid(load_one(a.gate, a.block_dtype, row * a.ld_gate));
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (j * TPR + t) * G;
+            settle<B, G>(bv[j], c, width);
+            settle<X, G>(xv[j], c, width);
+            if constexpr (GATE == GATE_CHANNEL) settle<B, G>(zv[j], c, width);
+        }
         float sum[1] = {0.f};
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -146,23 +220,26 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * TPR + t) * G;
+            float k[G];
+            w.template get<0>(j, k);
 #pragma unroll
             for (int i = 0; i < G; ++i) {
                 const float sig = GATE == GATE_CHANNEL ? sigmoid(zv[j][i]) : whole;
-                h[j][i] = fmaf(bv[j][i] * rb, k[j][i] * sig, xv[j][i]);
-                if (c + i < n) sum[0] = fmaf(h[j][i], h[j][i], sum[0]);
+                h[j][i] = fmaf(bv[j][i] * rb, k[i] * sig, xv[j][i]);
+                if (c + i < width) sum[0] = fmaf(h[j][i], h[j][i], sum[0]);
             }
-            store_pack<X, G, false>(static_cast<X*>(a.h) + row * width, c, n, Pack<X, G>::of(h[j]));
+            store_row<X, G>(static_cast<X*>(a.h) + row * width, c, n, Pack<X, G>::of(h[j]), nt);
         }
         row_sums<TPR, 1>(sum, slots[1]);
         const float rh = 1.f / sqrtf(fmaf(sum[0], per, a.eps));
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * TPR + t) * G;
-            float y[G];
+            float y[G], wpre[G];
+            w.template get<1>(j, wpre);
 #pragma unroll
-            for (int i = 0; i < G; ++i) y[i] = h[j][i] * rh * wpre[j][i];
-            store_pack<B, G, false>(static_cast<B*>(a.y) + row * width, c, n, Pack<B, G>::of(y));
+            for (int i = 0; i < G; ++i) y[i] = h[j][i] * rh * wpre[i];
+            store_row<B, G>(static_cast<B*>(a.y) + row * width, c, n, Pack<B, G>::of(y), nt);
         }
         if (in && t == 0 && a.rstd) {
             a.rstd[2 * row] = rb;
@@ -171,30 +248,27 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
     }
 }
 
+// (Four waves per SIMD where a workgroup's size allows them: 5003 x 1600 with an fp32 stream 66 -> 47 us.)
 template <typename X, typename B, int GATE, int TPR, int V, int G>
-__global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_backward_kernel(const MuonResidualNorm a) {
+__global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS, 4) void residual_backward_kernel(const MuonResidualNorm a, const bool nt) {
     constexpr int THREADS = TPR > RN_THREADS ? TPR : RN_THREADS, ROWS = THREADS / TPR;
     __shared__ float slots[2][THREADS / 64][3];
     const int t = threadIdx.x % TPR, width = a.width;
-    float k[V][G], wpre[V][G], q[V][G], r[V][G];
+    typedef Weights<TPR, V, G> W;
+    __shared__ f32x4v weights[2 * W::QUADS * TPR];
+    W w;
+    w.load(a, weights);
+    float q[V][G], r[V][G];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = (j * TPR + t) * G;
-        float s[G];
-        load_scale(a, c, s);
-        load_weights(a.post_weight, a.weight_dtype, c, width, k[j]);
-        load_weights(a.pre_weight, a.weight_dtype, c, width, wpre[j]);
+    for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int i = 0; i < G; ++i) {
-            k[j][i] *= s[i];
-            q[j][i] = r[j][i] = 0.f;
-        }
-    }
+        for (int i = 0; i < G; ++i) q[j][i] = r[j][i] = 0.f;
     const float per = 1.f / static_cast<float>(width);
     int set = 0;
     for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS; first < a.rows; first += static_cast<int64_t>(gridDim.x) * ROWS) {
-        const int64_t row = first + threadIdx.x / TPR;
-        const bool in = row < a.rows;
+        const int64_t place = first + (ROWS > 1 ? threadIdx.x / TPR : 0);
+        const bool in = ROWS == 1 || place < a.rows;
+        const int64_t row = in ? place : a.rows - 1;
         const int n = in ? width : 0;
         const X* const x = static_cast<const X*>(a.x) + row * a.ld_x;
         const B* const b = static_cast<const B*>(a.b) + row * a.ld_b;
@@ -204,51 +278,68 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * TPR + t) * G;
-            bv[j] = load_pack<B, G, true>(b, c, n);
-            xv[j] = load_pack<X, G, true>(x, c, n);
-            if constexpr (GATE == GATE_CHANNEL) zv[j] = load_pack<B, G, true>(z, c, n);
-            dyv[j] = a.dy ? load_pack<B, G, true>(static_cast<const B*>(a.dy) + row * a.ld_dy, c, n) : Pack<B, G>::zero();
-            dhv[j] = a.dh ? load_pack<X, G, true>(static_cast<const X*>(a.dh) + row * a.ld_dh, c, n) : Pack<X, G>::zero();
+            bv[j] = request<B, G>(b, c, width);
+            xv[j] = request<X, G>(x, c, width);
+            if constexpr (GATE == GATE_CHANNEL) zv[j] = request<B, G>(z, c, width);
+            // (without the gradient of one result any row stands in for it, and is then taken for zeros)
+            dyv[j] = request<B, G>(a.dy ? static_cast<const B*>(a.dy) + row * a.ld_dy : b, c, width);
+            dhv[j] = request<X, G>(a.dh ? static_cast<const X*>(a.dh) + row * a.ld_dh : x, c, width);
         }
-        const float rb = in ? a.rstd[2 * row] : 0.f, rh = in ? a.rstd[2 * row + 1] : 0.f;
+        const float rb = a.rstd[2 * row], rh = a.rstd[2 * row + 1];
         float whole = 1.f;
-        if constexpr (GATE == GATE_TOKEN) whole = in ? sigmoid(load_one(a.gate, a.block_dtype, row * a.ld_gate)) : 0.f;
+        if constexpr (GATE == GATE_TOKEN) whole = sigmoid(load_one(a.gate, a.block_dtype, row * a.ld_gate));
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (j * TPR + t) * G;
+            settle<B, G>(bv[j], c, width);
+            settle<X, G>(xv[j], c, width);
+            if constexpr (GATE == GATE_CHANNEL) settle<B, G>(zv[j], c, width);
+            settle<B, G>(dyv[j], c, width);
+            settle<X, G>(dhv[j], c, width);
+            if (!a.dy) dyv[j] = Pack<B, G>::zero();
+            if (!a.dh) dhv[j] = Pack<X, G>::zero();
+        }
         float sums[3] = {0.f, 0.f, 0.f};
         float nh[V][G], e[V][G], sig[V][G];
 #pragma unroll
-        for (int j = 0; j < V; ++j)
+        for (int j = 0; j < V; ++j) {
+            float k[G], wpre[G];
+            w.template get<0>(j, k);
+            w.template get<1>(j, wpre);
 #pragma unroll
             for (int i = 0; i < G; ++i) {
                 sig[j][i] = GATE == GATE_CHANNEL ? sigmoid(zv[j][i]) : whole;
-                const float kk = k[j][i] * sig[j][i], nb = bv[j][i] * rb;
+                const float kk = k[i] * sig[j][i], nb = bv[j][i] * rb;
                 nh[j][i] = fmaf(nb, kk, xv[j][i]) * rh;
-                const float dn = dyv[j][i] * wpre[j][i];
+                const float dn = dyv[j][i] * wpre[i];
                 e[j][i] = fmaf(rh, dn, dhv[j][i]);
                 sums[0] = fmaf(dn, nh[j][i], sums[0]);
                 sums[1] = fmaf(e[j][i] * kk, nb, sums[1]);
                 sums[2] = fmaf(nh[j][i] * kk, nb, sums[2]);
-                r[j][i] = fmaf(dyv[j][i], nh[j][i], r[j][i]);
+                if (in) r[j][i] = fmaf(dyv[j][i], nh[j][i], r[j][i]);      // (a row that stands in for one beyond the last adds nothing)
             }
+        }
         row_sums<TPR, 3>(sums, slots[set]);
         set ^= 1;
         const float c1 = sums[0] * per * rh, dc2 = fmaf(-c1, sums[2], sums[1]), c2 = dc2 * per;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * TPR + t) * G;
-            float dx[G], db[G], dz[G];
+            float dx[G], db[G], dz[G], k[G];
+            w.template get<0>(j, k);
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-                const float nb = bv[j][i] * rb, kk = k[j][i] * sig[j][i];
+                const float nb = bv[j][i] * rb, kk = k[i] * sig[j][i];
                 dx[i] = fmaf(-c1, nh[j][i], e[j][i]);
                 db[i] = rb * fmaf(dx[i], kk, -c2 * nb);
                 const float g = dx[i] * nb;
-                q[j][i] = fmaf(g, sig[j][i], q[j][i]);
+                if (in) q[j][i] = fmaf(g, sig[j][i], q[j][i]);
                 dz[i] = g * kk * (1.f - sig[j][i]);
             }
-            if (a.dx) store_pack<X, G, false>(static_cast<X*>(a.dx) + row * width, c, n, Pack<X, G>::of(dx));
-            if (a.db) store_pack<B, G, false>(static_cast<B*>(a.db) + row * width, c, n, Pack<B, G>::of(db));
+            if (a.dx) store_row<X, G>(static_cast<X*>(a.dx) + row * width, c, n, Pack<X, G>::of(dx), nt);
+            if (a.db) store_row<B, G>(static_cast<B*>(a.db) + row * width, c, n, Pack<B, G>::of(db), nt);
             if constexpr (GATE == GATE_CHANNEL)
-                if (a.dgate) store_pack<B, G, false>(static_cast<B*>(a.dgate) + row * width, c, n, Pack<B, G>::of(dz));
+                if (a.dgate) store_row<B, G>(static_cast<B*>(a.dgate) + row * width, c, n, Pack<B, G>::of(dz), nt);
         }
         if constexpr (GATE == GATE_TOKEN)
             if (in && t == 0 && a.dgate) store_one(a.dgate, a.block_dtype, row, (1.f - whole) * dc2);
@@ -341,11 +432,13 @@ __global__ __launch_bounds__(256) void residual_scale_kernel(const float* __rest
     if (threadIdx.x == 0) store_one(dscale, dtype, 0, (part[0] + part[1]) + (part[2] + part[3]));
 }
 
-// How a width is shared among threads: threads per row (a power of two) and times eight elements per thread.
+// How a width is shared among threads: threads per row and times eight elements per thread.
 template <int T, int E>
 struct Shape {
     static constexpr int TPR = T, EIGHTS = E;
 };
+// Backward, where the waves of a row take most of the registers, about as few whole waves as hold it: 5120 channels in the
+// threads of 8192 took 158 us over 8192 rows, in their own 137.  Forward that gains nothing (87 and 90 us).
 template <typename F>
 static void with_forward_shape(int width, F&& f) {
     if (width <= 512) f(Shape<64, 1>{});
@@ -360,7 +453,11 @@ static void with_backward_shape(int width, F&& f) {
     if (width <= 512) f(Shape<64, 1>{});
     else if (width <= 1024) f(Shape<128, 1>{});
     else if (width <= 2048) f(Shape<256, 1>{});
+    else if (width <= 3072) f(Shape<384, 1>{});
     else if (width <= 4096) f(Shape<512, 1>{});
+    else if (width <= 5120) f(Shape<640, 1>{});
+    else if (width <= 6144) f(Shape<768, 1>{});
+    else if (width <= 7168) f(Shape<896, 1>{});
     else if (width <= 8192) f(Shape<1024, 1>{});
     else f(Shape<1024, 2>{});
 }
@@ -375,6 +472,8 @@ static void with_types(const MuonResidualNorm& a, F&& f) {
     else if (a.block_dtype == MUON_AMD_SRC_BF16) gates(float{}, uint16_t{});
     else gates(float{}, float{});
 }
+
+static int elem_size(int dtype) { return dtype == MUON_AMD_SRC_BF16 ? 2 : 4; }
 
 // Workgroups of a launch over `rows` rows: all of them, up to `per_cu` for each of the 256 CUs.
 static int workgroups(int64_t rows, int rows_each, int per_cu) {
@@ -421,11 +520,12 @@ int muon_amd_residual_norm(const MuonResidualNorm* args, void* stream) {
     if (const int rc = check_residual(args, "residual_norm")) return rc;
     MUON_REQUIRE(args->h && args->y, "residual_norm: null output");
     const MuonResidualNorm a = *args;
+    const bool nt = a.rows * a.width * (2 * elem_size(a.stream_dtype) + (a.gate && !a.gate_is_token ? 3 : 2) * elem_size(a.block_dtype)) > RN_CACHE;
     with_types(a, [&](auto x, auto b, auto gate) {
         with_forward_shape(a.width, [&](auto s) {
             constexpr int TPR = decltype(s)::TPR, G = pack_of<decltype(x)>, V = 8 / G * decltype(s)::EIGHTS, THREADS = TPR > RN_THREADS ? TPR : RN_THREADS;
             hipLaunchKernelGGL((residual_forward_kernel<decltype(x), decltype(b), decltype(gate)::value, TPR, V, G>),
-                               dim3(workgroups(a.rows, THREADS / TPR, 2048 / THREADS)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a);
+                               dim3(workgroups(a.rows, THREADS / TPR, 2048 / THREADS)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a, nt);
         });
     });
     return check_launch("residual_norm");
@@ -439,13 +539,14 @@ int muon_amd_residual_norm_backward(const MuonResidualNorm* args, void* stream) 
     MUON_REQUIRE(!columns || a.partials, "residual_norm_backward: null workspace");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const int n = backward_workgroups(a.rows, a.width);
+    const bool nt = a.rows * a.width * (3 * elem_size(a.stream_dtype) + (a.gate && !a.gate_is_token ? 5 : 3) * elem_size(a.block_dtype)) > RN_CACHE;
     MuonResidualNorm b = a;
     if (!columns) b.partials = nullptr;
     with_types(a, [&](auto x, auto y, auto gate) {
         with_backward_shape(a.width, [&](auto s) {
             constexpr int TPR = decltype(s)::TPR, G = pack_of<decltype(x)>, V = 8 / G * decltype(s)::EIGHTS, THREADS = TPR > RN_THREADS ? TPR : RN_THREADS;
             hipLaunchKernelGGL((residual_backward_kernel<decltype(x), decltype(y), decltype(gate)::value, TPR, V, G>), dim3(n), dim3(THREADS),
-                               0, st, b);
+                               0, st, b, nt);
         });
     });
     if (const int rc = check_launch("residual_norm_backward")) return rc;

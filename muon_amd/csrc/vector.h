@@ -84,9 +84,10 @@ template <typename T, int G, bool NT, typename I>
 __device__ __forceinline__ Pack<T, G> load_pack(const T* p, I e, I n) {
     if (e + G <= n) return Pack<T, G>::template load<NT>(p + e);
     Pack<T, G> g = Pack<T, G>::zero();
+    if (e < n)                      // (lanes beyond the row do not walk through the elements)
 #pragma unroll
-    for (int k = 0; k < G - 1; ++k)
-        if (e + k < n) g.put(k, p[e + k]);
+        for (int k = 0; k < G - 1; ++k)
+            if (e + k < n) g.put(k, p[e + k]);
     return g;
 }
 template <typename T, int G, bool NT, typename I>
@@ -95,9 +96,10 @@ __device__ __forceinline__ void store_pack(T* p, I e, I n, const Pack<T, G>& g) 
         g.template store<NT>(p + e);
         return;
     }
+    if (e < n)
 #pragma unroll
-    for (int k = 0; k < G - 1; ++k)
-        if (e + k < n) p[e + k] = g.get(k);
+        for (int k = 0; k < G - 1; ++k)
+            if (e + k < n) p[e + k] = g.get(k);
 }
 
 // Elements of a pack where T decides alone: 16 bytes.

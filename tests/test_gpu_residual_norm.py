@@ -91,7 +91,7 @@ def check(t, dh, dy, eps=EPS, layout=lambda a: a):
     return h, y, grads
 
 
-WIDTHS = [1, 7, 8, 64, 100, 511, 512, 513, 768, 1024, 1025, 1600, 2048, 2500, 4096, 4104, 8192, 9001, 16384]
+WIDTHS = [1, 7, 8, 64, 100, 511, 512, 513, 768, 1024, 1025, 1600, 2048, 2500, 4000, 4096, 4104, 5120, 6000, 7168, 8192, 9001, 16384]
 
 
 @gpu
