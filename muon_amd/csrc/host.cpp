@@ -18,6 +18,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <array>
 #include <cstring>
 #include <list>
 #include <optional>
@@ -46,6 +47,7 @@ struct Api {
     decltype(&muon_amd_grad_clip) grad_clip;
     decltype(&muon_amd_validate_adamw_values) validate_adamw_values;
     decltype(&muon_amd_adamw_values) adamw_values;
+    decltype(&muon_amd_adamw) adamw;
     int max_width, max_experts, max_k, shared_elems, block_elems, norm_partials;
 } api{};
 
@@ -451,6 +453,17 @@ class AdamWTable {
     const py::str step_{"step"};
 };
 
+// The AdamW launch on the current stream of a device (addresses as numbers; hyper: lr, 1 - lr weight_decay, 1 - beta1,
+// 1 - beta2, eps, 1 - beta1^t, 1 - beta2^t, t).
+void adamw_launch(int device, uintptr_t descs, uintptr_t prefix, int n, int blocks, int dtype, int bits, const std::array<double, 8>& hyper,
+                  uintptr_t grad_scale, uintptr_t scalars) {
+    const auto f = [&](int i) { return static_cast<float>(hyper[i]); };
+    check(api.adamw(reinterpret_cast<const MuonAdamWDesc*>(descs), reinterpret_cast<const int32_t*>(prefix), n, blocks, dtype, bits, f(0), f(1),
+                    f(2), f(3), f(4), f(5), f(6), static_cast<uint32_t>(hyper[7]), reinterpret_cast<const float*>(grad_scale),
+                    reinterpret_cast<const float*>(scalars), c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream()),
+          "adamw");
+}
+
 // A table of descriptors and its block prefix on the device.  A table is never rewritten: other contents get memory of
 // their own, so a launch on one stream cannot see what a call on another stream uploads.
 class Table {
@@ -616,6 +629,7 @@ void bind(const py::dict& addresses, const py::object& error) {
     get(api.grad_clip, "muon_amd_grad_clip");
     get(api.validate_adamw_values, "muon_amd_validate_adamw_values");
     get(api.adamw_values, "muon_amd_adamw_values");
+    get(api.adamw, "muon_amd_adamw");
     const auto number = [&](const char* name) {
         int (*f)(void);
         get(f, name);
@@ -654,6 +668,7 @@ PYBIND11_MODULE(_native, m) {
     m.def("abi_version", [] { return MUON_AMD_ABI_VERSION; });
     m.def("residual_norm", &residual_norm);
     m.def("route_topk", &route_topk);
+    m.def("adamw_launch", &adamw_launch);
     m.def("clip", &clip);
     m.def("clip_list", &clip_list);
     m.def("clear_tables", [] { grad_tables().clear(); });

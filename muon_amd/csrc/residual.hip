@@ -150,28 +150,6 @@ __device__ __forceinline__ void store_row(T* p, int c, int n, const Pack<T, G>& 
     else store_pack<T, G, false>(p, c, n, g);
 }
 
-// The pack at channel c of a row of `width`.  It is requested whole and without a branch, from where it lies in the row
-// (the last one of a row that ends within it: from its last G elements), so that all loads of a row go out
-// together; settle() then moves what a lane at the end of the row got to its place, with zeros beyond the row.  (With a
-// branch at each load 5003 x 1600 took 46 us backward, and 38 without.)
-template <typename T, int G>
-__device__ __forceinline__ Pack<T, G> request(const T* row, int c, int width) {
-    if (width < G) return load_pack<T, G, true>(row, c, width);
-    return Pack<T, G>::template load<true>(row + min(c, width - G));
-}
-template <typename T, int G>
-__device__ __forceinline__ void settle(Pack<T, G>& v, int c, int width) {
-    if (width < G || c + G <= width) return;
-    const int shift = min(c - (width - G), G);
-#pragma unroll
-    for (int by = 1; by <= G; by <<= 1) {
-        Pack<T, G> moved = Pack<T, G>::zero();
-#pragma unroll
-        for (int k = 0; k + by < G; ++k) moved.put(k, v.get(k + by));
-        if (shift & by) v = moved;
-    }
-}
-
 template <typename X, typename B, int GATE, int TPR, int V, int G>
 __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_forward_kernel(const MuonResidualNorm a, const bool nt) {
     constexpr int THREADS = TPR > RN_THREADS ? TPR : RN_THREADS, ROWS = THREADS / TPR;
@@ -195,9 +173,9 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * TPR + t) * G;
-            bv[j] = request<B, G>(b, c, width);
-            xv[j] = request<X, G>(x, c, width);
-            if constexpr (GATE == GATE_CHANNEL) zv[j] = request<B, G>(z, c, width);
+            bv[j] = request<B, G, true>(b, c, width);
+            xv[j] = request<X, G, true>(x, c, width);
+            if constexpr (GATE == GATE_CHANNEL) zv[j] = request<B, G, true>(z, c, width);
         }
         float whole = 1.f;
         if constexpr (GATE == GATE_TOKEN) whole = sigmoid(load_one(a.gate, a.block_dtype, row * a.ld_gate));
@@ -278,12 +256,12 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS, 4) void residu
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * TPR + t) * G;
-            bv[j] = request<B, G>(b, c, width);
-            xv[j] = request<X, G>(x, c, width);
-            if constexpr (GATE == GATE_CHANNEL) zv[j] = request<B, G>(z, c, width);
+            bv[j] = request<B, G, true>(b, c, width);
+            xv[j] = request<X, G, true>(x, c, width);
+            if constexpr (GATE == GATE_CHANNEL) zv[j] = request<B, G, true>(z, c, width);
             // (without the gradient of one result any row stands in for it, and is then taken for zeros)
-            dyv[j] = request<B, G>(a.dy ? static_cast<const B*>(a.dy) + row * a.ld_dy : b, c, width);
-            dhv[j] = request<X, G>(a.dh ? static_cast<const X*>(a.dh) + row * a.ld_dh : x, c, width);
+            dyv[j] = request<B, G, true>(a.dy ? static_cast<const B*>(a.dy) + row * a.ld_dy : b, c, width);
+            dhv[j] = request<X, G, true>(a.dh ? static_cast<const X*>(a.dh) + row * a.ld_dh : x, c, width);
         }
         const float rb = a.rstd[2 * row], rh = a.rstd[2 * row + 1];
         float whole = 1.f;

@@ -20,23 +20,60 @@ namespace muon_amd {
 
 constexpr int RT_MAX_EXPERTS = 1024;
 constexpr int RT_MAX_K = 32;
-constexpr int RT_THREADS = 256;
+constexpr int RT_THREADS = 512;
+constexpr int RT_WAVES = RT_THREADS / 64;
 constexpr int RT_GROUPS = 512;             // workgroups at most: their partial sums are joined by one launch
 
-// The value of `v` in the lane a power of two away, within groups of L lanes.
-template <typename T>
-__device__ __forceinline__ T lane_xor(T v, int mask) {
-    return __shfl_xor(v, mask, 64);
+// Another lane's value, by one of the moves that vector instructions make on the way (data through LDS has ten times
+// the latency, and the choices of a row are a chain of such moves).
+template <int CTRL, typename T>
+__device__ __forceinline__ T moved(T v) {
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(T, static_cast<uint64_t>(moved<CTRL>(static_cast<uint32_t>(b >> 32))) << 32 | moved<CTRL>(static_cast<uint32_t>(b)));
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+    }
 }
+// Both 16-lane rows of each 32 lanes (ROWS) or both halves of the wave, each in every lane of the two, joined by f.
+template <bool ROWS, typename T, typename F>
+__device__ __forceinline__ T joined(T v, F&& f) {
+    const auto swap = [](uint32_t w) {
+        const auto r = ROWS ? __builtin_amdgcn_permlane16_swap(w, w, false, false) : __builtin_amdgcn_permlane32_swap(w, w, false, false);
+        return u32x2v{r[0], r[1]};
+    };
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const u32x2v hi = swap(static_cast<uint32_t>(b >> 32)), lo = swap(static_cast<uint32_t>(b));
+        return f(__builtin_bit_cast(T, static_cast<uint64_t>(hi[0]) << 32 | lo[0]), __builtin_bit_cast(T, static_cast<uint64_t>(hi[1]) << 32 | lo[1]));
+    } else {
+        const u32x2v r = swap(__builtin_bit_cast(uint32_t, v));
+        return f(__builtin_bit_cast(T, static_cast<uint32_t>(r[0])), __builtin_bit_cast(T, static_cast<uint32_t>(r[1])));
+    }
+}
+// f over L lanes next to each other, in every one of them.
 template <int L, typename T, typename F>
 __device__ __forceinline__ T group_reduce(T v, F&& f) {
-#pragma unroll
-    for (int m = 1; m < L; m <<= 1) v = f(v, lane_xor(v, m));
+    if constexpr (L >= 2) v = f(v, moved<0xB1>(v));              // quad_perm 1,0,3,2
+    if constexpr (L >= 4) v = f(v, moved<0x4E>(v));              // quad_perm 2,3,0,1
+    if constexpr (L >= 8) v = f(v, moved<0x141>(v));             // row_half_mirror
+    if constexpr (L >= 16) v = f(v, moved<0x140>(v));            // row_mirror
+    if constexpr (L >= 32) v = joined<true>(v, f);
+    if constexpr (L >= 64) v = joined<false>(v, f);
     return v;
 }
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {
     return group_reduce<L>(v, [](float a, float b) { return a + b; });
+}
+
+// e^d for d at most 0 (or not a number): 2^(d log2 e) by the target's instruction, with what the product lost put back, so
+// about two units off over the whole range.
+__device__ __forceinline__ float exp_of(float d) {
+    constexpr float L = 1.44269504088896341f, LN2 = 0.69314718055994531f;
+    d = d < -200.f ? -200.f : d;                                 // (e^-200 is zero; -infinity would leave no number in `lost`)
+    const float t = d * L, lost = fmaf(d, L, -t), e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e * LN2, lost, e);
 }
 
 // A logit's bits in the order of its value: negative numbers below positive ones, both zeros equal, NaN above all.
@@ -76,27 +113,39 @@ __device__ __forceinline__ const T* row_of(const MuonRoute& a, int64_t t) {
 }
 __device__ __forceinline__ bool unmasked(const MuonRoute& a, int64_t t) { return t < a.tokens && (!a.mask || a.mask[t]); }
 
-template <typename T, int N, int L>
-__device__ __forceinline__ void load_row(const T* row, int base, int experts, bool in, float (&x)[N]) {
-    constexpr int G = pack_of<T>;
+// A row's packs as they are requested, and its logits in fp32 once they are there: -infinity beyond the row and where the
+// token takes no part.
+template <typename T, int N>
+struct RowPacks {
+    static constexpr int G = pack_of<T>;
+    Pack<T, G> v[N / G];
+    __device__ __forceinline__ void load(const T* row, int base, int experts) {
 #pragma unroll
-    for (int g = 0; g < N / G; ++g) {
-        const Pack<T, G> v = load_pack<T, G, false>(row, base + G * g, in ? experts : 0);
-#pragma unroll
-        for (int i = 0; i < G; ++i) x[G * g + i] = in && base + G * g + i < experts ? v[i] : -__builtin_inff();
+        for (int g = 0; g < N / G; ++g) v[g] = request<T, G, false>(row, base + G * g, experts);
     }
-}
+    __device__ __forceinline__ void get(int base, int experts, bool in, float (&x)[N]) {
+#pragma unroll
+        for (int g = 0; g < N / G; ++g) {
+            settle<T, G>(v[g], base + G * g, experts);
+#pragma unroll
+            for (int i = 0; i < G; ++i) x[G * g + i] = in && base + G * g + i < experts ? v[g][i] : -__builtin_inff();
+        }
+    }
+};
 
-// partials: workgroups x experts pairs {sum of p, tokens}, then workgroups x {sum of lse^2, tokens that take part}.
+// partials: workgroups x experts pairs {sum of p, tokens}, then workgroups x {sum of lse^2, tokens that take part}, then
+// what the launch that joins them needs (a counter, which this one clears, and a float for each of its workgroups).
 template <typename T, int N, int L>
 __global__ __launch_bounds__(RT_THREADS) void route_forward_kernel(const MuonRoute a) {
     constexpr int ROWS = RT_THREADS / L;
     typedef Key<T> K;
-    __shared__ float sums[ROWS][N * L + 1];
+    typedef typename K::type key_t;
+    __shared__ float sums[RT_WAVES][N * L];
     __shared__ int tokens[N * L];
-    __shared__ float squares[RT_THREADS / 64];
-    __shared__ int parts[RT_THREADS / 64];
+    __shared__ float squares[RT_WAVES];
+    __shared__ int parts[RT_WAVES];
     const int lane = threadIdx.x % L, sub = threadIdx.x / L, base = lane * N, E = a.experts;
+    const auto larger = [](key_t u, key_t v) { return max(u, v); };
     for (int e = threadIdx.x; e < N * L; e += RT_THREADS) tokens[e] = 0;
     __syncthreads();
     float acc[N];
@@ -104,48 +153,50 @@ __global__ __launch_bounds__(RT_THREADS) void route_forward_kernel(const MuonRou
     for (int i = 0; i < N; ++i) acc[i] = 0.f;
     float square = 0.f;
     int part = 0;
-    for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS; first < a.tokens; first += static_cast<int64_t>(gridDim.x) * ROWS) {
-        const int64_t t = first + sub;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * ROWS + sub; t - sub < a.tokens; t += step) {
+        RowPacks<T, N> row;
+        row.load(row_of<T>(a, t < a.tokens ? t : a.tokens - 1), base, E);
         const bool in = unmasked(a, t);
         float x[N];
-        load_row<T, N, L>(row_of<T>(a, t), base, E, in, x);
-        typename K::type key[N];
+        row.get(base, E, in, x);
+        key_t key[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) key[i] = K::of(x[i], base + i);
         // The k largest, one after the other (all keys differ and there are at least k, so this never wraps around).  Lane
         // j mod L takes choice j; where there are more choices than lanes, it leaves the earlier ones unscaled.
-        typename K::type best = 0;
+        key_t best = 0, mine = 0;
         float top = 0.f, chosen = 0.f, my_part = 0.f;
         int my_expert = -1;
         bool on = false;
         for (int j = 0; j < a.k; ++j) {
-            typename K::type m = 0;
+            key_t m = 0;
 #pragma unroll
-            for (int i = 0; i < N; ++i) m = max(m, static_cast<typename K::type>(key[i] - best));
-            m = group_reduce<L>(m, [](typename K::type u, typename K::type v) { return max(u, v); });
-            best += m;
-            const bool there = in && K::available(best);
+            for (int i = 0; i < N; ++i) m = max(m, static_cast<key_t>(key[i] - best));
+            best += group_reduce<L>(m, larger);
             if (j == 0) {
-                on = there;
+                on = in && K::available(best);
                 top = K::value(best);
             }
-            const float ex = there ? expf(K::value(best) - top) : 0.f;
-            chosen += ex;
-            if (lane == j % L) {
-                my_part = ex;
-                my_expert = there ? K::index(best) : -1;
-                if (there) atomicAdd(&tokens[my_expert], 1);
-                if (j + L < a.k && t < a.tokens) {
-                    a.weights[t * a.k + j] = my_part;
-                    a.indices[t * a.k + j] = my_expert;
-                }
+            if (lane == j % L) mine = best;
+            if (j % L != L - 1 && j != a.k - 1) continue;
+            // the lanes have a choice each, or it is the last
+            const bool has = lane <= j % L, there = has && in && K::available(mine);
+            my_part = there ? exp_of(K::value(mine) - top) : 0.f;
+            my_expert = there ? K::index(mine) : -1;
+            chosen += group_sum<L>(my_part);
+            if (there) atomicAdd(&tokens[my_expert], 1);
+            const int64_t o = t * a.k + (j - j % L) + lane;
+            if (has && t < a.tokens) {
+                a.indices[o] = my_expert;
+                if (j != a.k - 1) a.weights[o] = my_part;
             }
         }
         // softmax over the row
         float ex[N], total = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            ex[i] = on ? expf(x[i] - top) : 0.f;
+            ex[i] = on ? exp_of(x[i] - top) : 0.f;
             total += ex[i];
         }
         total = group_sum<L>(total);
@@ -155,9 +206,8 @@ __global__ __launch_bounds__(RT_THREADS) void route_forward_kernel(const MuonRou
         if (t >= a.tokens) continue;
         const float scale = on ? (a.normalize ? 1.f / chosen : per) : 0.f;
         for (int j = lane; j < a.k; j += L) {
-            const bool last = j + L >= a.k;
+            const bool last = j + L >= a.k && j / L == (a.k - 1) / L;
             a.weights[t * a.k + j] = (last ? my_part : a.weights[t * a.k + j]) * scale;
-            if (last) a.indices[t * a.k + j] = my_expert;
         }
         if (lane == 0) {
             a.lse[t] = on ? lse : -__builtin_inff();
@@ -165,14 +215,15 @@ __global__ __launch_bounds__(RT_THREADS) void route_forward_kernel(const MuonRou
             part += on;
         }
     }
-    // join the workgroup's rows
+    // join the workgroup's rows: those of a wave, then the waves
 #pragma unroll
-    for (int i = 0; i < N; ++i) sums[sub][base + i] = acc[i];
+    for (int i = 0; i < N; ++i) {
 #pragma unroll
-    for (int m = 32; m > 0; m >>= 1) {
-        square += lane_xor(square, m);
-        part += lane_xor(part, m);
+        for (int m = L; m < 64; m <<= 1) acc[i] += __shfl_xor(acc[i], m, 64);
+        if ((threadIdx.x & 63) < L) sums[threadIdx.x >> 6][base + i] = acc[i];
     }
+    square = group_sum<64>(square);
+    part = group_reduce<64>(part, [](int u, int v) { return u + v; });
     if ((threadIdx.x & 63) == 0) {
         squares[threadIdx.x >> 6] = square;
         parts[threadIdx.x >> 6] = part;
@@ -181,92 +232,105 @@ __global__ __launch_bounds__(RT_THREADS) void route_forward_kernel(const MuonRou
     float* const out = a.partials + static_cast<int64_t>(blockIdx.x) * 2 * E;
     for (int e = threadIdx.x; e < E; e += RT_THREADS) {
         float s = 0.f;
-        for (int r = 0; r < ROWS; ++r) s += sums[r][e];
+#pragma unroll
+        for (int w = 0; w < RT_WAVES; ++w) s += sums[w][e];
         out[2 * e] = s;
         out[2 * e + 1] = __int_as_float(tokens[e]);
     }
     if (threadIdx.x == 0) {
-        float* const tail = a.partials + static_cast<int64_t>(gridDim.x) * 2 * E + 2 * blockIdx.x;
-        tail[0] = (squares[0] + squares[1]) + (squares[2] + squares[3]);
-        tail[1] = __int_as_float((parts[0] + parts[1]) + (parts[2] + parts[3]));
+        float* const tail = a.partials + static_cast<int64_t>(gridDim.x) * 2 * E;
+        float s = 0.f;
+        int n = 0;
+        for (int w = 0; w < RT_WAVES; ++w) {
+            s += squares[w];
+            n += parts[w];
+        }
+        tail[2 * blockIdx.x] = s;
+        tail[2 * blockIdx.x + 1] = __int_as_float(n);
+        if (blockIdx.x == 0) tail[2 * gridDim.x] = __int_as_float(0);
     }
 }
 
-// One workgroup joins the partial sums: counts, both losses, and the number of tokens that take part.
-constexpr int RJ_THREADS = 1024;
+// Joins the partial sums: a workgroup for every RJ_EXPERTS experts, whose threads share the partial sums of each and read
+// four of them at a time; the workgroup that is done last adds what the others left, in their order (one workgroup for all
+// of 512 partial sums of 256 experts took 18 us, and 36 with one load at a time).
+constexpr int RJ_THREADS = 1024, RJ_EXPERTS = 16, RJ_SHARES = RJ_THREADS / RJ_EXPERTS;
 __global__ __launch_bounds__(RJ_THREADS) void route_join_kernel(const MuonRoute a, int groups) {
-    __shared__ float psum[RJ_THREADS];
-    __shared__ int csum[RJ_THREADS];
-    __shared__ float red[RJ_THREADS / 64];
-    __shared__ float shared_square;
-    __shared__ int shared_part;
-    const int E = a.experts;
-    // shares of the workgroups for each expert: a power of two that fills the launch
-    int width = 64;
-    while (width < E) width <<= 1;
-    const int shares = RJ_THREADS / width, e = threadIdx.x % width, share = threadIdx.x / width;
+    __shared__ float psum[RJ_SHARES][RJ_EXPERTS];
+    __shared__ int csum[RJ_SHARES][RJ_EXPERTS];
+    __shared__ bool last;
+    __shared__ float squares[RJ_THREADS / 64];
+    __shared__ int parts[RJ_THREADS / 64];
+    const int E = a.experts, lane = threadIdx.x % RJ_EXPERTS, share = threadIdx.x / RJ_EXPERTS, e = blockIdx.x * RJ_EXPERTS + lane;
+    const float* const tail = a.partials + static_cast<int64_t>(groups) * 2 * E;
+    int* const counter = reinterpret_cast<int*>(a.partials + static_cast<int64_t>(groups) * 2 * (E + 1));
+    float* const dots = reinterpret_cast<float*>(counter) + 1;
     float p = 0.f;
     int c = 0;
     if (e < E) {
         const f32x2_t* const at = reinterpret_cast<const f32x2_t*>(a.partials) + e;
-        int g = share;
-        for (; g + 7 * shares < groups; g += 8 * shares) {       // (eight loads on their way at once: one at a time took 36 us)
-            f32x2_t v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = at[static_cast<int64_t>(g + i * shares) * E];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                p += v[i][0];
-                c += __float_as_int(v[i][1]);
-            }
-        }
-        for (; g < groups; g += shares) {
-            const f32x2_t v = at[static_cast<int64_t>(g) * E];
+        const auto add = [&](f32x2_t v) {
             p += v[0];
             c += __float_as_int(v[1]);
-        }
-    }
-    psum[threadIdx.x] = p;
-    csum[threadIdx.x] = c;
-    if (threadIdx.x < 64) {
-        const float* const tail = a.partials + static_cast<int64_t>(groups) * 2 * E;
-        float s = 0.f;
-        int n = 0;
-        for (int g = threadIdx.x; g < groups; g += 64) {
-            s += tail[2 * g];
-            n += __float_as_int(tail[2 * g + 1]);
-        }
+        };
+        int g = share;
+        for (; g + 3 * RJ_SHARES < groups; g += 4 * RJ_SHARES) {
+            f32x2_t v[4];
 #pragma unroll
-        for (int m = 32; m > 0; m >>= 1) {
-            s += lane_xor(s, m);
-            n += lane_xor(n, m);
+            for (int i = 0; i < 4; ++i) v[i] = at[static_cast<int64_t>(g + i * RJ_SHARES) * E];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) add(v[i]);
         }
+        for (; g < groups; g += RJ_SHARES) add(at[static_cast<int64_t>(g) * E]);
+    }
+    psum[share][lane] = p;
+    csum[share][lane] = c;
+    __syncthreads();
+    for (int half = RJ_SHARES / 2; half > 0; half >>= 1) {
+        if (share < half) {
+            psum[share][lane] += psum[share + half][lane];
+            csum[share][lane] += csum[share + half][lane];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x < 64) {
+        float dot = 0.f;
+        if (share == 0 && e < E) {
+            a.counts[e] = csum[0][lane];
+            dot = static_cast<float>(csum[0][lane]) * psum[0][lane];
+        }
+        dot = group_sum<64>(dot);
         if (threadIdx.x == 0) {
-            shared_square = s;
-            shared_part = n;
+            __hip_atomic_store(&dots[blockIdx.x], dot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.x) - 1;
         }
     }
     __syncthreads();
-    float dot = 0.f;
-    if (share == 0 && e < E) {
-        for (int o = 1; o < shares; ++o) {
-            p += psum[o * width + e];
-            c += csum[o * width + e];
-        }
-        a.counts[e] = c;
-        dot = static_cast<float>(c) * p;
+    if (!last) return;
+    float s = 0.f;
+    int n = 0;
+    for (int g = threadIdx.x; g < groups; g += RJ_THREADS) {
+        s += tail[2 * g];
+        n += __float_as_int(tail[2 * g + 1]);
     }
-    dot = wave_sum(dot);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = dot;
+    s = group_sum<64>(s);
+    n = group_reduce<64>(n, [](int u, int v) { return u + v; });
+    if ((threadIdx.x & 63) == 0) {
+        squares[threadIdx.x >> 6] = s;
+        parts[threadIdx.x >> 6] = n;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        float total = 0.f;
-        for (int w = 0; w < RJ_THREADS / 64; ++w) total += red[w];
-        const float n = static_cast<float>(shared_part > 0 ? shared_part : 1);
-        *a.balance = static_cast<float>(E) * (total / (n * static_cast<float>(a.k))) / n;
-        *a.z = shared_square / n;
-        *a.part = n;
+    if (threadIdx.x > 0) return;
+    for (int w = 1; w < RJ_THREADS / 64; ++w) {
+        s += squares[w];
+        n += parts[w];
     }
+    float total = 0.f;
+    for (unsigned g = 0; g < gridDim.x; ++g) total += __hip_atomic_load(&dots[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const float part = static_cast<float>(n > 0 ? n : 1);
+    *a.balance = static_cast<float>(E) * (total / (part * static_cast<float>(a.k))) / part;
+    *a.z = s / part;
+    *a.part = part;
 }
 
 // What lanes of a wave left in LDS is there for its other lanes (whose accesses are in order), for the compiler too.
@@ -275,54 +339,85 @@ __device__ __forceinline__ void wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+constexpr int RB_THREADS = 256;
+constexpr int RB_GROUPS = 1024;            // workgroups: four for each CU (65536 x 256: 25 us; 1536: 28, 3072: 37; each is set up once)
 template <typename T, int N, int L>
-__global__ __launch_bounds__(RT_THREADS) void route_backward_kernel(const MuonRoute a) {
-    constexpr int ROWS = RT_THREADS / L, G = pack_of<T>;
-    __shared__ float extra[ROWS][N * L + 4];          // what the weights' gradients add, by expert
+__global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRoute a) {
+    constexpr int ROWS = RB_THREADS / L, G = pack_of<T>;
+    // What the weights' gradients add, by expert.  Four experts of a lane lie next to those of the next lane, so that the
+    // lanes' reads of 16 bytes fall on all banks.
+    __shared__ f32x4v extra[ROWS][N / 4 * L];
     const int lane = threadIdx.x % L, sub = threadIdx.x / L, base = lane * N, E = a.experts;
+    const auto slot = [&](int e) { return reinterpret_cast<float*>(extra[sub]) + (e / 4 % (N / 4) * L + e / N) * 4 + e % 4; };
     const float n = *a.part;
     const float cb = a.dbalance ? *a.dbalance * static_cast<float>(E) / (n * n * static_cast<float>(a.k)) : 0.f;
     const float cz = a.dz ? *a.dz * 2.f / n : 0.f;
     float g[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        g[i] = base + i < E ? cb * static_cast<float>(a.counts[base + i]) : 0.f;
-        extra[sub][base + i] = 0.f;
-    }
+    for (int i = 0; i < N; ++i) g[i] = base + i < E ? cb * static_cast<float>(a.counts[base + i]) : 0.f;
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) extra[sub][q * L + lane] = f32x4v{0.f, 0.f, 0.f, 0.f};
     wave_order();
-    for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS; first < a.tokens; first += static_cast<int64_t>(gridDim.x) * ROWS) {
-        const int64_t t = first + sub;
-        const float lse = t < a.tokens ? a.lse[t] : -__builtin_inff();
-        const bool on = lse != -__builtin_inff();
-        float x[N];
-        load_row<T, N, L>(row_of<T>(a, t), base, E, on, x);
-        // the weights' part: lanes of the row take the k choices in turn
-        if (a.dweights && on) {
-            float dot = 0.f;
-            for (int j = lane; j < a.k; j += L) dot = fmaf(a.weights[t * a.k + j], a.dweights[t * a.ld_dweights + j], dot);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS, begin = static_cast<int64_t>(blockIdx.x) * ROWS + sub;
+    // The next row is on its way while this one is worked on: its logits, and each lane's first choice.
+    RowPacks<T, N> next;
+    float next_lse, next_w = 0.f, next_dw = 0.f;
+    int next_e = -1;
+    const bool chooses = a.dweights && lane < a.k;
+    const auto fetch = [&](int64_t t) {
+        const int64_t row = t < a.tokens ? t : a.tokens - 1;
+        next.load(row_of<T>(a, row), base, E);
+        next_lse = a.lse[row];
+        if (chooses) {
+            next_w = a.weights[row * a.k + lane];
+            next_dw = a.dweights[row * a.ld_dweights + lane];
+            next_e = a.indices[row * a.k + lane];
+        }
+    };
+    fetch(begin);
+    for (int64_t t = begin; t - sub < a.tokens; t += step) {
+        RowPacks<T, N> packs = next;
+        const float lse = next_lse, w = next_w, dw = next_dw;
+        const bool on = t < a.tokens && lse != -__builtin_inff();
+        const int mine = on ? next_e : -1;
+        fetch(t + step);
+        // The weights' part; lanes of the row take the k choices in turn.
+        if (a.dweights) {
+            float dot = w * dw;
+            for (int j = lane + L; j < a.k; j += L)
+                if (on) dot = fmaf(a.weights[t * a.k + j], a.dweights[t * a.ld_dweights + j], dot);
             dot = a.normalize ? group_sum<L>(dot) : 0.f;
-            for (int j = lane; j < a.k; j += L) {
-                const int e = a.indices[t * a.k + j];
-                if (e >= 0) extra[sub][e] = a.weights[t * a.k + j] * (a.dweights[t * a.ld_dweights + j] - dot);
+            if (mine >= 0) *slot(mine) = w * (dw - dot);
+            for (int j = lane + L; j < a.k; j += L) {
+                const int e = on ? a.indices[t * a.k + j] : -1;
+                if (e >= 0) *slot(e) = a.weights[t * a.k + j] * (a.dweights[t * a.ld_dweights + j] - dot);
             }
         }
         wave_order();
-        float p[N], u[N], dot = 0.f;
+        float x[N], p[N], u[N], dot = 0.f;
+        packs.get(base, E, on, x);
+#pragma unroll
+        for (int q = 0; q < N / 4; ++q) {
+            const f32x4v v = extra[sub][q * L + lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[4 * q + i] = v[i];
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            p[i] = on ? expf(x[i] - lse) : 0.f;
-            u[i] = extra[sub][base + i];
+            p[i] = on ? exp_of(x[i] - lse) : 0.f;
             dot = fmaf(p[i], g[i], dot);
             if (!a.normalize) dot += u[i];         // p dw: what comes through the probabilities themselves
         }
         dot = group_sum<L>(dot);
         const float all = on ? fmaf(cz, lse, -dot) : 0.f;
         wave_order();
-        if (a.dweights && on)
-            for (int j = lane; j < a.k; j += L) {
-                const int e = a.indices[t * a.k + j];
-                if (e >= 0) extra[sub][e] = 0.f;
+        if (a.dweights) {
+            if (mine >= 0) *slot(mine) = 0.f;
+            for (int j = lane + L; j < a.k; j += L) {
+                const int e = on ? a.indices[t * a.k + j] : -1;
+                if (e >= 0) *slot(e) = 0.f;
             }
+        }
         if (t >= a.tokens) continue;
 #pragma unroll
         for (int q = 0; q < N / G; ++q) {
@@ -387,7 +482,7 @@ int muon_amd_route_max_k(void) { return RT_MAX_K; }
 
 int64_t muon_amd_route_partials(int64_t tokens, int experts) {
     if (tokens <= 0 || experts <= 0 || experts > RT_MAX_EXPERTS) return 0;
-    return static_cast<int64_t>(route_groups(tokens, experts)) * 2 * (experts + 1);
+    return static_cast<int64_t>(route_groups(tokens, experts)) * 2 * (experts + 1) + 1 + (experts + RJ_EXPERTS - 1) / RJ_EXPERTS;
 }
 
 int muon_amd_route(const MuonRoute* args, void* stream) {
@@ -400,7 +495,7 @@ int muon_amd_route(const MuonRoute* args, void* stream) {
         hipLaunchKernelGGL((route_forward_kernel<decltype(x), decltype(s)::N, decltype(s)::L>), dim3(n), dim3(RT_THREADS), 0, st, a);
     });
     if (const int rc = check_launch("route")) return rc;
-    hipLaunchKernelGGL(route_join_kernel, dim3(1), dim3(RJ_THREADS), 0, st, a, n);
+    hipLaunchKernelGGL(route_join_kernel, dim3((a.experts + RJ_EXPERTS - 1) / RJ_EXPERTS), dim3(RJ_THREADS), 0, st, a, n);
     return check_launch("route");
 }
 
@@ -409,10 +504,10 @@ int muon_amd_route_backward(const MuonRoute* args, void* stream) {
     const MuonRoute a = *args;
     MUON_REQUIRE(a.dlogits, "route_backward: null output");
     with_route(a, [&](auto x, auto s) {
-        constexpr int ROWS = RT_THREADS / decltype(s)::L;
+        constexpr int ROWS = RB_THREADS / decltype(s)::L;
         const int64_t n = (a.tokens + ROWS - 1) / ROWS;
-        hipLaunchKernelGGL((route_backward_kernel<decltype(x), decltype(s)::N, decltype(s)::L>), dim3(n < 2048 ? n : 2048), dim3(RT_THREADS),
-                           0, static_cast<hipStream_t>(stream), a);
+        hipLaunchKernelGGL((route_backward_kernel<decltype(x), decltype(s)::N, decltype(s)::L>), dim3(n < RB_GROUPS ? n : RB_GROUPS),
+                           dim3(RB_THREADS), 0, static_cast<hipStream_t>(stream), a);
     });
     return check_launch("route_backward");
 }

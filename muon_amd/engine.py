@@ -557,7 +557,6 @@ class AdamWGroupEngine:
     STEP_MODULUS = 1 << 24     # the dither goes by the step modulo this: fp32 scalars hold it exactly
 
     def __init__(self, numels, dtypes, state_bits, device):
-        _lib.load()
         self.device = torch.device(device)
         self.state_bits = int(state_bits)
         self.dtype = dtypes[0] if len(set(dtypes)) == 1 else -1
@@ -601,11 +600,10 @@ class AdamWGroupEngine:
         pass
 
     def enqueue(self, scalars_ptr: int = 0, join: bool = True):
-        lib = _lib.load()
-        scale = None if self._grad_scale is None else self._grad_scale.data_ptr()
-        _launch("adamw", self.nbytes, lambda: _lib.check(lib.muon_amd_adamw(
-            self.desc_dev.data_ptr(), self.prefix_dev.data_ptr(), len(self.descs), self.nblocks, self.dtype, self.state_bits, *self._hyper,
-            scale, scalars_ptr or None, _stream_ptr(self.device)), "adamw"))
+        scale = 0 if self._grad_scale is None else self._grad_scale.data_ptr()
+        _launch("adamw", self.nbytes, lambda: _lib.native().adamw_launch(
+            self.device.index, self.desc_dev.data_ptr(), self.prefix_dev.data_ptr(), len(self.descs), self.nblocks, self.dtype,
+            self.state_bits, self._hyper, scale, scalars_ptr))
 
 
 class StepGraph:
