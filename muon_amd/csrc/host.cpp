@@ -359,6 +359,35 @@ bool plain_gradient(const Tensor& g, const Tensor& p) {
            g.sizes() == p.sizes() && g.is_contiguous();
 }
 
+// The state of parameter `p`, or null where it has none or one that is empty.  `at` walks along: states are in the order
+// of their first step, as a rule that of the parameters.
+PyObject* state_of(const py::dict& state, PyObject* p, Py_ssize_t& at) {
+    PyObject *key, *s;
+    if (!(PyDict_Next(state.ptr(), &at, &key, &s) && key == p)) {
+        s = PyDict_GetItemWithError(state.ptr(), p);
+        if (!s) PyErr_Clear();
+    }
+    return s && PyDict_Check(s) && PyDict_GET_SIZE(s) > 0 ? s : nullptr;
+}
+// The names of a state's tensors, in the order of a launch's table.
+const py::str& state_name(int i) {
+    static const py::str* const names = new py::str[4]{py::str("exp_avg"), py::str("exp_avg_sq"), py::str("exp_avg_exponent"),
+                                                       py::str("exp_avg_sq_exponent")};
+    return names[i];
+}
+// Tensor i of parameter t's state of `bits` bits, or null where it is not what the kernels take.
+const Tensor* state_tensor(PyObject* s, int i, const Tensor& t, int bits) {
+    PyObject* const v = PyDict_GetItemWithError(s, state_name(i).ptr());
+    if (!v || !THPVariable_Check(v)) {
+        PyErr_Clear();
+        return nullptr;
+    }
+    const Tensor& x = THPVariable_Unpack(v);
+    if (x.scalar_type() != (bits == 8 ? at::kByte : at::kFloat) || x.device() != t.device() || !x.is_contiguous()) return nullptr;
+    if (i < 2) return x.sizes() == t.sizes() ? &x : nullptr;
+    return x.dim() == 1 && x.size(0) == (t.numel() + api.shared_elems - 1) / api.shared_elems ? &x : nullptr;
+}
+
 // The rows of an AdamW launch over a fixed list of parameters.  collect() reads the addresses of parameters, gradients and
 // states as they are now; nothing is taken from an earlier step but the answer to whether they are the same.
 class AdamWTable {
@@ -381,31 +410,15 @@ class AdamWTable {
             if (!t || t->numel() != numels_[i] || dtype_of(*t) != dtypes_[i]) return -1;
             if (!device) device = t->device();
             if (t->device() != *device || !plain_gradient(t->grad(), *t)) return -1;
-            // states are in the order of their first step, as a rule that of the parameters
-            PyObject *key, *s;
-            if (!(PyDict_Next(state.ptr(), &at, &key, &s) && key == p)) {
-                s = PyDict_GetItemWithError(state.ptr(), p);
-                if (!s) {
-                    PyErr_Clear();
-                    return -1;
-                }
-            }
-            if (!PyDict_Check(s)) return -1;
+            PyObject* const s = state_of(state, p, at);
+            if (!s) return -1;
             int64_t* const row = &now_[i * columns_];
             row[0] = reinterpret_cast<int64_t>(t->data_ptr());
             row[1] = reinterpret_cast<int64_t>(t->grad().data_ptr());
-            const int64_t shared = (numels_[i] + api.shared_elems - 1) / api.shared_elems;
             for (int c = 2; c < columns_; ++c) {
-                PyObject* const v = PyDict_GetItemWithError(s, names_[c - 2].ptr());
-                if (!v || !THPVariable_Check(v)) {
-                    PyErr_Clear();
-                    return -1;
-                }
-                const Tensor& x = THPVariable_Unpack(v);
-                const bool codes = bits_ == 8;
-                if (x.scalar_type() != (codes ? at::kByte : at::kFloat) || x.device() != *device || !x.is_contiguous()) return -1;
-                if (c < 4 ? x.sizes() != t->sizes() : (x.dim() != 1 || x.size(0) != shared)) return -1;
-                row[c] = reinterpret_cast<int64_t>(x.data_ptr());
+                const Tensor* const x = state_tensor(s, c - 2, *t, bits_);
+                if (!x) return -1;
+                row[c] = reinterpret_cast<int64_t>(x->data_ptr());
             }
             PyObject* const count = PyDict_GetItemWithError(s, step_.ptr());
             if (!count || !PyLong_Check(count)) {
@@ -449,7 +462,6 @@ class AdamWTable {
     std::vector<int64_t> rows_, now_;
     int64_t version_ = 0;
     std::vector<py::dict> dicts_;
-    const std::vector<py::str> names_{py::str("exp_avg"), py::str("exp_avg_sq"), py::str("exp_avg_exponent"), py::str("exp_avg_sq_exponent")};
     const py::str step_{"step"};
 };
 
@@ -590,14 +602,49 @@ std::tuple<Tensor, Tensor> clip_list(const std::vector<Tensor>& grads, double ma
 class ValueTable {
    public:
     void run(const std::vector<std::vector<Tensor>>& rows) {
-        std::vector<MuonAdamWValuesDesc> descs(rows.size());
-        const auto bytes = [](const Tensor& t) { return static_cast<const uint8_t*>(t.data_ptr()); };
-        for (size_t i = 0; i < rows.size(); ++i) {
-            const auto& r = rows[i];
-            descs[i] = {bytes(r[0]), bytes(r[1]), bytes(r[2]), bytes(r[3]), static_cast<uint16_t*>(r[4].data_ptr()),
-                        static_cast<uint16_t*>(r[5].data_ptr()), r[0].numel()};
+        std::vector<MuonAdamWValuesDesc> descs;
+        for (const auto& r : rows) add(descs, {&r[0], &r[1], &r[2], &r[3], &r[4], &r[5]});
+        launch(std::move(descs), rows[0][0].device());
+    }
+    // The same for the parameters that have a state, into `out` (pairs, in their order); false: not the common case.
+    bool run_plain(const py::list& params, const py::dict& state, const py::list& out) {
+        std::vector<MuonAdamWValuesDesc> descs;
+        std::optional<c10::Device> device;
+        Py_ssize_t at = 0;
+        const Py_ssize_t n = PyList_GET_SIZE(params.ptr());
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* const p = PyList_GET_ITEM(params.ptr(), i);
+            PyObject* const s = state_of(state, p, at);
+            if (!s) continue;
+            const Tensor* const t = plain_parameter(p);
+            if (!t || (device && t->device() != *device) || static_cast<Py_ssize_t>(descs.size()) >= PyList_GET_SIZE(out.ptr())) return false;
+            device = t->device();
+            PyObject* const pair = PyList_GET_ITEM(out.ptr(), descs.size());
+            if (!PyTuple_Check(pair) || PyTuple_GET_SIZE(pair) != 2) return false;
+            std::array<const Tensor*, 6> row;
+            for (int c = 0; c < 4; ++c)
+                if (!(row[c] = state_tensor(s, c, *t, 8))) return false;
+            for (int c = 0; c < 2; ++c) {
+                PyObject* const v = PyTuple_GET_ITEM(pair, c);
+                if (!THPVariable_Check(v)) return false;
+                const Tensor& x = THPVariable_Unpack(v);
+                if (x.scalar_type() != at::kBFloat16 || x.numel() != t->numel() || x.device() != *device || !x.is_contiguous()) return false;
+                row[4 + c] = &x;
+            }
+            add(descs, row);
         }
-        const c10::Device device = rows[0][0].device();
+        if (descs.empty() || static_cast<Py_ssize_t>(descs.size()) != PyList_GET_SIZE(out.ptr())) return false;
+        launch(std::move(descs), *device);
+        return true;
+    }
+
+   private:
+    static void add(std::vector<MuonAdamWValuesDesc>& descs, const std::array<const Tensor*, 6>& r) {
+        const auto bytes = [&](int c) { return static_cast<const uint8_t*>(r[c]->data_ptr()); };
+        descs.push_back({bytes(0), bytes(1), bytes(2), bytes(3), static_cast<uint16_t*>(r[4]->data_ptr()),
+                         static_cast<uint16_t*>(r[5]->data_ptr()), r[0]->numel()});
+    }
+    void launch(std::vector<MuonAdamWValuesDesc> descs, const c10::Device& device) {
         const c10::DeviceGuard guard(device);
         if (descs.size() != descs_.size() || std::memcmp(descs.data(), descs_.data(), descs.size() * sizeof(descs[0])) != 0) {
             table_.upload(descs, device);
@@ -607,8 +654,6 @@ class ValueTable {
         check(api.adamw_values(table_.descs<MuonAdamWValuesDesc>(), table_.prefix(), table_.size(), table_.blocks(), current_stream(device)),
               "adamw_values");
     }
-
-   private:
     std::vector<MuonAdamWValuesDesc> descs_;
     Table table_;
 };
@@ -672,7 +717,7 @@ PYBIND11_MODULE(_native, m) {
     m.def("clip", &clip);
     m.def("clip_list", &clip_list);
     m.def("clear_tables", [] { grad_tables().clear(); });
-    py::class_<ValueTable>(m, "ValueTable").def(py::init<>()).def("run", &ValueTable::run);
+    py::class_<ValueTable>(m, "ValueTable").def(py::init<>()).def("run", &ValueTable::run).def("run_plain", &ValueTable::run_plain);
     py::class_<AdamWTable>(m, "AdamWTable")
         .def(py::init<std::vector<int64_t>, std::vector<int>, int>())
         .def("collect", &AdamWTable::collect)

@@ -565,7 +565,14 @@ class AdamW(_MuonBase):
         """The moments of the parameters that have a state, in the order of the groups, as a list of pairs (exp_avg,
         exp_avg_sq).  32 bits: the state tensors.  8 bits: bf16 tensors, which hold every value exactly while the
         largest of its 128 is at least 2^-100; `out`: a list of pairs of contiguous bf16 tensors that take them."""
-        params = [p for g in self.param_groups for p in g["params"] if self.state.get(p)]
+        params = [p for g in self.param_groups for p in g["params"]]
+        if self._state_bits == 8 and out is not None and _engine.PROFILE is None:
+            table = self._value_tables.get(None)
+            if table is None:
+                table = self._value_tables[None] = _lib.native().ValueTable()
+            if table.run_plain(params, self.state, list(out)):
+                return list(out)
+        params = [p for p in params if self.state.get(p)]
         if self._state_bits == 32:
             if out is not None:
                 raise ValueError("states of 32 bits are returned as they are: out is for 8 bits")

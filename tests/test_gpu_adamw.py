@@ -218,6 +218,8 @@ def test_state_values_are_what_the_codes_stand_for():
     opt.step()
     outs = [tuple(torch.full((p.numel() + 1,), 7.0, dtype=torch.bfloat16, device=DEV)[1:] for _ in range(2)) for p in params]
     got = opt.state_values(out=outs)
+    as_lists = opt.state_values(out=[[torch.empty_like(t) for t in pair] for pair in outs])       # (the general way)
+    assert all(torch.equal(a, b) for x, y in zip(got, as_lists) for a, b in zip(x, y))
     for p, (m, v), fresh in zip(params, got, opt.state_values()):
         for t, k, kind, f in ((m, "exp_avg", "m", fresh[0]), (v, "exp_avg_sq", "v", fresh[1])):
             want = values(opt.state[p][k].cpu().numpy(), opt.state[p][k + "_exponent"].cpu().numpy(), kind)
