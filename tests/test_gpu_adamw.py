@@ -42,12 +42,12 @@ def mix(t):
     return t
 
 
-def rounded(x, kind, step, slack, E):
-    """The value that x's code stands for, with y = |x| / step + dither moved by `slack`."""
+def rounded(x, kind, step, slack, E, first=0):
+    """The value that x's code stands for, with y = |x| / step + dither moved by `slack`; first: the place of x[0]."""
     f = FORMATS[kind]
     b, E = blocks_of(x), E[:, None]
     power = np.maximum(np.frexp(np.abs(b))[1] - 1, E - 127 - (f["top"] - 1))
-    i = np.arange(b.size, dtype=np.uint64).reshape(b.shape)
+    i = (np.arange(b.size, dtype=np.uint64) + np.uint64(first)).reshape(b.shape) % np.uint64(1 << 32)
     h = (i * np.uint64(0x9E3779B9) + np.uint64(mix(step))) % np.uint64(1 << 32)
     u = ((h ^ h >> np.uint64(15)) % np.uint64(1 << 24) * np.uint64(f["factor"]) % np.uint64(1 << 32) >> np.uint64(12)).astype(np.float64) / (1 << 20)
     y = np.ldexp(np.abs(b), 3 - power) + u + slack
@@ -419,3 +419,35 @@ def test_tables_are_checked():
         assert check(bad, prefix, 32) == -1
     assert lib.muon_amd_adamw(None, None, 1, 1, -1, 8, 0.1, 1.0, 0.1, 0.1, 1e-8, 0.5, 0.5, 1, None, None, None) == -1
     assert lib.muon_amd_adamw_values(None, None, 1, 1, None) == -1
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_places_beyond_32_bits(bits):
+    """A tensor of more than 2^32 elements: the last ones are stepped like those of a small tensor at their place."""
+    n, last = 2 ** 32 + 4099, 4096 + 128 * 3
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device=DEV))
+    p.grad = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    tail = slice(n - n % SHARED - last, n)
+    g = torch.Generator().manual_seed(2)
+    p.data[tail] = (torch.randn(p[tail].numel(), generator=g) * 0.05).to(torch.bfloat16).to(DEV)
+    p.grad[tail] = (torch.randn(p[tail].numel(), generator=g) * 1e-3).to(torch.bfloat16).to(DEV)
+    p.grad[:8] = 1e-3
+    small = torch.nn.Parameter(p.detach()[tail].clone())
+    small.grad = p.grad[tail].clone()
+    opts = [muon_amd.AdamW([q], lr=LR, betas=BETAS, eps=EPS, weight_decay=WD, state_bits=bits) for q in (p, small)]
+    for opt in opts:
+        opt.step()
+    assert torch.equal(p[tail], small)
+    if bits == 32:
+        assert torch.equal(opts[0].state[p]["exp_avg"][tail], opts[1].state[small]["exp_avg"])
+        return
+    s = opts[0].state[p]
+    gt = small.grad.double().cpu().numpy()
+    in32 = lerp32(np.zeros_like(gt), gt, np.float64(np.float32(1 - BETAS[0])))
+    E = s["exp_avg_exponent"][tail.start // SHARED:].cpu().numpy()
+    np.testing.assert_array_equal(E, shared_exponent(in32, "m"))
+    got = np.abs(values(s["exp_avg"][tail].cpu().numpy(), E, "m"))
+    lo, hi = (np.abs(rounded(in32, "m", 1, slack, E.astype(np.int64), tail.start)) for slack in (-2.0 ** -16, 2.0 ** -16))
+    assert ((got >= lo) & (got <= hi)).all()
+    assert (s["exp_avg"][:8] != 0).all() and not s["exp_avg"][8:4096].any()

@@ -277,3 +277,25 @@ def test_no_second_derivatives():
     g, = torch.autograd.grad((h.sum() + y.sum()), t["x"], create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), t["x"])
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements in rows a distance apart that passes 2^32 elements over the tensor: the last rows are those
+    of a small call, bit for bit."""
+    rows, width = 2 ** 31 // 8192 + 7, 8192
+    wide = torch.zeros(rows, 2 * width + 8, dtype=BF16, device=DEV)
+    x = wide[:, :width]
+    t, dh, dy = make((5, width), BF16, BF16, BF16, gate="token", scale="channel")
+    x[-5:] = t["x"].detach()
+    block, gate = torch.zeros(rows, width, dtype=BF16, device=DEV), torch.zeros(rows, 1, dtype=BF16, device=DEV)
+    block[-5:], gate[-5:] = t["block"].detach(), t["gate"].detach()
+    gh, gy = torch.zeros_like(block), torch.zeros_like(block)
+    gh[-5:], gy[-5:] = dh, dy
+    args = [v.requires_grad_() for v in (x, block, gate)]
+    small = muon_amd.residual_norm(t["x"], t["block"], t["post_weight"], t["pre_weight"], gate=t["gate"], scale=t["scale"])
+    big = muon_amd.residual_norm(args[0], args[1], t["post_weight"], t["pre_weight"], gate=args[2], scale=t["scale"])
+    for a, b in zip(small, big):
+        assert torch.equal(a, b[-5:]) and not b[:4].any()
+    for a, b in zip(torch.autograd.grad(small, [t["x"], t["block"], t["gate"]], (dh, dy)), torch.autograd.grad(big, args, (gh, gy))):
+        assert torch.equal(a, b[-5:])

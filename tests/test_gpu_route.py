@@ -262,3 +262,28 @@ def test_no_second_derivatives():
     g, = torch.autograd.grad(muon_amd.route_topk(leaf, 2).balance_loss, leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), leaf)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 logits in rows that pass 2^32 elements over the tensor: the last tokens are chosen for as in a small
+    call, and the counts are whole."""
+    tokens, experts, k = 2 ** 31 // 512 + 5, 512, 2
+    wide = torch.zeros(tokens, 2 * experts, dtype=BF16, device=DEV)
+    logits = wide[:, :experts]
+    small, _, dw = make((40, experts), k, BF16)
+    logits[-40:] = small.to(DEV)
+    leaf = logits.requires_grad_()
+    r = muon_amd.route_topk(leaf, k)
+    few = small.to(DEV).requires_grad_()
+    want = muon_amd.route_topk(few, k)
+    assert torch.equal(r.indices[-40:], want.indices) and torch.equal(r.weights[-40:], want.weights)
+    assert (r.indices[:-40] == torch.tensor([0, 1], dtype=torch.int32, device=DEV)).all()
+    counts = want.counts.clone()
+    counts[:2] += tokens - 40
+    assert torch.equal(r.counts, counts)
+    grads = torch.zeros(tokens, k, device=DEV)
+    grads[-40:] = dw.to(DEV)
+    a, = torch.autograd.grad(r.weights, leaf, grads)
+    b, = torch.autograd.grad(want.weights, few, dw.to(DEV))
+    assert torch.equal(a[-40:], b) and not a[:-40].any()
