@@ -482,6 +482,9 @@ class Table {
    public:
     template <typename D>
     void upload(const std::vector<D>& descs, const c10::Device& device) {
+        if (capturing()) throw LibraryError("tensors that no call has seen before cannot be uploaded while a HIP graph is captured: make the call once before");
+        if (captured_) kept_.push_back(memory_);
+        captured_ = false;
         std::vector<int32_t> prefix(descs.size() + 1, 0);
         for (size_t i = 0; i < descs.size(); ++i)
             prefix[i + 1] = prefix[i] + static_cast<int32_t>((descs[i].numel + api.block_elems - 1) / api.block_elems);
@@ -498,9 +501,13 @@ class Table {
         uploaded_.record(stream_of(device));
     }
     // Before a launch on the current stream: its table is there, and stays while it runs.
-    // (What a HIP graph records cannot wait for an event from outside of it: a caller that captures has made the call before.)
+    // (What a HIP graph records cannot wait for an event from outside of it: a caller that captures has made the call
+    // before.  The graph keeps the table's address: from then on its memory is not given back.)
     void use(const c10::Device& device) {
-        if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) return;
+        if (capturing()) {
+            captured_ = true;
+            return;
+        }
         const c10::Stream stream = stream_of(device);
         uploaded_.block(stream);
         memory_.record_stream(stream);
@@ -510,8 +517,10 @@ class Table {
     const int32_t* prefix() const { return reinterpret_cast<const int32_t*>(static_cast<const char*>(memory_.data_ptr()) + prefix_); }
     int size() const { return n_; }
     int blocks() const { return blocks_; }
+    bool captured() const { return captured_; }
 
    private:
+    static bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
     template <typename D>
     static auto validator() {
         if constexpr (std::is_same_v<D, MuonGradDesc>) return api.validate_grads;
@@ -520,6 +529,8 @@ class Table {
     Tensor memory_;
     size_t prefix_ = 0;
     int n_ = 0, blocks_ = 0;
+    bool captured_ = false;
+    std::vector<Tensor> kept_;
     c10::Event uploaded_{c10::DeviceType::CUDA};
 };
 
@@ -553,7 +564,9 @@ std::tuple<Tensor, Tensor> clip_tensors(const std::vector<const Tensor*>& grads,
         GradTable fresh{device, std::move(descs), {}};
         fresh.table.upload(fresh.descs, device);
         tables.push_front(std::move(fresh));
-        if (tables.size() > GRAD_TABLES) tables.pop_back();
+        size_t others = 0;
+        for (auto i = tables.begin(); i != tables.end();)
+            i = !i->table.captured() && ++others > GRAD_TABLES ? tables.erase(i) : std::next(i);
     }
     Table& table = tables.front().table;
     const auto options = at::TensorOptions().device(device);

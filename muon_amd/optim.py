@@ -534,7 +534,7 @@ class AdamW(_MuonBase):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         self._init_runtime("reference", False, None, use_graph=use_graph)
         self._state_bits = state_bits
-        self._value_tables = {}
+        self._value_tables, self._scale_buffers = {}, {}
 
     def _hook_group(self, group):                 # no matrix of this optimizer has an early stage
         pass
@@ -542,7 +542,7 @@ class AdamW(_MuonBase):
     def __setstate__(self, state):
         bits = state.get("muon_amd_options", {}).get("_state_bits", getattr(self, "_state_bits", 32))
         super().__setstate__(state)
-        self._state_bits, self._value_tables = bits, {}
+        self._state_bits, self._value_tables, self._scale_buffers = bits, {}, {}
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
@@ -555,6 +555,11 @@ class AdamW(_MuonBase):
             require_gpu_tensor(grad_scale, "grad_scale")
             if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
                 raise TypeError(f"grad_scale must be one fp32 number, got {grad_scale.dtype} of shape {tuple(grad_scale.shape)}")
+            if self._use_graph:                   # recorded launches read it from one place
+                kept = self._scale_buffers.get(grad_scale.device)
+                if kept is None:
+                    kept = self._scale_buffers[grad_scale.device] = torch.empty(1, dtype=torch.float32, device=grad_scale.device)
+                grad_scale = kept.copy_(grad_scale.reshape(1))
         for gi, group in enumerate(self.param_groups):
             self._adamw_group_step(gi, group, self._state_bits, grad_scale, missing_grad_is_zero=False)
         self._launch_pending()

@@ -302,13 +302,15 @@ def test_state_survives(bits, how):
 def test_recorded_steps_are_the_eager_ones(bits):
     pairs = [make([1000, (129, 65)], torch.bfloat16) for _ in range(2)]
     opts = [muon_amd.AdamW(ps, lr=LR, state_bits=bits, use_graph=g) for ps, g in zip(pairs, (False, True))]
-    scale = torch.ones((), device=DEV)
+    scale, graphs, kept = torch.ones((), device=DEV), set(), []
     for k in range(5):
         scale.fill_(0.5 + 0.1 * k)
         for opt, ps in zip(opts, pairs):
             for group in opt.param_groups:
                 group["lr"] = LR / (k + 1)
-            opt.step(grad_scale=scale)
+            kept.append(scale.clone())                            # (a tensor of its own at every step)
+            opt.step(grad_scale=kept[-1])
+            graphs.add(id(opts[1]._graphs[torch.device(DEV)].graph) if opt is opts[1] else None)
             if k % 2:
                 for p in ps:
                     p.grad.mul_(0.75)
@@ -320,7 +322,7 @@ def test_recorded_steps_are_the_eager_ones(bits):
             # (the bias corrections are formed on the device in a recorded step)
             torch.testing.assert_close(p.float(), q.float(), rtol=2 * U16, atol=0)
             assert opts[0].state[p]["step"] == opts[1].state[q]["step"]
-    assert opts[1]._graphs[torch.device(DEV)].replays == 5
+    assert opts[1]._graphs[torch.device(DEV)].replays == 5 and len(graphs) == 2      # recorded once (and None)
 
 
 @gpu

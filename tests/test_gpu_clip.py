@@ -153,3 +153,35 @@ def test_tables_are_checked():
         bad[name] = value
         assert lib.muon_amd_validate_grads(_lib.host_ptr(bad), 1, _lib.host_ptr(prefix)) == -1
     assert lib.muon_amd_grad_norm(None, None, 1, 1, None, 1.0, None, None) == -1
+
+
+@gpu
+def test_captured_calls():
+    """Recorded into a graph, both calls read the gradients as they are at each replay; a list that no call has seen
+    cannot be recorded; other lists do not take the recorded one's table away."""
+    params = make([5000, 300], [torch.float32, torch.bfloat16])
+    other = make([77], [torch.float32])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        muon_amd.clip_coefficient(params, 0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm, coefficient = muon_amd.clip_coefficient(params, 0.1)
+        with pytest.raises(muon_amd.MuonAmdError):
+            muon_amd.clip_coefficient(other, 0.1)
+        muon_amd.clip_grad_norm_(params, 0.1)
+    for _ in range(40):                                           # more lists than are kept
+        muon_amd.clip_coefficient(make([50], [torch.float32]), 1.0)
+    for k in range(4):
+        for i, p in enumerate(params):
+            p.grad.copy_(torch.randn(p.numel(), generator=torch.Generator().manual_seed(10 * k + i)) * (k + 1))
+        before = [p.grad.clone() for p in params]
+        want = muon_amd.clip_coefficient(params, 0.1)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert float(norm) == float(want[0]) and float(coefficient) == float(want[1])
+        for p, g in zip(params, before):
+            assert torch.equal(p.grad, (g.float() * want[1]).to(g.dtype))
