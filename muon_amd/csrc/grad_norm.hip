@@ -49,13 +49,17 @@ __device__ __forceinline__ void for_blocks(const MuonGradDesc* __restrict__ desc
     }
 }
 
-template <typename T>
+// Gradients that the memory-side cache holds are left in it for the pass that comes next (AdamW over 65 M bf16 gradients
+// then takes 225 us instead of 242); more than that are read with the non-temporal hint (531 M: 177 -> 156 us).
+constexpr int64_t GN_CACHED = 1ll << 27;
+
+template <typename T, bool NT>
 __device__ __forceinline__ double squares_of_block(const MuonGradDesc& d, int64_t base) {
     const T* __restrict__ const g = static_cast<const T*>(d.grad);
     constexpr int G = pack_of<T>, PACKS = GN_EACH / G;
     Pack<T, G> gv[PACKS];
 #pragma unroll
-    for (int i = 0; i < PACKS; ++i) gv[i] = load_pack<T, G, true>(g, base + (i * GN_THREADS + threadIdx.x) * G, d.numel);
+    for (int i = 0; i < PACKS; ++i) gv[i] = load_pack<T, G, NT>(g, base + (i * GN_THREADS + threadIdx.x) * G, d.numel);
     double s[2] = {0., 0.};
 #pragma unroll
     for (int i = 0; i < PACKS; ++i)
@@ -67,13 +71,14 @@ __device__ __forceinline__ double squares_of_block(const MuonGradDesc& d, int64_
     return s[0] + s[1];
 }
 
+template <bool NT>
 __global__ __launch_bounds__(GN_THREADS) void grad_squares_kernel(const MuonGradDesc* __restrict__ descs,
                                                                  const int32_t* __restrict__ prefix, int ntensors, int nblocks,
                                                                  double* __restrict__ partials) {
     __shared__ double red[4];
     double s = 0.;
     for_blocks(descs, prefix, ntensors, nblocks, [&](const MuonGradDesc& d, int64_t base) {
-        s += d.dtype == MUON_AMD_SRC_BF16 ? squares_of_block<uint16_t>(d, base) : squares_of_block<float>(d, base);
+        s += d.dtype == MUON_AMD_SRC_BF16 ? squares_of_block<uint16_t, NT>(d, base) : squares_of_block<float, NT>(d, base);
     });
     const double total = block_sum<GN_THREADS>(s, red);
     if (threadIdx.x == 0) partials[blockIdx.x] = total;
@@ -169,7 +174,8 @@ static int grad_squares(const MuonGradDesc* descs_dev, const int32_t* prefix_dev
     MUON_REQUIRE(descs_dev && prefix_dev && partials_dev && out_dev, "grad_norm: null table, workspace or output");
     MUON_REQUIRE(ntensors > 0 && nblocks > 0, "grad_norm: ntensors=%d nblocks=%d", ntensors, nblocks);
     MUON_REQUIRE(max_norm >= 0.f, "grad_norm: max_norm=%g", max_norm);
-    hipLaunchKernelGGL(grad_squares_kernel, dim3(nblocks < GN_PARTIALS ? nblocks : GN_PARTIALS), dim3(GN_THREADS), 0, stream,
+    const auto kernel = static_cast<int64_t>(nblocks) * GN_BLOCK_ELEMS > GN_CACHED ? grad_squares_kernel<true> : grad_squares_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3(nblocks < GN_PARTIALS ? nblocks : GN_PARTIALS), dim3(GN_THREADS), 0, stream,
                        descs_dev, prefix_dev, ntensors, nblocks, partials_dev);
     return check_launch("grad_norm");
 }
