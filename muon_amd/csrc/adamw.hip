@@ -26,8 +26,12 @@
 namespace muon_amd {
 
 constexpr int AW_THREADS = 256;
-constexpr int AW_EACH = 32;                                     // elements per thread: all their loads go out first
-constexpr int AW_BLOCK_ELEMS = AW_THREADS * AW_EACH;            // elements per workgroup
+constexpr int AW_BLOCK_ELEMS = 8192;                            // elements of a block of the table
+// Elements per thread, whose loads all go out first: 16, and two workgroups for each block, or 32 where codes go with fp32
+// parameters.  (16 and 32: 32-bit states over 32000 x 2048 bf16 217 and 226 us, 8-bit states over 50257 x 768 bf16 67.6
+// and 69.5, their values 40 and 43; 8-bit states over 128256 x 4096 fp32 1444 and 1391.)
+constexpr int AW_EACH = 16, AW8_EACH_F32 = 32;
+constexpr int workgroups_per_block(int each) { return AW_BLOCK_ELEMS / (AW_THREADS * each); }
 constexpr int AW_SHARED = 128;                                  // elements that share an exponent
 
 struct AdamWArgs {
@@ -61,18 +65,21 @@ __device__ __forceinline__ AdamWArgs read_args(AdamWArgs a, const float* sc) {
 }
 
 // The two moments; the square is rounded before it is subtracted from, as for tensors of fp32.  A weight of a half and
-// more is taken from the other end, new + (w - 1)(new - old), which is `new` itself for w = 1; which end is the same for
-// the whole launch.
+// more is taken from the other end, new + (w - 1)(new - old), which is `new` itself for w = 1.  NEAR: neither weight is,
+// as in every ordinary run (the two selections for each element are then left out).
+template <bool NEAR>
 __device__ __forceinline__ float lerp_from(float old, float now, float w) {
-    const bool far = fabsf(w) >= 0.5f;
+    const bool far = !NEAR && fabsf(w) >= 0.5f;
     return fmaf(far ? w - 1.f : w, now - old, far ? now : old);
 }
+template <bool NEAR>
 __device__ __forceinline__ void moments(float& m, float& v, float g, const AdamWArgs& a) {
 #pragma clang fp contract(off)
     const float gg = g * g;
-    m = lerp_from(m, g, a.w1);
-    v = lerp_from(v, gg, a.w2);
+    m = lerp_from<NEAR>(m, g, a.w1);
+    v = lerp_from<NEAR>(v, gg, a.w2);
 }
+__device__ __forceinline__ bool near_weights(const AdamWArgs& a) { return fabsf(a.w1) < 0.5f && fabsf(a.w2) < 0.5f; }
 
 // ---- states in 32 bits -------------------------------------------------------------------------------------
 template <typename T>
@@ -82,7 +89,7 @@ __device__ __forceinline__ void adamw32_pack(Pack<T, 4>& p, const Pack<T, 4>& g,
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         float mk = m[k], vk = v[k];
-        moments(mk, vk, g[k] * c, a);
+        moments<false>(mk, vk, g[k] * c, a);
         m.v[k] = mk;
         v.v[k] = vk;
         pn[k] = fmaf(a.neg_lr, mk / fmaf(sqrtf(vk), a.rsqrt_bias2, a.eps), p[k] * a.wd_factor);
@@ -92,13 +99,13 @@ __device__ __forceinline__ void adamw32_pack(Pack<T, 4>& p, const Pack<T, 4>& g,
 
 template <typename T>
 __device__ __forceinline__ void adamw32_block(const MuonAdamWDesc& d, int64_t base, float c, const AdamWArgs& a) {
-    constexpr int PACKS = AW_EACH / 4;
+    constexpr int PACKS = AW_EACH / 4, ELEMS = AW_THREADS * AW_EACH;
     const int64_t numel = d.numel;
     T* __restrict__ const p = static_cast<T*>(d.param);
     const T* __restrict__ const g = static_cast<const T*>(d.grad);
     float* __restrict__ const m = static_cast<float*>(d.exp_avg);
     float* __restrict__ const v = static_cast<float*>(d.exp_avg_sq);
-    if (base + AW_BLOCK_ELEMS <= numel) {
+    if (base + ELEMS <= numel) {
         Pack<T, 4> pv[PACKS], gv[PACKS];
         Pack<float, 4> mv[PACKS], vv[PACKS];
 #pragma unroll
@@ -120,7 +127,7 @@ __device__ __forceinline__ void adamw32_block(const MuonAdamWDesc& d, int64_t ba
         return;
     }
 #pragma unroll 1
-    for (int64_t e = base + threadIdx.x * 4; e < numel; e += AW_THREADS * 4) {
+    for (int64_t e = base + threadIdx.x * 4; e < numel && e < base + ELEMS; e += AW_THREADS * 4) {
         Pack<T, 4> pv = load_pack<T, 4, true>(p, e, numel);
         const Pack<T, 4> gv = load_pack<T, 4, true>(g, e, numel);
         Pack<float, 4> mv = load_pack<float, 4, true>(m, e, numel), vv = load_pack<float, 4, true>(v, e, numel);
@@ -146,9 +153,10 @@ __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(const MuonAdamWDesc
                                                             const float* __restrict__ grad_scale, const float* __restrict__ sc) {
     const AdamWArgs a = read_args(args, sc);
     const float c = grad_scale ? *grad_scale : 1.f;
-    const int b = blockIdx.x, ti = find_segment_wave(prefix, ntensors, b);
+    constexpr int PARTS = workgroups_per_block(AW_EACH);
+    const int b = blockIdx.x / PARTS, ti = find_segment_wave(prefix, ntensors, b);
     const MuonAdamWDesc d = descs[ti];
-    const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS;
+    const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS + blockIdx.x % PARTS * (AW_THREADS * AW_EACH);
     with_type<DTYPE>(d, [&](auto t) { adamw32_block<decltype(t)>(d, base, c, a); });
 }
 
@@ -216,55 +224,67 @@ __device__ __forceinline__ void decode_v(const Codes<G>& c, int E, float (&v)[G]
     for (int k = 0; k < G; ++k) v[k] = ldexpf(__uint_as_float(((c.w[k >> 2] >> (8 * (k & 3))) & 0xffu) << 20), E - 31);
 }
 
+// The top bytes of four words, in their order.
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t (&w)[4]) {
+    return __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0703u) | __builtin_amdgcn_perm(w[3], w[2], 0x07030c0cu);
+}
+
 // One pack: parameters and moments after the step, the new codes, and the new shared exponents of its block, which is
 // that of 128 / G lanes (every lane of the wave calls this; what is beyond the tensor is zero).
-template <typename T, int G>
+// Its arithmetic (about 40 instructions an element) takes nearly as long as bf16 parameters take to move: so codes are rounded where they end up in the top
+// byte of a word (the magnitude's bits and the dither's, both four bits higher than the code's own place), four of
+// which two byte permutations collect, and zeros among the codes of v are looked for four at a time.
+template <typename T, int G, bool NEAR>
 __device__ __forceinline__ void adamw8_pack(Pack<T, G>& p, const Pack<T, G>& g, Codes<G>& mc, Codes<G>& vc, int& Em, int& Ev,
                                             uint32_t i0, float c, const AdamWArgs& a) {
     float m[G], v[G], pn[G];
     decode_m<G>(mc, Em, m);
     decode_v<G>(vc, Ev, v);
     const float poison = max(Em, Ev) == 255 ? __builtin_nanf("") : 0.f;
-    uint32_t most_m = 0, most_v = 0;
+    float most_m = 0.f;
+    uint32_t most_v = 0;
 #pragma unroll
     for (int k = 0; k < G; ++k) {
         const float gk = fmaf(g[k], c, poison);
-        moments(m[k], v[k], gk, a);
-        most_m = max(most_m, __float_as_uint(m[k]) & 0x7fffffffu);
-        most_v = max(most_v, __float_as_uint(v[k]) & 0x7fffffffu);
+        moments<NEAR>(m[k], v[k], gk, a);
+        most_m = fmaxf(most_m, fabsf(m[k]));
+        most_v = max(most_v, __float_as_uint(v[k]));         // (the bits, so that NaN counts; m is not finite only where v is not)
         const float denominator = fmaf(__builtin_amdgcn_sqrtf(v[k]), a.rsqrt_bias2, a.eps);
         pn[k] = fmaf(a.neg_lr, m[k] * __builtin_amdgcn_rcpf(denominator), p[k] * a.wd_factor);
     }
     p = Pack<T, G>::of(pn);
     // exponent fields, one more where three bits of mantissa are not enough below the next power (m: 1.75 is the last)
-    const uint32_t both = lanes_max2<AW_SHARED / G>(((most_m + 0x1fffffu) >> 23) | ((most_v + 0xfffffu) >> 23 << 16));
+    const uint32_t both = lanes_max2<AW_SHARED / G>(((__float_as_uint(most_m) + 0x1fffffu) >> 23) | ((most_v + 0xfffffu) >> 23 << 16));
     Em = static_cast<int>(both & 0xffffu);
     Ev = static_cast<int>(both >> 16);
     if (max(Em, Ev) >= 255) Em = Ev = 255;
     uint32_t h32 = i0 * DITHER_I + a.dither;
 #pragma unroll
     for (int h = 0; h < G / 4; ++h) {
-        uint32_t cm = 0, cv = 0;
+        uint32_t sm[4], sv[4], signs[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float mk = m[4 * h + k], vk = v[4 * h + k];
-            const uint32_t ym = __float_as_uint(ldexpf(fabsf(mk), 15 - Em));
-            const uint32_t yv = __float_as_uint(ldexpf(vk, 31 - Ev));
             const uint32_t x = (h32 ^ (h32 >> 15)) & 0xffffffu;
-            const uint32_t qm = ((ym + (x * DITHER_M >> 12)) >> 20) | ((__float_as_uint(mk) >> 24) & 0x80u);
-            const uint32_t qv = max((yv + (x * DITHER_V >> 12)) >> 20, min(__float_as_uint(vk), 1u));
-            cm |= qm << (8 * k);
-            cv |= qv << (8 * k);
+            // (the bits of a product below the dither's 20 change no code: they end below the magnitude's lowest)
+            sm[k] = (__float_as_uint(ldexpf(fabsf(mk), 15 - Em)) << 4) + (x * DITHER_M >> 8);
+            sv[k] = (__float_as_uint(ldexpf(vk, 31 - Ev)) << 4) + (x * DITHER_V >> 8);
+            signs[k] = __float_as_uint(mk);
             h32 += DITHER_I;
         }
-        mc.w[h] = cm;
+        mc.w[h] = top_bytes(sm) | (top_bytes(signs) & 0x80808080u);
+        uint32_t cv = top_bytes(sv);
+        if ((cv - 0x01010101u) & ~cv & 0x80808080u)           // a code is zero: the least one unless v is zero itself
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (!(cv >> (8 * k) & 0xffu) && v[4 * h + k] != 0.f) cv |= 1u << (8 * k);
         vc.w[h] = cv;
     }
 }
 
-template <typename T>
+template <typename T, int EACH, bool NEAR>
 __device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t base, float c, const AdamWArgs& a) {
-    constexpr int G = pack_of<T>, PACKS = AW_EACH / G, LANES = AW_SHARED / G;
+    constexpr int G = pack_of<T>, PACKS = EACH / G, LANES = AW_SHARED / G, ELEMS = AW_THREADS * EACH;
     const int64_t numel = d.numel;
     T* __restrict__ const p = static_cast<T*>(d.param);
     const T* __restrict__ const g = static_cast<const T*>(d.grad);
@@ -272,7 +292,7 @@ __device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t bas
     uint8_t* __restrict__ const v = static_cast<uint8_t*>(d.exp_avg_sq);
     uint8_t* __restrict__ const me = d.exp_avg_exponent;
     uint8_t* __restrict__ const ve = d.exp_avg_sq_exponent;
-    if (base + AW_BLOCK_ELEMS <= numel) {
+    if (base + ELEMS <= numel) {
         Pack<T, G> pv[PACKS], gv[PACKS];
         Codes<G> mv[PACKS], vv[PACKS];
         int Em[PACKS], Ev[PACKS];
@@ -289,7 +309,7 @@ __device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t bas
 #pragma unroll
         for (int i = 0; i < PACKS; ++i) {
             const int64_t e = base + (i * AW_THREADS + threadIdx.x) * G;
-            adamw8_pack<T, G>(pv[i], gv[i], mv[i], vv[i], Em[i], Ev[i], static_cast<uint32_t>(e), c, a);
+            adamw8_pack<T, G, NEAR>(pv[i], gv[i], mv[i], vv[i], Em[i], Ev[i], static_cast<uint32_t>(e), c, a);
             mv[i].store(m + e);
             vv[i].store(v + e);
             pv[i].template store<true>(p + e);
@@ -301,14 +321,14 @@ __device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t bas
         return;
     }
 #pragma unroll 1
-    for (int64_t at = base; at < numel; at += AW_THREADS * G) {      // (the wave stays whole: its lanes exchange maxima)
+    for (int64_t at = base; at < numel && at < base + ELEMS; at += AW_THREADS * G) {      // (the wave stays whole: its lanes exchange maxima)
         const int64_t e = at + threadIdx.x * G;
         const bool any = e < numel;
         int Em = any ? me[e / AW_SHARED] : 0, Ev = any ? ve[e / AW_SHARED] : 0;
         Codes<G> mv = Codes<G>::load(m, e, numel), vv = Codes<G>::load(v, e, numel);
         Pack<T, G> pv = load_pack<T, G, true>(p, e, numel);
         const Pack<T, G> gv = load_pack<T, G, true>(g, e, numel);
-        adamw8_pack<T, G>(pv, gv, mv, vv, Em, Ev, static_cast<uint32_t>(e), c, a);
+        adamw8_pack<T, G, NEAR>(pv, gv, mv, vv, Em, Ev, static_cast<uint32_t>(e), c, a);
         mv.store(m, e, numel);
         vv.store(v, e, numel);
         store_pack<T, G, true>(p, e, numel, pv);
@@ -319,25 +339,31 @@ __device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t bas
     }
 }
 
+constexpr int adamw8_each(int dtype) { return dtype == MUON_AMD_SRC_BF16 ? AW_EACH : AW8_EACH_F32; }
 template <int DTYPE>
 __global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(const MuonAdamWDesc* __restrict__ descs,
                                                            const int32_t* __restrict__ prefix, int ntensors, AdamWArgs args,
                                                            const float* __restrict__ grad_scale, const float* __restrict__ sc) {
     const AdamWArgs a = read_args(args, sc);
     const float c = grad_scale ? *grad_scale : 1.f;
-    const int b = blockIdx.x, ti = find_segment_wave(prefix, ntensors, b);
+    constexpr int EACH = adamw8_each(DTYPE), PARTS = workgroups_per_block(EACH);
+    const int b = blockIdx.x / PARTS, ti = find_segment_wave(prefix, ntensors, b);
     const MuonAdamWDesc d = descs[ti];
-    const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS;
-    with_type<DTYPE>(d, [&](auto t) { adamw8_block<decltype(t)>(d, base, c, a); });
+    const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS + blockIdx.x % PARTS * (AW_THREADS * EACH);
+    with_type<DTYPE>(d, [&](auto t) {
+        if (near_weights(a)) adamw8_block<decltype(t), EACH, true>(d, base, c, a);
+        else adamw8_block<decltype(t), EACH, false>(d, base, c, a);
+    });
 }
 
 // The values of 8-bit states in bf16, which holds each of them exactly down to the least one that it has (three bits of
 // mantissa; only blocks below 2^-100 reach bf16's own subnormal numbers).
 __global__ __launch_bounds__(AW_THREADS) void adamw_values_kernel(const MuonAdamWValuesDesc* __restrict__ descs,
                                                                  const int32_t* __restrict__ prefix, int ntensors) {
-    const int b = blockIdx.x, ti = find_segment_wave(prefix, ntensors, b);
+    constexpr int PARTS = workgroups_per_block(AW_EACH);
+    const int b = blockIdx.x / PARTS, ti = find_segment_wave(prefix, ntensors, b);
     const MuonAdamWValuesDesc d = descs[ti];
-    const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS, numel = d.numel;
+    const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS + blockIdx.x % PARTS * (AW_THREADS * AW_EACH), numel = d.numel;
 #pragma unroll
     for (int i = 0; i < AW_EACH / 8; ++i) {
         const int64_t e = base + (i * AW_THREADS + threadIdx.x) * 8;
@@ -423,7 +449,9 @@ int muon_amd_adamw(const MuonAdamWDesc* descs_dev, const int32_t* block_prefix_d
     const auto kernel = state_bits == 8
                             ? pick(adamw8_kernel<MUON_AMD_SRC_F32>, adamw8_kernel<MUON_AMD_SRC_BF16>, adamw8_kernel<AW_MIXED>)
                             : pick(adamw32_kernel<MUON_AMD_SRC_F32>, adamw32_kernel<MUON_AMD_SRC_BF16>, adamw32_kernel<AW_MIXED>);
-    hipLaunchKernelGGL(kernel, dim3(nblocks), dim3(AW_THREADS), 0, static_cast<hipStream_t>(stream), descs_dev, block_prefix_dev,
+    const int parts = workgroups_per_block(state_bits == 8 ? adamw8_each(dtype) : AW_EACH);
+    MUON_REQUIRE(nblocks <= INT32_MAX / parts, "adamw: nblocks=%d", nblocks);
+    hipLaunchKernelGGL(kernel, dim3(nblocks * parts), dim3(AW_THREADS), 0, static_cast<hipStream_t>(stream), descs_dev, block_prefix_dev,
                        ntensors, a, grad_scale_dev, scalars_dev);
     return check_launch("adamw");
 }
@@ -432,7 +460,8 @@ int muon_amd_adamw_values(const MuonAdamWValuesDesc* descs_dev, const int32_t* b
                           void* stream) {
     MUON_REQUIRE(descs_dev && block_prefix_dev, "adamw_values: null table");
     MUON_REQUIRE(ntensors > 0 && nblocks > 0, "adamw_values: ntensors=%d nblocks=%d", ntensors, nblocks);
-    hipLaunchKernelGGL(adamw_values_kernel, dim3(nblocks), dim3(AW_THREADS), 0, static_cast<hipStream_t>(stream), descs_dev,
+    MUON_REQUIRE(nblocks <= INT32_MAX / workgroups_per_block(AW_EACH), "adamw_values: nblocks=%d", nblocks);
+    hipLaunchKernelGGL(adamw_values_kernel, dim3(nblocks * workgroups_per_block(AW_EACH)), dim3(AW_THREADS), 0, static_cast<hipStream_t>(stream), descs_dev,
                        block_prefix_dev, ntensors);
     return check_launch("adamw_values");
 }

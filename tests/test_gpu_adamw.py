@@ -136,7 +136,7 @@ def make(sizes, dtype, seed=0, offset=0, gstd=1e-3):
     return params
 
 
-SIZES = [[1], [7, 8, 9], [127, 128, 129, 255], [(3, 5), 0, 8191, (8, 1024), 8193], [(129, 257), 16384 + 5]]
+SIZES = [[1], [7, 8, 9], [127, 128, 129, 255], [4095, 4096, 4097], [(3, 5), 0, 8191, (8, 1024), 8193], [(129, 257), 16384 + 5]]
 
 
 @gpu
