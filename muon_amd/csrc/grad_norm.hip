@@ -26,8 +26,7 @@ __device__ __forceinline__ double block_sum(double v, double (&waves)[THREADS / 
 
 // Calls f(tensor, first element there) for a workgroup's share of the table's blocks, every gridDim.x-th: workgroups that
 // run together then read next to each other (a contiguous share for each took 10 % longer over 531 M bf16 gradients).
-// The tensor is looked up once and followed from there.  (From the last block to
-// the first, to find what the pass before read last in the cache, gained nothing.)
+// The tensor is looked up once and followed from there.
 template <typename F>
 __device__ __forceinline__ void for_blocks(const MuonGradDesc* __restrict__ descs, const int32_t* __restrict__ prefix, int ntensors,
                                            int nblocks, F&& f) {
@@ -109,38 +108,58 @@ __global__ __launch_bounds__(GN_JOIN) void grad_norm_kernel(const double* __rest
     }
 }
 
+// A workgroup scales a part of a block, whose loads all go out first (531 M bf16 gradients: 326 us; whole blocks 336, quarters 391,
+// and 4096 workgroups that stride over the blocks 358).
+constexpr int GN_PARTS = 2, GN_PART_ELEMS = GN_BLOCK_ELEMS / GN_PARTS;
 template <typename T>
-__device__ __forceinline__ void scale_block(const MuonGradDesc& d, int64_t base, float c) {
+__device__ __forceinline__ void scale_part(const MuonGradDesc& d, int64_t base, float c) {
     T* __restrict__ const g = static_cast<T*>(d.grad);
-    constexpr int G = pack_of<T>, PACKS = GN_EACH / G;
-    Pack<T, G> gv[PACKS];
-#pragma unroll
-    for (int i = 0; i < PACKS; ++i) gv[i] = load_pack<T, G, true>(g, base + (i * GN_THREADS + threadIdx.x) * G, d.numel);
-#pragma unroll
-    for (int i = 0; i < PACKS; ++i) {
+    constexpr int G = pack_of<T>, PACKS = GN_PART_ELEMS / GN_THREADS / G;
+    const auto scaled = [&](const Pack<T, G>& v) {
         float x[G];
 #pragma unroll
-        for (int k = 0; k < G; ++k) x[k] = gv[i][k] * c;
-        store_pack<T, G, true>(g, base + (i * GN_THREADS + threadIdx.x) * G, d.numel, Pack<T, G>::of(x));
+        for (int k = 0; k < G; ++k) x[k] = v[k] * c;
+        return Pack<T, G>::of(x);
+    };
+    if (base + GN_PART_ELEMS <= d.numel) {
+        Pack<T, G> v[PACKS];
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) v[i] = Pack<T, G>::template load<true>(g + base + (i * GN_THREADS + threadIdx.x) * G);
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) scaled(v[i]).template store<true>(g + base + (i * GN_THREADS + threadIdx.x) * G);
+        return;
     }
+#pragma unroll 1
+    for (int64_t e = base + threadIdx.x * G; e < d.numel && e < base + GN_PART_ELEMS; e += GN_THREADS * G)
+        store_pack<T, G, true>(g, e, d.numel, scaled(load_pack<T, G, true>(g, e, d.numel)));
 }
 
-// Every workgroup forms the coefficient from the partial sums (32 KB, from the L2), which saves a launch between the
-// two passes; it leaves at once where nothing is to be scaled.
+// JOIN: every workgroup forms the coefficient from the partial sums (8 bytes for each block, from the L2) instead of
+// a launch between the two passes.  Up to 8 M gradients that is faster whether they are then scaled or not (bf16, scaled: 1 M 8.2 ->
+// 6.7 us, 8 M 16.7 -> 15.5, 64 M 65 -> 72; fp32, not scaled: 1 M 6.6 -> 5.3, 8 M 9.5 -> 8.6, 16 M 17.7 -> 18.9, 64 M 54 -> 76).
+constexpr int GN_JOINED = 1024;            // blocks
+template <bool JOIN>
 __global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const MuonGradDesc* __restrict__ descs,
-                                                               const int32_t* __restrict__ prefix, int ntensors, int nblocks,
+                                                               const int32_t* __restrict__ prefix, int ntensors,
                                                                const double* __restrict__ partials, int n, float max_norm,
                                                                float* __restrict__ out) {
-    const float norm = norm_of<GN_THREADS>(partials, n), c = coefficient_of(norm, max_norm);
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        out[0] = norm;
-        out[1] = c;
+    float c;
+    if constexpr (JOIN) {
+        const float norm = norm_of<GN_THREADS>(partials, n);
+        c = coefficient_of(norm, max_norm);
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            out[0] = norm;
+            out[1] = c;
+        }
+    } else {
+        c = out[1];
     }
-    if (c == 1.f) return;
-    for_blocks(descs, prefix, ntensors, nblocks, [&](const MuonGradDesc& d, int64_t base) {
-        if (d.dtype == MUON_AMD_SRC_BF16) scale_block<uint16_t>(d, base, c);
-        else scale_block<float>(d, base, c);
-    });
+    if (c == 1.f) return;                 // (a coefficient that is not a number goes on)
+    const int b = blockIdx.x / GN_PARTS, ti = find_segment_wave(prefix, ntensors, b);
+    const MuonGradDesc d = descs[ti];
+    const int64_t base = static_cast<int64_t>(b - prefix[ti]) * GN_BLOCK_ELEMS + blockIdx.x % GN_PARTS * GN_PART_ELEMS;
+    if (d.dtype == MUON_AMD_SRC_BF16) scale_part<uint16_t>(d, base, c);
+    else scale_part<float>(d, base, c);
 }
 
 }  // namespace muon_amd
@@ -173,6 +192,7 @@ static int grad_squares(const MuonGradDesc* descs_dev, const int32_t* prefix_dev
                         float max_norm, const float* out_dev, hipStream_t stream) {
     MUON_REQUIRE(descs_dev && prefix_dev && partials_dev && out_dev, "grad_norm: null table, workspace or output");
     MUON_REQUIRE(ntensors > 0 && nblocks > 0, "grad_norm: ntensors=%d nblocks=%d", ntensors, nblocks);
+    MUON_REQUIRE(nblocks <= INT32_MAX / GN_PARTS, "grad_norm: nblocks=%d", nblocks);
     MUON_REQUIRE(max_norm >= 0.f, "grad_norm: max_norm=%g", max_norm);
     const auto kernel = static_cast<int64_t>(nblocks) * GN_BLOCK_ELEMS > GN_CACHED ? grad_squares_kernel<true> : grad_squares_kernel<false>;
     hipLaunchKernelGGL(kernel, dim3(nblocks < GN_PARTIALS ? nblocks : GN_PARTIALS), dim3(GN_THREADS), 0, stream,
@@ -194,8 +214,13 @@ int muon_amd_grad_clip(const MuonGradDesc* descs_dev, const int32_t* block_prefi
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (const int rc = grad_squares(descs_dev, block_prefix_dev, ntensors, nblocks, partials_dev, max_norm, out_dev, s)) return rc;
     const int n = nblocks < GN_PARTIALS ? nblocks : GN_PARTIALS;
-    hipLaunchKernelGGL(grad_scale_kernel, dim3(n), dim3(GN_THREADS), 0, s, descs_dev, block_prefix_dev, ntensors, nblocks, partials_dev,
-                       n, max_norm, out_dev);
+    const bool join = nblocks <= GN_JOINED;
+    if (!join) {
+        hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(GN_JOIN), 0, s, partials_dev, n, max_norm, out_dev);
+        if (const int rc = check_launch("grad_norm")) return rc;
+    }
+    hipLaunchKernelGGL(join ? grad_scale_kernel<true> : grad_scale_kernel<false>, dim3(nblocks * GN_PARTS), dim3(GN_THREADS), 0, s, descs_dev,
+                       block_prefix_dev, ntensors, partials_dev, n, max_norm, out_dev);
     return check_launch("grad_clip");
 }
 

@@ -46,7 +46,7 @@ def check(params, max_norm, in_place):
 @gpu
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("offset", [0, 1, 3])
-@pytest.mark.parametrize("sizes", [[1], [7, 8, 9], [8191, 8192, 8193, 5], [1 << 20, 3, 70001]], ids=str)
+@pytest.mark.parametrize("sizes", [[1], [7, 8, 9], [4095, 4096, 4097], [8191, 8192, 8193, 5], [1 << 20, 3, 70001]], ids=str)
 @pytest.mark.parametrize("types", ["fp32", "bf16", "both"])
 def test_norm_and_clip(types, sizes, offset, in_place):
     kinds = {"fp32": [torch.float32], "bf16": [torch.bfloat16], "both": [torch.bfloat16, torch.float32]}[types]
