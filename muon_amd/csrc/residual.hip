@@ -12,9 +12,11 @@
 //   D c2 = sum(e k sig nb) - rh c1 sum(nh k sig nb)
 // so that a row takes one reduction; the gradient of a gate for the whole row is (1 - sig) D c2.
 //
-// Memory bounds both passes.  A row stays in the registers of TPR threads (one wave up to 1024 channels forward, 512
-// backward: no barrier), 16 bytes of the residual stream per access; a workgroup takes row after row with the weights of its channels, and
-// backward their sums, held in registers, and the workgroups' sums are joined in a fixed order by a second launch.
+// Memory bounds both passes (16384 x 4096 bf16 with a gate per element: forward 119 us, 5.6 TB/s; backward 195 us, 5.5 TB/s; their
+// bytes at 6.5 TB/s: 103 and 165).  Backward is at the registers' limit: the next row ahead of time spills, fewer registers
+// recompute.  A row stays in the registers of TPR threads (one wave up to 1024 channels forward, 512
+// backward: no barrier), 16 bytes of the residual stream per access; a workgroup takes row after row with the weights of
+// its channels in LDS and, backward, their sums in registers; the workgroups' sums are joined in a fixed order by a second launch (7 us).
 #include <type_traits>
 
 #include "vector.h"
@@ -141,7 +143,7 @@ struct Weights {
 };
 
 // A result that is larger than what the memory-side cache keeps of a launch goes out with the non-temporal hint, so that it
-// does not push out what is still to be read: 16384 x 4096 bf16 128 -> 121 us forward and 205 -> 197 backward; with everything
+// does not push out what is still to be read: 16384 x 4096 bf16 6 % longer without the hint forward and 4 % backward; with everything
 // in the cache the hint costs (8192 x 2048: 26.2 -> 28.6 and 39.9 -> 42.5 us).
 constexpr int64_t RN_CACHE = 256ll << 20;
 template <typename T, int G>
@@ -458,6 +460,14 @@ static int workgroups(int64_t rows, int rows_each, int per_cu) {
     const int64_t n = (rows + rows_each - 1) / rows_each;
     return static_cast<int>(n < 256 * per_cu ? n : 256 * per_cu);
 }
+// Forward: as many as fit the CUs at once, and up to four times that where each still takes four rows for
+// each row's threads, to be worth the weights that it loads: 32768 x 4096 bf16 243 -> 231 us, 32768 x 2048 126 -> 119, 16384 x 4096
+// 122 -> 119.  Rows of more than 256 threads, whose weights are many: 16384 x 5120 166 -> 173, so not there.
+static int forward_workgroups(int64_t rows, int threads, int tpr) {
+    const int each = threads / tpr, per_cu = 2048 / threads;
+    const int once = workgroups(rows, each, per_cu), most = tpr > RN_THREADS ? 0 : workgroups(rows, 4 * each, 4 * per_cu);
+    return once > most ? once : most;
+}
 static int backward_workgroups(int64_t rows, int width) {
     int n = 0;
     with_backward_shape(width, [&](auto s) {
@@ -503,7 +513,7 @@ int muon_amd_residual_norm(const MuonResidualNorm* args, void* stream) {
         with_forward_shape(a.width, [&](auto s) {
             constexpr int TPR = decltype(s)::TPR, G = pack_of<decltype(x)>, V = 8 / G * decltype(s)::EIGHTS, THREADS = TPR > RN_THREADS ? TPR : RN_THREADS;
             hipLaunchKernelGGL((residual_forward_kernel<decltype(x), decltype(b), decltype(gate)::value, TPR, V, G>),
-                               dim3(workgroups(a.rows, THREADS / TPR, 2048 / THREADS)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a, nt);
+                               dim3(forward_workgroups(a.rows, THREADS, TPR)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a, nt);
         });
     });
     return check_launch("residual_norm");

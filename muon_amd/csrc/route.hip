@@ -10,6 +10,8 @@
 // to be found is the k largest: one 32-bit key holds a bf16 logit (in the order of its value) above the complement of
 // its index, so that the largest key is the largest logit at the lowest index; for fp32 logits the key has 64 bits.  The
 // largest key below the last one found follows from one wrapping subtraction and one maximum per element.
+// Instructions bound both passes where there are many experts (65536 tokens, 8 of 256, bf16: 26 us forward for 38 MB, about half
+// of it the eight maxima; 25 us backward for 74 MB), launches where there are few (1024 tokens, 2 of 8: 5.4, 3.6 and 4.8 us).
 // Sums over tokens: each lane adds the probabilities of its experts over its rows, a workgroup joins its lanes in a
 // fixed order, and a second launch joins the workgroups; counts are whole numbers, in any order the same.
 #include <type_traits>
