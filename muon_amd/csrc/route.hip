@@ -11,7 +11,7 @@
 // its index, so that the largest key is the largest logit at the lowest index; for fp32 logits the key has 64 bits.  The
 // largest key below the last one found follows from one wrapping subtraction and one maximum per element.
 // Instructions bound both passes where there are many experts (65536 tokens, 8 of 256, bf16: 26 us forward for 38 MB, about half
-// of it the eight maxima; 25 us backward for 74 MB), launches where there are few (1024 tokens, 2 of 8: 5.4, 3.6 and 4.8 us).
+// of it the eight maxima; 21 us backward for 74 MB), launches where there are few (1024 tokens, 2 of 8: 4.4, 3.6 and 4.4 us).
 // Sums over tokens: each lane adds the probabilities of its experts over its rows, a workgroup joins its lanes in a
 // fixed order, and a second launch joins the workgroups; counts are whole numbers, in any order the same.
 #include <type_traits>
@@ -64,16 +64,29 @@ __device__ __forceinline__ T group_reduce(T v, F&& f) {
     if constexpr (L >= 64) v = joined<false>(v, f);
     return v;
 }
+// The sum over the lanes of a wave that have the same place in groups of L lanes, in every one of them.
+template <int L>
+__device__ __forceinline__ float sum_of_groups(float v) {
+    if constexpr (L <= 1) v += moved<0xB1>(v);
+    if constexpr (L <= 2) v += moved<0x4E>(v);
+    if constexpr (L <= 4) v += moved<0x124>(v);                  // row_ror:4
+    if constexpr (L <= 8) v += moved<0x128>(v);                  // row_ror:8
+    const auto sum = [](float a, float b) { return a + b; };
+    if constexpr (L <= 16) v = joined<true>(v, sum);
+    if constexpr (L <= 32) v = joined<false>(v, sum);
+    return v;
+}
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {
     return group_reduce<L>(v, [](float a, float b) { return a + b; });
 }
 
-// e^d for d at most 0 (or not a number): 2^(d log2 e) by the target's instruction, with what the product lost put back, so
-// about two units off over the whole range.
+// e^d for d at most 0: 2^(d log2 e) by the target's instruction, with what the product lost put back, so
+// about two units off over the whole range.  Not a number gives zero like -infinity: what a row with such a logit, or with
+// +infinity, returns then follows from its sum of zero (1 / 0 times 0) or from its lse, neither of which is a number.
 __device__ __forceinline__ float exp_of(float d) {
     constexpr float L = 1.44269504088896341f, LN2 = 0.69314718055994531f;
-    d = d < -200.f ? -200.f : d;                                 // (e^-200 is zero; -infinity would leave no number in `lost`)
+    d = fmaxf(d, -200.f);                                        // (e^-200 is zero; -infinity would leave no number in `lost`)
     const float t = d * L, lost = fmaf(d, L, -t), e = __builtin_amdgcn_exp2f(t);
     return fmaf(e * LN2, lost, e);
 }
@@ -178,7 +191,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_forward_kernel(const MuonRou
             best += group_reduce<L>(m, larger);
             if (j == 0) {
                 on = in && K::available(best);
-                top = K::value(best);
+                top = on ? K::value(best) : 0.f;
             }
             if (lane == j % L) mine = best;
             if (j % L != L - 1 && j != a.k - 1) continue;
@@ -194,11 +207,11 @@ __global__ __launch_bounds__(RT_THREADS) void route_forward_kernel(const MuonRou
                 if (j != a.k - 1) a.weights[o] = my_part;
             }
         }
-        // softmax over the row
+        // softmax over the row (zeros where it takes no part: all of x is -infinity)
         float ex[N], total = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            ex[i] = on ? exp_of(x[i] - top) : 0.f;
+            ex[i] = exp_of(x[i] - top);
             total += ex[i];
         }
         total = group_sum<L>(total);
@@ -220,8 +233,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_forward_kernel(const MuonRou
     // join the workgroup's rows: those of a wave, then the waves
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-#pragma unroll
-        for (int m = L; m < 64; m <<= 1) acc[i] += __shfl_xor(acc[i], m, 64);
+        acc[i] = sum_of_groups<L>(acc[i]);
         if ((threadIdx.x & 63) < L) sums[threadIdx.x >> 6][base + i] = acc[i];
     }
     square = group_sum<64>(square);
@@ -342,7 +354,7 @@ __device__ __forceinline__ void wave_order() {
 }
 
 constexpr int RB_THREADS = 256;
-constexpr int RB_GROUPS = 1024;            // workgroups: four for each CU (65536 x 256: 25 us; 1536: 28, 3072: 37; each is set up once)
+constexpr int RB_GROUPS = 1024;            // workgroups: four for each CU, each set up once (65536 x 256: 20.8 us; 1536: 20.6, 2048: 22)
 template <typename T, int N, int L>
 __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRoute a) {
     constexpr int ROWS = RB_THREADS / L, G = pack_of<T>;
@@ -356,7 +368,9 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
     const float cz = a.dz ? *a.dz * 2.f / n : 0.f;
     float g[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) g[i] = base + i < E ? cb * static_cast<float>(a.counts[base + i]) : 0.f;
+    for (int i = 0; i < N; ++i) g[i] = static_cast<float>(a.counts[base + i < E ? base + i : E - 1]);       // (all requested together)
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] = base + i < E ? cb * g[i] : 0.f;
 #pragma unroll
     for (int q = 0; q < N / 4; ++q) extra[sub][q * L + lane] = f32x4v{0.f, 0.f, 0.f, 0.f};
     wave_order();
@@ -379,8 +393,8 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
     fetch(begin);
     for (int64_t t = begin; t - sub < a.tokens; t += step) {
         RowPacks<T, N> packs = next;
-        const float lse = next_lse, w = next_w, dw = next_dw;
-        const bool on = t < a.tokens && lse != -__builtin_inff();
+        const bool on = t < a.tokens && next_lse != -__builtin_inff();
+        const float lse = on ? next_lse : 0.f, w = next_w, dw = next_dw;
         const int mine = on ? next_e : -1;
         fetch(t + step);
         // The weights' part; lanes of the row take the k choices in turn.
@@ -406,7 +420,7 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            p[i] = on ? exp_of(x[i] - lse) : 0.f;
+            p[i] = exp_of(x[i] - lse);             // (zero where the token takes no part: x is -infinity)
             dot = fmaf(p[i], g[i], dot);
             if (!a.normalize) dot += u[i];         // p dw: what comes through the probabilities themselves
         }
@@ -446,6 +460,16 @@ static void with_route_shape(int experts, F&& f) {
     else if (experts <= 512) f(RouteShape<16, 32>{});
     else f(RouteShape<16, 64>{});
 }
+// Forward 16 elements for each lane keep the reductions short (65536 x 256 26 us; 8 elements 29, 32 elements 31); backward, with
+// one reduction, 8 leave room for twice the waves (21 us; 16 elements 23, 32 elements 29).
+template <typename F>
+static void with_route_backward_shape(int experts, F&& f) {
+    if (experts <= 64) with_route_shape(experts, f);
+    else if (experts <= 128) f(RouteShape<8, 16>{});
+    else if (experts <= 256) f(RouteShape<8, 32>{});
+    else if (experts <= 512) f(RouteShape<8, 64>{});
+    else f(RouteShape<16, 64>{});
+}
 static int route_groups(int64_t tokens, int experts) {
     int rows = 1;
     with_route_shape(experts, [&](auto s) { rows = RT_THREADS / decltype(s)::L; });
@@ -465,11 +489,9 @@ static int check_route(const MuonRoute* a, const char* what) {
 
 
 template <typename F>
-static void with_route(const MuonRoute& a, F&& f) {
-    with_route_shape(a.experts, [&](auto s) {
-        if (a.dtype == MUON_AMD_SRC_BF16) f(uint16_t{}, s);
-        else f(float{}, s);
-    });
+static void with_route_type(int dtype, F&& f) {
+    if (dtype == MUON_AMD_SRC_BF16) f(uint16_t{});
+    else f(float{});
 }
 
 }  // namespace muon_amd
@@ -493,8 +515,10 @@ int muon_amd_route(const MuonRoute* args, void* stream) {
     MUON_REQUIRE(a.partials && a.balance && a.z, "route: null workspace or output");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const int n = route_groups(a.tokens, a.experts);
-    with_route(a, [&](auto x, auto s) {
-        hipLaunchKernelGGL((route_forward_kernel<decltype(x), decltype(s)::N, decltype(s)::L>), dim3(n), dim3(RT_THREADS), 0, st, a);
+    with_route_type(a.dtype, [&](auto x) {
+        with_route_shape(a.experts, [&](auto s) {
+            hipLaunchKernelGGL((route_forward_kernel<decltype(x), decltype(s)::N, decltype(s)::L>), dim3(n), dim3(RT_THREADS), 0, st, a);
+        });
     });
     if (const int rc = check_launch("route")) return rc;
     hipLaunchKernelGGL(route_join_kernel, dim3((a.experts + RJ_EXPERTS - 1) / RJ_EXPERTS), dim3(RJ_THREADS), 0, st, a, n);
@@ -505,11 +529,13 @@ int muon_amd_route_backward(const MuonRoute* args, void* stream) {
     if (const int rc = check_route(args, "route_backward")) return rc;
     const MuonRoute a = *args;
     MUON_REQUIRE(a.dlogits, "route_backward: null output");
-    with_route(a, [&](auto x, auto s) {
-        constexpr int ROWS = RB_THREADS / decltype(s)::L;
-        const int64_t n = (a.tokens + ROWS - 1) / ROWS;
-        hipLaunchKernelGGL((route_backward_kernel<decltype(x), decltype(s)::N, decltype(s)::L>), dim3(n < RB_GROUPS ? n : RB_GROUPS),
-                           dim3(RB_THREADS), 0, static_cast<hipStream_t>(stream), a);
+    with_route_type(a.dtype, [&](auto x) {
+        with_route_backward_shape(a.experts, [&](auto s) {
+            constexpr int ROWS = RB_THREADS / decltype(s)::L;
+            const int64_t n = (a.tokens + ROWS - 1) / ROWS;
+            hipLaunchKernelGGL((route_backward_kernel<decltype(x), decltype(s)::N, decltype(s)::L>), dim3(n < RB_GROUPS ? n : RB_GROUPS),
+                               dim3(RB_THREADS), 0, static_cast<hipStream_t>(stream), a);
+        });
     });
     return check_launch("route_backward");
 }
