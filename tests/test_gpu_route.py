@@ -162,6 +162,26 @@ def test_nan_shows_and_stays_in_its_row():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")], ids=["inf", "nan"])
+@pytest.mark.parametrize("experts", [8, 48, 200, 300])
+def test_rows_whose_softmax_is_not_a_number(experts, bad, normalize, dtype):
+    logits = torch.randn(40, experts, generator=torch.Generator().manual_seed(5)).to(dtype)
+    clean = logits.clone()
+    logits[11, 5] = bad
+    x, c = (t.to(DEV).requires_grad_() for t in (logits, clean))
+    r, q = (muon_amd.route_topk(t, 3, normalize=normalize) for t in (x, c))
+    rest = torch.arange(40) != 11
+    assert r.indices[11, 0] == 5 and torch.isnan(r.weights[11]).all() and torch.isnan(r.balance_loss) and not torch.isfinite(r.z_loss)
+    assert torch.equal(r.weights[rest], q.weights[rest]) and torch.equal(r.indices[rest], q.indices[rest])
+    up = torch.ones_like(r.weights)
+    up[:, 0] = 2.0
+    g, h = (torch.autograd.grad(t.weights, u, up)[0] for t, u in ((r, x), (q, c)))
+    assert torch.isnan(g[11]).all() and torch.equal(g[rest], h[rest])
+
+
+@gpu
 def test_strides_dimensions_and_addresses():
     for dtype in (F32, BF16):
         l, m, dw = make((3, 5, 40), 4, dtype, masked=True)
