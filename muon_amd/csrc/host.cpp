@@ -537,8 +537,20 @@ class Table {
 struct GradTable {
     c10::Device device;
     std::vector<MuonGradDesc> descs;
+    bool overlap;                          // of gradients with each other
     Table table;
 };
+bool overlapping(const std::vector<MuonGradDesc>& descs) {
+    std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
+    for (const MuonGradDesc& d : descs) {
+        const uintptr_t begin = reinterpret_cast<uintptr_t>(d.grad);
+        ranges.emplace_back(begin, begin + d.numel * (d.dtype == MUON_AMD_SRC_BF16 ? 2 : 4));
+    }
+    std::sort(ranges.begin(), ranges.end());
+    for (size_t i = 1; i < ranges.size(); ++i)
+        if (ranges[i].first < ranges[i - 1].second) return true;
+    return false;
+}
 // The tables of the last gradient lists, newest first (calls hold the interpreter's lock).
 std::list<GradTable>& grad_tables() {
     static std::list<GradTable> tables;
@@ -561,13 +573,15 @@ std::tuple<Tensor, Tensor> clip_tensors(const std::vector<const Tensor*>& grads,
     if (found != tables.end()) {
         tables.splice(tables.begin(), tables, found);
     } else {
-        GradTable fresh{device, std::move(descs), {}};
+        const bool overlap = overlapping(descs);
+        GradTable fresh{device, std::move(descs), overlap, {}};
         fresh.table.upload(fresh.descs, device);
         tables.push_front(std::move(fresh));
         size_t others = 0;
         for (auto i = tables.begin(); i != tables.end();)
             i = !i->table.captured() && ++others > GRAD_TABLES ? tables.erase(i) : std::next(i);
     }
+    if (in_place && tables.front().overlap) throw py::value_error("gradients that share memory cannot be scaled in place");
     Table& table = tables.front().table;
     const auto options = at::TensorOptions().device(device);
     const Tensor out = at::empty({2}, options.dtype(at::kFloat));

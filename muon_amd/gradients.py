@@ -72,7 +72,7 @@ def clip_coefficient(parameters, max_norm: float):
 
 def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales the gradients in place so that their joint 2-norm is at most max_norm; returns the norm before that as a
-    0-dim fp32 tensor.  Gradients whose norm is small enough are not written.  error_if_nonfinite raises before anything
+    0-dim fp32 tensor.  Gradients whose norm is small enough are not written; ones that share memory are refused.  error_if_nonfinite raises before anything
     is scaled if the norm is infinite or not a number, and waits for the device to know."""
     with torch.no_grad():
         if error_if_nonfinite:

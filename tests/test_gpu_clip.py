@@ -185,3 +185,20 @@ def test_captured_calls():
         assert float(norm) == float(want[0]) and float(coefficient) == float(want[1])
         for p, g in zip(params, before):
             assert torch.equal(p.grad, (g.float() * want[1]).to(g.dtype))
+
+
+@gpu
+def test_gradients_that_share_memory():
+    params = make([1000, 1000, 500], [torch.float32] * 3)
+    params[1].grad = params[0].grad                               # counted twice by the norm; scaled twice it would be a race
+    check(params, 1e-3, False)
+    for other in (params[0].grad, params[0].grad[250:750]):
+        params[2 if other.numel() == 500 else 1].grad = other
+        before = [p.grad.clone() for p in params]
+        with pytest.raises(ValueError, match="share memory"):
+            muon_amd.clip_grad_norm_(params, 1e-3)
+        assert all(torch.equal(p.grad, g) for p, g in zip(params, before))
+        params[1].grad = params[0].grad.clone()
+    whole = torch.full((1500,), 0.5, device=DEV)                  # views of one buffer that lie next to each other
+    params[0].grad, params[2].grad = whole[:1000], whole[1000:]
+    check(params, 1e-3, True)
