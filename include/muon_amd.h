@@ -493,7 +493,7 @@ int muon_amd_adamw_values(const MuonAdamWValuesDesc* descs_dev, const int32_t* b
 
 /* ---- the norm of all gradients, and clipping by it ------------------------------------------- */
 /* out_dev[0] = sqrt(sum of squares of all elements), out_dev[1] = min(1, max_norm / (out_dev[0] + 1e-6));
- * muon_amd_grad_clip also multiplies every gradient by out_dev[1] in place.  partials_dev: workspace of
+ * muon_amd_grad_clip also multiplies every gradient by out_dev[1] in place (none may overlap another).  partials_dev: workspace of
  * muon_amd_grad_norm_partials() doubles.  Blocks as in muon_amd_adamw.                          */
 int muon_amd_grad_norm_partials(void);
 int muon_amd_validate_grads(const MuonGradDesc* descs_host, int ntensors, const int32_t* block_prefix_host);
