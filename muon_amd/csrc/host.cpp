@@ -392,8 +392,9 @@ const Tensor* state_tensor(PyObject* s, int i, const Tensor& t, int bits) {
 // states as they are now; nothing is taken from an earlier step but the answer to whether they are the same.
 class AdamWTable {
    public:
-    AdamWTable(std::vector<int64_t> numels, std::vector<int> dtypes, int bits)
-        : numels_(std::move(numels)), dtypes_(std::move(dtypes)), bits_(bits), columns_(bits == 8 ? 6 : 4),
+    // device: the index of the GPU that the launch runs on (-1: whichever the tensors are on).
+    AdamWTable(std::vector<int64_t> numels, std::vector<int> dtypes, int bits, int device)
+        : numels_(std::move(numels)), dtypes_(std::move(dtypes)), bits_(bits), device_(device), columns_(bits == 8 ? 6 : 4),
           rows_(numels_.size() * columns_), now_(rows_.size()) {}
 
     // The step these parameters are about to take (one for all), or -1: not the common case.
@@ -409,7 +410,7 @@ class AdamWTable {
             const Tensor* const t = plain_parameter(p);
             if (!t || t->numel() != numels_[i] || dtype_of(*t) != dtypes_[i]) return -1;
             if (!device) device = t->device();
-            if (t->device() != *device || !plain_gradient(t->grad(), *t)) return -1;
+            if (t->device() != *device || (device_ >= 0 && device->index() != device_) || !plain_gradient(t->grad(), *t)) return -1;
             PyObject* const s = state_of(state, p, at);
             if (!s) return -1;
             int64_t* const row = &now_[i * columns_];
@@ -458,7 +459,7 @@ class AdamWTable {
    private:
     const std::vector<int64_t> numels_;
     const std::vector<int> dtypes_;
-    const int bits_, columns_;
+    const int bits_, device_, columns_;
     std::vector<int64_t> rows_, now_;
     int64_t version_ = 0;
     std::vector<py::dict> dicts_;
@@ -746,7 +747,7 @@ PYBIND11_MODULE(_native, m) {
     m.def("clear_tables", [] { grad_tables().clear(); });
     py::class_<ValueTable>(m, "ValueTable").def(py::init<>()).def("run", &ValueTable::run).def("run_plain", &ValueTable::run_plain);
     py::class_<AdamWTable>(m, "AdamWTable")
-        .def(py::init<std::vector<int64_t>, std::vector<int>, int>())
+        .def(py::init<std::vector<int64_t>, std::vector<int>, int, int>(), py::arg("numels"), py::arg("dtypes"), py::arg("bits"), py::arg("device") = -1)
         .def("collect", &AdamWTable::collect)
         .def("columns", &AdamWTable::columns)
         .def_property_readonly("version", &AdamWTable::version)

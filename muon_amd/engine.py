@@ -550,27 +550,40 @@ class AdamGroupEngine:
 
 
 class AdamWGroupEngine:
-    """One AdamW launch over a fixed list of tensors with states in 32 or 8 bits (prepare / enqueue as above)."""
+    """One AdamW launch over a list of tensors with states in 32 or 8 bits (lay_out, bind, prepare, enqueue)."""
 
     N_SCALARS = 8          # {lr, 1 - lr * weight_decay, 1 - beta1, 1 - beta2, eps, 1 - beta1**t, 1 - beta2**t, t}
     POINTERS = ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_exponent", "exp_avg_sq_exponent")
     STEP_MODULUS = 1 << 24     # the dither goes by the step modulo this: fp32 scalars hold it exactly
 
-    def __init__(self, numels, dtypes, state_bits, device):
+    def __init__(self, state_bits, device):
         self.device = torch.device(device)
         self.state_bits = int(state_bits)
+        self.layout = None
+        self.revision = 0          # of the tables' memory: recorded launches hold its address
+        self.desc_dev = self.prefix_dev = None
+        self.staging = _Staging(self.device)
+        self.key = None
+        self._hyper = None
+        self._grad_scale = None
+
+    def lay_out(self, numels, dtypes):
+        """The sizes and types of the tensors that follow (at every step: a parameter may have been resized, converted or
+        replaced since the last one)."""
+        layout = (tuple(numels), tuple(dtypes))
+        if layout == self.layout:
+            return
         self.dtype = dtypes[0] if len(set(dtypes)) == 1 else -1
         self.descs = np.zeros(len(numels), dtype=_lib.ADAMW_DESC)
         self.descs["numel"], self.descs["dtype"] = numels, dtypes
         self.prefix = _plan.adam_block_prefix(numels)
         self.nblocks = int(self.prefix[-1])
+        self.nbytes = sum(int(n) * ((6 if t == _lib.SRC_BF16 else 12) + (4 if self.state_bits == 8 else 16)) for n, t in zip(numels, dtypes))
         self.prefix_dev = _upload(self.prefix, self.device)
         self.desc_dev = torch.empty(self.descs.nbytes, dtype=torch.uint8, device=self.device)
-        self.staging = _Staging(self.device)
-        self.nbytes = sum(int(n) * ((6 if t == _lib.SRC_BF16 else 12) + (4 if self.state_bits == 8 else 16)) for n, t in zip(numels, dtypes))
-        self.key = None
-        self._hyper = None
-        self._grad_scale = None
+        self.home = _stream_ptr(self.device)
+        self.layout, self.key = layout, None
+        self.revision += 1
 
     def bind(self, key, columns):
         """Rewrites the table if `key`, which stands for the addresses, is another than at the last call.  columns(): for
@@ -589,12 +602,15 @@ class AdamWGroupEngine:
         self._hyper = [lr, 1 - lr * weight_decay, 1 - betas[0], 1 - betas[1], eps,
                        1 - betas[0] ** step, 1 - betas[1] ** step, step % self.STEP_MODULUS]
         self._grad_scale = grad_scale
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self.home:
+            for table in (self.desc_dev, self.prefix_dev):          # (they may be replaced while the step's launch runs)
+                table.record_stream(torch.cuda.current_stream(self.device))
 
     def scalars(self):
         return [float(x) for x in self._hyper]
 
     def structure_key(self):
-        return (id(self), None if self._grad_scale is None else self._grad_scale.data_ptr())
+        return (id(self), self.revision, None if self._grad_scale is None else self._grad_scale.data_ptr())
 
     def join(self):
         pass

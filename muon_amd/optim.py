@@ -49,7 +49,8 @@ class _MuonBase(torch.optim.Optimizer):
         self._writebacks = []         # (destination, contiguous copy) pairs to copy back after the launches
         self._keepalive = []          # temporaries whose addresses the pending launches use
         self._step_bumps = []         # (Adam state, new step count) written when the launches go out
-        self._adamw_tables = {}       # group index -> (_native.AdamWTable, engine, device): the addresses of a plain group
+        self._adamw_engines = {}      # (group index, state bits, device, launch of the group) -> AdamWGroupEngine
+        self._adamw_tables = {}       # (group index, state bits) -> (_native.AdamWTable, engine, device): a plain group's addresses
         self._table_bumps = []        # (table, new step count), likewise
 
     _RUNTIME_OPTIONS = ("_ns_rounding", "_mutate_grad", "_workspace_bytes", "_ns_variant", "_use_graph",
@@ -343,7 +344,7 @@ class _MuonBase(torch.optim.Optimizer):
         hyper = dict(lr=float(group["lr"]), weight_decay=float(group["weight_decay"]),
                      betas=(float(group["betas"][0]), float(group["betas"][1])), eps=float(group["eps"]), grad_scale=grad_scale)
         # a group whose tensors were all plain at the last step: their addresses, read again, are all there is to do
-        table, eng, device = self._adamw_tables.get(gi, (None, None, None))
+        table, eng, device = self._adamw_tables.get((gi, bits), (None, None, None))
         if table is not None and (grad_scale is None or grad_scale.device == device):
             step = table.collect(group["params"], self.state)
             if step > 0:
@@ -366,24 +367,23 @@ class _MuonBase(torch.optim.Optimizer):
             if p.numel() > 0:
                 by_step.setdefault((step_now, p.device), []).append(
                     (p, (self._dense(p, writebacks), self._dense(g, writebacks, written=False), *tensors)))
-        self._adamw_tables.pop(gi, None)
-        for (step, device), items in by_step.items():
+        self._adamw_tables.pop((gi, bits), None)
+        for k, ((step, device), items) in enumerate(by_step.items()):
             if grad_scale is not None and grad_scale.device != device:
                 raise _lib.MuonAmdError(f"grad_scale is on {grad_scale.device}, parameters are on {device}")
-            key = (gi, device, tuple(id(p) for p, _ in items))
-            numels, dtypes = [p.numel() for p, _ in items], [_src_dtype(p) for p, _ in items]
-            eng = self._adam_engines.get(key)
+            eng = self._adamw_engines.get((gi, bits, device, k))
             if eng is None:
-                with torch.cuda.device(device):
-                    eng = AdamWGroupEngine(numels, dtypes, bits, device)
-                self._adam_engines[key] = eng
+                eng = self._adamw_engines[gi, bits, device, k] = AdamWGroupEngine(bits, device)
+            numels, dtypes = [p.numel() for p, _ in items], [_src_dtype(p) for p, _ in items]
             columns = [[t[j].data_ptr() for _, t in items] for j in range(4 if bits == 32 else 6)]
+            with torch.cuda.device(device):
+                eng.lay_out(numels, dtypes)
             eng.bind(columns, lambda: columns)
             eng.prepare(step=step, **hyper)
             self._pending.append(eng)
             self._keepalive.append((items, grad_scale))
             if not writebacks and len(items) == len(group["params"]):
-                self._adamw_tables[gi] = (_lib.native().AdamWTable(numels, dtypes, bits), eng, device)
+                self._adamw_tables[gi, bits] = (_lib.native().AdamWTable(numels, dtypes, bits, device.index), eng, device)
         self._writebacks += writebacks
 
     def _load_adamw_state(self, state_dict, params):
