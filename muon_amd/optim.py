@@ -298,10 +298,11 @@ class _MuonBase(torch.optim.Optimizer):
                 by_step.setdefault(step_now, []).append((p, item))
         for step, items in by_step.items():
             device = items[0][0].device
-            key = (gi, device, tuple(id(p) for p, _ in items))
+            numels = tuple(p.numel() for p, _ in items)          # (a parameter may have been resized since)
+            key = (gi, device, tuple(id(p) for p, _ in items), numels)
             eng = self._adam_engines.get(key)
             if eng is None:
-                eng = AdamGroupEngine([p.numel() for p, _ in items], device)
+                eng = AdamGroupEngine(numels, device)
                 self._adam_engines[key] = eng
             eng.prepare([t[0].data_ptr() for _, t in items], [t[1].data_ptr() for _, t in items],
                         [t[2].data_ptr() for _, t in items], [t[3].data_ptr() for _, t in items],
