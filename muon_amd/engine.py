@@ -549,8 +549,20 @@ class AdamGroupEngine:
         self.enqueue()
 
 
+# Tables that a HIP graph of the program reads: a replay holds their addresses for as long as the program keeps it.
+_TABLES_OF_GRAPHS = []
+
+
+def refuse_in_capture(what: str) -> None:
+    """Before what a HIP graph must not record: a table's upload (a replay would read the host's buffer as it is then), or
+    the zeros of a new state."""
+    if torch.cuda.is_current_stream_capturing():
+        raise _lib.MuonAmdError(f"{what} while a HIP graph is captured: take a step over the same tensors before")
+
+
 class AdamWGroupEngine:
-    """One AdamW launch over a list of tensors with states in 32 or 8 bits (lay_out, bind, prepare, enqueue)."""
+    """One AdamW launch over a list of tensors with states in 32 or 8 bits (lay_out, bind, prepare, enqueue).  A graph that the
+    program captures may record it over a list that was bound before; its tables are from then on neither written nor freed."""
 
     N_SCALARS = 8          # {lr, 1 - lr * weight_decay, 1 - beta1, 1 - beta2, eps, 1 - beta1**t, 1 - beta2**t, t}
     POINTERS = ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_exponent", "exp_avg_sq_exponent")
@@ -562,6 +574,7 @@ class AdamWGroupEngine:
         self.layout = None
         self.revision = 0          # of the tables' memory: recorded launches hold its address
         self.desc_dev = self.prefix_dev = None
+        self.of_graph = False      # a graph of the program reads them
         self.staging = _Staging(self.device)
         self.key = None
         self._hyper = None
@@ -573,28 +586,40 @@ class AdamWGroupEngine:
         layout = (tuple(numels), tuple(dtypes))
         if layout == self.layout:
             return
+        refuse_in_capture("AdamW cannot take another list of tensors")
         self.dtype = dtypes[0] if len(set(dtypes)) == 1 else -1
         self.descs = np.zeros(len(numels), dtype=_lib.ADAMW_DESC)
         self.descs["numel"], self.descs["dtype"] = numels, dtypes
         self.prefix = _plan.adam_block_prefix(numels)
         self.nblocks = int(self.prefix[-1])
         self.nbytes = sum(int(n) * ((6 if t == _lib.SRC_BF16 else 12) + (4 if self.state_bits == 8 else 16)) for n, t in zip(numels, dtypes))
+        self.layout = layout
+        self._new_tables()
+
+    def _new_tables(self):
         self.prefix_dev = _upload(self.prefix, self.device)
         self.desc_dev = torch.empty(self.descs.nbytes, dtype=torch.uint8, device=self.device)
         self.home = _stream_ptr(self.device)
-        self.layout, self.key = layout, None
+        self.of_graph, self.key = False, None
         self.revision += 1
 
     def bind(self, key, columns):
         """Rewrites the table if `key`, which stands for the addresses, is another than at the last call.  columns(): for
         each name of POINTERS the tensors' addresses (the last two only with 8 bits)."""
-        if key != self.key:
-            for name, column in zip(self.POINTERS, columns()):
-                self.descs[name] = column
-            _lib.check(_lib.load().muon_amd_validate_adamw(_lib.host_ptr(self.descs), len(self.descs), _lib.host_ptr(self.prefix),
+        if key == self.key:
+            return
+        descs = self.descs.copy()
+        for name, column in zip(self.POINTERS, columns()):
+            descs[name] = column
+        if self.key is None or descs.tobytes() != self.descs.tobytes():
+            refuse_in_capture("AdamW cannot take tensors at other addresses")
+            _lib.check(_lib.load().muon_amd_validate_adamw(_lib.host_ptr(descs), len(descs), _lib.host_ptr(self.prefix),
                                                            self.state_bits), "validate_adamw")
-            self.staging.upload(self.descs, self.desc_dev)
-            self.key = key
+            if self.of_graph:
+                self._new_tables()
+            self.descs = descs
+            self.staging.upload(descs, self.desc_dev)
+        self.key = key
 
     def prepare(self, *, lr, weight_decay, betas, eps, step, grad_scale=None):
         """grad_scale: a one-element fp32 tensor on the device, or None."""
@@ -616,6 +641,10 @@ class AdamWGroupEngine:
         pass
 
     def enqueue(self, scalars_ptr: int = 0, join: bool = True):
+        # (a StepGraph, which passes its scalars, knows the tables' revision; any other capture is the program's)
+        if not scalars_ptr and not self.of_graph and torch.cuda.is_current_stream_capturing():
+            _TABLES_OF_GRAPHS.append((self.desc_dev, self.prefix_dev))
+            self.of_graph = True
         scale = 0 if self._grad_scale is None else self._grad_scale.data_ptr()
         _launch("adamw", self.nbytes, lambda: _lib.native().adamw_launch(
             self.device.index, self.desc_dev.data_ptr(), self.prefix_dev.data_ptr(), len(self.descs), self.nblocks, self.dtype,

@@ -13,7 +13,7 @@ import weakref
 import torch
 
 from . import _lib, engine as _engine
-from .engine import AdamGroupEngine, AdamWGroupEngine, MuonGroupEngine, StepGraph, _launch, require_gpu_tensor
+from .engine import AdamGroupEngine, AdamWGroupEngine, MuonGroupEngine, StepGraph, _launch, refuse_in_capture, require_gpu_tensor
 from .functional import _rounding_flag, _src_dtype
 
 NS_STEPS = 5          # the reference classes never pass a step count: muon_update's default rules
@@ -318,6 +318,7 @@ class _MuonBase(torch.optim.Optimizer):
     def _adamw_state(self, p, state, bits):
         """A parameter's state tensors in the engine's order, made on its first step and checked on every one."""
         if len(state) == 0:
+            refuse_in_capture("AdamW cannot take its first step over a parameter")
             if bits == 32:
                 state["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 state["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
@@ -551,6 +552,8 @@ class AdamW(_MuonBase):
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale=None):
+        if self._use_graph:
+            refuse_in_capture("AdamW(use_graph=True), which keeps a graph of its own, cannot step")
         loss = self._run_closure(closure)
         if grad_scale is not None:
             require_gpu_tensor(grad_scale, "grad_scale")
