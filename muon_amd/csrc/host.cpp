@@ -477,6 +477,13 @@ void adamw_launch(int device, uintptr_t descs, uintptr_t prefix, int n, int bloc
           "adamw");
 }
 
+// The memory of tables that a captured HIP graph reads: a replay holds their addresses for as long as the program keeps it,
+// whatever becomes of the tables' owners.  (Never destroyed: the process ends with it.)
+std::vector<Tensor>& tables_of_graphs() {
+    static auto* const kept = new std::vector<Tensor>;
+    return *kept;
+}
+
 // A table of descriptors and its block prefix on the device.  A table is never rewritten: other contents get memory of
 // their own, so a launch on one stream cannot see what a call on another stream uploads.
 class Table {
@@ -484,7 +491,6 @@ class Table {
     template <typename D>
     void upload(const std::vector<D>& descs, const c10::Device& device) {
         if (capturing()) throw LibraryError("tensors that no call has seen before cannot be uploaded while a HIP graph is captured: make the call once before");
-        if (captured_) kept_.push_back(memory_);
         captured_ = false;
         std::vector<int32_t> prefix(descs.size() + 1, 0);
         for (size_t i = 0; i < descs.size(); ++i)
@@ -506,6 +512,7 @@ class Table {
     // before.  The graph keeps the table's address: from then on its memory is not given back.)
     void use(const c10::Device& device) {
         if (capturing()) {
+            if (!captured_) tables_of_graphs().push_back(memory_);
             captured_ = true;
             return;
         }
@@ -531,7 +538,6 @@ class Table {
     size_t prefix_ = 0;
     int n_ = 0, blocks_ = 0;
     bool captured_ = false;
-    std::vector<Tensor> kept_;
     c10::Event uploaded_{c10::DeviceType::CUDA};
 };
 
@@ -745,6 +751,7 @@ PYBIND11_MODULE(_native, m) {
     m.def("clip", &clip);
     m.def("clip_list", &clip_list);
     m.def("clear_tables", [] { grad_tables().clear(); });
+    m.def("tables_of_graphs", [] { return tables_of_graphs().size(); });
     py::class_<ValueTable>(m, "ValueTable").def(py::init<>()).def("run", &ValueTable::run).def("run_plain", &ValueTable::run_plain);
     py::class_<AdamWTable>(m, "AdamWTable")
         .def(py::init<std::vector<int64_t>, std::vector<int>, int, int>(), py::arg("numels"), py::arg("dtypes"), py::arg("bits"), py::arg("device") = -1)
