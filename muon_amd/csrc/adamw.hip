@@ -258,6 +258,7 @@ __device__ __forceinline__ void adamw8_pack(Pack<T, G>& p, const Pack<T, G>& g, 
         pn[k] = fmaf(a.neg_lr, m[k] * __builtin_amdgcn_rcpf(denominator), p[k] * a.wd_factor);
     }
     p = Pack<T, G>::of(pn);
+    most_v = min(most_v, 0x7fffffffu);                       // (a NaN's sign and the carry would wrap around to a small exponent)
     // exponent fields, one more where three bits of mantissa are not enough below the next power (m: 1.75 is the last)
     const uint32_t both = lanes_max2<AW_SHARED / G>(((__float_as_uint(most_m) + 0x1fffffu) >> 23) | ((most_v + 0xfffffu) >> 23 << 16));
     Em = static_cast<int>(both & 0xffffu);
