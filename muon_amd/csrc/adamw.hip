@@ -65,21 +65,26 @@ __device__ __forceinline__ AdamWArgs read_args(AdamWArgs a, const float* sc) {
 }
 
 // The two moments; the square is rounded before it is subtracted from, as for tensors of fp32.  A weight of a half and
-// more is taken from the other end, new + (w - 1)(new - old), which is `new` itself for w = 1.  NEAR: neither weight is,
-// as in every ordinary run (the two selections for each element are then left out).
-template <bool NEAR>
+// more is taken from the other end, new + (w - 1)(new - old), which is `new` itself for w = 1.  ORDINARY: neither weight is
+// (the two selections for each element are then left out).
+template <bool ORDINARY>
 __device__ __forceinline__ float lerp_from(float old, float now, float w) {
-    const bool far = !NEAR && fabsf(w) >= 0.5f;
+    const bool far = !ORDINARY && fabsf(w) >= 0.5f;
     return fmaf(far ? w - 1.f : w, now - old, far ? now : old);
 }
-template <bool NEAR>
+template <bool ORDINARY>
 __device__ __forceinline__ void moments(float& m, float& v, float g, const AdamWArgs& a) {
 #pragma clang fp contract(off)
     const float gg = g * g;
-    m = lerp_from<NEAR>(m, g, a.w1);
-    v = lerp_from<NEAR>(v, gg, a.w2);
+    m = lerp_from<ORDINARY>(m, g, a.w1);
+    v = lerp_from<ORDINARY>(v, gg, a.w2);
 }
-__device__ __forceinline__ bool near_weights(const AdamWArgs& a) { return fabsf(a.w1) < 0.5f && fabsf(a.w2) < 0.5f; }
+// Whether the arguments are those of an ordinary run, for which 8-bit states have a kernel path of their own: small weights, and
+// an eps beside which the root of a subnormal v (below 2^-63) is lost, so that the path may take it for zero.  (131 M fp32
+// elements: 347 us that way, 367 the other; 39 M in bf16: 68 both ways.)
+__device__ __forceinline__ bool ordinary(const AdamWArgs& a) {
+    return fabsf(a.w1) < 0.5f && fabsf(a.w2) < 0.5f && a.eps >= 0x1p-39f * a.rsqrt_bias2;
+}
 
 // ---- states in 32 bits -------------------------------------------------------------------------------------
 // Memory bounds it: 22 bytes an element with bf16 parameters, 28 with fp32 (32000 x 2048 bf16: 218 us, 6.6 TB/s).  Lists of small
@@ -234,12 +239,22 @@ __device__ __forceinline__ uint32_t top_bytes(const uint32_t (&w)[4]) {
     return __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0703u) | __builtin_amdgcn_perm(w[3], w[2], 0x07030c0cu);
 }
 
+// The root of v by the target's instruction, which is a unit off and takes subnormal numbers for zero; they are scaled up
+// unless ORDINARY allows that.  (A unit each of the root and of the reciprocal below is a relative 2^-22 of an update that
+// goes by codes of three bits; the correctly rounded ones of the 32-bit states are about 20 instructions longer.)
+template <bool ORDINARY>
+__device__ __forceinline__ float root(float v) {
+    if (ORDINARY) return __builtin_amdgcn_sqrtf(v);
+    const bool low = v < 0x1p-96f;
+    return __builtin_amdgcn_sqrtf(low ? v * 0x1p32f : v) * (low ? 0x1p-16f : 1.f);
+}
+
 // One pack: parameters and moments after the step, the new codes, and the new shared exponents of its block, which is
 // that of 128 / G lanes (every lane of the wave calls this; what is beyond the tensor is zero).
 // Its arithmetic (about 40 instructions an element) takes nearly as long as bf16 parameters take to move: so codes are rounded where they end up in the top
 // byte of a word (the magnitude's bits and the dither's, both four bits higher than the code's own place), four of
 // which two byte permutations collect, and zeros among the codes of v are looked for four at a time.
-template <typename T, int G, bool NEAR>
+template <typename T, int G, bool ORDINARY>
 __device__ __forceinline__ void adamw8_pack(Pack<T, G>& p, const Pack<T, G>& g, Codes<G>& mc, Codes<G>& vc, int& Em, int& Ev,
                                             uint32_t i0, float c, const AdamWArgs& a) {
     float m[G], v[G], pn[G];
@@ -251,10 +266,10 @@ __device__ __forceinline__ void adamw8_pack(Pack<T, G>& p, const Pack<T, G>& g, 
 #pragma unroll
     for (int k = 0; k < G; ++k) {
         const float gk = fmaf(g[k], c, poison);
-        moments<NEAR>(m[k], v[k], gk, a);
+        moments<ORDINARY>(m[k], v[k], gk, a);
         most_m = fmaxf(most_m, fabsf(m[k]));
         most_v = max(most_v, __float_as_uint(v[k]));         // (the bits, so that NaN counts; m is not finite only where v is not)
-        const float denominator = fmaf(__builtin_amdgcn_sqrtf(v[k]), a.rsqrt_bias2, a.eps);
+        const float denominator = fmaf(root<ORDINARY>(v[k]), a.rsqrt_bias2, a.eps);
         pn[k] = fmaf(a.neg_lr, m[k] * __builtin_amdgcn_rcpf(denominator), p[k] * a.wd_factor);
     }
     p = Pack<T, G>::of(pn);
@@ -288,7 +303,7 @@ __device__ __forceinline__ void adamw8_pack(Pack<T, G>& p, const Pack<T, G>& g, 
     }
 }
 
-template <typename T, int EACH, bool NEAR>
+template <typename T, int EACH, bool ORDINARY>
 __device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t base, float c, const AdamWArgs& a) {
     constexpr int G = pack_of<T>, PACKS = EACH / G, LANES = AW_SHARED / G, ELEMS = AW_THREADS * EACH;
     const int64_t numel = d.numel;
@@ -315,7 +330,7 @@ __device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t bas
 #pragma unroll
         for (int i = 0; i < PACKS; ++i) {
             const int64_t e = base + (i * AW_THREADS + threadIdx.x) * G;
-            adamw8_pack<T, G, NEAR>(pv[i], gv[i], mv[i], vv[i], Em[i], Ev[i], static_cast<uint32_t>(e), c, a);
+            adamw8_pack<T, G, ORDINARY>(pv[i], gv[i], mv[i], vv[i], Em[i], Ev[i], static_cast<uint32_t>(e), c, a);
             mv[i].store(m + e);
             vv[i].store(v + e);
             pv[i].template store<true>(p + e);
@@ -334,7 +349,7 @@ __device__ __forceinline__ void adamw8_block(const MuonAdamWDesc& d, int64_t bas
         Codes<G> mv = Codes<G>::load(m, e, numel), vv = Codes<G>::load(v, e, numel);
         Pack<T, G> pv = load_pack<T, G, true>(p, e, numel);
         const Pack<T, G> gv = load_pack<T, G, true>(g, e, numel);
-        adamw8_pack<T, G, NEAR>(pv, gv, mv, vv, Em, Ev, static_cast<uint32_t>(e), c, a);
+        adamw8_pack<T, G, ORDINARY>(pv, gv, mv, vv, Em, Ev, static_cast<uint32_t>(e), c, a);
         mv.store(m, e, numel);
         vv.store(v, e, numel);
         store_pack<T, G, true>(p, e, numel, pv);
@@ -357,7 +372,7 @@ __global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(const MuonAdamWDesc*
     const MuonAdamWDesc d = descs[ti];
     const int64_t base = static_cast<int64_t>(b - prefix[ti]) * AW_BLOCK_ELEMS + blockIdx.x % PARTS * (AW_THREADS * EACH);
     with_type<DTYPE>(d, [&](auto t) {
-        if (near_weights(a)) adamw8_block<decltype(t), EACH, true>(d, base, c, a);
+        if (ordinary(a)) adamw8_block<decltype(t), EACH, true>(d, base, c, a);
         else adamw8_block<decltype(t), EACH, false>(d, base, c, a);
     });
 }
