@@ -399,9 +399,9 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
         fetch(t + step);
         // The weights' part; lanes of the row take the k choices in turn.
         if (a.dweights) {
-            float dot = w * dw;
+            float dot = mine >= 0 ? w * dw : 0.f;        // (what arrives for a choice that is not there may be no number)
             for (int j = lane + L; j < a.k; j += L)
-                if (on) dot = fmaf(a.weights[t * a.k + j], a.dweights[t * a.ld_dweights + j], dot);
+                if (on && a.indices[t * a.k + j] >= 0) dot = fmaf(a.weights[t * a.k + j], a.dweights[t * a.ld_dweights + j], dot);
             dot = a.normalize ? group_sum<L>(dot) : 0.f;
             if (mine >= 0) *slot(mine) = w * (dw - dot);
             for (int j = lane + L; j < a.k; j += L) {
