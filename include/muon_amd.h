@@ -228,6 +228,7 @@ typedef struct MuonRoute {
     float* balance;  float* z;   /* one float each                                                */
     float* part;                 /* one float: tokens that take part, at least 1                  */
     float* lse;                  /* tokens: log sum exp; -infinity for a token that takes no part */
+    float* lse_rest;             /* tokens: what rounding it to fp32 left out                     */
     float* partials;             /* forward: muon_amd_route_partials() floats                     */
     const float* dweights;       /* backward: tokens x k, ld_dweights from row to row; NULL: zeros */
     const float* dbalance;  const float* dz;             /* backward: one float each; NULL: zero  */

@@ -82,7 +82,7 @@ class ResidualNormArgs(ctypes.Structure):
 
 
 class RouteArgs(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "mask", "weights", "indices", "counts", "balance", "z", "part", "lse", "partials",
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "mask", "weights", "indices", "counts", "balance", "z", "part", "lse", "lse_rest", "partials",
                                                 "dweights", "dbalance", "dz", "dlogits")] +
                 [(n, ctypes.c_int64) for n in ("tokens", "ld_logits", "ld_dweights")] +
                 [(n, ctypes.c_int32) for n in ("experts", "k", "dtype", "normalize")])

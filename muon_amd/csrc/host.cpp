@@ -259,6 +259,7 @@ MuonRoute route_args(const Tensor& logits, const Tensor& mask, const RouteOut& o
     a.counts = o.counts.data_ptr<int32_t>();
     a.part = o.part.data_ptr<float>();
     a.lse = o.lse.data_ptr<float>();
+    a.lse_rest = a.lse + a.tokens;
     a.k = static_cast<int32_t>(o.weights.size(-1));
     a.normalize = normalize;
     return a;
@@ -282,7 +283,7 @@ RouteOut route_forward(const Tensor& logits, int64_t k, const Tensor& mask, bool
     o.balance = at::empty({}, f32);
     o.z = at::empty({}, f32);
     o.part = at::empty({}, f32);
-    o.lse = at::empty({tokens}, f32);
+    o.lse = at::empty({2, tokens}, f32);              // and what rounding it left out
     const Tensor partials = at::empty({api.route_partials(tokens, static_cast<int>(experts))}, f32);
     std::vector<Tensor> keep;
     keep.reserve(2);

@@ -215,7 +215,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_forward_kernel(const MuonRou
             total += ex[i];
         }
         total = group_sum<L>(total);
-        const float lse = on ? top + logf(total) : 0.f, per = on ? 1.f / total : 0.f;
+        const float log_total = on ? logf(total) : 0.f, lse = top + log_total, per = on ? 1.f / total : 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = fmaf(ex[i], per, acc[i]);
         if (t >= a.tokens) continue;
@@ -226,6 +226,9 @@ __global__ __launch_bounds__(RT_THREADS) void route_forward_kernel(const MuonRou
         }
         if (lane == 0) {
             a.lse[t] = on ? lse : -__builtin_inff();
+            // what the sum's rounding left out, exactly (D. Knuth, "The Art of Computer Programming", volume 2, 4.2.2)
+            const float part_of_log = lse - top;
+            a.lse_rest[t] = (top - (lse - part_of_log)) + (log_total - part_of_log);
             square = fmaf(lse, lse, square);
             part += on;
         }
@@ -377,13 +380,14 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
     const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS, begin = static_cast<int64_t>(blockIdx.x) * ROWS + sub;
     // The next row is on its way while this one is worked on: its logits, and each lane's first choice.
     RowPacks<T, N> next;
-    float next_lse, next_w = 0.f, next_dw = 0.f;
+    float next_lse, next_rest, next_w = 0.f, next_dw = 0.f;
     int next_e = -1;
     const bool chooses = a.dweights && lane < a.k;
     const auto fetch = [&](int64_t t) {
         const int64_t row = t < a.tokens ? t : a.tokens - 1;
         next.load(row_of<T>(a, row), base, E);
         next_lse = a.lse[row];
+        next_rest = a.lse_rest[row];
         if (chooses) {
             next_w = a.weights[row * a.k + lane];
             next_dw = a.dweights[row * a.ld_dweights + lane];
@@ -394,7 +398,9 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
     for (int64_t t = begin; t - sub < a.tokens; t += step) {
         RowPacks<T, N> packs = next;
         const bool on = t < a.tokens && next_lse != -__builtin_inff();
-        const float lse = on ? next_lse : 0.f, w = next_w, dw = next_dw;
+        // (what rounding lse left out would go into every probability: all of a row's logits at a value far from zero, as
+        // the type's lowest one, lose the logarithm of their number)
+        const float lse = on ? next_lse : 0.f, rest = on ? next_rest : 0.f, w = next_w, dw = next_dw;
         const int mine = on ? next_e : -1;
         fetch(t + step);
         // The weights' part; lanes of the row take the k choices in turn.
@@ -420,7 +426,7 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            p[i] = exp_of(x[i] - lse);             // (zero where the token takes no part: x is -infinity)
+            p[i] = exp_of(x[i] - lse - rest);      // (zero where the token takes no part: x is -infinity)
             dot = fmaf(p[i], g[i], dot);
             if (!a.normalize) dot += u[i];         // p dw: what comes through the probabilities themselves
         }
@@ -482,7 +488,7 @@ static int check_route(const MuonRoute* a, const char* what) {
     MUON_REQUIRE(a->tokens > 0 && a->experts > 0 && a->experts <= RT_MAX_EXPERTS, "%s: tokens=%lld experts=%d (at most %d)", what,
                  static_cast<long long>(a->tokens), a->experts, RT_MAX_EXPERTS);
     MUON_REQUIRE(a->k > 0 && a->k <= a->experts && a->k <= RT_MAX_K, "%s: k=%d of %d experts (at most %d)", what, a->k, a->experts, RT_MAX_K);
-    MUON_REQUIRE(a->logits && a->weights && a->indices && a->counts && a->part && a->lse, "%s: null pointer", what);
+    MUON_REQUIRE(a->logits && a->weights && a->indices && a->counts && a->part && a->lse && a->lse_rest, "%s: null pointer", what);
     MUON_REQUIRE(a->dtype == MUON_AMD_SRC_F32 || a->dtype == MUON_AMD_SRC_BF16, "%s: dtype=%d", what, a->dtype);
     return MUON_AMD_OK;
 }
