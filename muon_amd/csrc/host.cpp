@@ -194,6 +194,13 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     }
 };
 
+// Whether one of them carries a forward-mode derivative: these functions have none, and must not drop it.
+bool any_tangent(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t && t->_fw_grad(0).defined()) return true;
+    return false;
+}
+
 bool residual_taken(const Tensor& x, const Tensor& block, const Tensor& post, const Tensor& pre, const std::optional<Tensor>& gate,
                     const std::optional<Tensor>& scale, double eps) {
     if (!taken(x) || x.dim() < 1 || !(eps >= 0.)) return false;
@@ -213,7 +220,7 @@ bool residual_taken(const Tensor& x, const Tensor& block, const Tensor& post, co
         for (int64_t d = 0; d + 1 < x.dim(); ++d)
             if (gate->size(d) != x.size(d)) return false;
     }
-    return true;
+    return !any_tangent({&x, &block, &post, &pre, gate ? &*gate : nullptr, scale ? &*scale : nullptr});
 }
 
 bool any_requires_grad(std::initializer_list<const Tensor*> ts) {
@@ -339,6 +346,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>> route_topk(con
     if (mask && (mask->scalar_type() != at::kBool || mask->device() != logits.device() ||
                  mask->sizes() != logits.sizes().slice(0, logits.dim() - 1)))
         return std::nullopt;
+    if (any_tangent({&logits})) return std::nullopt;
     const py::gil_scoped_release released;
     if (any_requires_grad({&logits})) {
         const variable_list out = RouteTopk::apply(logits, k, mask, normalize);

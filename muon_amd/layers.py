@@ -26,6 +26,11 @@ def _dtype(t: torch.Tensor, name: str) -> int:
         raise TypeError(f"{name} is {t.dtype}: fp32 and bf16 tensors are taken") from None
 
 
+def _no_tangent(t: torch.Tensor, name: str) -> None:
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name} carries a forward-mode derivative: only gradients (reverse mode) are there")
+
+
 def residual_norm(x: torch.Tensor, block: torch.Tensor, post_weight: torch.Tensor, pre_weight: torch.Tensor, *,
                   gate: torch.Tensor | None = None, scale: torch.Tensor | None = None, eps: float = 1e-6):
     """The step between two blocks of a transformer over rows of D channels (the last dimension):
@@ -72,6 +77,8 @@ def _refuse_residual(x, block, post_weight, pre_weight, gate, scale, eps):
             raise TypeError(f"gate is {gate.dtype}, block {block.dtype}: they must have one type")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
+    for name, t in tensors:
+        _no_tangent(t, name)
     raise _lib.MuonAmdError("residual_norm does not take these arguments")
 
 
@@ -117,4 +124,5 @@ def _refuse_route(logits, k, mask):
         require_gpu_tensor(mask, "mask")
         if mask.dtype != torch.bool or mask.shape != logits.shape[:-1] or mask.device != logits.device:
             raise ValueError(f"mask must be a bool tensor of shape {tuple(logits.shape[:-1])} on {logits.device}, got {mask.dtype} {tuple(mask.shape)}")
+    _no_tangent(logits, "logits")
     raise _lib.MuonAmdError("route_topk does not take these arguments")
