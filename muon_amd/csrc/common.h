@@ -111,7 +111,9 @@ __device__ __forceinline__ int find_segment(const int32_t* __restrict__ prefix, 
 __device__ __forceinline__ int find_segment_wave(const int32_t* __restrict__ prefix, int n, int b) {
     int lo = 0;
     const int lane = static_cast<int>(threadIdx.x & 63);
-    for (int stride = n > 4096 ? 4096 : n > 64 ? 64 : 1; ; stride >>= 6) {
+    int stride = 1;                                // (64 strides cover the table: any number of tensors up to 2^30)
+    while (n > 64 * stride && stride < 1 << 24) stride <<= 6;
+    for (;; stride >>= 6) {
         // entries lo + stride, lo + 2 stride, ..: how many are at or below b
         const int i = lo + (lane + 1) * stride;
         const uint64_t below = __ballot(i < n && prefix[i < n ? i : n] <= b);
