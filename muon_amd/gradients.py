@@ -29,6 +29,8 @@ def _general(parameters, max_norm, in_place):
             raise ValueError("the same parameter is in the list twice")
         seen.add(id(p))
         if not g.is_contiguous():                 # the kernels address row-major memory
+            if in_place and any(n > 1 and st == 0 for n, st in zip(g.shape, g.stride())):
+                raise ValueError("gradients that share memory cannot be scaled in place (one is broadcast)")
             c = g.contiguous()
             writebacks.append((g, c))
             g = c
