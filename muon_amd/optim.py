@@ -388,16 +388,19 @@ class _MuonBase(torch.optim.Optimizer):
                 self._adamw_tables[gi, bits] = (_lib.native().AdamWTable(numels, dtypes, bits, device.index), eng, device)
         self._writebacks += writebacks
 
-    def _load_adamw_state(self, state_dict, params):
+    def _load_adamw_state(self, state_dict, params, bits):
         """After torch's load_state_dict, which converts every state tensor to its parameter's type: the tensors of
-        `params` as they were saved."""
+        `params` as they were saved, in row-major order; for states of 32 bits, bf16 and fp16 ones (torch.optim.AdamW's over
+        such parameters) widened to fp32."""
         mine = {id(p) for p in params}
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
             if id(p) in mine:
                 for key, value in state_dict["state"].get(i, {}).items():
                     if isinstance(value, torch.Tensor) and key != "step":
-                        self.state[p][key] = value.detach().to(p.device, copy=True)
+                        wide = bits == 32 and value.dtype in (torch.bfloat16, torch.float16)
+                        self.state[p][key] = value.detach().to(p.device, torch.float32 if wide else value.dtype, copy=True,
+                                                               memory_format=torch.contiguous_format)
 
     def _launch_pending(self):
         """Enqueue what the group loop prepared: eagerly, or (use_graph=True) as one recorded graph
@@ -548,7 +551,7 @@ class AdamW(_MuonBase):
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
-        self._load_adamw_state(state_dict, [p for g in self.param_groups for p in g["params"]])
+        self._load_adamw_state(state_dict, [p for g in self.param_groups for p in g["params"]], self._state_bits)
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale=None):
@@ -651,7 +654,8 @@ class SingleDeviceMuonWithAuxAdam(_MuonBase):
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
         if self._adam_state_bits is not None:
-            self._load_adamw_state(state_dict, [p for g in self.param_groups if not g["use_muon"] for p in g["params"]])
+            self._load_adamw_state(state_dict, [p for g in self.param_groups if not g["use_muon"] for p in g["params"]],
+                                   self._adam_state_bits)
 
     @torch.no_grad()
     def step(self, closure=None):
