@@ -550,6 +550,9 @@ class AdamW(_MuonBase):
         self._state_bits, self._value_tables, self._scale_buffers = bits, {}, {}
 
     def load_state_dict(self, state_dict):
+        for option in ("amsgrad", "maximize"):    # of torch.optim.AdamW: other updates than this one
+            if any(g.get(option) for g in state_dict["param_groups"]):
+                raise NotImplementedError(f"AdamW has no {option}: the state dict is of an optimizer with it")
         super().load_state_dict(state_dict)
         self._load_adamw_state(state_dict, [p for g in self.param_groups for p in g["params"]], self._state_bits)
 

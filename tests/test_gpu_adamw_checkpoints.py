@@ -49,3 +49,12 @@ def test_states_of_8_bits_are_not_made_from_others():
     new.load_state_dict(old.state_dict())
     with pytest.raises(NotImplementedError):
         new.step()
+
+
+@pytest.mark.parametrize("option", ["amsgrad", "maximize"])
+def test_other_algorithms_are_refused(option):
+    params, old = trained(torch.float32, **{option: True})
+    for new in (muon_amd.AdamW(params), muon_amd.AdamW(params, state_bits=8)):
+        with pytest.raises(NotImplementedError, match=option):
+            new.load_state_dict(old.state_dict())
+        assert not new.state and new.param_groups[0]["lr"] == 1e-3
