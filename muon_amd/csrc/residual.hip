@@ -64,7 +64,15 @@ __device__ __forceinline__ void row_sums(float (&s)[N], float (*slots)[N]) {
     }
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+// The gate of logits stored as B.  exp(-z) by the target's power of two alone is off by 2^-24 |z| relative to itself (60 units at
+// -80): a hundredth of a percent of what a bf16 logit's own rounding makes of it, but more than an fp32 result should be, so
+// fp32 logits take the exact one (8192 x 2048 all in fp32: 59 us forward and 100 backward both ways; for bf16 logits beside an
+// fp32 stream it would cost 2 to 7 %).  Below -87.3, where the gate is no normal number, it is zero.  1 - sigmoid, which the
+// gate's gradient takes, has the rounding of one: 2^-24 absolute.
+template <typename B>
+__device__ __forceinline__ float sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.f + (sizeof(B) == 4 ? expf(-z) : __expf(-z)));
+}
 
 // A pack's elements of a vector of weights in fp32 (zero beyond the row).
 template <int G>
@@ -180,7 +188,7 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
             if constexpr (GATE == GATE_CHANNEL) zv[j] = request<B, G, true>(z, c, width);
         }
         float whole = 1.f;
-        if constexpr (GATE == GATE_TOKEN) whole = sigmoid(load_one(a.gate, a.block_dtype, row * a.ld_gate));
+        if constexpr (GATE == GATE_TOKEN) whole = sigmoid<B>(load_one(a.gate, a.block_dtype, row * a.ld_gate));
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * TPR + t) * G;
@@ -204,7 +212,7 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS) void residual_
             w.template get<0>(j, k);
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-                const float sig = GATE == GATE_CHANNEL ? sigmoid(zv[j][i]) : whole;
+                const float sig = GATE == GATE_CHANNEL ? sigmoid<B>(zv[j][i]) : whole;
                 h[j][i] = fmaf(bv[j][i] * rb, k[i] * sig, xv[j][i]);
                 if (c + i < width) sum[0] = fmaf(h[j][i], h[j][i], sum[0]);
             }
@@ -267,7 +275,7 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS, 4) void residu
         }
         const float rb = a.rstd[2 * row], rh = a.rstd[2 * row + 1];
         float whole = 1.f;
-        if constexpr (GATE == GATE_TOKEN) whole = sigmoid(load_one(a.gate, a.block_dtype, row * a.ld_gate));
+        if constexpr (GATE == GATE_TOKEN) whole = sigmoid<B>(load_one(a.gate, a.block_dtype, row * a.ld_gate));
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * TPR + t) * G;
@@ -288,7 +296,7 @@ __global__ __launch_bounds__(TPR > RN_THREADS ? TPR : RN_THREADS, 4) void residu
             w.template get<1>(j, wpre);
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-                sig[j][i] = GATE == GATE_CHANNEL ? sigmoid(zv[j][i]) : whole;
+                sig[j][i] = GATE == GATE_CHANNEL ? sigmoid<B>(zv[j][i]) : whole;
                 const float kk = k[i] * sig[j][i], nb = bv[j][i] * rb;
                 nh[j][i] = fmaf(nb, kk, xv[j][i]) * rh;
                 const float dn = dyv[j][i] * wpre[i];
