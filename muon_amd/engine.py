@@ -613,6 +613,11 @@ class AdamWGroupEngine:
             descs[name] = column
         if self.key is None or descs.tobytes() != self.descs.tobytes():
             refuse_in_capture("AdamW cannot take tensors at other addresses")
+            order = np.argsort(descs["param"])    # (two workgroups would step the same element)
+            begins = descs["param"][order].astype(np.int64)
+            ends = begins + (descs["numel"] * np.where(descs["dtype"] == _lib.SRC_BF16, 2, 4))[order]
+            if (ends[:-1] > begins[1:]).any():
+                raise ValueError("parameters that share memory, or one that is in a group twice, cannot be stepped together")
             _lib.check(_lib.load().muon_amd_validate_adamw(_lib.host_ptr(descs), len(descs), _lib.host_ptr(self.prefix),
                                                            self.state_bits), "validate_adamw")
             if self.of_graph:
