@@ -66,6 +66,8 @@ void* current_stream(const c10::Device& device) {
 // The current stream as torch's device-independent interface names it.
 c10::Stream stream_of(const c10::Device& device) { return c10::impl::VirtualGuardImpl(device.type()).getStream(device); }
 
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? MUON_AMD_SRC_BF16 : MUON_AMD_SRC_F32; }
 bool taken(const Tensor& t) { return t.is_cuda() && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16); }
 
@@ -446,15 +448,14 @@ class AdamWTable {
         }
         return step;
     }
-    // What column c of the launch's table holds (valid after collect).
-    py::list columns() const {
-        py::list out;
-        for (int c = 0; c < columns_; ++c) {
-            py::list column;
-            for (size_t i = 0; i < numels_.size(); ++i) column.append(rows_[i * columns_ + c]);
-            out.append(column);
-        }
-        return out;
+    // Puts the addresses into the rows of the launch's table, which begin with them (valid after collect).
+    void write(const py::buffer& table) const {
+        const py::buffer_info rows = table.request(/*writable=*/true);
+        const size_t size = columns_ * sizeof(int64_t), stride = static_cast<size_t>(rows.itemsize);
+        if (rows.ndim != 1 || static_cast<size_t>(rows.size) != numels_.size() || stride < size || rows.strides[0] != rows.itemsize)
+            throw py::value_error("not this list's table");
+        for (size_t i = 0; i < numels_.size(); ++i)
+            std::memcpy(static_cast<char*>(rows.ptr) + i * stride, &rows_[i * columns_], size);
     }
     int64_t version() const { return version_; }
     // Writes the new step count to the states that collect() saw.
@@ -476,14 +477,15 @@ class AdamWTable {
 };
 
 // The AdamW launch on the current stream of a device (addresses as numbers; hyper: lr, 1 - lr weight_decay, 1 - beta1,
-// 1 - beta2, eps, 1 - beta1^t, 1 - beta2^t, t).
-void adamw_launch(int device, uintptr_t descs, uintptr_t prefix, int n, int blocks, int dtype, int bits, const std::array<double, 8>& hyper,
+// 1 - beta2, eps, 1 - beta1^t, 1 - beta2^t, t).  Whether a HIP graph records it.
+bool adamw_launch(int device, uintptr_t descs, uintptr_t prefix, int n, int blocks, int dtype, int bits, const std::array<double, 8>& hyper,
                   uintptr_t grad_scale, uintptr_t scalars) {
     const auto f = [&](int i) { return static_cast<float>(hyper[i]); };
     check(api.adamw(reinterpret_cast<const MuonAdamWDesc*>(descs), reinterpret_cast<const int32_t*>(prefix), n, blocks, dtype, bits, f(0), f(1),
                     f(2), f(3), f(4), f(5), f(6), static_cast<uint32_t>(hyper[7]), reinterpret_cast<const float*>(grad_scale),
                     reinterpret_cast<const float*>(scalars), c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream()),
           "adamw");
+    return capturing();
 }
 
 // The memory of tables that a captured HIP graph reads: a replay holds their addresses for as long as the program keeps it,
@@ -537,7 +539,6 @@ class Table {
     bool captured() const { return captured_; }
 
    private:
-    static bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
     template <typename D>
     static auto validator() {
         if constexpr (std::is_same_v<D, MuonGradDesc>) return api.validate_grads;
@@ -765,7 +766,7 @@ PYBIND11_MODULE(_native, m) {
     py::class_<AdamWTable>(m, "AdamWTable")
         .def(py::init<std::vector<int64_t>, std::vector<int>, int, int>(), py::arg("numels"), py::arg("dtypes"), py::arg("bits"), py::arg("device") = -1)
         .def("collect", &AdamWTable::collect)
-        .def("columns", &AdamWTable::columns)
+        .def("write", &AdamWTable::write)
         .def_property_readonly("version", &AdamWTable::version)
         .def("bump", &AdamWTable::bump);
 }

@@ -567,9 +567,11 @@ class AdamWGroupEngine:
     N_SCALARS = 8          # {lr, 1 - lr * weight_decay, 1 - beta1, 1 - beta2, eps, 1 - beta1**t, 1 - beta2**t, t}
     POINTERS = ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_exponent", "exp_avg_sq_exponent")
     STEP_MODULUS = 1 << 24     # the dither goes by the step modulo this: fp32 scalars hold it exactly
+    _current_stream = staticmethod(torch._C._cuda_getCurrentRawStream)
 
     def __init__(self, state_bits, device):
         self.device = torch.device(device)
+        self.index = self.device.index
         self.state_bits = int(state_bits)
         self.layout = None
         self.revision = 0          # of the tables' memory: recorded launches hold its address
@@ -599,32 +601,40 @@ class AdamWGroupEngine:
     def _new_tables(self):
         self.prefix_dev = _upload(self.prefix, self.device)
         self.desc_dev = torch.empty(self.descs.nbytes, dtype=torch.uint8, device=self.device)
-        self.home = _stream_ptr(self.device)
+        self.addresses = self.desc_dev.data_ptr(), self.prefix_dev.data_ptr(), len(self.descs)
+        self.home = self._current_stream(self.index)
         self.of_graph, self.key = False, None
         self.revision += 1
 
-    def bind(self, key, columns):
-        """Rewrites the table if `key`, which stands for the addresses, is another than at the last call.  columns(): for
-        each name of POINTERS the tensors' addresses (the last two only with 8 bits)."""
+    def bind(self, key, write):
+        """Rewrites the table if `key`, which stands for the addresses, is another than at the last call.  write(descs) puts
+        them into the table's rows, in the order of POINTERS (the last two only with 8 bits)."""
         if key == self.key:
             return
         descs = self.descs.copy()
-        for name, column in zip(self.POINTERS, columns()):
-            descs[name] = column
-        if self.key is None or descs.tobytes() != self.descs.tobytes():
-            refuse_in_capture("AdamW cannot take tensors at other addresses")
-            order = np.argsort(descs["param"])    # (two workgroups would step the same element)
-            begins = descs["param"][order].astype(np.int64)
-            ends = begins + (descs["numel"] * np.where(descs["dtype"] == _lib.SRC_BF16, 2, 4))[order]
-            if (ends[:-1] > begins[1:]).any():
-                raise ValueError("parameters that share memory, or one that is in a group twice, cannot be stepped together")
+        write(descs)
+        capturing = torch.cuda.is_current_stream_capturing()
+        if self.key is None or not (capturing or self.of_graph) or descs.tobytes() != self.descs.tobytes():
+            if capturing:
+                refuse_in_capture("AdamW cannot take tensors at other addresses")
             _lib.check(_lib.load().muon_amd_validate_adamw(_lib.host_ptr(descs), len(descs), _lib.host_ptr(self.prefix),
                                                            self.state_bits), "validate_adamw")
+            if self.key is None or (descs["param"] != self.descs["param"]).any():
+                self._check_apart(descs)
             if self.of_graph:
                 self._new_tables()
             self.descs = descs
             self.staging.upload(descs, self.desc_dev)
         self.key = key
+
+    @staticmethod
+    def _check_apart(descs):
+        """Two workgroups would step an element at once that two of the parameters hold."""
+        order = np.argsort(descs["param"])
+        begins = descs["param"][order].astype(np.int64)
+        ends = begins + (descs["numel"] * np.where(descs["dtype"] == _lib.SRC_BF16, 2, 4))[order]
+        if (ends[:-1] > begins[1:]).any():
+            raise ValueError("parameters that share memory, or one that is in a group twice, cannot be stepped together")
 
     def prepare(self, *, lr, weight_decay, betas, eps, step, grad_scale=None):
         """grad_scale: a one-element fp32 tensor on the device, or None."""
@@ -632,7 +642,7 @@ class AdamWGroupEngine:
         self._hyper = [lr, 1 - lr * weight_decay, 1 - betas[0], 1 - betas[1], eps,
                        1 - betas[0] ** step, 1 - betas[1] ** step, step % self.STEP_MODULUS]
         self._grad_scale = grad_scale
-        if torch._C._cuda_getCurrentRawStream(self.device.index) != self.home:
+        if self._current_stream(self.index) != self.home:
             for table in (self.desc_dev, self.prefix_dev):          # (they may be replaced while the step's launch runs)
                 table.record_stream(torch.cuda.current_stream(self.device))
 
@@ -646,14 +656,14 @@ class AdamWGroupEngine:
         pass
 
     def enqueue(self, scalars_ptr: int = 0, join: bool = True):
+        scale = 0 if self._grad_scale is None else self._grad_scale.data_ptr()
+        captured = []
+        _launch("adamw", self.nbytes, lambda: captured.append(_lib.native().adamw_launch(
+            self.index, *self.addresses, self.nblocks, self.dtype, self.state_bits, self._hyper, scale, scalars_ptr)))
         # (a StepGraph, which passes its scalars, knows the tables' revision; any other capture is the program's)
-        if not scalars_ptr and not self.of_graph and torch.cuda.is_current_stream_capturing():
+        if captured[0] and not scalars_ptr and not self.of_graph:
             _TABLES_OF_GRAPHS.append((self.desc_dev, self.prefix_dev))
             self.of_graph = True
-        scale = 0 if self._grad_scale is None else self._grad_scale.data_ptr()
-        _launch("adamw", self.nbytes, lambda: _lib.native().adamw_launch(
-            self.device.index, self.desc_dev.data_ptr(), self.prefix_dev.data_ptr(), len(self.descs), self.nblocks, self.dtype,
-            self.state_bits, self._hyper, scale, scalars_ptr))
 
 
 class StepGraph:

@@ -350,7 +350,7 @@ class _MuonBase(torch.optim.Optimizer):
         if table is not None and (grad_scale is None or grad_scale.device == device):
             step = table.collect(group["params"], self.state)
             if step > 0:
-                eng.bind((id(table), table.version), table.columns)
+                eng.bind((id(table), table.version), table.write)
                 eng.prepare(step=step, **hyper)
                 self._pending.append(eng)
                 self._table_bumps.append((table, step))
@@ -377,10 +377,15 @@ class _MuonBase(torch.optim.Optimizer):
             if eng is None:
                 eng = self._adamw_engines[gi, bits, device, k] = AdamWGroupEngine(bits, device)
             numels, dtypes = [p.numel() for p, _ in items], [_src_dtype(p) for p, _ in items]
-            columns = [[t[j].data_ptr() for _, t in items] for j in range(4 if bits == 32 else 6)]
+            addresses = tuple(tuple(t[j].data_ptr() for _, t in items) for j in range(4 if bits == 32 else 6))
+
+            def write(descs):
+                for name, column in zip(eng.POINTERS, addresses):
+                    descs[name] = column
+
             with torch.cuda.device(device):
                 eng.lay_out(numels, dtypes)
-            eng.bind(columns, lambda: columns)
+            eng.bind(addresses, write)
             eng.prepare(step=step, **hyper)
             self._pending.append(eng)
             self._keepalive.append((items, grad_scale))
