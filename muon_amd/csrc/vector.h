@@ -11,11 +11,8 @@
 namespace muon_amd {
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
 typedef float f32x4v_any __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint32_t u32x4v_any __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u32x2v_any __attribute__((ext_vector_type(2), aligned(2)));
 
 #define MUON_GLOBAL __attribute__((address_space(1)))
 
