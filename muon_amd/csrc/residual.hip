@@ -14,7 +14,8 @@
 //
 // Memory bounds both passes (16384 x 4096 bf16 with a gate per element: forward 119 us, 5.6 TB/s; backward 195 us, 5.5 TB/s; their
 // bytes at 6.5 TB/s: 103 and 165).  Backward is at the registers' limit: the next row ahead of time spills, fewer registers
-// recompute.  A row stays in the registers of TPR threads (one wave up to 1024 channels forward, 512
+// recompute; and from 5121 channels on (a workgroup of 768 threads and more, 128 registers each) some kernels spill as they are, 1
+// to 10 registers of a lane, above 8192 (16 channels a thread) all of them, 49 to 98.  A row stays in the registers of TPR threads (one wave up to 1024 channels forward, 512
 // backward: no barrier), 16 bytes of the residual stream per access; a workgroup takes row after row with the weights of
 // its channels in LDS and, backward, their sums in registers; the workgroups' sums are joined in a fixed order by a second launch (7 us).
 #include <type_traits>
@@ -65,7 +66,7 @@ __device__ __forceinline__ void row_sums(float (&s)[N], float (*slots)[N]) {
 }
 
 // The gate of logits stored as B.  exp(-z) by the target's power of two alone is off by 2^-24 |z| relative to itself (60 units at
-// -80): a hundredth of a percent of what a bf16 logit's own rounding makes of it, but more than an fp32 result should be, so
+// -80): 2^-15 of what a bf16 logit's own rounding makes of it, but more than an fp32 result should be, so
 // fp32 logits take the exact one (8192 x 2048 all in fp32: 59 us forward and 100 backward both ways; for bf16 logits beside an
 // fp32 stream it would cost 2 to 7 %).  Below -87.3, where the gate is no normal number, it is zero.  1 - sigmoid, which the
 // gate's gradient takes, has the rounding of one: 2^-24 absolute.
@@ -468,9 +469,10 @@ static int workgroups(int64_t rows, int rows_each, int per_cu) {
     const int64_t n = (rows + rows_each - 1) / rows_each;
     return static_cast<int>(n < 256 * per_cu ? n : 256 * per_cu);
 }
-// Forward: as many as fit the CUs at once, and up to four times that where each still takes four rows for
+// Forward: 2048 threads a CU, and up to four times that where each still takes four rows for
 // each row's threads, to be worth the weights that it loads: 32768 x 4096 bf16 243 -> 231 us, 32768 x 2048 126 -> 119, 16384 x 4096
-// 122 -> 119.  Rows of more than 256 threads, whose weights are many: 16384 x 5120 166 -> 173, so not there.
+// 122 -> 119.  (Up to 512 channels 1792 to 2048 threads fit a CU at once; the registers of wider rows leave 1024 to 1536 there, and
+// the rest of the launch follows as workgroups end.)  Rows of more than 256 threads, whose weights are many: 16384 x 5120 166 -> 173, so not there.
 static int forward_workgroups(int64_t rows, int threads, int tpr) {
     const int each = threads / tpr, per_cu = 2048 / threads;
     const int once = workgroups(rows, each, per_cu), most = tpr > RN_THREADS ? 0 : workgroups(rows, 4 * each, 4 * per_cu);

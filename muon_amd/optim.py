@@ -524,9 +524,13 @@ class AdamW(_MuonBase):
     state_bits=32: `exp_avg` and `exp_avg_sq` in fp32.  state_bits=8: codes of 8 bits (uint8 tensors of the parameter's
     shape) with one shared power of two for every 128 consecutive elements (`exp_avg_exponent`, `exp_avg_sq_exponent`):
     `exp_avg` in the codes of float8_e4m3fn, `exp_avg_sq` with five bits of exponent, three of mantissa and no sign.  An
-    element's code is within 1/16 (on average over the steps: equal) of its moment from 2^-14 (2^-30) of the largest of
+    element's code is within 1/8 (on average over the steps: equal) of its moment from 2^-14 (2^-30) of the largest of
     its 128 upwards, and a multiple of 2^-17 (2^-33) of that power below.  Rounding is by a fixed dither of the element's
     place and the step, so a run repeats bit for bit.  A moment that is not finite makes its 128 elements NaN.
+
+    load_state_dict takes torch.optim.AdamW's states with state_bits=32 (16-bit ones are widened).  Parameters that share
+    memory are refused.  A HIP graph of the program may record step() over tensors that a step has seen: a replay repeats that
+    step, with its hyper-parameters and step count.
 
     grad_scale of step(): a one-element fp32 tensor on the device that multiplies the gradients on the way, as
     clip_coefficient returns it (or the inverse of a loss scale).  use_graph records the launch into a HIP graph and
