@@ -556,7 +556,7 @@ _TABLES_OF_GRAPHS = []
 def refuse_in_capture(what: str) -> None:
     """Before what a HIP graph must not record: a table's upload (a replay would read the host's buffer as it is then), or
     the zeros of a new state."""
-    if torch.cuda.is_current_stream_capturing():
+    if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
         raise _lib.MuonAmdError(f"{what} while a HIP graph is captured: take a step over the same tensors before")
 
 
