@@ -237,6 +237,31 @@ typedef struct MuonRoute {
     int32_t experts, k, dtype, normalize;
 } MuonRoute;
 
+/* How a loss over tokens is returned: each token's, their sum, or the mean over those that take part. */
+#define MUON_AMD_REDUCE_NONE 0
+#define MUON_AMD_REDUCE_SUM  1
+#define MUON_AMD_REDUCE_MEAN 2
+
+/* Distillation from a teacher's top logits, forward and backward (a host struct that is read during the call). */
+typedef struct MuonDistill {
+    const void* logits;          /* tokens x vocab of dtype, ld_logits elements from row to row   */
+    const void* teacher;         /* tokens x top of teacher_dtype: the teacher's logits           */
+    const void* indices;         /* tokens x top whole numbers of index_bits; outside 0 .. vocab - 1: not there */
+    const uint8_t* mask;         /* tokens bytes, zero: the token takes no part; NULL: all do     */
+    float* losses;               /* forward: tokens                                               */
+    float* loss;                 /* forward: one float, their sum or mean (NULL: not written)     */
+    float* part;                 /* one float: tokens that take part, at least 1                  */
+    float* stats;                /* tokens x 4: what backward needs of the softmaxes              */
+    float* partials;             /* forward: muon_amd_distill_partials() floats                   */
+    int32_t* counter;            /* forward: one word                                             */
+    const float* dloss;          /* backward: the gradient of loss, or (MUON_AMD_REDUCE_NONE) of losses, ld_dloss apart */
+    void* dlogits;               /* backward: tokens x vocab of dtype                             */
+    int64_t tokens, ld_logits, ld_teacher, ld_indices, ld_dloss;
+    int32_t vocab, top, dtype, teacher_dtype, index_bits, reduction;
+    float temperature;
+    int32_t reserved;
+} MuonDistill;
+
 /* One matrix of the AOL rescaling step of the 4-iteration variant (muon.py:776-785), in the
  * wide orientation: X is m_p x n_p with m_p <= n_p (zero padded).                           */
 typedef struct MuonAolDesc {
@@ -524,6 +549,16 @@ int     muon_amd_route_max_k(void);
 int64_t muon_amd_route_partials(int64_t tokens, int experts);
 int     muon_amd_route(const MuonRoute* args_host, void* stream);
 int     muon_amd_route_backward(const MuonRoute* args_host, void* stream);
+
+/* ---- distillation from a teacher's top logits -------------------------------------------------- */
+/* Per token: T^2 sum_k q_k (log q_k - log p_{i_k}) with p = softmax(logits / T), q = softmax(teacher / T) over the token's list.
+ * Entries whose index is outside of the vocabulary or whose logit is -infinity are not there; a token without any takes no
+ * part.  Backward reads what forward wrote.                                                        */
+size_t  muon_amd_sizeof_distill(void);
+int     muon_amd_distill_max_top(void);
+int64_t muon_amd_distill_partials(int64_t tokens, int vocab, int dtype);
+int     muon_amd_distill(const MuonDistill* args_host, void* stream);
+int     muon_amd_distill_backward(const MuonDistill* args_host, void* stream);
 
 #ifdef __cplusplus
 }

@@ -24,6 +24,7 @@ AOL_SYMMETRIC = 0
 AOL_ROWS_ONLY = 1
 SRC_F32 = 0
 SRC_BF16 = 1
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 # numpy mirrors of the C structs (align=True reproduces the C layout; sizes are checked against
 # the library's own sizeof at load time).
@@ -86,6 +87,14 @@ class RouteArgs(ctypes.Structure):
                                                 "dweights", "dbalance", "dz", "dlogits")] +
                 [(n, ctypes.c_int64) for n in ("tokens", "ld_logits", "ld_dweights")] +
                 [(n, ctypes.c_int32) for n in ("experts", "k", "dtype", "normalize")])
+
+
+class DistillArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "teacher", "indices", "mask", "losses", "loss", "part", "stats", "partials", "counter",
+                                                "dloss", "dlogits")] +
+                [(n, ctypes.c_int64) for n in ("tokens", "ld_logits", "ld_teacher", "ld_indices", "ld_dloss")] +
+                [(n, ctypes.c_int32) for n in ("vocab", "top", "dtype", "teacher_dtype", "index_bits", "reduction")] +
+                [("temperature", ctypes.c_float), ("reserved", ctypes.c_int32)])
 
 
 _c_int = ctypes.c_int
@@ -152,6 +161,11 @@ SIGNATURES = {
     "muon_amd_route_partials": (ctypes.c_int64, [ctypes.c_int64, _c_int]),
     "muon_amd_route": (_c_int, [ctypes.POINTER(RouteArgs), _vp]),
     "muon_amd_route_backward": (_c_int, [ctypes.POINTER(RouteArgs), _vp]),
+    "muon_amd_sizeof_distill": (ctypes.c_size_t, []),
+    "muon_amd_distill_max_top": (_c_int, []),
+    "muon_amd_distill_partials": (ctypes.c_int64, [ctypes.c_int64, _c_int, _c_int]),
+    "muon_amd_distill": (_c_int, [ctypes.POINTER(DistillArgs), _vp]),
+    "muon_amd_distill_backward": (_c_int, [ctypes.POINTER(DistillArgs), _vp]),
     "muon_amd_grad_clip": (_c_int, [_vp, _vp, _c_int, _c_int, _vp, _c_float, _vp, _vp]),
 }
 
@@ -186,7 +200,8 @@ def load():
                    (GRAD_DESC, lib.muon_amd_sizeof_grad_desc)):
         if dt.itemsize != fn():
             raise MuonAmdError(f"struct layout mismatch: binding {dt.itemsize} bytes, library {fn()}")
-    for struct, fn in ((ResidualNormArgs, lib.muon_amd_sizeof_residual_norm), (RouteArgs, lib.muon_amd_sizeof_route)):
+    for struct, fn in ((ResidualNormArgs, lib.muon_amd_sizeof_residual_norm), (RouteArgs, lib.muon_amd_sizeof_route),
+                       (DistillArgs, lib.muon_amd_sizeof_distill)):
         if ctypes.sizeof(struct) != fn():
             raise MuonAmdError(f"struct layout mismatch: binding {ctypes.sizeof(struct)} bytes, library {fn()}")
     _lib = lib

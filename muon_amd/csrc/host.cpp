@@ -42,13 +42,16 @@ struct Api {
     decltype(&muon_amd_route) route;
     decltype(&muon_amd_route_backward) route_backward;
     decltype(&muon_amd_route_partials) route_partials;
+    decltype(&muon_amd_distill) distill;
+    decltype(&muon_amd_distill_backward) distill_backward;
+    decltype(&muon_amd_distill_partials) distill_partials;
     decltype(&muon_amd_validate_grads) validate_grads;
     decltype(&muon_amd_grad_norm) grad_norm;
     decltype(&muon_amd_grad_clip) grad_clip;
     decltype(&muon_amd_validate_adamw_values) validate_adamw_values;
     decltype(&muon_amd_adamw_values) adamw_values;
     decltype(&muon_amd_adamw) adamw;
-    int max_width, max_experts, max_k, shared_elems, block_elems, norm_partials;
+    int max_width, max_experts, max_k, max_top, shared_elems, block_elems, norm_partials;
 } api{};
 
 struct LibraryError : std::runtime_error {
@@ -356,6 +359,111 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>> route_topk(con
     }
     const RouteOut o = route_forward(logits, k, mask.value_or(Tensor()), normalize);
     return std::make_tuple(o.weights, o.indices, o.counts, o.balance, o.z);
+}
+
+// ---- distill_topk ------------------------------------------------------------------------------------------------
+bool whole_numbers(const Tensor& t) { return t.is_cuda() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong); }
+int bits_of(const Tensor& t) { return t.scalar_type() == at::kLong ? 64 : 32; }
+
+struct DistillTensors {
+    Tensor logits, teacher, indices, mask, part, stats;         // (the mask may be undefined)
+};
+MuonDistill distill_args(const DistillTensors& t, int64_t reduction, double temperature, std::vector<Tensor>& keep) {
+    const auto hold = [&](Tensor r) -> const Tensor& {
+        keep.push_back(std::move(r));
+        return keep.back();
+    };
+    keep.reserve(4);
+    MuonDistill a{};
+    const Tensor& x = hold(rows_of(t.logits, t.logits.size(-1)));
+    const Tensor& v = hold(rows_of(t.teacher, t.teacher.size(-1)));
+    const Tensor& i = hold(rows_of(t.indices, t.indices.size(-1)));
+    a.logits = x.data_ptr();
+    a.teacher = v.data_ptr();
+    a.indices = i.data_ptr();
+    a.mask = t.mask.defined() ? static_cast<const uint8_t*>(hold(t.mask.contiguous()).data_ptr()) : nullptr;
+    a.part = t.part.data_ptr<float>();
+    a.stats = t.stats.data_ptr<float>();
+    a.tokens = x.size(0);
+    a.ld_logits = x.stride(0);
+    a.ld_teacher = v.stride(0);
+    a.ld_indices = i.stride(0);
+    a.vocab = static_cast<int32_t>(x.size(1));
+    a.top = static_cast<int32_t>(v.size(1));
+    a.dtype = dtype_of(t.logits);
+    a.teacher_dtype = dtype_of(t.teacher);
+    a.index_bits = bits_of(t.indices);
+    a.reduction = static_cast<int32_t>(reduction);
+    a.temperature = static_cast<float>(temperature);
+    return a;
+}
+
+// The loss; `t` gets what backward needs.
+Tensor distill_forward(DistillTensors& t, int64_t reduction, double temperature) {
+    const auto f32 = t.logits.options().dtype(at::kFloat);
+    const auto shape = t.logits.sizes().slice(0, t.logits.dim() - 1);
+    const int64_t vocab = t.logits.size(-1), tokens = t.logits.numel() / vocab;
+    if (tokens == 0) return reduction ? at::zeros({}, f32) : at::zeros(shape, f32);
+    Tensor losses = at::empty(shape, f32), loss = reduction ? at::empty({}, f32) : Tensor();
+    t.part = at::empty({}, f32);
+    t.stats = at::empty({tokens, 4}, f32);
+    const Tensor partials = at::empty({api.distill_partials(tokens, static_cast<int>(vocab), dtype_of(t.logits)) + 1}, f32);
+    std::vector<Tensor> keep;
+    MuonDistill a = distill_args(t, reduction, temperature, keep);
+    a.losses = losses.data_ptr<float>();
+    a.loss = reduction ? loss.data_ptr<float>() : nullptr;
+    a.partials = partials.data_ptr<float>();
+    a.counter = reinterpret_cast<int32_t*>(a.partials + partials.numel() - 1);
+    const c10::DeviceGuard guard(t.logits.device());
+    check(api.distill(&a, current_stream(t.logits.device())), "distill");
+    return reduction ? loss : losses;
+}
+
+struct DistillTopk : torch::autograd::Function<DistillTopk> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& indices, const std::optional<Tensor>& mask,
+                          int64_t reduction, double temperature) {
+        DistillTensors t{logits, teacher, indices, mask.value_or(Tensor()), Tensor(), Tensor()};
+        const Tensor loss = distill_forward(t, reduction, temperature);
+        ctx->saved_data["reduction"] = reduction;
+        ctx->saved_data["temperature"] = temperature;
+        ctx->save_for_backward({t.logits, t.teacher, t.indices, t.mask, t.part, t.stats});
+        return loss;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list douts) {
+        const variable_list saved = ctx->get_saved_variables();
+        const DistillTensors t{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5]};
+        Tensor dlogits = at::empty(t.logits.sizes(), t.logits.options());
+        if (t.stats.defined()) {
+            std::vector<Tensor> keep;
+            MuonDistill a = distill_args(t, ctx->saved_data["reduction"].toInt(), ctx->saved_data["temperature"].toDouble(), keep);
+            const Tensor dloss = a.reduction == MUON_AMD_REDUCE_NONE ? douts[0].reshape({a.tokens}) : douts[0];
+            a.dloss = dloss.data_ptr<float>();
+            a.ld_dloss = dloss.dim() ? dloss.stride(0) : 0;
+            a.dlogits = dlogits.data_ptr();
+            const c10::DeviceGuard guard(t.logits.device());
+            check(api.distill_backward(&a, current_stream(t.logits.device())), "distill_backward");
+        }
+        return once({dlogits, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, "the gradients of distill_topk are not differentiable");
+    }
+};
+
+// None where the arguments are not taken.
+std::optional<Tensor> distill_topk(const Tensor& logits, const Tensor& teacher, const Tensor& indices, double temperature, const std::optional<Tensor>& mask,
+                                   int64_t reduction) {
+    const auto device = logits.device();
+    const auto rows = [&](const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); };
+    if (!taken(logits) || !taken(teacher) || !whole_numbers(indices) || teacher.device() != device || indices.device() != device) return std::nullopt;
+    if (logits.dim() < 1 || teacher.dim() != logits.dim() || indices.sizes() != teacher.sizes() || rows(teacher) != rows(logits)) return std::nullopt;
+    if (logits.size(-1) < 1 || logits.size(-1) > (int64_t(1) << 30) || logits.numel() / logits.size(-1) > (int64_t(1) << 24) || teacher.size(-1) < 1 ||
+        teacher.size(-1) > api.max_top)
+        return std::nullopt;
+    if (mask && (mask->scalar_type() != at::kBool || mask->device() != device || mask->sizes() != rows(logits))) return std::nullopt;
+    // (a temperature whose reciprocal is no normal number would leave none)
+    if (!(temperature >= 1e-30 && temperature <= 1e30) || reduction < 0 || any_tangent({&logits, &teacher}) || any_requires_grad({&teacher})) return std::nullopt;
+    const py::gil_scoped_release released;
+    if (any_requires_grad({&logits})) return DistillTopk::apply(logits, teacher, indices, mask, reduction, temperature);
+    DistillTensors t{logits, teacher, indices, mask.value_or(Tensor()), Tensor(), Tensor()};
+    return distill_forward(t, reduction, temperature);
 }
 
 // ---- addresses of an optimizer's tensors -------------------------------------------------------------------------
@@ -713,6 +821,9 @@ void bind(const py::dict& addresses, const py::object& error) {
     get(api.route, "muon_amd_route");
     get(api.route_backward, "muon_amd_route_backward");
     get(api.route_partials, "muon_amd_route_partials");
+    get(api.distill, "muon_amd_distill");
+    get(api.distill_backward, "muon_amd_distill_backward");
+    get(api.distill_partials, "muon_amd_distill_partials");
     get(api.validate_grads, "muon_amd_validate_grads");
     get(api.grad_norm, "muon_amd_grad_norm");
     get(api.grad_clip, "muon_amd_grad_clip");
@@ -727,6 +838,7 @@ void bind(const py::dict& addresses, const py::object& error) {
     api.max_width = number("muon_amd_residual_norm_max_width");
     api.max_experts = number("muon_amd_route_max_experts");
     api.max_k = number("muon_amd_route_max_k");
+    api.max_top = number("muon_amd_distill_max_top");
     api.shared_elems = number("muon_amd_adamw_shared_elems");
     api.block_elems = number("muon_amd_elementwise_block_elems");
     api.norm_partials = number("muon_amd_grad_norm_partials");
@@ -737,6 +849,7 @@ void bind(const py::dict& addresses, const py::object& error) {
     };
     same("muon_amd_sizeof_residual_norm", sizeof(MuonResidualNorm));
     same("muon_amd_sizeof_route", sizeof(MuonRoute));
+    same("muon_amd_sizeof_distill", sizeof(MuonDistill));
     same("muon_amd_sizeof_grad_desc", sizeof(MuonGradDesc));
     same("muon_amd_sizeof_adamw_values_desc", sizeof(MuonAdamWValuesDesc));
     static PyObject* raised;
@@ -757,6 +870,7 @@ PYBIND11_MODULE(_native, m) {
     m.def("abi_version", [] { return MUON_AMD_ABI_VERSION; });
     m.def("residual_norm", &residual_norm);
     m.def("route_topk", &route_topk);
+    m.def("distill_topk", &distill_topk);
     m.def("adamw_launch", &adamw_launch);
     m.def("clip", &clip);
     m.def("clip_list", &clip_list);
