@@ -242,6 +242,27 @@ typedef struct MuonRoute {
 #define MUON_AMD_REDUCE_SUM  1
 #define MUON_AMD_REDUCE_MEAN 2
 
+/* Cross entropy of a linear head, forward and backward (a host struct that is read during the call). */
+typedef struct MuonHeadLoss {
+    const void* hidden;          /* tokens x width bf16, ld_hidden elements from row to row       */
+    const void* weight;          /* vocab x width bf16, ld_weight from row to row                 */
+    const void* targets;         /* tokens whole numbers of target_bits; ignore_index: the token takes no part */
+    float* losses;               /* forward: tokens (zero where one takes no part; NaN where a target is outside of the vocabulary) */
+    float* lse;                  /* forward: tokens, log sum exp of the logits (zero likewise)    */
+    float* loss;                 /* forward: one float, their sum or mean (NULL: not written)     */
+    float* part;                 /* one float: tokens that take part, at least 1                  */
+    int32_t* order;              /* tokens + 1: the rows of the products (kept for backward)      */
+    int32_t* rows;               /* tokens: their targets (kept)                                  */
+    float* stats;                /* tokens x 2: their maximum and the logarithm of their sum (kept) */
+    int32_t* counter;            /* forward: one word                                             */
+    void* workspace;             /* muon_amd_head_loss_workspace() bytes at a multiple of 256     */
+    const float* dloss;          /* backward: the gradient of loss, or (MUON_AMD_REDUCE_NONE) of losses, ld_dloss apart; NULL: zero */
+    const float* dlse;           /* backward: the gradient of lse, ld_dlse apart; NULL: zeros     */
+    void* dhidden;  void* dweight;       /* backward: tokens x width and vocab x width bf16; NULL is not written */
+    int64_t tokens, ld_hidden, ld_weight, ignore_index, workspace_bytes, ld_dloss, ld_dlse;
+    int32_t width, vocab, target_bits, reduction;
+} MuonHeadLoss;
+
 /* Distillation from a teacher's top logits, forward and backward (a host struct that is read during the call). */
 typedef struct MuonDistill {
     const void* logits;          /* tokens x vocab of dtype, ld_logits elements from row to row   */
@@ -549,6 +570,14 @@ int     muon_amd_route_max_k(void);
 int64_t muon_amd_route_partials(int64_t tokens, int experts);
 int     muon_amd_route(const MuonRoute* args_host, void* stream);
 int     muon_amd_route_backward(const MuonRoute* args_host, void* stream);
+
+/* ---- cross entropy of a linear head without its logits ------------------------------------------ */
+/* x = hidden weight^T;  lse = log sum exp(x);  loss = lse - x[target], fp32 sums of bf16 products.  Backward forms the logits again in
+ * pieces of the vocabulary and reads what forward wrote; its workspace differs from forward's.  */
+size_t  muon_amd_sizeof_head_loss(void);
+int64_t muon_amd_head_loss_workspace(const MuonHeadLoss* args_host, int backward);
+int     muon_amd_head_loss(const MuonHeadLoss* args_host, void* stream);
+int     muon_amd_head_loss_backward(const MuonHeadLoss* args_host, void* stream);
 
 /* ---- distillation from a teacher's top logits -------------------------------------------------- */
 /* Per token: T^2 sum_k q_k (log q_k - log p_{i_k}) with p = softmax(logits / T), q = softmax(teacher / T) over the token's list.

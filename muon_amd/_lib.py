@@ -89,6 +89,13 @@ class RouteArgs(ctypes.Structure):
                 [(n, ctypes.c_int32) for n in ("experts", "k", "dtype", "normalize")])
 
 
+class HeadLossArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("hidden", "weight", "targets", "losses", "lse", "loss", "part", "order", "rows", "stats", "counter",
+                                                "workspace", "dloss", "dlse", "dhidden", "dweight")] +
+                [(n, ctypes.c_int64) for n in ("tokens", "ld_hidden", "ld_weight", "ignore_index", "workspace_bytes", "ld_dloss", "ld_dlse")] +
+                [(n, ctypes.c_int32) for n in ("width", "vocab", "target_bits", "reduction")])
+
+
 class DistillArgs(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "teacher", "indices", "mask", "losses", "loss", "part", "stats", "partials", "counter",
                                                 "dloss", "dlogits")] +
@@ -161,6 +168,10 @@ SIGNATURES = {
     "muon_amd_route_partials": (ctypes.c_int64, [ctypes.c_int64, _c_int]),
     "muon_amd_route": (_c_int, [ctypes.POINTER(RouteArgs), _vp]),
     "muon_amd_route_backward": (_c_int, [ctypes.POINTER(RouteArgs), _vp]),
+    "muon_amd_sizeof_head_loss": (ctypes.c_size_t, []),
+    "muon_amd_head_loss_workspace": (ctypes.c_int64, [ctypes.POINTER(HeadLossArgs), _c_int]),
+    "muon_amd_head_loss": (_c_int, [ctypes.POINTER(HeadLossArgs), _vp]),
+    "muon_amd_head_loss_backward": (_c_int, [ctypes.POINTER(HeadLossArgs), _vp]),
     "muon_amd_sizeof_distill": (ctypes.c_size_t, []),
     "muon_amd_distill_max_top": (_c_int, []),
     "muon_amd_distill_partials": (ctypes.c_int64, [ctypes.c_int64, _c_int, _c_int]),
@@ -201,7 +212,7 @@ def load():
         if dt.itemsize != fn():
             raise MuonAmdError(f"struct layout mismatch: binding {dt.itemsize} bytes, library {fn()}")
     for struct, fn in ((ResidualNormArgs, lib.muon_amd_sizeof_residual_norm), (RouteArgs, lib.muon_amd_sizeof_route),
-                       (DistillArgs, lib.muon_amd_sizeof_distill)):
+                       (DistillArgs, lib.muon_amd_sizeof_distill), (HeadLossArgs, lib.muon_amd_sizeof_head_loss)):
         if ctypes.sizeof(struct) != fn():
             raise MuonAmdError(f"struct layout mismatch: binding {ctypes.sizeof(struct)} bytes, library {fn()}")
     _lib = lib

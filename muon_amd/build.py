@@ -24,12 +24,14 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmuon_amd.so")
 NATIVE_OUT = os.path.join(HERE, "_native.so")
 SOURCES = ["capi.hip", "elementwise.hip", "aol.hip", "ns_gemm.hip", "small.hip", "step.hip", "adamw.hip", "grad_norm.hip",
-           "residual.hip", "route.hip", "distill.hip"]
+           "residual.hip", "route.hip", "distill.hip", "head.hip"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # hipcc -O3 must not form packed-fp32 instructions on this target
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
+# The kernels whose LDS reads are waited for by hand.
+CHECKED = {"ns_gemm.hip": "ns_gemm_kernel", "head.hip": "head_gemm_kernel"}
 # The GEMM kernels' arguments arrive in scalar registers with the dispatch instead of through a load of each wave's own: 0.2 us
 # for each of the 15 dependent launches of a small matrix (768 x 3072: 174.8 -> 171.2 us, runs of one build differ by 0.1 %).  In a
 # step of one launch that does not show in the call (64 x 64 x 3 x 3: the kernel 37.0 -> 36.7 us, the call 47.6-48.3 -> 46.9-48.1 us
@@ -50,17 +52,17 @@ def _vregs(text: str) -> frozenset:
     return frozenset(out)
 
 
-def check_fragment_waits(asm_text: str) -> int:
-    """Walks the control-flow graph of every ns_gemm_kernel in a hipcc -S listing.  A register that an
+def check_fragment_waits(asm_text: str, kernel: str = "ns_gemm_kernel", source: str = "ns_gemm.hip") -> int:
+    """Walks the control-flow graph of every ns_gemm_kernel (or other `kernel`) in a hipcc -S listing.  A register that an
     inline-assembly LDS read (ds_read_b128, ds_read_b64_tr_b16) has requested is pending until a `s_waitcnt lgkmcnt(n)` leaves at
     most n younger requests outstanding (LDS reads return in order).  Raises if any instruction --
     a copy the register allocator put at a loop edge, an address computation, an MFMA -- names a
     pending register: it would see the register before its data.  Returns the number of such reads
     it followed."""
     lines = asm_text.split("\n")
-    starts = [i for i, l in enumerate(lines) if re.match(r"^_ZN8muon_amd14ns_gemm_kernel\S*:", l)]
+    starts = [i for i, l in enumerate(lines) if re.match(rf"^_ZN8muon_amd{len(kernel)}{kernel}\S*:", l)]
     if not starts:
-        raise RuntimeError("check_fragment_waits: no ns_gemm_kernel in the listing")
+        raise RuntimeError(f"check_fragment_waits: no {kernel} in the listing")
     nreads = 0
     for k0 in starts:
         instrs, labels, inasm = [], {}, False
@@ -91,7 +93,7 @@ def check_fragment_waits(asm_text: str) -> int:
                 elif op in ("ds_read_b128", "ds_read_b64_tr_b16") and from_asm:
                     dst, addr = t.split(None, 1)[1].split(",")[:2]
                     if any(p & _vregs(addr) for p in pend):
-                        raise RuntimeError(f"ns_gemm.hip: line {line_no} of the listing reads LDS through a pending register: {t}")
+                        raise RuntimeError(f"{source}: line {line_no} of the listing reads LDS through a pending register: {t}")
                     pend = pend + (_vregs(dst),)
                     nreads += 1
                 elif op == "s_endpgm":
@@ -104,7 +106,7 @@ def check_fragment_waits(asm_text: str) -> int:
                         stack.append((labels[t.split()[1]], pend))
                     elif pend and any(p & _vregs(t) for p in pend):
                         raise RuntimeError(
-                            f"ns_gemm.hip: line {line_no} of the listing touches a fragment register whose LDS read "
+                            f"{source}: line {line_no} of the listing touches a fragment register whose LDS read "
                             f"is still in flight: {t}")
                 pc += 1
     if nreads == 0:
@@ -112,7 +114,7 @@ def check_fragment_waits(asm_text: str) -> int:
     return nreads
 
 
-def check_store_data(asm_text: str) -> int:
+def check_store_data(asm_text: str, source: str = "ns_gemm.hip") -> int:
     """No vector instruction may overwrite a data register of a buffer, global or flat store of more than 8 bytes
     within two wait states of it: the store still reads that register for its last lanes.  The compiler
     leaves out those wait states after a buffer store with a scalar offset.  A vector instruction writes its first
@@ -132,7 +134,7 @@ def check_store_data(asm_text: str) -> int:
             op, _, args = u.partition(" ")
             written = args if re.match(r"v_(permlane\d+_)?swap", op) else args.split(",")[0]
             if op.startswith("v_") and _vregs(written) & data:
-                raise RuntimeError(f"ns_gemm.hip: '{u}' overwrites the data of '{t}' while it is read")
+                raise RuntimeError(f"{source}: '{u}' overwrites the data of '{t}' while it is read")
             states += int(args) + 1 if op == "s_nop" else 1
     return nstores
 
@@ -174,18 +176,20 @@ def build(verbose: bool = True, check: bool = True) -> str:
             raise RuntimeError("building libmuon_amd.so and _native.so failed")
     if check:
         with tempfile.TemporaryDirectory() as d:
-            listing = os.path.join(d, "ns_gemm.s")
             flags = [f for f in FLAGS if f not in ("-shared", "-fPIC")]
-            cmd = [hipcc, *flags, *SOURCE_FLAGS["ns_gemm.hip"], "-S", "--cuda-device-only", os.path.join(CSRC, "ns_gemm.hip"), "-o", listing]
-            proc = subprocess.run(cmd, capture_output=True, text=True)
-            if proc.returncode != 0:
-                sys.stderr.write(proc.stdout + proc.stderr)
-                raise RuntimeError("hipcc failed writing the assembly listing of ns_gemm.hip")
-            text = open(listing).read()
-            n = check_fragment_waits(text)
-            check_store_data(text)
-            if verbose:
-                print(f"ns_gemm.hip: {n} hand-waited fragment reads followed through the listing, none touched early", flush=True)
+            listings = {src: os.path.join(d, src + ".s") for src in CHECKED}
+            procs = {src: subprocess.Popen([hipcc, *flags, *SOURCE_FLAGS.get(src, []), "-S", "--cuda-device-only", os.path.join(CSRC, src), "-o", out],
+                                           stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for src, out in listings.items()}
+            outputs = {src: proc.communicate()[0] for src, proc in procs.items()}
+            for src, kernel in CHECKED.items():
+                if procs[src].returncode != 0:
+                    sys.stderr.write(outputs[src])
+                    raise RuntimeError(f"hipcc failed writing the assembly listing of {src}")
+                text = open(listings[src]).read()
+                n = check_fragment_waits(text, kernel, src)
+                check_store_data(text, src)
+                if verbose:
+                    print(f"{src}: {n} hand-waited fragment reads followed through the listing, none touched early", flush=True)
     os.replace(tmp, OUT)
     os.replace(native_tmp, NATIVE_OUT)
     return OUT

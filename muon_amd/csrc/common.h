@@ -34,6 +34,8 @@ int launch_norm_normalize(const MuonMatDesc* descs_dev, const int32_t* tile_pref
 
 // Raises the dynamic-LDS limit of the kernels of small.hip (part of muon_amd_init).
 int raise_small_limits();
+// The same for head.hip.
+int raise_head_limits();
 
 // ---- bf16 <-> fp32 -----------------------------------------------------------------------
 // bf16 values are carried as uint16_t (upper half of the fp32 pattern).  The fp32 -> bf16

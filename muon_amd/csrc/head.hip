@@ -1,0 +1,963 @@
+// Cross entropy of a linear head over a large vocabulary, without its logits.  Over N tokens of D channels h, a matrix W of
+// V rows, targets t:
+//   x_nv = h_n . W_v,  lse_n = log sum_v exp(x_nv),  loss_n = lse_n - x_{n, t_n}
+// Backward, from the gradients g_n of loss_n and z_n of lse_n:
+//   e_nv = (g_n + z_n) exp(x_nv - lse_n) - g_n [v = t_n],   dh_n = sum_v e_nv W_v,   dW_v = sum_n e_nv h_n
+//
+// Forward is one matrix product whose epilogue leaves the maximum and the sum of exponentials of each row of its tile, 8 bytes for
+// 256 logits, joined by a second launch.  Backward goes through the vocabulary in pieces: the logits of a piece are formed again
+// (the same product, so the same bits), e is written once in bf16 (a relative rounding of 2^-9 of each term of sums over the
+// vocabulary or the tokens, next to the 2^-9 of h and W themselves), and two products follow, whose second operand (and for
+// dW the first one too) lies k-major and is read through transposing LDS reads, so nothing is written twice.  8 N V D operations
+// instead of the 6 N V D of a backward pass that keeps N V logits.
+//
+// Tokens that are ignored leave the products: a first launch numbers those that take part, and their hidden states are copied
+// to consecutive rows (zeros up to whole tiles).  The products take the tokens' number from the device; workgroups beyond it end
+// at once.  Up to 64 tokens forward (evaluation, single tokens) the matrix is streamed once through registers instead.
+//
+// The products bound everything: matrix instructions at 256 x 256 tiles of 8 waves, k-blocks of 64 in an LDS ring filled by
+// buffer_load ... lds a block and a half ahead, as in ns_gemm.hip.
+#include <stdlib.h>
+
+#include "lanes.h"
+#include "tile.h"
+
+namespace muon_amd {
+
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
+constexpr int HD_TILE = 256;                        // rows of the copy of the hidden states are padded to this
+constexpr int HD_FEW = 64;                          // tokens that the streaming kernel takes
+
+// ---------------------------------------------------------------------------------------------
+// The products
+// ---------------------------------------------------------------------------------------------
+enum HeadProduct {
+    HEAD_STATS,      // x = h W^T: row statistics
+    HEAD_GRAD,       // x = h W^T again: e
+    HEAD_DHIDDEN,    // e W, a share of the vocabulary
+    HEAD_DWEIGHT,    // e^T h
+};
+
+// acc[i][j] = sum_k P(i, k) Q(j, k).  An operand is row-major (k along the row) or k-major; `end_*` is the byte offset of the last
+// 16 bytes that may be read from the base: what lies beyond (rows and columns of a tile that are in no output, rows that
+// meet zeros of the other operand) is read from there instead.
+struct HeadGemm {
+    const uint16_t* P;
+    const uint16_t* Q;
+    int64_t ldp, ldq;
+    int64_t end_p, end_q;
+    const int32_t* count;          // tokens that take part
+    int row_tiles, col_tiles, splits;   // (row_tiles of a product over tokens: at most; the count decides)
+    int rows, cols, kblocks;       // rows / cols of the output (rows of a product over tokens: from the count), k-blocks (HEAD_DWEIGHT: from the count)
+    int col_limit;                 // columns of a k-major Q row that may be read
+    int row_limit;                 // likewise of a k-major P row
+    // HEAD_STATS, HEAD_GRAD
+    int vocab_begin, vocab;        // first column in the vocabulary, size of the vocabulary
+    const int32_t* target;         // of each row
+    f32x2_t* stats;                // [column tile][row]: maximum, sum of 2^((x - maximum) log2 e)
+    float* target_logit;
+    int64_t ld_stats;
+    const f32x4v* coef;            // of each row: g + z, g, the row's maximum, log2 of its sum
+    // outputs
+    uint16_t* out;                 // HEAD_GRAD, HEAD_DWEIGHT
+    float* part;                   // HEAD_DHIDDEN: [split][row][column]
+    int64_t ld_out, part_stride;
+    int add;                       // HEAD_DHIDDEN: to what a piece before left there
+};
+
+template <int BT_, int WGM_, int WGN_, int MINB_, int NHALF_>
+struct HeadCfg {
+    static constexpr int BT = BT_, WGM = WGM_, WGN = WGN_, MINB = MINB_, NHALF = NHALF_;
+    static constexpr int NW = WGM * WGN, NT = NW * 64, WM = BT / WGM, WN = BT / WGN, TM = WM / 32, TN = WN / 32;
+    static constexpr int HALF_BYTES = BT * ROW_BYTES, DPH = BT / 8 / NW, RING = (NHALF - 1) / 2;
+    static constexpr size_t LDS_BYTES = static_cast<size_t>(NHALF) * HALF_BYTES;
+    static_assert(WN == 64, "an epilogue's strip is 64 columns");
+    static_assert(RING == 2 && NHALF % 2 == 1, "one copy of the k-block for each of the last two");
+    static_assert(LDS_BYTES * MINB <= 163840, "LDS of a CU");
+};
+typedef HeadCfg<256, 2, 4, 1, 5> HeadLarge;
+typedef HeadCfg<128, 2, 2, 2, 5> HeadSmall;
+
+// Tile `t` of row_tiles x col_tiles: strips of 8 column tiles, row by row, so that 32 neighbours are 4 x 8 tiles.
+struct TileAt {
+    int row, col;
+};
+__device__ __forceinline__ TileAt tile_at(int t, int row_tiles, int col_tiles) {
+    const int strip = t / (8 * row_tiles), first = strip * 8, width = min(8, col_tiles - first), in = t - first * row_tiles;
+    return {in / width, first + in % width};
+}
+// Workgroup b of `total` to its place in that order: workgroups are dealt to the eight XCDs in turn, and each XCD gets runs of 32
+// neighbours, which share operand panels in its L2 (what is left over after whole sets of eight runs: one run for each XCD).
+__device__ __forceinline__ int place_of(int b, int total) {
+    const int full = total / 256 * 256;
+    const int x = b % 8, s = b / 8;
+    if (b < full) return ((s / 32) * 8 + x) * 32 + s % 32;
+    const int rem = total - full;
+    return full + x * (rem / 8) + min(x, rem % 8) + (b - full) / 8;
+}
+
+// Fragments of one k-step for a side of the product: N fragments, row-major or k-major.
+template <int N, bool K>
+struct Frags {
+    u32x4 row[K ? 1 : N];
+    u32x2 tr[K ? 2 * N : 1];
+    __device__ __forceinline__ u32x4 get(int i) const {
+        if constexpr (K) return u32x4{tr[2 * i].x, tr[2 * i].y, tr[2 * i + 1].x, tr[2 * i + 1].y};
+        else return row[i];
+    }
+};
+// The wait for the older fragments while CNT younger reads are in flight, tied to their registers.
+template <int CNT, typename A, typename B>
+__device__ __forceinline__ void wait_both(A& a, B& b) {
+    constexpr bool ka = sizeof(a.tr) > sizeof(u32x2), kb = sizeof(b.tr) > sizeof(u32x2);
+    if constexpr (!ka && !kb) {
+        wait_frags<CNT>(a.row, b.row);
+    } else if constexpr (!ka) {
+        wait_frags_tr<CNT>(a.row, b.tr);
+    } else if constexpr (sizeof(a.tr) / sizeof(u32x2) == 8) {
+        static_assert(sizeof(b.tr) / sizeof(u32x2) == 4, "operand lists below");
+        asm volatile("s_waitcnt lgkmcnt(%12)"
+                     : "+v"(a.tr[0]), "+v"(a.tr[1]), "+v"(a.tr[2]), "+v"(a.tr[3]), "+v"(a.tr[4]), "+v"(a.tr[5]), "+v"(a.tr[6]), "+v"(a.tr[7]),
+                       "+v"(b.tr[0]), "+v"(b.tr[1]), "+v"(b.tr[2]), "+v"(b.tr[3])
+                     : "n"(CNT));
+    } else {
+        static_assert(sizeof(a.tr) / sizeof(u32x2) == 4 && sizeof(b.tr) / sizeof(u32x2) == 4, "operand lists below");
+        asm volatile("s_waitcnt lgkmcnt(%8)"
+                     : "+v"(a.tr[0]), "+v"(a.tr[1]), "+v"(a.tr[2]), "+v"(a.tr[3]), "+v"(b.tr[0]), "+v"(b.tr[1]), "+v"(b.tr[2]), "+v"(b.tr[3])
+                     : "n"(CNT));
+    }
+}
+
+// An operand's half-stages: where a lane's pieces lie from the tile's base, and how the base moves from k-block to k-block.
+template <typename Cfg, bool K>
+struct Source {
+    uint32_t off[Cfg::DPH];
+    uint64_t base;                 // (wave-uniform)
+    int64_t step, end;
+    // first: the tile's first row (k-major: column); limit: columns of a k-major row that may be read
+    __device__ __forceinline__ void set(const uint16_t* p, int64_t ld, int64_t end_bytes, int first, int limit, int k0, int lane, int wave) {
+        constexpr int ROWK = Cfg::BT * 2;
+        const int gchunk = (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4));
+        const int64_t corner = K ? (static_cast<int64_t>(k0) * ld + first) * 2 : (static_cast<int64_t>(first) * ld + k0) * 2;
+#pragma unroll
+        for (int j = 0; j < Cfg::DPH; ++j) {
+            if constexpr (K) {
+                const int o = (j * Cfg::NW + wave) * 1024 + lane * 16, k = o / ROWK, w = o % ROWK;
+                const int col = ((w / 64) ^ (k & 3)) * 32 + ((w % 64) >> 1);
+                off[j] = static_cast<uint32_t>((k * ld + min(col, limit - first - 8)) * 2);
+            } else {
+                const int r = (j * Cfg::NW + wave) * 8 + (lane >> 3);
+                off[j] = static_cast<uint32_t>((r * ld + gchunk * 8) * 2);
+            }
+        }
+        base = reinterpret_cast<uint64_t>(p) + corner;
+        end = end_bytes - corner;
+        step = K ? BK * ld * 2 : BK * 2;
+    }
+    // Piece j of k-block kb.
+    __device__ __forceinline__ void issue(int j, int kb, uint32_t lds_addr) const {
+        const int64_t moved = kb * step, left = end - moved;
+        const uint64_t b = base + moved;
+        const u32x4 rsrc = {static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
+        const uint32_t last = left > 0xfffffff0ll ? 0xfffffff0u : static_cast<uint32_t>(left);
+        dma16(rsrc, min(off[j], last), 0u, lds_addr);
+    }
+};
+
+template <typename Cfg, int PRODUCT>
+__global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const HeadGemm a) {
+    constexpr int NW = Cfg::NW, WGN = Cfg::WGN, WM = Cfg::WM, WN = Cfg::WN, TM = Cfg::TM, TN = Cfg::TN, NHALF = Cfg::NHALF;
+    constexpr int HALF_BYTES = Cfg::HALF_BYTES, DPH = Cfg::DPH, RING = Cfg::RING, ROWK = Cfg::BT * 2;
+    constexpr bool PK = PRODUCT == HEAD_DWEIGHT, QK = PRODUCT == HEAD_DHIDDEN || PRODUCT == HEAD_DWEIGHT;
+    extern __shared__ __align__(16) uint16_t lds[];
+    const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint16_t*)lds));
+    const int count = *a.count;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WGN, wn = wave % WGN;
+    const int rows = PRODUCT == HEAD_DWEIGHT ? a.rows : count;
+    const int row_tiles = (rows + Cfg::BT - 1) / Cfg::BT, tiles = row_tiles * a.col_tiles;
+    const int id = static_cast<int>(blockIdx.x);
+    if (id >= tiles * a.splits) return;
+    const int place = place_of(id, tiles * a.splits), split = place / tiles;
+    const TileAt tile = tile_at(place - split * tiles, row_tiles, a.col_tiles);
+    const int i0 = tile.row * Cfg::BT, j0 = tile.col * Cfg::BT;
+    // k-blocks of this share
+    const int all = PRODUCT == HEAD_DWEIGHT ? (count + BK - 1) / BK : a.kblocks;
+    const int k0 = static_cast<int>(static_cast<int64_t>(all) * split / a.splits), nk = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - k0;
+
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int x = 0; x < TM; ++x)
+#pragma unroll
+        for (int y = 0; y < TN; ++y)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[x][y][i] = 0.f;
+
+    if (nk > 0) {
+        Source<Cfg, PK> sp_;
+        Source<Cfg, QK> sq_;
+        sp_.set(a.P, a.ldp, a.end_p, i0, a.row_limit, k0 * BK, lane, wave);
+        sq_.set(a.Q, a.ldq, a.end_q, j0, a.col_limit, k0 * BK, lane, wave);
+        const uint32_t dst0 = lds_base + wave * 1024;
+#pragma unroll
+        for (int h = 0; h < NHALF; ++h)
+            if (h < 2 * nk) {
+#pragma unroll
+                for (int j = 0; j < DPH; ++j) {
+                    if (h & 1) sq_.issue(j, h >> 1, dst0 + h * HALF_BYTES + j * NW * 1024);
+                    else sp_.issue(j, h >> 1, dst0 + h * HALF_BYTES + j * NW * 1024);
+                }
+            }
+
+        const int swz = (lane >> 1) & 7, c0 = (lane >> 5) ^ swz, r4 = (lane & 15) >> 2;
+        const int koff[4] = {c0 * 16, (c0 ^ 2) * 16, (c0 ^ 4) * 16, (c0 ^ 6) * 16};
+        const uint32_t pfrag = lds_base + (wm * WM + (lane & 31)) * ROW_BYTES, qfrag = lds_base + (wn * WN + (lane & 31)) * ROW_BYTES;
+        uint32_t ptr_off[TM], qtr_off[TN];
+#pragma unroll
+        for (int x = 0; x < TM; ++x)
+            ptr_off[x] = ((lane >> 5) * 8 + r4) * ROWK + (lane & 3) * 8 + ((wm * (WM / 32) + x) ^ r4) * 64 + ((lane >> 4) & 1) * 32;
+#pragma unroll
+        for (int y = 0; y < TN; ++y)
+            qtr_off[y] = ((lane >> 5) * 8 + r4) * ROWK + (lane & 3) * 8 + ((wn * (WN / 32) + y) ^ r4) * 64 + ((lane >> 4) & 1) * 32;
+
+        if (2 * nk >= NHALF) NS_WAIT_VMCNT((NHALF - 2) * DPH);
+        else NS_WAIT_VMCNT(0);
+        __syncthreads();
+
+        // The loop is that of ns_gemm_kernel: fragments double buffered over k-steps across blocks, reads and waits written out, the
+        // transfers of a pair of half-stages spread over four k-steps (there: why each is where it is).
+        Frags<TM, PK> af[2];
+        Frags<TN, QK> bf[2];
+        constexpr int KSTEPS = BK / 16, NFRAG = (PK ? 2 * TM : TM) + (QK ? 2 * TN : TN), DPK = 2 * DPH / KSTEPS;
+        static_assert(NFRAG < 16 && 2 * DPH % KSTEPS == 0 && DPH % DPK == 0 && DPK <= TM, "reads in flight, transfers per k-step");
+        const auto load = [&](int buf, int sp, int sq, int ks) __attribute__((always_inline)) {
+            if constexpr (PK) FragLoadTr<TM, ROWK>::run(af[buf].tr, ptr_off, lds_base + sp * HALF_BYTES + ks * 16 * ROWK);
+            else FragLoad<TM>::run(af[buf].row, pfrag + sp * HALF_BYTES + koff[ks]);
+            if constexpr (QK) FragLoadTr<TN, ROWK>::run(bf[buf].tr, qtr_off, lds_base + sq * HALF_BYTES + ks * 16 * ROWK);
+            else FragLoad<TN>::run(bf[buf].row, qfrag + sq * HALF_BYTES + koff[ks]);
+        };
+        const auto multiply = [&](int x, int buf) __attribute__((always_inline)) {
+#pragma unroll
+            for (int y = 0; y < TN; ++y)
+                acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, bf[buf].get(y)),
+                                                                    __builtin_bit_cast(bf16x8, af[buf].get(x)), acc[x][y], 0, 0, 0);
+        };
+        uint32_t ddst[2] = {0, 0};
+        int dk[2] = {0, 0};
+        const auto transfer = [&](int jj) __attribute__((always_inline)) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (jj / DPH == 0) sq_.issue(jj % DPH, dk[0], ddst[0] + (jj % DPH) * NW * 1024);
+            else sp_.issue(jj % DPH, dk[1], ddst[1] + (jj % DPH) * NW * 1024);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        load(0, 0, 1, 0);
+        wait_both<0>(af[0], bf[0]);
+        int sp = 0, sq = 1, kb = 0;
+        const auto block = [&](auto more) __attribute__((always_inline)) {
+            constexpr int MORE = decltype(more)::value;
+            int spn = sp + 2, sqn = sq + 2;
+            spn = spn >= NHALF ? spn - NHALF : spn;
+            sqn = sqn >= NHALF ? sqn - NHALF : sqn;
+#pragma unroll
+            for (int ks = 0; ks + 1 < KSTEPS; ++ks) {
+                const int cur = ks & 1, nxt = cur ^ 1;
+                load(nxt, sp, sq, ks + 1);
+                wait_both<NFRAG>(af[cur], bf[cur]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < TM; ++x) {
+                    multiply(x, cur);
+                    if (x < DPK && kb > 0 && (MORE == RING || (MORE == RING - 1 && (ks + 1) * DPK + x < DPH))) transfer((ks + 1) * DPK + x);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            constexpr int cur = (KSTEPS - 1) & 1, nxt = cur ^ 1;
+            wait_both<0>(af[cur], bf[cur]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < TM / 2; ++x) multiply(x, cur);
+            __builtin_amdgcn_sched_barrier(0);
+            if (MORE > 0) {
+                NS_WAIT_VMCNT((MORE == RING ? NHALF - 4 : MORE > 0 ? 2 * MORE - 2 : 0) * DPH);
+                __builtin_amdgcn_s_barrier();
+                const int h0 = 2 * kb + NHALF;
+                ddst[0] = dst0 + sp * HALF_BYTES;
+                ddst[1] = dst0 + sq * HALF_BYTES;
+                dk[0] = h0 >> 1;
+                dk[1] = (h0 + 1) >> 1;
+                load(nxt, spn, sqn, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int x = TM / 2; x < TM; ++x) {
+                multiply(x, cur);
+                if (MORE == RING) {
+#pragma unroll
+                    for (int jj = 0; jj < DPK; ++jj)
+                        if (jj * (TM - TM / 2) / DPK == x - TM / 2) transfer(jj);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (MORE > 0) wait_both<0>(af[0], bf[0]);
+            sp = spn;
+            sq = sqn;
+        };
+        for (; kb < nk - RING; ++kb) block(std::integral_constant<int, RING>{});
+        if (nk - kb == 2) {
+            block(std::integral_constant<int, 1>{});
+            ++kb;
+        }
+        block(std::integral_constant<int, 0>{});
+        __syncthreads();            // every wave is done with the ring
+    }
+
+    // ---- epilogue: a lane's accumulators are 4 x 4 columns of row lane % 32 in each 32 x 32 tile --------------------
+    int tid_e = threadIdx.x;
+    asm volatile("" : "+v"(tid_e));            // (nothing of it is formed ahead of the loop and kept there)
+    const int lane_e = tid_e & 63, lr = lane_e & 31, g = lane_e >> 5;
+    const int row0 = i0 + wm * WM, col0 = j0 + wn * WN;
+    if constexpr (PRODUCT == HEAD_STATS) {
+        // columns beyond the vocabulary do not count
+        const int limit = a.vocab - col0;
+        f32x2_t* const red = reinterpret_cast<f32x2_t*>(lds);               // [wave column][row of the tile]
+#pragma unroll
+        for (int x = 0; x < TM; ++x) {
+            if (limit < WN) {
+#pragma unroll
+                for (int y = 0; y < TN; ++y)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (y * 32 + (i / 4) * 8 + g * 4 + i % 4 >= limit) acc[x][y][i] = -__builtin_inff();
+            }
+            float m = acc[x][0][0];
+#pragma unroll
+            for (int y = 0; y < TN; ++y)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, acc[x][y][i]);
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            const float ref = m == -__builtin_inff() ? 0.f : m;
+            float s = 0.f;
+#pragma unroll
+            for (int y = 0; y < TN; ++y)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s += __builtin_amdgcn_exp2f((acc[x][y][i] - ref) * LOG2E);
+            s += __shfl_xor(s, 32, 64);
+            if (g == 0) red[wn * Cfg::BT + wm * WM + x * 32 + lr] = f32x2_t{m, s};
+            // the target's logit, where it is one of these columns
+            const int row = row0 + x * 32 + lr, at = row < rows ? a.target[row] - col0 : -1;
+            const bool mine = at >= 0 && at < WN && ((at >> 2) & 1) == g;
+            if (__ballot(mine)) {
+                float value = 0.f;
+#pragma unroll
+                for (int y = 0; y < TN; ++y)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (y * 32 + (i / 4) * 8 + g * 4 + i % 4 == at) value = acc[x][y][i];
+                if (mine) a.target_logit[row] = value;
+            }
+        }
+        __syncthreads();
+        for (int r = tid_e; r < Cfg::BT; r += Cfg::NT) {
+            float m = red[r][0], s = red[r][1];
+#pragma unroll
+            for (int w = 1; w < WGN; ++w) {
+                const f32x2_t o = red[w * Cfg::BT + r];
+                const float top = fmaxf(m, o[0]), ref = top == -__builtin_inff() ? 0.f : top;
+                s = s * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + o[1] * __builtin_amdgcn_exp2f((o[0] - ref) * LOG2E);
+                m = top;
+            }
+            if (i0 + r < rows) a.stats[tile.col * a.ld_stats + i0 + r] = f32x2_t{m, s};
+        }
+    } else if constexpr (PRODUCT == HEAD_DHIDDEN) {
+        float* const part = a.part + split * a.part_stride;
+#pragma unroll
+        for (int x = 0; x < TM; ++x) {
+            const int row = row0 + x * 32 + lr;
+            if (row >= rows) continue;
+#pragma unroll
+            for (int y = 0; y < TN; ++y)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int col = col0 + y * 32 + q * 8 + g * 4;           // (the columns are padded to 64)
+                    if (col >= a.cols) continue;
+                    f32x4v v = {acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2], acc[x][y][4 * q + 3]};
+                    float* const at = part + row * a.ld_out + col;
+                    if (a.add) v += load_as<false, f32x4v>(at);
+                    store_as<false>(at, v);
+                }
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < TM; ++x) {
+            const int row = row0 + x * 32 + lr;
+            [[maybe_unused]] float both = 0.f, own = 0.f, m = 0.f, l = 0.f;
+            [[maybe_unused]] int at = -1;
+            if constexpr (PRODUCT == HEAD_GRAD) {
+                // (rows of the tile beyond the tokens are rows of zeros, and so are their coefficients)
+                const f32x4v c = a.coef[row];
+                both = c[0];
+                own = c[1];
+                m = c[2];
+                l = c[3];
+                at = row < rows ? a.target[row] - a.vocab_begin - col0 : -1;
+            }
+#pragma unroll
+            for (int y = 0; y < TN; ++y) {
+                uint32_t po[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    float v[2] = {acc[x][y][2 * k], acc[x][y][2 * k + 1]};
+                    if constexpr (PRODUCT == HEAD_GRAD) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int c = y * 32 + (k / 2) * 8 + g * 4 + (k % 2) * 2 + i;
+                            v[i] = both * __builtin_amdgcn_exp2f((v[i] - m) * LOG2E - l) - (c == at ? own : 0.f);
+                            if (a.vocab_begin + col0 + c >= a.vocab) v[i] = 0.f;
+                        }
+                    }
+                    po[k] = pack2bf(v[0], v[1]);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; q += 2) {
+                    const auto u = __builtin_amdgcn_permlane32_swap(po[2 * q], po[2 * q + 2], false, false);
+                    const auto w = __builtin_amdgcn_permlane32_swap(po[2 * q + 1], po[2 * q + 3], false, false);
+                    const Pack<uint16_t, 8> v = {{u[0], w[0], u[1], w[1]}};
+                    const int col = col0 + y * 32 + (q + g) * 8;
+                    if (PRODUCT == HEAD_GRAD || row < rows) store_pack<uint16_t, 8, false>(a.out + row * a.ld_out, col, a.cols, v);
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Few tokens: W streamed through registers
+// ---------------------------------------------------------------------------------------------
+// A workgroup takes 64 rows of W, its four waves every fourth block of 64 channels: fragments of 16 rows x 32 channels straight from
+// memory (a 128-byte line of a row is two of them), against those of up to 64 tokens, which the caches hold.  The waves'
+// sums are added in LDS.  W's bytes bound it.
+constexpr int HF_THREADS = 256, HF_VOCAB = 64;
+typedef float f32x4a __attribute__((ext_vector_type(4)));
+template <int NT, bool TAIL>
+__device__ __forceinline__ bf16x8 few_chunk(const uint16_t* row, int k, int width) {
+    if constexpr (!TAIL) return __builtin_bit_cast(bf16x8, Pack<uint16_t, 8>::load<false>(row + k).v);
+    else return __builtin_bit_cast(bf16x8, load_pack<uint16_t, 8, false>(row, k, width).v);
+}
+template <int NT>
+__global__ __launch_bounds__(HF_THREADS) void head_few_kernel(const uint16_t* hidden, int64_t ld_hidden, const uint16_t* weight, int64_t ld_weight, int tokens,
+                                                              int width, int vocab, const void* targets, int target_bits, f32x2_t* stats, int64_t ld_stats,
+                                                              float* target_logit) {
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    // a row's columns exchanged by its number, four at a time: the lanes of a token's 16 then write to different banks
+    __shared__ float sums[4][16 * NT][HF_VOCAB];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = (lane >> 4) * 8;
+    const int v0 = blockIdx.x * HF_VOCAB;
+    const uint16_t* wrow[4];
+    const uint16_t* hrow[NT];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) wrow[f] = weight + min(v0 + 16 * f + r, vocab - 1) * ld_weight;
+#pragma unroll
+    for (int f = 0; f < NT; ++f) hrow[f] = hidden + min(16 * f + r, tokens - 1) * ld_hidden;
+    f32x4a acc[4][NT];
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[f][t] = f32x4a{0.f, 0.f, 0.f, 0.f};
+    const auto steps = [&](auto tail, int k) __attribute__((always_inline)) {
+        constexpr bool TAIL = decltype(tail)::value;
+        bf16x8 w[2][4], h[2][NT];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int f = 0; f < 4; ++f) w[s][f] = few_chunk<NT, TAIL>(wrow[f], k + 32 * s + kq, width);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) h[s][t] = few_chunk<NT, TAIL>(hrow[t], k + 32 * s + kq, width);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[s][f], h[s][t], acc[f][t], 0, 0, 0);
+    };
+    const int whole = width / 64;
+#pragma unroll 2
+    for (int b = wave; b < whole; b += 4) steps(std::false_type{}, b * 64);
+    if (width % 64 && wave == whole % 4) steps(std::true_type{}, whole * 64);
+    // a lane holds rows 4 (lane / 16) .. + 3 of W for token lane % 16
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+*reinterpret_cast<f32x4a*>(&sums[wave][16 * t + r][(16 * f + 4 * (lane >> 4)) ^ (r << 2)]) = acc[f][t];
+    __syncthreads();
+    for (int t = wave; t < tokens; t += 4) {
+        const int v = v0 + lane;
+        const int at = lane ^ ((t & 15) << 2);
+        float x = (sums[0][t][at] + sums[1][t][at]) + (sums[2][t][at] + sums[3][t][at]);
+        if (v >= vocab) x = -__builtin_inff();
+        const int64_t target = target_bits == 64 ? static_cast<const int64_t*>(targets)[t] : static_cast<const int32_t*>(targets)[t];
+        if (v == target) target_logit[t] = x;
+        const float m = group_reduce<64>(x, [](float p, float q) { return fmaxf(p, q); });
+        const float s = group_sum<64>(__builtin_amdgcn_exp2f((x - (m == -__builtin_inff() ? 0.f : m)) * LOG2E));
+        if (lane == 0) stats[blockIdx.x * ld_stats + t] = f32x2_t{m, s};
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// The launches around the products
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ int64_t target_of(const MuonHeadLoss& a, int64_t t) {
+    return a.target_bits == 64 ? static_cast<const int64_t*>(a.targets)[t] : static_cast<const int32_t*>(a.targets)[t];
+}
+// A target as the other kernels see it: -1 where it is outside of the vocabulary.
+__device__ __forceinline__ int target_in(const MuonHeadLoss& a, int64_t target) { return target >= 0 && target < a.vocab ? static_cast<int>(target) : -1; }
+
+// Numbers the tokens that take part, in order: order[row] = token for the first `count` rows, after them ~token of the ignored
+// ones (whose outputs are written here); rows[row] = target.  order[tokens] = count.  COMPACT: otherwise every token keeps its row, order[token]
+// = ~token where it is ignored, and the count is the number of tokens.
+constexpr int HO_THREADS = 1024;
+template <bool COMPACT>
+__global__ __launch_bounds__(HO_THREADS) void head_order_kernel(const MuonHeadLoss a) {
+    __shared__ int before[HO_THREADS / 64 + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t each = (a.tokens + HO_THREADS - 1) / HO_THREADS, begin = min(threadIdx.x * each, a.tokens), end = min(begin + each, a.tokens);
+    int n = 0;
+    for (int64_t t = begin; t < end; ++t) n += target_of(a, t) != a.ignore_index;
+    int upto = n;                                            // of this lane and those before it
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += o;
+    }
+    if (lane == 63) before[wave + 1] = upto;
+    if (threadIdx.x == 0) before[0] = 0;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int w = 0; w < HO_THREADS / 64; ++w) before[w + 1] += before[w];
+    __syncthreads();
+    const int count = before[HO_THREADS / 64];
+    int64_t at = before[wave] + upto - n, out = count + (begin - at);
+    for (int64_t t = begin; t < end; ++t) {
+        const int64_t target = target_of(a, t);
+        const bool on = target != a.ignore_index;
+        const int64_t row = COMPACT ? (on ? at++ : out++) : t;
+        a.order[row] = static_cast<int32_t>(on ? t : ~t);
+        a.rows[row] = on ? target_in(a, target) : -1;
+        if (!on) {
+            a.losses[t] = 0.f;
+            a.lse[t] = 0.f;
+        }
+    }
+    if (threadIdx.x == 0) {
+        a.order[a.tokens] = static_cast<int32_t>(COMPACT ? count : a.tokens);
+        *a.part = static_cast<float>(count > 0 ? count : 1);
+        *a.counter = 0;
+    }
+}
+
+// The hidden states of the rows, in bf16 rows of `ld` elements with zeros beyond the width, up to a whole tile of rows; backward their
+// coefficients too.  A wave for each row.
+__global__ __launch_bounds__(256) void head_gather_kernel(const MuonHeadLoss a, uint16_t* rows, int ld, f32x4v* coef) {
+    const int lane = threadIdx.x & 63;
+    const int64_t count = a.order[a.tokens], padded = (count + HD_TILE - 1) / HD_TILE * HD_TILE;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < padded; r += static_cast<int64_t>(gridDim.x) * 4) {
+        const int token = r < count ? a.order[r] : -1;
+        const uint16_t* const from = static_cast<const uint16_t*>(a.hidden) + (token >= 0 ? token : 0) * a.ld_hidden;
+        for (int e = lane * 8; e < ld; e += 512)
+            (token >= 0 ? load_pack<uint16_t, 8, false>(from, e, a.width) : Pack<uint16_t, 8>::zero()).template store<false>(rows + r * ld + e);
+        if (coef && lane == 0) {
+            f32x4v c = {0.f, 0.f, 0.f, 0.f};
+            if (token >= 0) {
+                float g = a.dloss ? a.dloss[a.reduction == MUON_AMD_REDUCE_NONE ? token * a.ld_dloss : 0] : 0.f;
+                if (a.reduction == MUON_AMD_REDUCE_MEAN) g /= *a.part;
+                const float z = a.dlse ? a.dlse[token * a.ld_dlse] : 0.f;
+                // (a target outside of the vocabulary: no number, as the loss)
+                c = f32x4v{a.rows[r] >= 0 ? g + z : __builtin_nanf(""), g, a.stats[2 * r], a.stats[2 * r + 1]};
+            }
+            coef[r] = c;
+        }
+    }
+}
+
+// W with rows of `ld` elements, zeros beyond its width: where its own rows are no multiples of 128 bytes at 16-byte addresses.
+__global__ __launch_bounds__(256) void head_pad_kernel(const uint16_t* weight, int64_t ld_weight, int64_t vocab, int width, uint16_t* out, int ld) {
+    const int64_t packs = vocab * (ld / 8);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < packs; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / (ld / 8);
+        const int e = static_cast<int>(i % (ld / 8)) * 8;
+        load_pack<uint16_t, 8, false>(weight + r * ld_weight, e, width).template store<false>(out + r * ld + e);
+    }
+}
+
+// Joins the statistics of a row's column tiles, and forms its loss; the workgroup that is done last adds up the losses.  16 rows to a
+// workgroup, 64 threads to each.
+constexpr int HJ_THREADS = 1024, HJ_ROWS = 16, HJ_SHARES = HJ_THREADS / HJ_ROWS;
+__global__ __launch_bounds__(HJ_THREADS) void head_join_kernel(const MuonHeadLoss a, const f32x2_t* stats, int64_t ld_stats, int tiles, const float* target_logit,
+                                                               float* left) {
+    __shared__ float tops[HJ_SHARES][HJ_ROWS], sums[HJ_SHARES][HJ_ROWS];
+    __shared__ bool last;
+    const int r = threadIdx.x % HJ_ROWS, share = threadIdx.x / HJ_ROWS;
+    const int64_t count = a.order[a.tokens], row = static_cast<int64_t>(blockIdx.x) * HJ_ROWS + r;
+    const auto join = [](float& m, float& s, float m2, float s2) {
+        const float top = fmaxf(m, m2), ref = top == -__builtin_inff() ? 0.f : top;
+        s = s * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * LOG2E);
+        m = top;
+    };
+    float m = -__builtin_inff(), s = 0.f;
+    if (row < count) {
+        int i = share;
+        for (; i + 3 * HJ_SHARES < tiles; i += 4 * HJ_SHARES) {
+            f32x2_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = stats[(i + k * HJ_SHARES) * ld_stats + row];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) join(m, s, v[k][0], v[k][1]);
+        }
+        for (; i < tiles; i += HJ_SHARES) {
+            const f32x2_t v = stats[i * ld_stats + row];
+            join(m, s, v[0], v[1]);
+        }
+    }
+    tops[share][r] = m;
+    sums[share][r] = s;
+    __syncthreads();
+    for (int half = HJ_SHARES / 2; half > 0; half >>= 1) {
+        if (share < half) {
+            float m1 = tops[share][r], s1 = sums[share][r];
+            join(m1, s1, tops[share + half][r], sums[share + half][r]);
+            tops[share][r] = m1;
+            sums[share][r] = s1;
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x < 64) {
+        float loss = 0.f;
+        if (share == 0 && row < count && a.order[row] >= 0) {
+            const int token = a.order[row];
+            m = tops[0][r] == -__builtin_inff() ? 0.f : tops[0][r];
+            const float l = __log2f(sums[0][r]);
+            a.stats[2 * row] = m;
+            a.stats[2 * row + 1] = l;
+            loss = a.rows[row] >= 0 ? fmaf(l, LN2, m - target_logit[row]) : __builtin_nanf("");
+            a.losses[token] = loss;
+            a.lse[token] = fmaf(l, LN2, m);
+        }
+        loss = group_sum<64>(loss);
+        if (threadIdx.x == 0) {
+            __hip_atomic_store(&left[blockIdx.x], loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = __hip_atomic_fetch_add(a.counter, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.x) - 1;
+        }
+    }
+    __syncthreads();
+    if (!last || !a.loss) return;
+    float total = 0.f;
+    for (unsigned g = threadIdx.x; g < gridDim.x; g += HJ_THREADS) total += __hip_atomic_load(&left[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    total = group_sum<64>(total);
+    if ((threadIdx.x & 63) == 0) tops[0][threadIdx.x >> 6] = total;
+    __syncthreads();
+    if (threadIdx.x > 0) return;
+    total = 0.f;
+    for (int w = 0; w < HJ_THREADS / 64; ++w) total += tops[0][w];
+    *a.loss = a.reduction == MUON_AMD_REDUCE_MEAN ? total / *a.part : total;
+}
+
+// Adds the shares of the hidden states' gradient and writes it to the tokens; zeros for those that take no part.  A wave for each row.
+__global__ __launch_bounds__(256) void head_dhidden_kernel(const MuonHeadLoss a, const float* part, int64_t stride, int ld, int shares) {
+    const int lane = threadIdx.x & 63;
+    const int64_t count = a.order[a.tokens];
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < a.tokens; r += static_cast<int64_t>(gridDim.x) * 4) {
+        const int at = a.order[r];
+        const bool on = at >= 0;
+        uint16_t* const out = static_cast<uint16_t*>(a.dhidden) + static_cast<int64_t>(on ? at : ~at) * a.width;
+        for (int e = lane * 8; e < a.width; e += 512) {
+            float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (on && r < count)
+                for (int s = 0; s < shares; ++s) {
+                    const float* const p = part + s * stride + r * ld + e;
+                    const f32x4v lo = load_as<true, f32x4v>(p), hi = load_as<true, f32x4v>(p + 4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sum[i] += lo[i];
+                        sum[4 + i] += hi[i];
+                    }
+                }
+            store_pack<uint16_t, 8, false>(out, e, a.width, Pack<uint16_t, 8>::of(sum));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// How a call is laid out
+// ---------------------------------------------------------------------------------------------
+// Bytes of e: the larger the piece of the vocabulary, the less its sums' reading and writing weighs.  At least 4096 columns
+// whatever the number of tokens.
+constexpr int64_t HD_PIECE_BYTES = int64_t(1) << 30;
+
+static int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+struct HeadPlan {
+    bool few, padded;              // streamed; W through a padded copy
+    bool large;                    // 256 x 256 tiles in the products over tokens
+    int64_t rows, ld;              // padded rows and width
+    int tile, col_tiles;           // of the statistics
+    int64_t piece;                 // columns of e
+    int pieces, splits;
+    // offsets in the workspace, in bytes
+    int64_t hidden, weight, stats, logit, left, coef, e, part, bytes;
+};
+
+static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
+    HeadPlan p{};
+    const int64_t n = a.tokens, d = a.width, v = a.vocab;
+    p.few = !backward && n <= HD_FEW;
+    p.ld = up(d, BK);
+    p.rows = up(n, HD_TILE);
+    // (whether W can be read as it is goes by its address too: a plan without one leaves room for the copy)
+    p.padded = !p.few && (d % BK != 0 || a.ld_weight % 8 != 0 || reinterpret_cast<uintptr_t>(a.weight) % 16 != 0 || !a.weight);
+    p.large = (p.rows / 256) * up(v, 256) / 256 >= 512;
+    p.tile = p.few ? HF_VOCAB : p.large ? 256 : 128;
+    p.col_tiles = static_cast<int>(up(v, p.tile) / p.tile);
+    int64_t at = 0;
+    const auto take = [&](int64_t bytes) {
+        const int64_t begin = at;
+        at += up(bytes, 256);
+        return begin;
+    };
+    if (!p.few) p.hidden = take(p.rows * p.ld * 2);
+    if (p.padded) p.weight = take(v * p.ld * 2);
+    if (!backward) {
+        p.stats = take(p.rows * p.col_tiles * 8);
+        p.logit = take(p.rows * 4);
+        p.left = take((n + HJ_ROWS - 1) / HJ_ROWS * 4);
+    } else {
+        p.coef = take(p.rows * 16);
+        const int64_t fit = HD_PIECE_BYTES / (p.rows * 2) / 256 * 256, most = fit < 4096 ? 4096 : fit;
+        p.pieces = static_cast<int>((up(v, 256) + most - 1) / most);
+        p.piece = up((v + p.pieces - 1) / p.pieces, 256);
+        p.pieces = static_cast<int>((v + p.piece - 1) / p.piece);
+        p.e = take(p.rows * p.piece * 2);
+        const int64_t tiles = (p.rows / 256) * ((d + 255) / 256), wanted = (512 + tiles - 1) / tiles, most_splits = p.piece / BK / 8;
+        p.splits = static_cast<int>(wanted < most_splits ? wanted : most_splits > 0 ? most_splits : 1);
+        p.part = take(p.splits * p.rows * p.ld * 4);
+    }
+    p.bytes = at;
+    return p;
+}
+
+static int check_head(const MuonHeadLoss* a, const char* what) {
+    MUON_REQUIRE(a, "%s: null arguments", what);
+    MUON_REQUIRE(a->tokens > 0 && a->tokens <= (1 << 24) && a->vocab > 0 && a->vocab <= (1 << 24) && a->width > 0 && a->width <= (1 << 16),
+                 "%s: tokens=%lld vocab=%d width=%d", what, static_cast<long long>(a->tokens), a->vocab, a->width);
+    MUON_REQUIRE(a->hidden && a->weight && a->targets && a->order && a->rows && a->stats && a->part && a->workspace, "%s: null pointer", what);
+    MUON_REQUIRE(a->target_bits == 32 || a->target_bits == 64, "%s: target_bits=%d", what, a->target_bits);
+    MUON_REQUIRE(a->reduction >= MUON_AMD_REDUCE_NONE && a->reduction <= MUON_AMD_REDUCE_MEAN, "%s: reduction=%d", what, a->reduction);
+    MUON_REQUIRE(reinterpret_cast<uintptr_t>(a->workspace) % 256 == 0, "%s: the workspace is not at a multiple of 256 bytes", what);
+    MUON_REQUIRE(a->ld_weight >= 0 && a->ld_weight <= (int64_t(1) << 21), "%s: ld_weight=%lld", what, static_cast<long long>(a->ld_weight));
+    return MUON_AMD_OK;
+}
+
+template <typename Cfg, int PRODUCT>
+static int launch_product(const HeadGemm& g, hipStream_t s) {
+    const int64_t grid = static_cast<int64_t>(g.row_tiles) * g.col_tiles * g.splits;
+    MUON_REQUIRE(grid > 0 && grid <= 0x7fffffff, "linear_cross_entropy: %lld tiles", static_cast<long long>(grid));
+    hipLaunchKernelGGL((head_gemm_kernel<Cfg, PRODUCT>), dim3(static_cast<unsigned>(grid)), dim3(Cfg::NT), Cfg::LDS_BYTES, s, g);
+    return check_launch("linear_cross_entropy");
+}
+template <int PRODUCT>
+static int launch_product(const HeadGemm& g, bool large, hipStream_t s) {
+    return large ? launch_product<HeadLarge, PRODUCT>(g, s) : launch_product<HeadSmall, PRODUCT>(g, s);
+}
+
+template <typename Cfg, int PRODUCT>
+static int raise_head_limit() {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(head_gemm_kernel<Cfg, PRODUCT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                            static_cast<int>(Cfg::LDS_BYTES)) != hipSuccess) {
+        (void)hipGetLastError();
+        set_error("linear_cross_entropy: cannot raise dynamic LDS to %zu bytes", Cfg::LDS_BYTES);
+        return MUON_AMD_ELAUNCH;
+    }
+    return MUON_AMD_OK;
+}
+template <typename Cfg>
+static int raise_head_limits_of() {
+    int rc = raise_head_limit<Cfg, HEAD_STATS>();
+    if (rc == MUON_AMD_OK) rc = raise_head_limit<Cfg, HEAD_GRAD>();
+    if (rc == MUON_AMD_OK) rc = raise_head_limit<Cfg, HEAD_DHIDDEN>();
+    if (rc == MUON_AMD_OK) rc = raise_head_limit<Cfg, HEAD_DWEIGHT>();
+    return rc;
+}
+int raise_head_limits() {
+    const int rc = raise_head_limits_of<HeadLarge>();
+    return rc == MUON_AMD_OK ? raise_head_limits_of<HeadSmall>() : rc;
+}
+
+// The copies that the products read; W is then (w, ld).
+static int gather(const MuonHeadLoss& a, const HeadPlan& p, char* ws, f32x4v* coef, const uint16_t** w, int64_t* ld, hipStream_t s) {
+    const int64_t blocks = p.rows / 4 < 4096 ? p.rows / 4 : 4096;
+    hipLaunchKernelGGL(head_gather_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, reinterpret_cast<uint16_t*>(ws + p.hidden), static_cast<int>(p.ld), coef);
+    if (const int rc = check_launch("linear_cross_entropy: rows")) return rc;
+    *w = static_cast<const uint16_t*>(a.weight);
+    *ld = a.ld_weight;
+    if (p.padded) {
+        *w = reinterpret_cast<uint16_t*>(ws + p.weight);
+        *ld = p.ld;
+        hipLaunchKernelGGL(head_pad_kernel, dim3(4096), dim3(256), 0, s, static_cast<const uint16_t*>(a.weight), a.ld_weight, static_cast<int64_t>(a.vocab), a.width,
+                           reinterpret_cast<uint16_t*>(ws + p.weight), static_cast<int>(p.ld));
+        return check_launch("linear_cross_entropy: matrix");
+    }
+    return MUON_AMD_OK;
+}
+
+}  // namespace muon_amd
+
+using namespace muon_amd;
+
+extern "C" {
+
+size_t muon_amd_sizeof_head_loss(void) { return sizeof(MuonHeadLoss); }
+
+int64_t muon_amd_head_loss_workspace(const MuonHeadLoss* args, int backward) {
+    if (!args || args->tokens <= 0 || args->vocab <= 0 || args->width <= 0) return 0;
+    return head_plan(*args, backward != 0).bytes;
+}
+
+int muon_amd_head_loss(const MuonHeadLoss* args, void* stream) {
+    if (const int rc = check_head(args, "head_loss")) return rc;
+    const MuonHeadLoss a = *args;
+    MUON_REQUIRE(a.losses && a.lse && a.counter, "head_loss: null output");
+    const HeadPlan p = head_plan(a, false);
+    MUON_REQUIRE(a.workspace_bytes >= p.bytes, "head_loss: a workspace of %lld bytes, %lld needed", static_cast<long long>(a.workspace_bytes), static_cast<long long>(p.bytes));
+    if (const int rc = muon_amd_init()) return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    char* const ws = static_cast<char*>(a.workspace);
+    f32x2_t* const stats = reinterpret_cast<f32x2_t*>(ws + p.stats);
+    float* const logit = reinterpret_cast<float*>(ws + p.logit);
+    if (p.few) hipLaunchKernelGGL(head_order_kernel<false>, dim3(1), dim3(HO_THREADS), 0, s, a);
+    else hipLaunchKernelGGL(head_order_kernel<true>, dim3(1), dim3(HO_THREADS), 0, s, a);
+    if (const int rc = check_launch("head_loss: order")) return rc;
+    if (p.few) {
+        const auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(p.col_tiles), dim3(HF_THREADS), 0, s, static_cast<const uint16_t*>(a.hidden), a.ld_hidden,
+                               static_cast<const uint16_t*>(a.weight), a.ld_weight, static_cast<int>(a.tokens), a.width, a.vocab, a.targets, a.target_bits, stats, p.rows, logit);
+        };
+        if (a.tokens <= 16) go(head_few_kernel<1>);
+        else if (a.tokens <= 32) go(head_few_kernel<2>);
+        else go(head_few_kernel<4>);
+        if (const int rc = check_launch("head_loss: few")) return rc;
+    } else {
+        HeadGemm g{};
+        if (const int rc = gather(a, p, ws, nullptr, &g.Q, &g.ldq, s)) return rc;
+        g.P = reinterpret_cast<const uint16_t*>(ws + p.hidden);
+        g.ldp = p.ld;
+        g.end_p = (p.rows * p.ld - 8) * 2;
+        g.end_q = ((a.vocab - 1) * g.ldq + p.ld - 8) * 2;
+        g.count = a.order + a.tokens;
+        g.row_tiles = static_cast<int>(p.rows / p.tile);
+        g.col_tiles = p.col_tiles;
+        g.splits = 1;
+        g.kblocks = static_cast<int>(p.ld / BK);
+        g.vocab = a.vocab;
+        g.target = a.rows;
+        g.stats = stats;
+        g.ld_stats = p.rows;
+        g.target_logit = logit;
+        if (const int rc = launch_product<HEAD_STATS>(g, p.large, s)) return rc;
+    }
+    hipLaunchKernelGGL(head_join_kernel, dim3(static_cast<unsigned>((a.tokens + HJ_ROWS - 1) / HJ_ROWS)), dim3(HJ_THREADS), 0, s, a, stats, p.rows, p.col_tiles, logit,
+                       reinterpret_cast<float*>(ws + p.left));
+    return check_launch("head_loss: join");
+}
+
+int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
+    if (const int rc = check_head(args, "head_loss_backward")) return rc;
+    const MuonHeadLoss a = *args;
+    MUON_REQUIRE(a.dhidden || a.dweight, "head_loss_backward: no output");
+    const HeadPlan p = head_plan(a, true);
+    MUON_REQUIRE(a.workspace_bytes >= p.bytes, "head_loss_backward: a workspace of %lld bytes, %lld needed", static_cast<long long>(a.workspace_bytes),
+                 static_cast<long long>(p.bytes));
+    if (const int rc = muon_amd_init()) return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    char* const ws = static_cast<char*>(a.workspace);
+    f32x4v* const coef = reinterpret_cast<f32x4v*>(ws + p.coef);
+    const uint16_t* w;
+    int64_t ldw;
+    if (const int rc = gather(a, p, ws, coef, &w, &ldw, s)) return rc;
+    uint16_t* const rows = reinterpret_cast<uint16_t*>(ws + p.hidden);
+    uint16_t* const e = reinterpret_cast<uint16_t*>(ws + p.e);
+    float* const part = reinterpret_cast<float*>(ws + p.part);
+    for (int i = 0; i < p.pieces; ++i) {
+        const int begin = static_cast<int>(i * p.piece), size = static_cast<int>(a.vocab - begin < p.piece ? a.vocab - begin : p.piece);
+        const uint16_t* const piece = w + begin * ldw;
+        HeadGemm g{};
+        g.count = a.order + a.tokens;
+        g.splits = 1;
+        // e of the piece
+        const int tile = p.large ? 256 : 128;
+        g.P = rows;
+        g.ldp = p.ld;
+        g.end_p = (p.rows * p.ld - 8) * 2;
+        g.Q = piece;
+        g.ldq = ldw;
+        g.end_q = ((size - 1) * ldw + p.ld - 8) * 2;
+        g.row_tiles = static_cast<int>(p.rows / tile);
+        g.col_tiles = static_cast<int>(up(size, tile) / tile);
+        g.cols = static_cast<int>(p.piece);
+        g.kblocks = static_cast<int>(p.ld / BK);
+        g.vocab_begin = begin;
+        g.vocab = a.vocab;
+        g.target = a.rows;
+        g.coef = coef;
+        g.out = e;
+        g.ld_out = p.piece;
+        if (const int rc = launch_product<HEAD_GRAD>(g, p.large, s)) return rc;
+        if (a.dhidden) {
+            HeadGemm h{};
+            h.count = g.count;
+            h.P = e;
+            h.ldp = p.piece;
+            h.end_p = (p.rows * p.piece - 8) * 2;
+            h.Q = piece;
+            h.ldq = ldw;
+            h.end_q = ((size - 1) * ldw + p.ld - 8) * 2;
+            h.col_limit = static_cast<int>(p.ld);
+            h.row_tiles = static_cast<int>(p.rows / 256);
+            h.col_tiles = static_cast<int>(up(p.ld, 256) / 256);
+            h.splits = p.splits;
+            h.cols = static_cast<int>(p.ld);
+            h.kblocks = static_cast<int>(up(size, BK) / BK);
+            h.part = part;
+            h.add = i > 0;
+            h.part_stride = p.rows * p.ld;
+            h.ld_out = p.ld;
+            if (const int rc = launch_product<HeadLarge, HEAD_DHIDDEN>(h, s)) return rc;
+        }
+        if (a.dweight) {
+            HeadGemm h{};
+            h.count = g.count;
+            h.P = e;
+            h.ldp = p.piece;
+            h.end_p = (p.rows * p.piece - 8) * 2;
+            h.row_limit = static_cast<int>(p.piece);
+            h.Q = rows;
+            h.ldq = p.ld;
+            h.end_q = (p.rows * p.ld - 8) * 2;
+            h.col_limit = static_cast<int>(p.ld);
+            h.rows = size;
+            h.row_tiles = static_cast<int>(up(size, 256) / 256);
+            h.col_tiles = static_cast<int>(up(a.width, 256) / 256);
+            h.splits = 1;
+            h.cols = a.width;
+            h.out = static_cast<uint16_t*>(a.dweight) + static_cast<int64_t>(begin) * a.width;
+            h.ld_out = a.width;
+            if (const int rc = launch_product<HeadLarge, HEAD_DWEIGHT>(h, s)) return rc;
+        }
+    }
+    if (a.dhidden) {
+        const int64_t blocks = (a.tokens + 3) / 4 < 8192 ? (a.tokens + 3) / 4 : 8192;
+        hipLaunchKernelGGL(head_dhidden_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, part, p.rows * p.ld, static_cast<int>(p.ld), p.splits);
+        return check_launch("head_loss_backward: hidden");
+    }
+    return MUON_AMD_OK;
+}
+
+}  // extern "C"

@@ -42,6 +42,9 @@ struct Api {
     decltype(&muon_amd_route) route;
     decltype(&muon_amd_route_backward) route_backward;
     decltype(&muon_amd_route_partials) route_partials;
+    decltype(&muon_amd_head_loss) head_loss;
+    decltype(&muon_amd_head_loss_backward) head_loss_backward;
+    decltype(&muon_amd_head_loss_workspace) head_loss_workspace;
     decltype(&muon_amd_distill) distill;
     decltype(&muon_amd_distill_backward) distill_backward;
     decltype(&muon_amd_distill_partials) distill_partials;
@@ -361,10 +364,138 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>> route_topk(con
     return std::make_tuple(o.weights, o.indices, o.counts, o.balance, o.z);
 }
 
-// ---- distill_topk ------------------------------------------------------------------------------------------------
 bool whole_numbers(const Tensor& t) { return t.is_cuda() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong); }
 int bits_of(const Tensor& t) { return t.scalar_type() == at::kLong ? 64 : 32; }
 
+// ---- linear_cross_entropy ----------------------------------------------------------------------------------------
+struct HeadTensors {
+    Tensor hidden, weight, targets, part, order, rows, stats;
+};
+constexpr int64_t HEAD_MAX_DISTANCE = int64_t(1) << 21;          // between rows of the matrix
+
+MuonHeadLoss head_args(const HeadTensors& t, int64_t reduction, int64_t ignore_index, std::vector<Tensor>& keep) {
+    const int64_t width = t.hidden.size(-1);
+    const auto hold = [&](Tensor r) -> const Tensor& {
+        keep.push_back(std::move(r));
+        return keep.back();
+    };
+    keep.reserve(3);
+    MuonHeadLoss a{};
+    const Tensor& h = hold(rows_of(t.hidden, width));
+    const Tensor rows = rows_of(t.weight, width);
+    const Tensor& w = hold(rows.stride(0) > HEAD_MAX_DISTANCE ? rows.contiguous() : rows);
+    a.hidden = h.data_ptr();
+    a.weight = w.data_ptr();
+    a.targets = hold(t.targets.contiguous()).data_ptr();
+    a.part = t.part.data_ptr<float>();
+    a.order = t.order.data_ptr<int32_t>();
+    a.rows = t.rows.data_ptr<int32_t>();
+    a.stats = t.stats.data_ptr<float>();
+    a.tokens = h.size(0);
+    a.ld_hidden = h.stride(0);
+    a.ld_weight = w.stride(0);
+    a.ignore_index = ignore_index;
+    a.width = static_cast<int32_t>(width);
+    a.vocab = static_cast<int32_t>(w.size(0));
+    a.target_bits = bits_of(t.targets);
+    a.reduction = static_cast<int32_t>(reduction);
+    return a;
+}
+Tensor head_workspace(MuonHeadLoss& a, bool backward, const Tensor& like) {
+    a.workspace_bytes = api.head_loss_workspace(&a, backward);
+    const Tensor ws = at::empty({std::max<int64_t>(a.workspace_bytes, 256)}, like.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+    return ws;
+}
+
+// (loss, lse); `t` gets what backward needs.
+std::tuple<Tensor, Tensor> head_forward(HeadTensors& t, int64_t reduction, int64_t ignore_index) {
+    const auto f32 = t.hidden.options().dtype(at::kFloat), i32 = t.hidden.options().dtype(at::kInt);
+    const auto shape = t.targets.sizes();
+    const int64_t tokens = t.targets.numel();
+    Tensor lse = at::empty(shape, f32);
+    if (tokens == 0) return {reduction ? at::zeros({}, f32) : at::zeros(shape, f32), lse};
+    const Tensor losses = at::empty(shape, f32), loss = reduction ? at::empty({}, f32) : Tensor(), counter = at::empty({}, i32);
+    t.part = at::empty({}, f32);
+    t.order = at::empty({tokens + 1}, i32);
+    t.rows = at::empty({tokens}, i32);
+    t.stats = at::empty({tokens, 2}, f32);
+    std::vector<Tensor> keep;
+    MuonHeadLoss a = head_args(t, reduction, ignore_index, keep);
+    a.losses = losses.data_ptr<float>();
+    a.lse = lse.data_ptr<float>();
+    a.loss = reduction ? loss.data_ptr<float>() : nullptr;
+    a.counter = counter.data_ptr<int32_t>();
+    const Tensor ws = head_workspace(a, false, t.hidden);
+    const c10::DeviceGuard guard(t.hidden.device());
+    check(api.head_loss(&a, current_stream(t.hidden.device())), "linear_cross_entropy");
+    return {reduction ? loss : losses, lse};
+}
+
+struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t reduction,
+                                 int64_t ignore_index) {
+        HeadTensors t{hidden, weight, targets, Tensor(), Tensor(), Tensor(), Tensor()};
+        auto [loss, lse] = head_forward(t, reduction, ignore_index);
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["reduction"] = reduction;
+        ctx->saved_data["ignore_index"] = ignore_index;
+        ctx->save_for_backward({t.hidden, t.weight, t.targets, t.part, t.order, t.rows, t.stats});
+        return {loss, lse};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list douts) {
+        const variable_list saved = ctx->get_saved_variables();
+        const HeadTensors t{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], saved[6]};
+        const bool nothing = !t.order.defined() || (!douts[0].defined() && !douts[1].defined());
+        const auto gradient = [&](size_t edge, const Tensor& of) {
+            if (!ctx->needs_input_grad(edge)) return Tensor();
+            return nothing ? at::zeros(of.sizes(), of.options()) : at::empty(of.sizes(), of.options());
+        };
+        Tensor dhidden = gradient(0, t.hidden), dweight = gradient(1, t.weight);
+        if (!nothing && (dhidden.defined() || dweight.defined())) {
+            std::vector<Tensor> keep;
+            MuonHeadLoss a = head_args(t, ctx->saved_data["reduction"].toInt(), ctx->saved_data["ignore_index"].toInt(), keep);
+            const auto each = [&](const Tensor& g) { return g.reshape({a.tokens}); };
+            Tensor dloss, dlse;
+            if (douts[0].defined()) {
+                dloss = a.reduction == MUON_AMD_REDUCE_NONE ? each(douts[0]) : douts[0];
+                a.dloss = dloss.data_ptr<float>();
+                a.ld_dloss = dloss.dim() ? dloss.stride(0) : 0;
+            }
+            if (douts[1].defined()) {
+                dlse = each(douts[1]);
+                a.dlse = dlse.data_ptr<float>();
+                a.ld_dlse = dlse.stride(0);
+            }
+            a.dhidden = dhidden.defined() ? dhidden.data_ptr() : nullptr;
+            a.dweight = dweight.defined() ? dweight.data_ptr() : nullptr;
+            const Tensor ws = head_workspace(a, true, t.hidden);
+            const c10::DeviceGuard guard(t.hidden.device());
+            check(api.head_loss_backward(&a, current_stream(t.hidden.device())), "linear_cross_entropy backward");
+        }
+        return once({dhidden, dweight, Tensor(), Tensor(), Tensor()}, "the gradients of linear_cross_entropy are not differentiable");
+    }
+};
+
+// None where the arguments are not taken.
+std::optional<std::tuple<Tensor, Tensor>> linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore_index,
+                                                               int64_t reduction) {
+    const auto bf16 = [&](const Tensor& t) { return t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.device() == hidden.device(); };
+    if (!bf16(hidden) || !bf16(weight) || !whole_numbers(targets) || targets.device() != hidden.device()) return std::nullopt;
+    if (hidden.dim() < 1 || weight.dim() != 2 || weight.size(1) != hidden.size(-1) || targets.sizes() != hidden.sizes().slice(0, hidden.dim() - 1))
+        return std::nullopt;
+    if (weight.size(1) < 1 || weight.size(1) > (1 << 16) || weight.size(0) < 1 || weight.size(0) > (1 << 24) || targets.numel() > (1 << 24)) return std::nullopt;
+    if (reduction < 0 || any_tangent({&hidden, &weight})) return std::nullopt;
+    const py::gil_scoped_release released;
+    if (any_requires_grad({&hidden, &weight})) {
+        const variable_list out = LinearCrossEntropy::apply(hidden, weight, targets, reduction, ignore_index);
+        return std::make_tuple(out[0], out[1]);
+    }
+    HeadTensors t{hidden, weight, targets, Tensor(), Tensor(), Tensor(), Tensor()};
+    return head_forward(t, reduction, ignore_index);
+}
+
+// ---- distill_topk ------------------------------------------------------------------------------------------------
 struct DistillTensors {
     Tensor logits, teacher, indices, mask, part, stats;         // (the mask may be undefined)
 };
@@ -821,6 +952,9 @@ void bind(const py::dict& addresses, const py::object& error) {
     get(api.route, "muon_amd_route");
     get(api.route_backward, "muon_amd_route_backward");
     get(api.route_partials, "muon_amd_route_partials");
+    get(api.head_loss, "muon_amd_head_loss");
+    get(api.head_loss_backward, "muon_amd_head_loss_backward");
+    get(api.head_loss_workspace, "muon_amd_head_loss_workspace");
     get(api.distill, "muon_amd_distill");
     get(api.distill_backward, "muon_amd_distill_backward");
     get(api.distill_partials, "muon_amd_distill_partials");
@@ -849,6 +983,7 @@ void bind(const py::dict& addresses, const py::object& error) {
     };
     same("muon_amd_sizeof_residual_norm", sizeof(MuonResidualNorm));
     same("muon_amd_sizeof_route", sizeof(MuonRoute));
+    same("muon_amd_sizeof_head_loss", sizeof(MuonHeadLoss));
     same("muon_amd_sizeof_distill", sizeof(MuonDistill));
     same("muon_amd_sizeof_grad_desc", sizeof(MuonGradDesc));
     same("muon_amd_sizeof_adamw_values_desc", sizeof(MuonAdamWValuesDesc));
@@ -870,6 +1005,7 @@ PYBIND11_MODULE(_native, m) {
     m.def("abi_version", [] { return MUON_AMD_ABI_VERSION; });
     m.def("residual_norm", &residual_norm);
     m.def("route_topk", &route_topk);
+    m.def("linear_cross_entropy", &linear_cross_entropy);
     m.def("distill_topk", &distill_topk);
     m.def("adamw_launch", &adamw_launch);
     m.def("clip", &clip);

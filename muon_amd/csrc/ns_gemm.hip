@@ -1053,6 +1053,7 @@ static int device_setup(const DeviceState** out) {
         if (rc == MUON_AMD_OK) rc = raise_lds_limits<Cfg1>();
         if (rc == MUON_AMD_OK) rc = raise_lds_limits<Cfg2>();
         if (rc == MUON_AMD_OK) rc = raise_small_limits();
+        if (rc == MUON_AMD_OK) rc = raise_head_limits();
         if (rc != MUON_AMD_OK) return rc;
         void* ptr = nullptr;
         if (hipGetSymbolAddress(&ptr, HIP_SYMBOL(scratch)) != hipSuccess || ptr == nullptr) {

@@ -6,8 +6,6 @@ functions with gradients.
         the next block, in one pass
     route_topk(logits, k)  -> weights, indices, counts, balance_loss, z_loss
         the experts of each token, tokens per expert, and the losses that keep them balanced
-    distill_topk(logits, teacher_logits, teacher_indices, temperature=...)  -> loss
-        distillation from the largest logits of a teacher
 """
 from __future__ import annotations
 
@@ -128,67 +126,3 @@ def _refuse_route(logits, k, mask):
             raise ValueError(f"mask must be a bool tensor of shape {tuple(logits.shape[:-1])} on {logits.device}, got {mask.dtype} {tuple(mask.shape)}")
     _no_tangent(logits, "logits")
     raise _lib.MuonAmdError("route_topk does not take these arguments")
-
-
-def _reduction(reduction) -> int:
-    """The reduction's number, or -1 for what is none."""
-    return _lib.REDUCTIONS.get(reduction, -1) if isinstance(reduction, str) else -1
-
-
-def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_indices: torch.Tensor, *, temperature: float = 1.0,
-                 mask: torch.Tensor | None = None, reduction: str = "mean") -> torch.Tensor:
-    """Distillation of a student, logits (..., vocabulary) in fp32 or bf16, from the largest logits that a teacher kept for
-    each token: teacher_logits (..., k), fp32 or bf16, at teacher_indices (..., k), int32 or int64, T = temperature:
-
-        p = softmax(logits / T) over the vocabulary;  q = softmax(teacher_logits / T) over the token's list
-        loss = T^2 sum_k q_k (log q_k - log p[teacher_indices_k])
-
-    as the mean over the tokens that take part (zero where none does), their "sum", or ("none") of each token, fp32.  Entries
-    whose index is outside of the vocabulary (-1 by habit) or whose teacher logit is -infinity are not there; a token whose
-    list has none, or whose `mask` (bool, the shape of logits without its last dimension) is false, takes no part: its loss and
-    gradient are zero, whatever its logits hold.  An index that comes several times counts with the sum of its
-    q.  The gradient flows to logits alone.  At most 1024 entries a token.  Sums are fp32 in a fixed order."""
-    if isinstance(temperature, (int, float)):
-        out = _lib.native().distill_topk(logits, teacher_logits, teacher_indices, float(temperature), mask, _reduction(reduction))
-        if out is not None:
-            return out
-    _refuse_distill(logits, teacher_logits, teacher_indices, temperature, mask, reduction)
-
-
-def _refuse_reduction(reduction):
-    if _reduction(reduction) < 0:
-        raise ValueError(f"reduction must be one of {', '.join(sorted(_lib.REDUCTIONS))}, got {reduction!r}")
-
-
-def _refuse_distill(logits, teacher_logits, teacher_indices, temperature, mask, reduction):
-    """Says what is wrong with arguments that were not taken."""
-    for name, t in (("logits", logits), ("teacher_logits", teacher_logits)):
-        require_gpu_tensor(t, name)
-        _dtype(t, name)
-    require_gpu_tensor(teacher_indices, "teacher_indices")
-    if teacher_indices.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"teacher_indices is {teacher_indices.dtype}: int32 and int64 are taken")
-    for name, t in (("teacher_logits", teacher_logits), ("teacher_indices", teacher_indices)):
-        if t.device != logits.device:
-            raise _lib.MuonAmdError(f"{name} is on {t.device}, logits on {logits.device}")
-    if logits.ndim < 1 or not 1 <= logits.size(-1) <= 1 << 30:
-        raise ValueError(f"logits must have 1 to 2^30 classes as their last dimension, got {tuple(logits.shape)}")
-    limit = _lib.load().muon_amd_distill_max_top()
-    if teacher_logits.ndim != logits.ndim or teacher_logits.shape[:-1] != logits.shape[:-1] or not 1 <= teacher_logits.size(-1) <= limit:
-        raise ValueError(f"teacher_logits must be {tuple(logits.shape[:-1])} lists of 1 to {limit} entries, got {tuple(teacher_logits.shape)}")
-    if teacher_indices.shape != teacher_logits.shape:
-        raise ValueError(f"teacher_indices must have the shape of teacher_logits, {tuple(teacher_logits.shape)}, got {tuple(teacher_indices.shape)}")
-    if logits.numel() // logits.size(-1) > 1 << 24:
-        raise ValueError(f"{logits.numel() // logits.size(-1)} tokens: at most 2^24 are taken")
-    if mask is not None:
-        require_gpu_tensor(mask, "mask")
-        if mask.dtype != torch.bool or mask.shape != logits.shape[:-1] or mask.device != logits.device:
-            raise ValueError(f"mask must be a bool tensor of shape {tuple(logits.shape[:-1])} on {logits.device}, got {mask.dtype} {tuple(mask.shape)}")
-    if not isinstance(temperature, (int, float)) or not 1e-30 <= temperature <= 1e30:
-        raise ValueError(f"temperature must be a number from 1e-30 to 1e30, got {temperature!r}")
-    _refuse_reduction(reduction)
-    _no_tangent(logits, "logits")
-    _no_tangent(teacher_logits, "teacher_logits")
-    if torch.is_grad_enabled() and teacher_logits.requires_grad:
-        raise ValueError("teacher_logits requires a gradient: there is none for the teacher (detach it)")
-    raise _lib.MuonAmdError("distill_topk does not take these arguments")
