@@ -571,6 +571,17 @@ int64_t muon_amd_route_partials(int64_t tokens, int experts);
 int     muon_amd_route(const MuonRoute* args_host, void* stream);
 int     muon_amd_route_backward(const MuonRoute* args_host, void* stream);
 
+/* ---- routing by scores with a bias, within groups of experts ------------------------------------- */
+/* The same with scores s = softmax(logits) or sigmoid(logits): the choice is by c = s + bias (experts floats, NULL: 0), ties at the
+ * lowest index, among the groups_kept of `groups` equal runs of experts whose two largest c have the largest sum; the weights and the balance
+ * loss (over s / sum s) know nothing of the bias.  An expert whose logit or bias is -infinity is never chosen.  c is compared as in 64 bits.  Backward:
+ * with what the scored forward wrote.                                                               */
+#define MUON_AMD_SCORES_SOFTMAX 0
+#define MUON_AMD_SCORES_SIGMOID 1
+int     muon_amd_route_max_groups(void);
+int     muon_amd_route_scored(const MuonRoute* args_host, int scores, const float* bias_dev, int groups, int groups_kept, void* stream);
+int     muon_amd_route_scored_backward(const MuonRoute* args_host, int scores, void* stream);
+
 /* ---- cross entropy of a linear head without its logits ------------------------------------------ */
 /* x = hidden weight^T;  lse = log sum exp(x);  loss = lse - x[target], fp32 sums of bf16 products.  Backward forms the logits again in
  * pieces of the vocabulary and reads what forward wrote; its workspace differs from forward's.  */

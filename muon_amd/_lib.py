@@ -24,6 +24,7 @@ AOL_SYMMETRIC = 0
 AOL_ROWS_ONLY = 1
 SRC_F32 = 0
 SRC_BF16 = 1
+SCORES = {"softmax": 0, "sigmoid": 1}
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 # numpy mirrors of the C structs (align=True reproduces the C layout; sizes are checked against
@@ -168,6 +169,9 @@ SIGNATURES = {
     "muon_amd_route_partials": (ctypes.c_int64, [ctypes.c_int64, _c_int]),
     "muon_amd_route": (_c_int, [ctypes.POINTER(RouteArgs), _vp]),
     "muon_amd_route_backward": (_c_int, [ctypes.POINTER(RouteArgs), _vp]),
+    "muon_amd_route_max_groups": (_c_int, []),
+    "muon_amd_route_scored": (_c_int, [ctypes.POINTER(RouteArgs), _c_int, _vp, _c_int, _c_int, _vp]),
+    "muon_amd_route_scored_backward": (_c_int, [ctypes.POINTER(RouteArgs), _c_int, _vp]),
     "muon_amd_sizeof_head_loss": (ctypes.c_size_t, []),
     "muon_amd_head_loss_workspace": (ctypes.c_int64, [ctypes.POINTER(HeadLossArgs), _c_int]),
     "muon_amd_head_loss": (_c_int, [ctypes.POINTER(HeadLossArgs), _vp]),

@@ -24,7 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmuon_amd.so")
 NATIVE_OUT = os.path.join(HERE, "_native.so")
 SOURCES = ["capi.hip", "elementwise.hip", "aol.hip", "ns_gemm.hip", "small.hip", "step.hip", "adamw.hip", "grad_norm.hip",
-           "residual.hip", "route.hip", "distill.hip", "head.hip"]
+           "residual.hip", "route.hip", "route_scored.hip", "distill.hip", "head.hip"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # hipcc -O3 must not form packed-fp32 instructions on this target

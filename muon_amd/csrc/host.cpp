@@ -40,7 +40,8 @@ struct Api {
     decltype(&muon_amd_residual_norm_backward) residual_norm_backward;
     decltype(&muon_amd_residual_norm_partials) residual_norm_partials;
     decltype(&muon_amd_route) route;
-    decltype(&muon_amd_route_backward) route_backward;
+    decltype(&muon_amd_route_scored) route_scored;
+    decltype(&muon_amd_route_scored_backward) route_backward;
     decltype(&muon_amd_route_partials) route_partials;
     decltype(&muon_amd_head_loss) head_loss;
     decltype(&muon_amd_head_loss_backward) head_loss_backward;
@@ -54,7 +55,7 @@ struct Api {
     decltype(&muon_amd_validate_adamw_values) validate_adamw_values;
     decltype(&muon_amd_adamw_values) adamw_values;
     decltype(&muon_amd_adamw) adamw;
-    int max_width, max_experts, max_k, max_top, shared_elems, block_elems, norm_partials;
+    int max_width, max_experts, max_k, max_groups, max_top, shared_elems, block_elems, norm_partials;
 } api{};
 
 struct LibraryError : std::runtime_error {
@@ -280,7 +281,15 @@ MuonRoute route_args(const Tensor& logits, const Tensor& mask, const RouteOut& o
     return a;
 }
 
-RouteOut route_forward(const Tensor& logits, int64_t k, const Tensor& mask, bool normalize) {
+// What the choice goes by.
+struct RouteScores {
+    int64_t scores = MUON_AMD_SCORES_SOFTMAX, groups = 1, kept = 1;
+    Tensor bias;
+    // the order of the logits, which has kernels of its own
+    bool plain() const { return scores == MUON_AMD_SCORES_SOFTMAX && !bias.defined() && kept == groups; }
+};
+
+RouteOut route_forward(const Tensor& logits, int64_t k, const Tensor& mask, bool normalize, const RouteScores& by) {
     const int64_t experts = logits.size(-1), tokens = logits.numel() / experts;
     const auto f32 = logits.options().dtype(at::kFloat), i32 = logits.options().dtype(at::kInt);
     std::vector<int64_t> shape = logits.sizes().vec();
@@ -307,15 +316,24 @@ RouteOut route_forward(const Tensor& logits, int64_t k, const Tensor& mask, bool
     a.z = o.z.data_ptr<float>();
     a.partials = partials.data_ptr<float>();
     const c10::DeviceGuard guard(logits.device());
-    check(api.route(&a, current_stream(logits.device())), "route");
+    if (by.plain()) {
+        check(api.route(&a, current_stream(logits.device())), "route");
+    } else {
+        const Tensor bias = by.bias.defined() ? by.bias.contiguous() : Tensor();
+        check(api.route_scored(&a, static_cast<int>(by.scores), bias.defined() ? bias.data_ptr<float>() : nullptr, static_cast<int>(by.groups),
+                               static_cast<int>(by.kept), current_stream(logits.device())),
+              "route_scored");
+    }
     return o;
 }
 
 struct RouteTopk : torch::autograd::Function<RouteTopk> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t k, const std::optional<Tensor>& mask, bool normalize) {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t k, const std::optional<Tensor>& mask, bool normalize,
+                                 const RouteScores& by) {
         const Tensor m = mask.value_or(Tensor());
-        const RouteOut o = route_forward(logits, k, m, normalize);
+        const RouteOut o = route_forward(logits, k, m, normalize, by);
         ctx->set_materialize_grads(false);
+        ctx->saved_data["scores"] = by.scores;
         ctx->saved_data["normalize"] = normalize;
         ctx->save_for_backward({logits, m, o.weights, o.indices, o.counts, o.part, o.lse});
         ctx->mark_non_differentiable({o.indices, o.counts});
@@ -340,27 +358,36 @@ struct RouteTopk : torch::autograd::Function<RouteTopk> {
             a.dbalance = douts[3].defined() ? douts[3].data_ptr<float>() : nullptr;
             a.dz = douts[4].defined() ? douts[4].data_ptr<float>() : nullptr;
             const c10::DeviceGuard guard(logits.device());
-            check(api.route_backward(&a, current_stream(logits.device())), "route_backward");
+            check(api.route_backward(&a, static_cast<int>(ctx->saved_data["scores"].toInt()), current_stream(logits.device())), "route_backward");
         }
-        return once({dlogits, Tensor(), Tensor(), Tensor()}, "the gradients of route_topk are not differentiable");
+        return once({dlogits, Tensor(), Tensor(), Tensor(), Tensor()}, "the gradients of route_topk are not differentiable");
     }
 };
 
 std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>> route_topk(const Tensor& logits, int64_t k, const std::optional<Tensor>& mask,
-                                                                             bool normalize) {
+                                                                             bool normalize, int64_t scores, const std::optional<Tensor>& bias,
+                                                                             int64_t groups, int64_t kept) {
     if (!taken(logits) || logits.dim() < 1 || logits.size(-1) < 1 || logits.size(-1) > api.max_experts || k < 1 ||
         k > std::min<int64_t>(logits.size(-1), api.max_k))
         return std::nullopt;
     if (mask && (mask->scalar_type() != at::kBool || mask->device() != logits.device() ||
                  mask->sizes() != logits.sizes().slice(0, logits.dim() - 1)))
         return std::nullopt;
+    const int64_t experts = logits.size(-1);
+    if (scores < 0 || groups < 1 || groups > std::min<int64_t>(experts, api.max_groups) || experts % groups != 0 || kept < 1 || kept > groups ||
+        k > kept * (experts / groups))
+        return std::nullopt;
+    if (bias && (bias->scalar_type() != at::kFloat || bias->device() != logits.device() || bias->dim() != 1 || bias->size(0) != experts ||
+                 any_requires_grad({&*bias}) || any_tangent({&*bias})))
+        return std::nullopt;
     if (any_tangent({&logits})) return std::nullopt;
+    const RouteScores by{scores, groups, kept, bias.value_or(Tensor())};
     const py::gil_scoped_release released;
     if (any_requires_grad({&logits})) {
-        const variable_list out = RouteTopk::apply(logits, k, mask, normalize);
+        const variable_list out = RouteTopk::apply(logits, k, mask, normalize, by);
         return std::make_tuple(out[0], out[1], out[2], out[3], out[4]);
     }
-    const RouteOut o = route_forward(logits, k, mask.value_or(Tensor()), normalize);
+    const RouteOut o = route_forward(logits, k, mask.value_or(Tensor()), normalize, by);
     return std::make_tuple(o.weights, o.indices, o.counts, o.balance, o.z);
 }
 
@@ -950,7 +977,8 @@ void bind(const py::dict& addresses, const py::object& error) {
     get(api.residual_norm_backward, "muon_amd_residual_norm_backward");
     get(api.residual_norm_partials, "muon_amd_residual_norm_partials");
     get(api.route, "muon_amd_route");
-    get(api.route_backward, "muon_amd_route_backward");
+    get(api.route_scored, "muon_amd_route_scored");
+    get(api.route_backward, "muon_amd_route_scored_backward");
     get(api.route_partials, "muon_amd_route_partials");
     get(api.head_loss, "muon_amd_head_loss");
     get(api.head_loss_backward, "muon_amd_head_loss_backward");
@@ -972,6 +1000,7 @@ void bind(const py::dict& addresses, const py::object& error) {
     api.max_width = number("muon_amd_residual_norm_max_width");
     api.max_experts = number("muon_amd_route_max_experts");
     api.max_k = number("muon_amd_route_max_k");
+    api.max_groups = number("muon_amd_route_max_groups");
     api.max_top = number("muon_amd_distill_max_top");
     api.shared_elems = number("muon_amd_adamw_shared_elems");
     api.block_elems = number("muon_amd_elementwise_block_elems");
@@ -1004,7 +1033,9 @@ PYBIND11_MODULE(_native, m) {
     m.def("bind", &bind);
     m.def("abi_version", [] { return MUON_AMD_ABI_VERSION; });
     m.def("residual_norm", &residual_norm);
-    m.def("route_topk", &route_topk);
+    m.def("route_topk", &route_topk, py::arg("logits"), py::arg("k"), py::arg("mask"), py::arg("normalize"),
+          py::arg("scores") = static_cast<int64_t>(MUON_AMD_SCORES_SOFTMAX), py::arg("bias") = py::none(), py::arg("groups") = static_cast<int64_t>(1),
+          py::arg("kept") = static_cast<int64_t>(1));
     m.def("linear_cross_entropy", &linear_cross_entropy);
     m.def("distill_topk", &distill_topk);
     m.def("adamw_launch", &adamw_launch);

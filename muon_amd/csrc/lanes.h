@@ -70,4 +70,11 @@ __device__ __forceinline__ float exp_of(float d) {
     return fmaf(e * LN2, lost, e);
 }
 
+// 1 / (1 + e^-x) and, with it, 1 / (1 + e^x): about four units off, relative to themselves.  Not a number gives what is none.
+__device__ __forceinline__ float sigmoid_of(float x, float& rest) {
+    const float t = exp_of(-fabsf(x)), r = __builtin_amdgcn_rcpf(1.f + t), small = t * r;
+    rest = x >= 0.f ? small : r;
+    return x != x ? x : x >= 0.f ? r : small;
+}
+
 }  // namespace muon_amd

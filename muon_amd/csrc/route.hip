@@ -14,74 +14,9 @@
 // of it the eight maxima; 21 us backward for 74 MB), launches where there are few (1024 tokens, 2 of 8: 4.4, 3.6 and 4.4 us).
 // Sums over tokens: each lane adds the probabilities of its experts over its rows, a workgroup joins its lanes in a
 // fixed order, and a second launch joins the workgroups; counts are whole numbers, in any order the same.
-#include <type_traits>
-
-#include "lanes.h"
+#include "route.h"
 
 namespace muon_amd {
-
-constexpr int RT_MAX_EXPERTS = 1024;
-constexpr int RT_MAX_K = 32;
-constexpr int RT_THREADS = 512;
-constexpr int RT_WAVES = RT_THREADS / 64;
-constexpr int RT_GROUPS = 512;             // workgroups at most: their partial sums are joined by one launch
-
-// A logit's bits in the order of its value: negative numbers below positive ones, both zeros equal, NaN above all.
-__device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t b = __float_as_uint(x == x ? x + 0.f : __builtin_nanf(""));
-    return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
-}
-__device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
-constexpr uint32_t ORDERED_MINUS_INF = 0x007fffffu;          // of -infinity
-
-template <typename T>
-struct Key;
-template <>
-struct Key<uint16_t> {
-    typedef uint32_t type;
-    static __device__ __forceinline__ type of(float x, int e) { return (ordered(x) & 0xffff0000u) | (0xffffu - static_cast<uint32_t>(e)); }
-    static __device__ __forceinline__ int index(type k) { return static_cast<int>(0xffffu - (k & 0xffffu)); }
-    // (-infinity and what is beyond the row: 0x007f in the upper half and below)
-    static __device__ __forceinline__ bool available(type k) { return (k >> 16) > (ORDERED_MINUS_INF >> 16); }
-    static __device__ __forceinline__ float value(type k) { return __uint_as_float(__float_as_uint(value_of(k)) & 0xffff0000u); }
-};
-template <>
-struct Key<float> {
-    typedef uint64_t type;
-    static __device__ __forceinline__ type of(float x, int e) {
-        return (static_cast<uint64_t>(ordered(x)) << 32) | (0xffffffffu - static_cast<uint32_t>(e));
-    }
-    static __device__ __forceinline__ int index(type k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
-    static __device__ __forceinline__ bool available(type k) { return static_cast<uint32_t>(k >> 32) > ORDERED_MINUS_INF; }
-    static __device__ __forceinline__ float value(type k) { return value_of(static_cast<uint32_t>(k >> 32)); }
-};
-
-// Where a token's row of logits is, and whether it takes part.
-template <typename T>
-__device__ __forceinline__ const T* row_of(const MuonRoute& a, int64_t t) {
-    return static_cast<const T*>(a.logits) + t * a.ld_logits;
-}
-__device__ __forceinline__ bool unmasked(const MuonRoute& a, int64_t t) { return t < a.tokens && (!a.mask || a.mask[t]); }
-
-// A row's packs as they are requested, and its logits in fp32 once they are there: -infinity beyond the row and where the
-// token takes no part.
-template <typename T, int N>
-struct RowPacks {
-    static constexpr int G = pack_of<T>;
-    Pack<T, G> v[N / G];
-    __device__ __forceinline__ void load(const T* row, int base, int experts) {
-#pragma unroll
-        for (int g = 0; g < N / G; ++g) v[g] = request<T, G, false>(row, base + G * g, experts);
-    }
-    __device__ __forceinline__ void get(int base, int experts, bool in, float (&x)[N]) {
-#pragma unroll
-        for (int g = 0; g < N / G; ++g) {
-            settle<T, G>(v[g], base + G * g, experts);
-#pragma unroll
-            for (int i = 0; i < G; ++i) x[G * g + i] = in && base + G * g + i < experts ? v[g][i] : -__builtin_inff();
-        }
-    }
-};
 
 // partials: workgroups x experts pairs {sum of p, tokens}, then workgroups x {sum of lse^2, tokens that take part}, then
 // what the launch that joins them needs (a counter, which this one clears, and a float for each of its workgroups).
@@ -285,15 +220,11 @@ __global__ __launch_bounds__(RJ_THREADS) void route_join_kernel(const MuonRoute 
     *a.part = part;
 }
 
-// What lanes of a wave left in LDS is there for its other lanes (whose accesses are in order), for the compiler too.
-__device__ __forceinline__ void wave_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 constexpr int RB_THREADS = 256;
 constexpr int RB_GROUPS = 1024;            // workgroups: four for each CU, each set up once (65536 x 256: 20.8 us; 1536: 20.6, 2048: 22)
-template <typename T, int N, int L>
+// SIGMOID: scores s = sigmoid(l) instead of p, with q = s / sum s in the balance loss (route_scored.hip):
+//   dl = s (1 - s) (g - sum q g) / sum s + 2 cz lse / N p + [at S] (1 - s) w (dw - sum w dw)
+template <typename T, int N, int L, bool SIGMOID>
 __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRoute a) {
     constexpr int ROWS = RB_THREADS / L, G = pack_of<T>;
     // What the weights' gradients add, by expert.  Four experts of a lane lie next to those of the next lane, so that the
@@ -352,6 +283,7 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
         }
         wave_order();
         float x[N], p[N], u[N], dot = 0.f;
+        [[maybe_unused]] float s[SIGMOID ? N : 1], rest_of[SIGMOID ? N : 1], norm = 0.f;
         packs.get(base, E, on, x);
 #pragma unroll
         for (int q = 0; q < N / 4; ++q) {
@@ -362,10 +294,21 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             p[i] = exp_of(x[i] - lse - rest);      // (zero where the token takes no part: x is -infinity)
-            dot = fmaf(p[i], g[i], dot);
-            if (!a.normalize) dot += u[i];         // p dw: what comes through the probabilities themselves
+            if constexpr (SIGMOID) {
+                s[i] = sigmoid_of(x[i], rest_of[i]);
+                norm += s[i];
+                dot = fmaf(s[i], g[i], dot);
+            } else {
+                dot = fmaf(p[i], g[i], dot);
+                if (!a.normalize) dot += u[i];     // p dw: what comes through the probabilities themselves
+            }
         }
         dot = group_sum<L>(dot);
+        if constexpr (SIGMOID) {
+            norm = group_sum<L>(norm);
+            norm = norm != 0.f ? 1.f / norm : 0.f;
+            dot *= norm;
+        }
         const float all = on ? fmaf(cz, lse, -dot) : 0.f;
         wave_order();
         if (a.dweights) {
@@ -380,27 +323,20 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
         for (int q = 0; q < N / G; ++q) {
             float d[G];
 #pragma unroll
-            for (int i = 0; i < G; ++i) d[i] = fmaf(p[G * q + i], g[G * q + i] + all, u[G * q + i]);
+            for (int i = 0; i < G; ++i) {
+                const int k = G * q + i;
+                if constexpr (SIGMOID) {
+                    const float from = s[k] * rest_of[k] * (norm * (g[k] - dot)) + u[k] * rest_of[k];
+                    d[i] = on ? fmaf(p[k], cz * lse, from) : 0.f;
+                } else {
+                    d[i] = fmaf(p[k], g[k] + all, u[k]);
+                }
+            }
             store_pack<T, G, false>(static_cast<T*>(a.dlogits) + t * E, base + G * q, E, Pack<T, G>::of(d));
         }
     }
 }
 
-template <int A, int B>
-struct RouteShape {
-    static constexpr int N = A, L = B;
-};
-template <typename F>
-static void with_route_shape(int experts, F&& f) {
-    if (experts <= 8) f(RouteShape<8, 1>{});
-    else if (experts <= 16) f(RouteShape<8, 2>{});
-    else if (experts <= 32) f(RouteShape<8, 4>{});
-    else if (experts <= 64) f(RouteShape<8, 8>{});
-    else if (experts <= 128) f(RouteShape<16, 8>{});
-    else if (experts <= 256) f(RouteShape<16, 16>{});
-    else if (experts <= 512) f(RouteShape<16, 32>{});
-    else f(RouteShape<16, 64>{});
-}
 // Forward 16 elements for each lane keep the reductions short (65536 x 256 26 us; 8 elements 29, 32 elements 31); backward, with
 // one reduction, 8 leave room for twice the waves (21 us; 16 elements 23, 32 elements 29).
 template <typename F>
@@ -411,28 +347,9 @@ static void with_route_backward_shape(int experts, F&& f) {
     else if (experts <= 512) f(RouteShape<8, 64>{});
     else f(RouteShape<16, 64>{});
 }
-static int route_groups(int64_t tokens, int experts) {
-    int rows = 1;
-    with_route_shape(experts, [&](auto s) { rows = RT_THREADS / decltype(s)::L; });
-    const int64_t n = (tokens + rows - 1) / rows;
-    return static_cast<int>(n < RT_GROUPS ? n : RT_GROUPS);
-}
-
-static int check_route(const MuonRoute* a, const char* what) {
-    MUON_REQUIRE(a, "%s: null arguments", what);
-    MUON_REQUIRE(a->tokens > 0 && a->experts > 0 && a->experts <= RT_MAX_EXPERTS, "%s: tokens=%lld experts=%d (at most %d)", what,
-                 static_cast<long long>(a->tokens), a->experts, RT_MAX_EXPERTS);
-    MUON_REQUIRE(a->k > 0 && a->k <= a->experts && a->k <= RT_MAX_K, "%s: k=%d of %d experts (at most %d)", what, a->k, a->experts, RT_MAX_K);
-    MUON_REQUIRE(a->logits && a->weights && a->indices && a->counts && a->part && a->lse && a->lse_rest, "%s: null pointer", what);
-    MUON_REQUIRE(a->dtype == MUON_AMD_SRC_F32 || a->dtype == MUON_AMD_SRC_BF16, "%s: dtype=%d", what, a->dtype);
-    return MUON_AMD_OK;
-}
-
-
-template <typename F>
-static void with_route_type(int dtype, F&& f) {
-    if (dtype == MUON_AMD_SRC_BF16) f(uint16_t{});
-    else f(float{});
+int launch_route_join(const MuonRoute& a, int groups, hipStream_t stream) {
+    hipLaunchKernelGGL(route_join_kernel, dim3((a.experts + RJ_EXPERTS - 1) / RJ_EXPERTS), dim3(RJ_THREADS), 0, stream, a, groups);
+    return check_launch("route");
 }
 
 }  // namespace muon_amd
@@ -462,20 +379,25 @@ int muon_amd_route(const MuonRoute* args, void* stream) {
         });
     });
     if (const int rc = check_launch("route")) return rc;
-    hipLaunchKernelGGL(route_join_kernel, dim3((a.experts + RJ_EXPERTS - 1) / RJ_EXPERTS), dim3(RJ_THREADS), 0, st, a, n);
-    return check_launch("route");
+    return launch_route_join(a, n, st);
 }
 
-int muon_amd_route_backward(const MuonRoute* args, void* stream) {
+int muon_amd_route_backward(const MuonRoute* args, void* stream) { return muon_amd_route_scored_backward(args, MUON_AMD_SCORES_SOFTMAX, stream); }
+
+int muon_amd_route_scored_backward(const MuonRoute* args, int scores, void* stream) {
     if (const int rc = check_route(args, "route_backward")) return rc;
     const MuonRoute a = *args;
     MUON_REQUIRE(a.dlogits, "route_backward: null output");
+    MUON_REQUIRE(scores == MUON_AMD_SCORES_SOFTMAX || scores == MUON_AMD_SCORES_SIGMOID, "route_backward: scores=%d", scores);
     with_route_type(a.dtype, [&](auto x) {
         with_route_backward_shape(a.experts, [&](auto s) {
             constexpr int ROWS = RB_THREADS / decltype(s)::L;
             const int64_t n = (a.tokens + ROWS - 1) / ROWS;
-            hipLaunchKernelGGL((route_backward_kernel<decltype(x), decltype(s)::N, decltype(s)::L>), dim3(n < RB_GROUPS ? n : RB_GROUPS),
-                               dim3(RB_THREADS), 0, static_cast<hipStream_t>(stream), a);
+            const auto go = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3(n < RB_GROUPS ? n : RB_GROUPS), dim3(RB_THREADS), 0, static_cast<hipStream_t>(stream), a);
+            };
+            if (scores == MUON_AMD_SCORES_SIGMOID) go(route_backward_kernel<decltype(x), decltype(s)::N, decltype(s)::L, true>);
+            else go(route_backward_kernel<decltype(x), decltype(s)::N, decltype(s)::L, false>);
         });
     });
     return check_launch("route_backward");

@@ -91,7 +91,8 @@ class Routing(NamedTuple):
     z_loss: torch.Tensor         # 0-dim fp32
 
 
-def route_topk(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = None, normalize: bool = True) -> Routing:
+def route_topk(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = None, normalize: bool = True, scores: str = "softmax",
+               bias: torch.Tensor | None = None, groups: int = 1, groups_kept: int | None = None) -> Routing:
     """The k experts of each token from its logits (..., experts), fp32 or bf16, with the losses of a balanced router:
 
         p = softmax(logits);  indices: the k largest logits, of equal ones the lowest index first
@@ -103,15 +104,26 @@ def route_topk(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = None
     that have an expert available at all.  An expert whose logit is -infinity is not available to that token; a
     choice that is not there has index -1 and weight 0.  A token that takes no part has indices -1, weights 0 and no
     gradient.  Gradients flow to the logits from weights, balance_loss (through p; counts are constants) and z_loss.
-    NaN counts as the largest logit.  At most 1024 experts and 32 choices.  Sums are fp32 in a fixed order."""
-    if isinstance(k, int) and not isinstance(k, bool):
-        out = _lib.native().route_topk(logits, k, mask, bool(normalize))
+    NaN counts as the largest logit.  At most 1024 experts and 32 choices.  Sums are fp32 in a fixed order.
+
+    A router that is balanced without a loss chooses by other numbers than it weighs with:
+
+        s = softmax(logits), or (scores="sigmoid") sigmoid(logits);  c = s + bias
+        the experts lie in `groups` equal runs, whose scores are the sums of their two largest c; the `groups_kept` best ones take part
+        indices: the k largest c among those, of equal ones the lowest index first;  weights: s at indices, as above
+
+    bias: one fp32 number for each expert, without a gradient (a program raises it for experts with few tokens and lowers it for
+    those with many); an expert whose bias is -infinity is not available.  balance_loss is then over s divided by its sum over the
+    experts.  What is chosen goes by the order of the c as in 64 bits, not by the rounding of an exponential.  At most 64 groups."""
+    if all(isinstance(n, int) and not isinstance(n, bool) for n in (k, groups, 1 if groups_kept is None else groups_kept)):
+        kept = groups if groups_kept is None else groups_kept
+        out = _lib.native().route_topk(logits, k, mask, bool(normalize), _lib.SCORES.get(scores, -1) if isinstance(scores, str) else -1, bias, groups, kept)
         if out is not None:
             return Routing(*out)
-    _refuse_route(logits, k, mask)
+    _refuse_route(logits, k, mask, scores, bias, groups, groups_kept)
 
 
-def _refuse_route(logits, k, mask):
+def _refuse_route(logits, k, mask, scores, bias, groups, groups_kept):
     """Says what is wrong with arguments that were not taken."""
     require_gpu_tensor(logits, "logits")
     _dtype(logits, "logits")
@@ -124,5 +136,22 @@ def _refuse_route(logits, k, mask):
         require_gpu_tensor(mask, "mask")
         if mask.dtype != torch.bool or mask.shape != logits.shape[:-1] or mask.device != logits.device:
             raise ValueError(f"mask must be a bool tensor of shape {tuple(logits.shape[:-1])} on {logits.device}, got {mask.dtype} {tuple(mask.shape)}")
+    if not isinstance(scores, str) or scores not in _lib.SCORES:
+        raise ValueError(f"scores must be one of {', '.join(sorted(_lib.SCORES))}, got {scores!r}")
+    experts, limit = logits.size(-1), lib.muon_amd_route_max_groups()
+    if not isinstance(groups, int) or isinstance(groups, bool) or not 1 <= groups <= limit or experts % groups:
+        raise ValueError(f"groups must be 1 to {limit} and divide the {experts} experts, got {groups!r}")
+    kept = groups if groups_kept is None else groups_kept
+    if not isinstance(kept, int) or isinstance(kept, bool) or not 1 <= kept <= groups or k > kept * (experts // groups):
+        raise ValueError(f"groups_kept must be 1 to {groups} and leave {k} experts to choose from, got {groups_kept!r}")
+    if bias is not None:
+        require_gpu_tensor(bias, "bias")
+        if bias.dtype != torch.float32:
+            raise TypeError(f"bias is {bias.dtype}: fp32 is taken")
+        if bias.shape != (experts,) or bias.device != logits.device:
+            raise ValueError(f"bias must have {experts} elements on {logits.device}, got {tuple(bias.shape)} on {bias.device}")
+        if torch.is_grad_enabled() and bias.requires_grad:
+            raise ValueError("bias requires a gradient: there is none (it steers the choice alone)")
+        _no_tangent(bias, "bias")
     _no_tangent(logits, "logits")
     raise _lib.MuonAmdError("route_topk does not take these arguments")
