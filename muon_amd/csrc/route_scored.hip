@@ -10,8 +10,8 @@
 // best one left out) are nearer than what that may be off, the wave does the row again in 64 bits: about 2 rows of a thousand
 // with sigmoid scores (8 of 256).  Equal logits with equal biases are a tie, not a near one.
 //
-// Layout as in route.hip: a row in the registers of L lanes, N elements each, the k largest by 64-bit keys (c above the complement of
-// the index).  The c go through LDS for the groups, which may begin anywhere in a lane's elements.
+// Layout as in route.hip: a row in the registers of L lanes, N elements each.  The c go through LDS for the groups, which may begin anywhere in a
+// lane's elements.
 #include "route.h"
 
 namespace muon_amd {
@@ -38,16 +38,19 @@ __device__ __forceinline__ T wave_best(T v) {
 
 // A row once more in 64 bits, by a whole wave: writes the k choices (-1 where there is none).  c: LDS of this wave for E doubles; best: for 64.
 template <typename T, bool SIGMOID>
-__device__ __noinline__ void choose_again(const T* row, const float* bias, int experts, int k, int groups, int kept, double* c, double* best, int* picks) {
+__device__ __forceinline__ void choose_again(const T* row, const float* bias, int experts, int k, int groups, int kept, double* c, double* best, int* picks) {
     const int lane = threadIdx.x & 63;
     float most = -__builtin_inff();
+#pragma unroll 1
     for (int e = lane; e < experts; e += 64) most = fmaxf(most, logit_of(row, e));
     const double top = group_reduce<64>(most, [](float x, float y) { return fmaxf(x, y); });
     double total = 0.0;
     if constexpr (!SIGMOID) {
+#pragma unroll 1
         for (int e = lane; e < experts; e += 64) total += exp(static_cast<double>(logit_of(row, e)) - top);
         total = group_reduce<64>(total, [](double x, double y) { return x + y; });
     }
+#pragma unroll 1
     for (int e = lane; e < experts; e += 64) {
         const float x = logit_of(row, e), b = bias ? bias[e] : 0.f;
         const double s = SIGMOID ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : exp(static_cast<double>(x) - top) / total;
@@ -59,6 +62,7 @@ __device__ __noinline__ void choose_again(const T* row, const float* bias, int e
         double first = -__builtin_inf(), second = -__builtin_inf();
         bool none = false;
         if (lane < groups)
+#pragma unroll 1
             for (int e = lane * size; e < (lane + 1) * size; ++e) {
                 const double v = c[e];
                 none |= v != v;
@@ -69,18 +73,22 @@ __device__ __noinline__ void choose_again(const T* row, const float* bias, int e
         best[lane] = score;
         wave_order();
         int before = 0;
+#pragma unroll 1
         for (int g = 0; g < groups; ++g) {
             const uint64_t other = ordered_double(best[g]), own = ordered_double(score);
             before += other > own || (other == own && g < lane);
         }
         const uint64_t in = __ballot(lane < groups && before < kept);
+#pragma unroll 1
         for (int e = lane; e < experts; e += 64)
             if (!(in >> (e / size) & 1)) c[e] = -__builtin_inf();
         wave_order();
     }
+#pragma unroll 1
     for (int j = 0; j < k; ++j) {
         uint64_t own = 0;
         int at = 0;
+#pragma unroll 1
         for (int e = lane; e < experts; e += 64) {
             const uint64_t v = ordered_double(c[e]);
             if (v > own) {
@@ -99,87 +107,160 @@ __device__ __noinline__ void choose_again(const T* row, const float* bias, int e
     }
 }
 
+// The weights and indices of a row by L lanes: scores of the choices, formed again from their logits (softmax: e^(l - top) per).
+constexpr int LATER = -2;                        // first index of a row that is to be done again
+template <typename T, int L, bool SIGMOID>
+__device__ __forceinline__ void put_choices(const MuonRoute& a, int64_t t, const T* row, float top, float per, const int* picks, int* tokens, int lane) {
+    const auto score_at = [&](int e) {
+        const float l = logit_of(row, e);
+        if constexpr (SIGMOID) {
+            float rest;
+            return sigmoid_of(l, rest);
+        } else {
+            const float d = l - top;
+            return (d == d ? exp_of(d) : d) * per;
+        }
+    };
+    float chosen = 0.f;
+    for (int j = lane; j < a.k; j += L) {
+        const int e = picks[j];
+        if (e >= 0) chosen += score_at(e);
+    }
+    chosen = a.normalize ? group_sum<L>(chosen) : 1.f;
+    for (int j = lane; j < a.k; j += L) {
+        const int e = picks[j];
+        const float score = e >= 0 ? score_at(e) : 0.f;
+        a.indices[t * a.k + j] = e;
+        a.weights[t * a.k + j] = chosen != 0.f ? score / chosen : 0.f;
+        if (e >= 0) atomicAdd(&tokens[e], 1);
+    }
+}
+
 template <typename T, int N, int L, bool SIGMOID>
-__global__ __launch_bounds__(RT_THREADS) void route_scored_kernel(const MuonRoute a, const float* bias, int groups, int kept) {
+__global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonRoute a, const float* bias, int groups, int kept) {
     constexpr int ROWS = RT_THREADS / L, WROWS = 64 / L;                      // rows of the workgroup, of a wave
     constexpr int PICKS = N * L < RT_MAX_K + 1 ? N * L : RT_MAX_K + 1, PG = N * L < RS_MAX_GROUPS ? N * L : RS_MAX_GROUPS;
     constexpr int ROWC = N * L + N * L / 32;                                  // a row's c, a place more every 32: groups a power of two apart
     constexpr int CFLOATS = WROWS * ROWC > 2 * N * L ? WROWS * ROWC : 2 * N * L, GFLOATS = 2 * WROWS * PG > 128 ? 2 * WROWS * PG : 128;
-    typedef Key<float> K;
+    constexpr int LIST = N * L / 2;
     __shared__ float sums[RT_WAVES][N * L];
     __shared__ int tokens[N * L];
+    __shared__ __align__(16) float biases[N * L];
     __shared__ float squares[RT_WAVES];
     __shared__ int parts[RT_WAVES];
     __shared__ __align__(8) float by_expert[RT_WAVES][CFLOATS];
     __shared__ __align__(8) float by_group[RT_WAVES][GFLOATS];
     __shared__ int pick_at[RT_WAVES][WROWS][PICKS];
     __shared__ float pick_c[RT_WAVES][WROWS][PICKS];
-    const int lane = threadIdx.x % L, sub = threadIdx.x / L, base = lane * N, E = a.experts, wave = threadIdx.x >> 6, slot = (threadIdx.x & 63) / L;
+    const int lane = threadIdx.x % L, sub = threadIdx.x / L, first_of_lane = lane * N, E = a.experts, wave = threadIdx.x >> 6, slot = (threadIdx.x & 63) / L;
     const int size = E / groups, wanted = a.k < E ? a.k + 1 : a.k;           // (one more than is chosen: what the last one is near to)
     float* const row_c = by_expert[wave] + slot * ROWC;
     float* const row_g = by_group[wave] + slot * 2 * PG;                      // scores of the groups, what each may be off by
     int* const row_at = pick_at[wave][slot];
     float* const row_pick = pick_c[wave][slot];
-    const auto larger = [](uint64_t u, uint64_t v) { return max(u, v); };
     const auto most_of = [](float u, float v) { return fmaxf(u, v); };
-    for (int e = threadIdx.x; e < N * L; e += RT_THREADS) tokens[e] = 0;
+    for (int e = threadIdx.x; e < N * L; e += RT_THREADS) {
+        tokens[e] = 0;
+        biases[e] = bias && e < E ? bias[e] : 0.f;
+    }
     __syncthreads();
-    float acc[N], b[N];
+    float acc[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        acc[i] = 0.f;
-        b[i] = bias && base + i < E ? bias[base + i] : 0.f;
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    // the groups of a lane's elements, a byte each
+    uint32_t group_of[N / 4];
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+        group_of[q] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) group_of[q] |= static_cast<uint32_t>(min((first_of_lane + 4 * q + i) / size, groups - 1)) << (8 * i);
     }
     float square = 0.f;
     int part = 0;
+    bool later = false;
     const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
     for (int64_t t = static_cast<int64_t>(blockIdx.x) * ROWS + sub; t - sub < a.tokens; t += step) {
+        // (opaque copies: what follows from them for each of N elements is formed where it is used, not kept in N registers each)
+        int base = first_of_lane;
+        asm volatile("" : "+v"(base));
         RowPacks<T, N> packs;
         const T* const row = row_of<T>(a, t < a.tokens ? t : a.tokens - 1);
         packs.load(row, base, E);
         const bool in = unmasked(a, t);
         float x[N], s[N];
         packs.get(base, E, in, x);
-        // logsumexp, scores
-        float top = -__builtin_inff(), total = 0.f;
+        // logsumexp, scores.  Where no logit is far from zero (in any row of the wave), a sigmoid's exponential serves both.
+        float top = -__builtin_inff(), total = 0.f, norm = 1.f, far = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);
         top = group_reduce<L>(top, most_of);
         if (top == -__builtin_inff()) top = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float d = x[i] - top;
-            s[i] = d == d ? exp_of(d) : d;
-            total += s[i];
-        }
-        total = group_sum<L>(total);
-        float per = total != 0.f ? 1.f / total : 0.f, norm = 0.f;
         if constexpr (SIGMOID) {
 #pragma unroll
+            for (int i = 0; i < N; ++i) far = fmaxf(far, x[i] == -__builtin_inff() ? 0.f : fabsf(x[i]));
+        }
+        if (SIGMOID && !__ballot(!(far <= 40.f))) {
+            top = 0.f;
+            norm = 0.f;
+#pragma unroll
             for (int i = 0; i < N; ++i) {
-                float rest;
-                s[i] = sigmoid_of(x[i], rest);
+                const float t = exp_of(-fabsf(x[i])), u = __builtin_amdgcn_rcpf(1.f + t);
+                // (-infinity: t is zero and stays it on this side; no number: nor is what follows)
+                const float e = x[i] >= 0.f ? __builtin_amdgcn_rcpf(t) : x[i] == x[i] ? t : x[i];
+                s[i] = x[i] >= 0.f ? u : e * u;
+                total += e;
                 norm += s[i];
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float d = x[i] - top;
+                s[i] = d == d ? exp_of(d) : d;
+                total += s[i];
+            }
+            if constexpr (SIGMOID) {
+                norm = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    float rest;
+                    s[i] = sigmoid_of(x[i], rest);
+                    norm += s[i];
+                }
+            }
+        }
+        total = group_sum<L>(total);
+        const float per = total != 0.f ? 1.f / total : 0.f;
+        if constexpr (SIGMOID) {
             norm = group_sum<L>(norm);
             norm = norm != 0.f ? 1.f / norm : 0.f;
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) s[i] *= per;
-            norm = 1.f;
         }
         // What a c may be off by, beside its own rounding: of scores up to 1 or the row's largest probability, or without a bias relative to itself
         // (softmax: that includes the rounding of differences of logits).
         constexpr float OFF = SIGMOID ? 8.f * RS_UNIT : 40.f * RS_UNIT, RELATIVE = SIGMOID ? 8.f * RS_UNIT : 128.f * RS_UNIT;
         const float off = bias ? OFF * (SIGMOID ? 1.f : per) : 0.f, relative = bias ? RS_UNIT : RELATIVE + RS_UNIT;
+        // from here on what is chosen by; the token takes part if anything is available
+        float c[N];
+        bool some = false;
+#pragma unroll
+        for (int q = 0; q < N / 4; ++q) {
+            const f32x4v b = *reinterpret_cast<const f32x4v*>(&biases[base + 4 * q]);
+#pragma unroll
+            for (int i = 4 * q; i < 4 * q + 4; ++i) {
+                c[i] = x[i] == -__builtin_inff() ? -__builtin_inff() : s[i] + b[i % 4];
+                some |= c[i] != -__builtin_inff();
+            }
+        }
+        const bool on = group_reduce<L>(static_cast<int>(some), [](int u, int v) { return u | v; }) != 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = on ? fmaf(s[i], norm, acc[i]) : acc[i];
         bool close = false;
         uint64_t in_groups = ~0ull;
         if (kept < groups) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int e = base + i;
-                row_c[e + e / 32] = x[i] == -__builtin_inff() ? -__builtin_inff() : s[i] + b[i];
-            }
+            for (int i = 0; i < N; ++i) row_c[base + base / 32 + i] = c[i];          // (a lane's elements lie within 32)
             wave_order();
             for (int g = lane; g < groups; g += L) {
                 float first = -__builtin_inff(), second = -__builtin_inff();
@@ -218,25 +299,58 @@ __global__ __launch_bounds__(RT_THREADS) void route_scored_kernel(const MuonRout
             high = group_reduce<L>(high, most_of);
             close = low <= high;
         }
-        uint64_t key[N];
+        // The `wanted` largest values, each below the one before (in `ordered` form: as in route.hip, one subtraction and one maximum for each
+        // element; there is always -infinity to end with).  Then every element that is as large as the last of them goes into a list, by
+        // index, and its place in the order is counted there: equal values are told apart by their index.
+        uint32_t key[N], best = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = base + i;
-            const bool there = x[i] != -__builtin_inff() && (kept == groups || (in_groups >> (e / size) & 1));
-            key[i] = K::of(there ? s[i] + b[i] : -__builtin_inff(), e);
+        for (int q = 0; q < N / 4; ++q) {
+            uint32_t four = group_of[q];
+            asm volatile("" : "+v"(four));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) key[4 * q + i] = in_groups >> (four >> (8 * i) & 255) & 1 ? ordered(c[4 * q + i]) : ORDERED_MINUS_INF;
         }
-        uint64_t best = 0;
-        bool on = false;
         for (int j = 0; j < wanted; ++j) {
-            uint64_t m = 0;
+            uint32_t m = ORDERED_MINUS_INF - best;
 #pragma unroll
             for (int i = 0; i < N; ++i) m = max(m, key[i] - best);
-            best += group_reduce<L>(m, larger);
-            if (j == 0) on = in && K::available(best);
-            if (lane == j % L) {
-                row_at[j] = in && K::available(best) ? K::index(best) : -1;
-                row_pick[j] = K::value(best);
+            m = group_reduce<L>(m, [](uint32_t u, uint32_t v) { return max(u, v); });
+            best += best == ORDERED_MINUS_INF ? 0u : m;
+        }
+        best = max(best, ORDERED_MINUS_INF + 1);
+        int listed = 0;
+        uint32_t* const list = reinterpret_cast<uint32_t*>(row_c);               // {value, index}, LIST of them
+        wave_order();
+        const uint64_t in_row = (L == 64 ? ~0ull : ((1ull << (L & 63)) - 1) << (slot * L)), below = in_row & ((1ull << (threadIdx.x & 63)) - 1);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool hit = key[i] >= best;
+            const uint64_t hits = __ballot(hit);
+            const int at = listed + __builtin_popcountll(hits & below);
+            if (hit && at < LIST) {
+                list[2 * at] = key[i];
+                list[2 * at + 1] = base + i;
             }
+            listed += __builtin_popcountll(hits & in_row);
+        }
+        wave_order();
+        for (int j = lane; j < wanted; j += L) row_at[j] = -1;
+        wave_order();
+        if (listed <= LIST) {
+            for (int q = lane; q < listed; q += L) {
+                const uint32_t value = list[2 * q], index = list[2 * q + 1];
+                int before = 0;
+                for (int o = 0; o < listed; ++o) {
+                    const uint32_t other = list[2 * o];
+                    before += other > value || (other == value && list[2 * o + 1] < index);
+                }
+                if (before < wanted) {
+                    row_at[before] = index;
+                    row_pick[before] = value_of(value);
+                }
+            }
+        } else {
+            close = true;                        // (many equal values: the way that needs no list)
         }
         wave_order();
         for (int j = lane + 1; j < wanted; j += L) {
@@ -245,44 +359,13 @@ __global__ __launch_bounds__(RT_THREADS) void route_scored_kernel(const MuonRout
             if (at < 0 || !(before - c <= 2.f * off + 2.f * relative * (fabsf(c) + fabsf(before)))) continue;
             if (!(logit_of(row, at) == logit_of(row, prev) && (!bias || bias[at] == bias[prev]))) close = true;
         }
-        const uint64_t again = __ballot(close && on);
-        if (again) {
-            // a row at a time, each by the whole wave
-            for (int q = 0; q < WROWS; ++q) {
-                const uint64_t lanes = L == 64 ? ~0ull : ((1ull << (L & 63)) - 1) << (q * L);
-                if (!(again & lanes)) continue;
-                const int64_t tq = t - slot + q;
-                choose_again<T, SIGMOID>(row_of<T>(a, tq), bias, E, a.k, groups, kept, reinterpret_cast<double*>(by_expert[wave]),
-                                         reinterpret_cast<double*>(by_group[wave]), pick_at[wave][q]);
-            }
-            wave_order();
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] = on ? fmaf(s[i], norm, acc[i]) : acc[i];
+        close = group_reduce<L>(static_cast<int>(close), [](int u, int v) { return u | v; }) != 0;
         if (t >= a.tokens) continue;
-        // the weights: scores of the choices, formed again from their logits
-        const auto score_at = [&](int e) {
-            const float l = logit_of(row, e);
-            if constexpr (SIGMOID) {
-                float rest;
-                return sigmoid_of(l, rest);
-            } else {
-                const float d = l - top;
-                return (d == d ? exp_of(d) : d) * per;
-            }
-        };
-        float chosen = 0.f;
-        for (int j = lane; j < a.k; j += L) {
-            const int e = row_at[j];
-            if (e >= 0) chosen += score_at(e);
-        }
-        chosen = a.normalize ? group_sum<L>(chosen) : 1.f;
-        for (int j = lane; j < a.k; j += L) {
-            const int e = row_at[j];
-            const float score = e >= 0 ? score_at(e) : 0.f;
-            a.indices[t * a.k + j] = e;
-            a.weights[t * a.k + j] = chosen != 0.f ? score / chosen : 0.f;
-            if (e >= 0) atomicAdd(&tokens[e], 1);
+        if (on && close) {                       // (the rows that are done again come after the loop, out of its registers' way)
+            if (lane == 0) a.indices[t * a.k] = LATER;
+            later = true;
+        } else {
+            put_choices<T, L, SIGMOID>(a, t, row, top, per, row_at, tokens, lane);
         }
         if (lane == 0) {
             const float log_total = logf(total), lse = top + log_total;
@@ -293,11 +376,26 @@ __global__ __launch_bounds__(RT_THREADS) void route_scored_kernel(const MuonRout
             part += on;
         }
     }
+    if (__ballot(later)) {
+        const int whole = threadIdx.x & 63;
+        for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS + sub - slot; first < a.tokens; first += step) {
+            const int64_t own = first + whole;
+            uint64_t again = __ballot(whole < WROWS && own < a.tokens && a.indices[(own < a.tokens ? own : first) * a.k] == LATER);
+            for (; again; again &= again - 1) {
+                const int64_t t = first + __builtin_ctzll(again);
+                const T* const row = row_of<T>(a, t);
+                choose_again<T, SIGMOID>(row, bias, E, a.k, groups, kept, reinterpret_cast<double*>(by_expert[wave]),
+                                         reinterpret_cast<double*>(by_group[wave]), pick_at[wave][0]);
+                put_choices<T, 64, SIGMOID>(a, t, row, a.lse[t], expf(-a.lse_rest[t]), pick_at[wave][0], tokens, whole);
+                wave_order();
+            }
+        }
+    }
     // join the workgroup's rows: those of a wave, then the waves
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         acc[i] = sum_of_groups<L>(acc[i]);
-        if ((threadIdx.x & 63) < L) sums[threadIdx.x >> 6][base + i] = acc[i];
+        if ((threadIdx.x & 63) < L) sums[threadIdx.x >> 6][first_of_lane + i] = acc[i];
     }
     square = group_sum<64>(square);
     part = group_reduce<64>(part, [](int u, int v) { return u + v; });
