@@ -63,12 +63,14 @@ __device__ __forceinline__ float group_sum(float v) {
 // e^d for d at most 0: 2^(d log2 e) by the target's instruction, with what the product lost put back, so
 // about two units off over the whole range.  Not a number gives zero like -infinity: what a row with such a logit, or with
 // +infinity, returns then follows from its sum of zero (1 / 0 times 0) or from its lse, neither of which is a number.
-__device__ __forceinline__ float exp_of(float d) {
+__device__ __forceinline__ float exp_of_bounded(float d) {       // (from -200 on)
     constexpr float L = 1.44269504088896341f, LN2 = 0.69314718055994531f;
-    d = fmaxf(d, -200.f);                                        // (e^-200 is zero; -infinity would leave no number in `lost`)
     const float t = d * L, lost = fmaf(d, L, -t), e = __builtin_amdgcn_exp2f(t);
     return fmaf(e * LN2, lost, e);
 }
+
+// (e^-200 is zero; -infinity would leave no number in `lost`)
+__device__ __forceinline__ float exp_of(float d) { return exp_of_bounded(fmaxf(d, -200.f)); }
 
 // 1 / (1 + e^-x) and, with it, 1 / (1 + e^x): about four units off, relative to themselves.  Not a number gives what is none.
 __device__ __forceinline__ float sigmoid_of(float x, float& rest) {

@@ -60,6 +60,15 @@ struct RowPacks {
 #pragma unroll
         for (int g = 0; g < N / G; ++g) v[g] = request<T, G, false>(row, base + G * g, experts);
     }
+    // (zeros beyond the row)
+    __device__ __forceinline__ void get(int base, int experts, float (&x)[N]) {
+#pragma unroll
+        for (int g = 0; g < N / G; ++g) {
+            settle<T, G>(v[g], base + G * g, experts);
+#pragma unroll
+            for (int i = 0; i < G; ++i) x[G * g + i] = v[g][i];
+        }
+    }
     __device__ __forceinline__ void get(int base, int experts, bool in, float (&x)[N]) {
 #pragma unroll
         for (int g = 0; g < N / G; ++g) {

@@ -31,6 +31,9 @@ __device__ __forceinline__ float logit_of(const T* row, int e) {
     else return row[e];
 }
 
+// exp_of that hands on what is no number.
+__device__ __forceinline__ float exp_with_nan(float d) { return exp_of_bounded(d < -200.f ? -200.f : d); }
+
 template <typename T>
 __device__ __forceinline__ T wave_best(T v) {
     return group_reduce<64>(v, [](T x, T y) { return x > y ? x : y; });
@@ -60,16 +63,14 @@ __device__ __forceinline__ void choose_again(const T* row, const float* bias, in
     if (kept < groups) {
         const int size = experts / groups;
         double first = -__builtin_inf(), second = -__builtin_inf();
-        bool none = false;
         if (lane < groups)
 #pragma unroll 1
             for (int e = lane * size; e < (lane + 1) * size; ++e) {
-                const double v = c[e];
-                none |= v != v;
+                const double v = c[e] == c[e] ? c[e] : __builtin_inf();
                 second = fmax(second, fmin(first, v));
                 first = fmax(first, v);
             }
-        const double score = none ? __builtin_nan("") : second == -__builtin_inf() ? first : first + second;
+        const double score = second == -__builtin_inf() ? first : first + second;
         best[lane] = score;
         wave_order();
         int before = 0;
@@ -177,7 +178,9 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
     }
     float square = 0.f;
     int part = 0;
-    bool later = false;
+    bool later = false, biases_none = false;
+    for (int e = 0; e < N; ++e) biases_none |= biases[first_of_lane + e] != biases[first_of_lane + e];
+    biases_none = __ballot(biases_none) != 0;
     const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
     for (int64_t t = static_cast<int64_t>(blockIdx.x) * ROWS + sub; t - sub < a.tokens; t += step) {
         // (opaque copies: what follows from them for each of N elements is formed where it is used, not kept in N registers each)
@@ -188,34 +191,33 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
         packs.load(row, base, E);
         const bool in = unmasked(a, t);
         float x[N], s[N];
-        packs.get(base, E, in, x);
-        // logsumexp, scores.  Where no logit is far from zero (in any row of the wave), a sigmoid's exponential serves both.
-        float top = -__builtin_inff(), total = 0.f, norm = 1.f, far = 0.f;
+        packs.get(base, E, x);
+        const int limit = in ? E - base : 0;
+        if (__ballot(limit < N)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = i < limit ? x[i] : -__builtin_inff();
+        }
+        // logsumexp, scores.  Where the largest logit (of every row of the wave) is not far from zero, a sigmoid's exponential serves both: what
+        // is lost of logits far below it is nothing beside its own.
+        float top = -__builtin_inff(), total = 0.f, norm = 1.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);
         top = group_reduce<L>(top, most_of);
         if (top == -__builtin_inff()) top = 0.f;
-        if constexpr (SIGMOID) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) far = fmaxf(far, x[i] == -__builtin_inff() ? 0.f : fabsf(x[i]));
-        }
-        if (SIGMOID && !__ballot(!(far <= 40.f))) {
+        if (SIGMOID && !__ballot(!(fabsf(top) <= 40.f))) {
             top = 0.f;
             norm = 0.f;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float t = exp_of(-fabsf(x[i])), u = __builtin_amdgcn_rcpf(1.f + t);
-                // (-infinity: t is zero and stays it on this side; no number: nor is what follows)
-                const float e = x[i] >= 0.f ? __builtin_amdgcn_rcpf(t) : x[i] == x[i] ? t : x[i];
-                s[i] = x[i] >= 0.f ? u : e * u;
+                const float t = exp_with_nan(-fabsf(x[i])), u = __builtin_amdgcn_rcpf(1.f + t), e = x[i] >= 0.f ? __builtin_amdgcn_rcpf(t) : t;
+                s[i] = x[i] >= 0.f ? u : t * u;
                 total += e;
                 norm += s[i];
             }
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float d = x[i] - top;
-                s[i] = d == d ? exp_of(d) : d;
+                s[i] = exp_with_nan(x[i] - top);
                 total += s[i];
             }
             if constexpr (SIGMOID) {
@@ -256,59 +258,86 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
         const bool on = group_reduce<L>(static_cast<int>(some), [](int u, int v) { return u | v; }) != 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = on ? fmaf(s[i], norm, acc[i]) : acc[i];
-        bool close = false;
-        uint64_t in_groups = ~0ull;
+        // (a row in which anything is no number is done again, where that is the largest value)
+        bool close = total != total || biases_none, lane_in = true;
+        uint64_t in_groups = 0;
         if (kept < groups) {
+            // the two largest c of each group: of a lane's elements where they are of one group, else through all of them in LDS
+            const bool whole = size % N == 0;
+            if (whole) {
+                float first = c[0], second = -__builtin_inff();
 #pragma unroll
-            for (int i = 0; i < N; ++i) row_c[base + base / 32 + i] = c[i];          // (a lane's elements lie within 32)
+                for (int i = 1; i < N; ++i) {
+                    second = fmaxf(second, fminf(first, c[i]));
+                    first = fmaxf(first, c[i]);
+                }
+                row_c[2 * lane] = first;
+                row_c[2 * lane + 1] = second;
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) row_c[base + base / 32 + i] = c[i];      // (a lane's elements lie within 32)
+            }
             wave_order();
             for (int g = lane; g < groups; g += L) {
                 float first = -__builtin_inff(), second = -__builtin_inff();
-                bool none = false;
-                for (int e = g * size; e < (g + 1) * size; ++e) {
-                    const float v = row_c[e + e / 32];
-                    none |= v != v;
-                    second = fmaxf(second, fminf(first, v));
-                    first = fmaxf(first, v);
+                if (whole) {
+                    for (int q = g * (size / N); q < (g + 1) * (size / N); ++q) {
+                        const float u = row_c[2 * q], v = row_c[2 * q + 1];
+                        second = fmaxf(fmaxf(second, v), fminf(first, u));
+                        first = fmaxf(first, u);
+                    }
+                } else {
+                    for (uint32_t e = g * size; e < static_cast<uint32_t>((g + 1) * size); ++e) {
+                        const float v = row_c[e + (e >> 5)];
+                        second = fmaxf(second, fminf(first, v));
+                        first = fmaxf(first, v);
+                    }
                 }
-                const float score = second == -__builtin_inff() ? first : first + second;
-                row_g[g] = none ? __builtin_nanf("") : score;
-                row_g[PG + g] = 2.f * off + 2.f * relative * (fabsf(first) + (second == -__builtin_inff() ? 0.f : fabsf(second)));
+                const bool one = second == -__builtin_inff();
+                row_g[g] = one ? first : first + second;
+                row_g[PG + g] = 2.f * off + 2.f * relative * (fabsf(first) + (one ? 0.f : fabsf(second)));
             }
             wave_order();
             // rank of each group; how near the two sides of the border may come
             float low = __builtin_inff(), high = -__builtin_inff();
-            uint64_t mine = 0;
             for (int g = lane; g < groups; g += L) {
                 const float score = row_g[g];
-                const uint32_t own = ordered(score);
                 int before = 0;
                 for (int o = 0; o < groups; ++o) {
-                    const uint32_t other = ordered(row_g[o]);
-                    before += other > own || (other == own && o < g);
+                    const float other = row_g[o];
+                    before += other > score || (other == score && o < g);
                 }
                 if (before < kept) {
-                    mine |= 1ull << g;
+                    in_groups |= 1ull << g;
                     low = fminf(low, score - row_g[PG + g]);
                 } else if (score != -__builtin_inff()) {
                     high = fmaxf(high, score + row_g[PG + g]);
                 }
             }
-            in_groups = group_reduce<L>(mine, [](uint64_t u, uint64_t v) { return u | v; });
+            in_groups = group_reduce<L>(in_groups, [](uint64_t u, uint64_t v) { return u | v; });
             low = -group_reduce<L>(-low, most_of);
             high = group_reduce<L>(high, most_of);
-            close = low <= high;
+            close |= low <= high;
+            if (whole) {
+                lane_in = in_groups >> (group_of[0] & 255) & 1;
+            } else {
+#pragma unroll
+                for (int q = 0; q < N / 4; ++q) {
+                    uint32_t four = group_of[q];
+                    asm volatile("" : "+v"(four));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) c[4 * q + i] = in_groups >> (four >> (8 * i) & 255) & 1 ? c[4 * q + i] : -__builtin_inff();
+                }
+            }
         }
-        // The `wanted` largest values, each below the one before (in `ordered` form: as in route.hip, one subtraction and one maximum for each
-        // element; there is always -infinity to end with).  Then every element that is as large as the last of them goes into a list, by
-        // index, and its place in the order is counted there: equal values are told apart by their index.
+        // The `wanted` largest values, each below the one before (in the order of their bits: as in route.hip, one subtraction and one maximum for
+        // each element; there is always -infinity to end with).  Then every element that is as large as the last of them goes into a list,
+        // by index, and its place in the order is counted there: equal values are told apart by their index.
         uint32_t key[N], best = 0;
 #pragma unroll
-        for (int q = 0; q < N / 4; ++q) {
-            uint32_t four = group_of[q];
-            asm volatile("" : "+v"(four));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) key[4 * q + i] = in_groups >> (four >> (8 * i) & 255) & 1 ? ordered(c[4 * q + i]) : ORDERED_MINUS_INF;
+        for (int i = 0; i < N; ++i) {
+            const uint32_t bits = __float_as_uint(lane_in ? c[i] : -__builtin_inff());
+            key[i] = bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
         }
         for (int j = 0; j < wanted; ++j) {
             uint32_t m = ORDERED_MINUS_INF - best;
@@ -319,20 +348,25 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
         }
         best = max(best, ORDERED_MINUS_INF + 1);
         int listed = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) listed += key[i] >= best;
+        int at = listed;                                     // of this lane and those before it
+#pragma unroll
+        for (int d = 1; d < L; d <<= 1) {
+            const int o = __shfl_up(at, d, L);
+            at += lane >= d ? o : 0;
+        }
+        at -= listed;
+        listed = group_reduce<L>(listed, [](int u, int v) { return u + v; });
         uint32_t* const list = reinterpret_cast<uint32_t*>(row_c);               // {value, index}, LIST of them
         wave_order();
-        const uint64_t in_row = (L == 64 ? ~0ull : ((1ull << (L & 63)) - 1) << (slot * L)), below = in_row & ((1ull << (threadIdx.x & 63)) - 1);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const bool hit = key[i] >= best;
-            const uint64_t hits = __ballot(hit);
-            const int at = listed + __builtin_popcountll(hits & below);
-            if (hit && at < LIST) {
+        for (int i = 0; i < N; ++i)
+            if (key[i] >= best && at < LIST) {
                 list[2 * at] = key[i];
                 list[2 * at + 1] = base + i;
+                ++at;
             }
-            listed += __builtin_popcountll(hits & in_row);
-        }
         wave_order();
         for (int j = lane; j < wanted; j += L) row_at[j] = -1;
         wave_order();
