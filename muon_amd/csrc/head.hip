@@ -26,6 +26,7 @@ namespace muon_amd {
 
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 constexpr int HD_TILE = 256;                        // rows of the copy of the hidden states are padded to this
+constexpr int HD_CUS = 256;                         // compute units
 constexpr int HD_FEW = 64;                          // tokens that the streaming kernel takes
 
 // ---------------------------------------------------------------------------------------------
@@ -47,7 +48,8 @@ struct HeadGemm {
     int64_t ldp, ldq;
     int64_t end_p, end_q;
     const int32_t* count;          // tokens that take part
-    int row_tiles, col_tiles, splits;   // (row_tiles of a product over tokens: at most; the count decides)
+    const int32_t* splits;         // HEAD_DHIDDEN: shares of the k-blocks
+    int row_tiles, col_tiles, most_splits;   // (row_tiles of a product over tokens: at most; the count decides)
     int rows, cols, kblocks;       // rows / cols of the output (rows of a product over tokens: from the count), k-blocks (HEAD_DWEIGHT: from the count)
     int col_limit;                 // columns of a k-major Q row that may be read
     int row_limit;                 // likewise of a k-major P row
@@ -176,14 +178,14 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const Hea
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WGN, wn = wave % WGN;
     const int rows = PRODUCT == HEAD_DWEIGHT ? a.rows : count;
     const int row_tiles = (rows + Cfg::BT - 1) / Cfg::BT, tiles = row_tiles * a.col_tiles;
-    const int id = static_cast<int>(blockIdx.x);
-    if (id >= tiles * a.splits) return;
-    const int place = place_of(id, tiles * a.splits), split = place / tiles;
+    const int id = static_cast<int>(blockIdx.x), splits = PRODUCT == HEAD_DHIDDEN ? *a.splits : 1;
+    if (id >= tiles * splits) return;
+    const int place = place_of(id, tiles * splits), split = place / tiles;
     const TileAt tile = tile_at(place - split * tiles, row_tiles, a.col_tiles);
     const int i0 = tile.row * Cfg::BT, j0 = tile.col * Cfg::BT;
     // k-blocks of this share
     const int all = PRODUCT == HEAD_DWEIGHT ? (count + BK - 1) / BK : a.kblocks;
-    const int k0 = static_cast<int>(static_cast<int64_t>(all) * split / a.splits), nk = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - k0;
+    const int k0 = static_cast<int>(static_cast<int64_t>(all) * split / splits), nk = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - k0;
 
     f32x16 acc[TM][TN];
 #pragma unroll
@@ -443,18 +445,19 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const Hea
 // sums are added in LDS.  W's bytes bound it.
 constexpr int HF_THREADS = 256, HF_VOCAB = 64;
 typedef float f32x4a __attribute__((ext_vector_type(4)));
-template <int NT, bool TAIL>
+template <bool TAIL>
 __device__ __forceinline__ bf16x8 few_chunk(const uint16_t* row, int k, int width) {
     if constexpr (!TAIL) return __builtin_bit_cast(bf16x8, Pack<uint16_t, 8>::load<false>(row + k).v);
     else return __builtin_bit_cast(bf16x8, load_pack<uint16_t, 8, false>(row, k, width).v);
 }
 template <int NT>
-__global__ __launch_bounds__(HF_THREADS) void head_few_kernel(const uint16_t* hidden, int64_t ld_hidden, const uint16_t* weight, int64_t ld_weight, int tokens,
+__global__ __launch_bounds__(HF_THREADS, NT == 4 ? 4 : 1) void head_few_kernel(const uint16_t* hidden, int64_t ld_hidden, const uint16_t* weight, int64_t ld_weight, int tokens,
                                                               int width, int vocab, const void* targets, int target_bits, f32x2_t* stats, int64_t ld_stats,
-                                                              float* target_logit) {
+                                                              float* target_logit, int32_t* counter) {
     typedef uint32_t words __attribute__((ext_vector_type(4)));
     // a row's columns exchanged by its number, four at a time: the lanes of a token's 16 then write to different banks
-    __shared__ float sums[4][16 * NT][HF_VOCAB];
+    constexpr int WAVES = NT == 4 ? 2 : 4;       // whose sums lie in LDS at once (what four of them take for 64 tokens would leave two workgroups a CU)
+    __shared__ __align__(16) float sums[WAVES][16 * NT][HF_VOCAB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = (lane >> 4) * 8;
     const int v0 = blockIdx.x * HF_VOCAB;
     const uint16_t* wrow[4];
@@ -463,46 +466,70 @@ __global__ __launch_bounds__(HF_THREADS) void head_few_kernel(const uint16_t* hi
     for (int f = 0; f < 4; ++f) wrow[f] = weight + min(v0 + 16 * f + r, vocab - 1) * ld_weight;
 #pragma unroll
     for (int f = 0; f < NT; ++f) hrow[f] = hidden + min(16 * f + r, tokens - 1) * ld_hidden;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;       // (of the launch that joins)
+    // each lane's token's target, where it is a row of W (requested before the rows: a load for each token at the end took a third of the time)
+    int target = -1;
+    if (lane < tokens) {
+        const int64_t at = target_bits == 64 ? static_cast<const int64_t*>(targets)[lane] : static_cast<const int32_t*>(targets)[lane];
+        if (at >= 0 && at < vocab) target = static_cast<int>(at);
+    }
     f32x4a acc[4][NT];
 #pragma unroll
     for (int f = 0; f < 4; ++f)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[f][t] = f32x4a{0.f, 0.f, 0.f, 0.f};
+    // S steps of 32 channels at a time: as many loads as the registers leave in flight
+    constexpr int S = NT == 4 ? 1 : 2;
     const auto steps = [&](auto tail, int k) __attribute__((always_inline)) {
         constexpr bool TAIL = decltype(tail)::value;
-        bf16x8 w[2][4], h[2][NT];
+        bf16x8 w[S][4], h[S][NT];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < S; ++s) {
 #pragma unroll
-            for (int f = 0; f < 4; ++f) w[s][f] = few_chunk<NT, TAIL>(wrow[f], k + 32 * s + kq, width);
+            for (int f = 0; f < 4; ++f) w[s][f] = few_chunk<TAIL>(wrow[f], k + 32 * s + kq, width);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) h[s][t] = few_chunk<NT, TAIL>(hrow[t], k + 32 * s + kq, width);
+            for (int t = 0; t < NT; ++t) h[s][t] = few_chunk<TAIL>(hrow[t], k + 32 * s + kq, width);
         }
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
                 for (int t = 0; t < NT; ++t) acc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[s][f], h[s][t], acc[f][t], 0, 0, 0);
     };
     const int whole = width / 64;
+    if constexpr (S == 2) {
 #pragma unroll 2
-    for (int b = wave; b < whole; b += 4) steps(std::false_type{}, b * 64);
-    if (width % 64 && wave == whole % 4) steps(std::true_type{}, whole * 64);
+        for (int b = wave; b < whole; b += 4) steps(std::false_type{}, b * 64);
+    } else {
+#pragma unroll 1
+        for (int i = 2 * wave; i < 2 * whole; i += i % 2 ? 7 : 1) steps(std::false_type{}, i * 32);
+    }
+    if (width % 64 && wave == whole % 4)
+        for (int k = whole * 64; k < width; k += 32 * S) steps(std::true_type{}, k);
     // a lane holds rows 4 (lane / 16) .. + 3 of W for token lane % 16
+    const auto slot = [&](int f, int t) { return reinterpret_cast<f32x4a*>(&sums[wave % WAVES][16 * t + r][(16 * f + 4 * (lane >> 4)) ^ (r << 2)]); };
+    if (wave >= 4 - WAVES) {
 #pragma unroll
-    for (int f = 0; f < 4; ++f)
+        for (int f = 0; f < 4; ++f)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-*reinterpret_cast<f32x4a*>(&sums[wave][16 * t + r][(16 * f + 4 * (lane >> 4)) ^ (r << 2)]) = acc[f][t];
+            for (int t = 0; t < NT; ++t) *slot(f, t) = acc[f][t];
+    }
+    if (WAVES < 4) __syncthreads();
+    if (wave < 4 - WAVES) {
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) *slot(f, t) += acc[f][t];
+    }
     __syncthreads();
     for (int t = wave; t < tokens; t += 4) {
         const int v = v0 + lane;
         const int at = lane ^ ((t & 15) << 2);
-        float x = (sums[0][t][at] + sums[1][t][at]) + (sums[2][t][at] + sums[3][t][at]);
+        float x = sums[0][t][at] + sums[1][t][at];
+        if constexpr (WAVES == 4) x += sums[2][t][at] + sums[3][t][at];
         if (v >= vocab) x = -__builtin_inff();
-        const int64_t target = target_bits == 64 ? static_cast<const int64_t*>(targets)[t] : static_cast<const int32_t*>(targets)[t];
-        if (v == target) target_logit[t] = x;
+        if (v == __builtin_amdgcn_readlane(target, t)) target_logit[t] = x;
         const float m = group_reduce<64>(x, [](float p, float q) { return fmaxf(p, q); });
         const float s = group_sum<64>(__builtin_amdgcn_exp2f((x - (m == -__builtin_inff() ? 0.f : m)) * LOG2E));
         if (lane == 0) stats[blockIdx.x * ld_stats + t] = f32x2_t{m, s};
@@ -519,10 +546,8 @@ __device__ __forceinline__ int64_t target_of(const MuonHeadLoss& a, int64_t t) {
 __device__ __forceinline__ int target_in(const MuonHeadLoss& a, int64_t target) { return target >= 0 && target < a.vocab ? static_cast<int>(target) : -1; }
 
 // Numbers the tokens that take part, in order: order[row] = token for the first `count` rows, after them ~token of the ignored
-// ones (whose outputs are written here); rows[row] = target.  order[tokens] = count.  COMPACT: otherwise every token keeps its row, order[token]
-// = ~token where it is ignored, and the count is the number of tokens.
+// ones (whose outputs are written here); rows[row] = target.  order[tokens] = count.
 constexpr int HO_THREADS = 1024;
-template <bool COMPACT>
 __global__ __launch_bounds__(HO_THREADS) void head_order_kernel(const MuonHeadLoss a) {
     __shared__ int before[HO_THREADS / 64 + 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -546,7 +571,7 @@ __global__ __launch_bounds__(HO_THREADS) void head_order_kernel(const MuonHeadLo
     for (int64_t t = begin; t < end; ++t) {
         const int64_t target = target_of(a, t);
         const bool on = target != a.ignore_index;
-        const int64_t row = COMPACT ? (on ? at++ : out++) : t;
+        const int64_t row = on ? at++ : out++;
         a.order[row] = static_cast<int32_t>(on ? t : ~t);
         a.rows[row] = on ? target_in(a, target) : -1;
         if (!on) {
@@ -555,10 +580,27 @@ __global__ __launch_bounds__(HO_THREADS) void head_order_kernel(const MuonHeadLo
         }
     }
     if (threadIdx.x == 0) {
-        a.order[a.tokens] = static_cast<int32_t>(COMPACT ? count : a.tokens);
+        a.order[a.tokens] = count;
         *a.part = static_cast<float>(count > 0 ? count : 1);
         *a.counter = 0;
     }
+}
+
+// The shares that the k-blocks of e W are cut into.  A launch takes as many rounds of workgroups as it has tiles for every CU, and a tile
+// as long as its share and about six k-blocks more (its prologue and epilogue): the number of shares with the least of that.
+// (4096 x 32000 x 2048: 504 -> 438 us against a fixed 4; 5003 x 50257 x 1600, a third ignored: 658 -> 534.)
+constexpr int HD_SPLITS = 12;
+__device__ __forceinline__ int splits_for(int64_t count, int ld, int kblocks, int most) {
+    const int tiles = static_cast<int>((count + 255) / 256) * ((ld + 255) / 256);
+    int best = 1, least = 0x7fffffff;
+    for (int s = 1; s <= most; ++s) {
+        const int cost = (tiles * s + HD_CUS - 1) / HD_CUS * ((kblocks + s - 1) / s + 6);
+        if (cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
 }
 
 // The tokens' common factor g of a mean or sum, without its power of two: e is formed and rounded without it, and the products are
@@ -572,11 +614,15 @@ __device__ __forceinline__ float common_factor(const MuonHeadLoss& a) {
 
 // The hidden states of the rows, in bf16 rows of `ld` elements with zeros beyond the width, up to a whole tile of rows; backward their
 // coefficients too.  A wave for each row.
-__global__ __launch_bounds__(256) void head_gather_kernel(const MuonHeadLoss a, uint16_t* rows, int ld, f32x4v* coef, float* scale) {
+__global__ __launch_bounds__(256) void head_gather_kernel(const MuonHeadLoss a, uint16_t* rows, int ld, f32x4v* coef, float* scale, int kblocks, int most_splits) {
     const int lane = threadIdx.x & 63;
     const float factor = coef ? common_factor(a) : 1.f;
-    if (coef && blockIdx.x == 0 && threadIdx.x == 0) *scale = factor;
-    const int64_t count = a.order[a.tokens], padded = (count + HD_TILE - 1) / HD_TILE * HD_TILE;
+    const int64_t count = a.order[a.tokens];
+    if (coef && blockIdx.x == 0 && threadIdx.x == 0) {
+        scale[0] = factor;
+        reinterpret_cast<int32_t*>(scale)[1] = splits_for(count, ld, kblocks, most_splits);
+    }
+    const int64_t padded = (count + HD_TILE - 1) / HD_TILE * HD_TILE;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < padded; r += static_cast<int64_t>(gridDim.x) * 4) {
         const int token = r < count ? a.order[r] : -1;
         const uint16_t* const from = static_cast<const uint16_t*>(a.hidden) + (token >= 0 ? token : 0) * a.ld_hidden;
@@ -607,14 +653,16 @@ __global__ __launch_bounds__(256) void head_pad_kernel(const uint16_t* weight, i
 }
 
 // Joins the statistics of a row's column tiles, and forms its loss; the workgroup that is done last adds up the losses.  16 rows to a
-// workgroup, 64 threads to each.
+// workgroup, 64 threads to each.  FEW: the rows are the tokens, order[token] = ~token where one is ignored, and nothing of that
+// has been written yet.
 constexpr int HJ_THREADS = 1024, HJ_ROWS = 16, HJ_SHARES = HJ_THREADS / HJ_ROWS;
+template <bool FEW>
 __global__ __launch_bounds__(HJ_THREADS) void head_join_kernel(const MuonHeadLoss a, const f32x2_t* stats, int64_t ld_stats, int tiles, const float* target_logit,
                                                                float* left) {
     __shared__ float tops[HJ_SHARES][HJ_ROWS], sums[HJ_SHARES][HJ_ROWS];
     __shared__ bool last;
     const int r = threadIdx.x % HJ_ROWS, share = threadIdx.x / HJ_ROWS;
-    const int64_t count = a.order[a.tokens], row = static_cast<int64_t>(blockIdx.x) * HJ_ROWS + r;
+    const int64_t count = FEW ? a.tokens : a.order[a.tokens], row = static_cast<int64_t>(blockIdx.x) * HJ_ROWS + r;
     const auto join = [](float& m, float& s, float m2, float s2) {
         const float top = fmaxf(m, m2), ref = top == -__builtin_inff() ? 0.f : top;
         s = s * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * LOG2E);
@@ -649,26 +697,59 @@ __global__ __launch_bounds__(HJ_THREADS) void head_join_kernel(const MuonHeadLos
     }
     if (threadIdx.x < 64) {
         float loss = 0.f;
-        if (share == 0 && row < count && a.order[row] >= 0) {
-            const int token = a.order[row];
+        int token = -1, target = -1;
+        if (share == 0 && row < count) {
+            if constexpr (FEW) {
+                const int64_t t = target_of(a, row);
+                token = static_cast<int>(t != a.ignore_index ? row : ~row);
+                target = token >= 0 ? target_in(a, t) : -1;
+                a.order[row] = token;
+                a.rows[row] = target;
+                if (token < 0) {
+                    a.losses[row] = 0.f;
+                    a.lse[row] = 0.f;
+                }
+            } else {
+                token = a.order[row];
+                target = a.rows[row];
+            }
+        }
+        if (token >= 0) {
             m = tops[0][r] == -__builtin_inff() ? 0.f : tops[0][r];
             const float l = __log2f(sums[0][r]);
             a.stats[2 * row] = m;
             a.stats[2 * row + 1] = l;
-            loss = a.rows[row] >= 0 ? fmaf(l, LN2, m - target_logit[row]) : __builtin_nanf("");
+            loss = target >= 0 ? fmaf(l, LN2, m - target_logit[row]) : __builtin_nanf("");
             a.losses[token] = loss;
             a.lse[token] = fmaf(l, LN2, m);
         }
         loss = group_sum<64>(loss);
+        const int part = FEW ? __builtin_popcountll(__ballot(token >= 0)) : 0;
         if (threadIdx.x == 0) {
-            __hip_atomic_store(&left[blockIdx.x], loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            last = __hip_atomic_fetch_add(a.counter, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.x) - 1;
+            __hip_atomic_store(&left[2 * blockIdx.x], loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (FEW) __hip_atomic_store(&left[2 * blockIdx.x + 1], __int_as_float(part), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = gridDim.x == 1 || __hip_atomic_fetch_add(a.counter, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.x) - 1;
         }
     }
     __syncthreads();
-    if (!last || !a.loss) return;
+    if (!last) return;
+    if constexpr (FEW) {                         // (few workgroups)
+        if (threadIdx.x > 0) return;
+        float total = 0.f;
+        int n = 0;
+        for (unsigned g = 0; g < gridDim.x; ++g) {
+            total += __hip_atomic_load(&left[2 * g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            n += __float_as_int(__hip_atomic_load(&left[2 * g + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        }
+        const float part = static_cast<float>(n > 0 ? n : 1);
+        a.order[a.tokens] = static_cast<int32_t>(a.tokens);
+        *a.part = part;
+        if (a.loss) *a.loss = a.reduction == MUON_AMD_REDUCE_MEAN ? total / part : total;
+        return;
+    }
+    if (!a.loss) return;
     float total = 0.f;
-    for (unsigned g = threadIdx.x; g < gridDim.x; g += HJ_THREADS) total += __hip_atomic_load(&left[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (unsigned g = threadIdx.x; g < gridDim.x; g += HJ_THREADS) total += __hip_atomic_load(&left[2 * g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     total = group_sum<64>(total);
     if ((threadIdx.x & 63) == 0) tops[0][threadIdx.x >> 6] = total;
     __syncthreads();
@@ -679,9 +760,9 @@ __global__ __launch_bounds__(HJ_THREADS) void head_join_kernel(const MuonHeadLos
 }
 
 // Adds the shares of the hidden states' gradient and writes it to the tokens; zeros for those that take no part.  A wave for each row.
-__global__ __launch_bounds__(256) void head_dhidden_kernel(const MuonHeadLoss a, const float* part, int64_t stride, int ld, int shares, const float* scale) {
-    const int lane = threadIdx.x & 63;
-    const float factor = *scale;
+__global__ __launch_bounds__(256) void head_dhidden_kernel(const MuonHeadLoss a, const float* part, int64_t stride, int ld, const float* scale) {
+    const int lane = threadIdx.x & 63, shares = reinterpret_cast<const int32_t*>(scale)[1];
+    const float factor = scale[0];
     const int64_t count = a.order[a.tokens];
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < a.tokens; r += static_cast<int64_t>(gridDim.x) * 4) {
         const int at = a.order[r];
@@ -748,17 +829,20 @@ static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
     if (!backward) {
         p.stats = take(p.rows * p.col_tiles * 8);
         p.logit = take(p.rows * 4);
-        p.left = take((n + HJ_ROWS - 1) / HJ_ROWS * 4);
+        p.left = take((n + HJ_ROWS - 1) / HJ_ROWS * 8);
     } else {
         p.coef = take(p.rows * 16);
-        p.scale = take(4);
+        p.scale = take(8);
         const int64_t fit = HD_PIECE_BYTES / (p.rows * 2) / 256 * 256, most = fit < 4096 ? 4096 : fit;
         p.pieces = static_cast<int>((up(v, 256) + most - 1) / most);
         p.piece = up((v + p.pieces - 1) / p.pieces, 256);
         p.pieces = static_cast<int>((v + p.piece - 1) / p.piece);
         p.e = take(p.rows * p.piece * 2);
-        const int64_t tiles = (p.rows / 256) * ((d + 255) / 256), wanted = (512 + tiles - 1) / tiles, most_splits = p.piece / BK / 8;
-        p.splits = static_cast<int>(wanted < most_splits ? wanted : most_splits > 0 ? most_splits : 1);
+        // at most so many shares (the tokens that take part decide, on the device): of 8 k-blocks or more each, in half a GiB or one share
+        int64_t most_splits = HD_SPLITS;
+        if (most_splits > p.piece / BK / 8) most_splits = p.piece / BK / 8;
+        if (most_splits > HD_PIECE_BYTES / 2 / (p.rows * p.ld * 4)) most_splits = HD_PIECE_BYTES / 2 / (p.rows * p.ld * 4);
+        p.splits = static_cast<int>(most_splits > 0 ? most_splits : 1);
         p.part = take(p.splits * p.rows * p.ld * 4);
     }
     p.bytes = at;
@@ -779,7 +863,7 @@ static int check_head(const MuonHeadLoss* a, const char* what) {
 
 template <typename Cfg, int PRODUCT>
 static int launch_product(const HeadGemm& g, hipStream_t s) {
-    const int64_t grid = static_cast<int64_t>(g.row_tiles) * g.col_tiles * g.splits;
+    const int64_t grid = static_cast<int64_t>(g.row_tiles) * g.col_tiles * (g.most_splits > 0 ? g.most_splits : 1);
     MUON_REQUIRE(grid > 0 && grid <= 0x7fffffff, "linear_cross_entropy: %lld tiles", static_cast<long long>(grid));
     hipLaunchKernelGGL((head_gemm_kernel<Cfg, PRODUCT>), dim3(static_cast<unsigned>(grid)), dim3(Cfg::NT), Cfg::LDS_BYTES, s, g);
     return check_launch("linear_cross_entropy");
@@ -816,7 +900,7 @@ int raise_head_limits() {
 static int gather(const MuonHeadLoss& a, const HeadPlan& p, char* ws, f32x4v* coef, const uint16_t** w, int64_t* ld, hipStream_t s) {
     const int64_t blocks = p.rows / 4 < 4096 ? p.rows / 4 : 4096;
     hipLaunchKernelGGL(head_gather_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, reinterpret_cast<uint16_t*>(ws + p.hidden), static_cast<int>(p.ld), coef,
-                       reinterpret_cast<float*>(ws + p.scale));
+                       reinterpret_cast<float*>(ws + p.scale), static_cast<int>(p.piece / BK), p.splits);
     if (const int rc = check_launch("linear_cross_entropy: rows")) return rc;
     *w = static_cast<const uint16_t*>(a.weight);
     *ld = a.ld_weight;
@@ -854,19 +938,24 @@ int muon_amd_head_loss(const MuonHeadLoss* args, void* stream) {
     char* const ws = static_cast<char*>(a.workspace);
     f32x2_t* const stats = reinterpret_cast<f32x2_t*>(ws + p.stats);
     float* const logit = reinterpret_cast<float*>(ws + p.logit);
-    if (p.few) hipLaunchKernelGGL(head_order_kernel<false>, dim3(1), dim3(HO_THREADS), 0, s, a);
-    else hipLaunchKernelGGL(head_order_kernel<true>, dim3(1), dim3(HO_THREADS), 0, s, a);
-    if (const int rc = check_launch("head_loss: order")) return rc;
+    const auto join = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((a.tokens + HJ_ROWS - 1) / HJ_ROWS)), dim3(HJ_THREADS), 0, s, a, stats, p.rows, p.col_tiles, logit,
+                           reinterpret_cast<float*>(ws + p.left));
+        return check_launch("head_loss: join");
+    };
     if (p.few) {
         const auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(p.col_tiles), dim3(HF_THREADS), 0, s, static_cast<const uint16_t*>(a.hidden), a.ld_hidden,
-                               static_cast<const uint16_t*>(a.weight), a.ld_weight, static_cast<int>(a.tokens), a.width, a.vocab, a.targets, a.target_bits, stats, p.rows, logit);
+                               static_cast<const uint16_t*>(a.weight), a.ld_weight, static_cast<int>(a.tokens), a.width, a.vocab, a.targets, a.target_bits, stats, p.rows, logit, a.counter);
         };
         if (a.tokens <= 16) go(head_few_kernel<1>);
         else if (a.tokens <= 32) go(head_few_kernel<2>);
         else go(head_few_kernel<4>);
         if (const int rc = check_launch("head_loss: few")) return rc;
+        return join(head_join_kernel<true>);
     } else {
+        hipLaunchKernelGGL(head_order_kernel, dim3(1), dim3(HO_THREADS), 0, s, a);
+        if (const int rc = check_launch("head_loss: order")) return rc;
         HeadGemm g{};
         if (const int rc = gather(a, p, ws, nullptr, &g.Q, &g.ldq, s)) return rc;
         g.P = reinterpret_cast<const uint16_t*>(ws + p.hidden);
@@ -876,7 +965,6 @@ int muon_amd_head_loss(const MuonHeadLoss* args, void* stream) {
         g.count = a.order + a.tokens;
         g.row_tiles = static_cast<int>(p.rows / p.tile);
         g.col_tiles = p.col_tiles;
-        g.splits = 1;
         g.kblocks = static_cast<int>(p.ld / BK);
         g.vocab = a.vocab;
         g.target = a.rows;
@@ -885,9 +973,7 @@ int muon_amd_head_loss(const MuonHeadLoss* args, void* stream) {
         g.target_logit = logit;
         if (const int rc = launch_product<HEAD_STATS>(g, p.large, s)) return rc;
     }
-    hipLaunchKernelGGL(head_join_kernel, dim3(static_cast<unsigned>((a.tokens + HJ_ROWS - 1) / HJ_ROWS)), dim3(HJ_THREADS), 0, s, a, stats, p.rows, p.col_tiles, logit,
-                       reinterpret_cast<float*>(ws + p.left));
-    return check_launch("head_loss: join");
+    return join(head_join_kernel<false>);
 }
 
 int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
@@ -907,12 +993,12 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
     uint16_t* const rows = reinterpret_cast<uint16_t*>(ws + p.hidden);
     uint16_t* const e = reinterpret_cast<uint16_t*>(ws + p.e);
     float* const part = reinterpret_cast<float*>(ws + p.part);
+    const int32_t* const splits = reinterpret_cast<const int32_t*>(ws + p.scale) + 1;
     for (int i = 0; i < p.pieces; ++i) {
         const int begin = static_cast<int>(i * p.piece), size = static_cast<int>(a.vocab - begin < p.piece ? a.vocab - begin : p.piece);
         const uint16_t* const piece = w + begin * ldw;
         HeadGemm g{};
         g.count = a.order + a.tokens;
-        g.splits = 1;
         // e of the piece
         const int tile = p.large ? 256 : 128;
         g.P = rows;
@@ -944,7 +1030,8 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
             h.col_limit = static_cast<int>(p.ld);
             h.row_tiles = static_cast<int>(p.rows / 256);
             h.col_tiles = static_cast<int>(up(p.ld, 256) / 256);
-            h.splits = p.splits;
+            h.splits = splits;
+            h.most_splits = p.splits;
             h.cols = static_cast<int>(p.ld);
             h.kblocks = static_cast<int>(up(size, BK) / BK);
             h.part = part;
@@ -967,7 +1054,6 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
             h.rows = size;
             h.row_tiles = static_cast<int>(up(size, 256) / 256);
             h.col_tiles = static_cast<int>(up(a.width, 256) / 256);
-            h.splits = 1;
             h.cols = a.width;
             h.scale = reinterpret_cast<const float*>(ws + p.scale);
             h.out = static_cast<uint16_t*>(a.dweight) + static_cast<int64_t>(begin) * a.width;
@@ -977,7 +1063,7 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
     }
     if (a.dhidden) {
         const int64_t blocks = (a.tokens + 3) / 4 < 8192 ? (a.tokens + 3) / 4 : 8192;
-        hipLaunchKernelGGL(head_dhidden_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, part, p.rows * p.ld, static_cast<int>(p.ld), p.splits,
+        hipLaunchKernelGGL(head_dhidden_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, part, p.rows * p.ld, static_cast<int>(p.ld),
                            reinterpret_cast<const float*>(ws + p.scale));
         return check_launch("head_loss_backward: hidden");
     }
