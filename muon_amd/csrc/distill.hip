@@ -11,7 +11,9 @@
 // them and writes the gradient.  Arithmetic is in base 2: with c = log2(e) / T a thread keeps m, its largest logit, and
 // s = sum 2^((x - m) c); m and log2(s) are kept apart for backward, so that probabilities go by differences of logits
 // however far from zero these are (with x c - m c in one instruction, a row at 1e30 is lost in the rounding of m c).  Rows are shared by several workgroups where
-// there are few of them, and joined in the order of their parts.
+// there are few of them, and joined in the order of their parts.  Loads and stores of the rows carry the non-temporal hint: nothing is read again
+// while it is in a cache, but for what fits the last one (8192 x 128256 bf16, both passes: 1140 -> 1021 us, 6.2 TB/s of the 6.3 GB; 4096 x
+// 32000: 155.6 -> 154.2, with plain loads backward 149.4).
 #include "lanes.h"
 
 namespace muon_amd {
@@ -79,7 +81,7 @@ __global__ __launch_bounds__(DT_THREADS) void distill_stats_kernel(const MuonDis
     for (; e - static_cast<int>(threadIdx.x) * G + DT_UNROLL * STEP <= end; e += DT_UNROLL * STEP) {
         Pack<T, G> v[DT_UNROLL];
 #pragma unroll
-        for (int u = 0; u < DT_UNROLL; ++u) v[u] = Pack<T, G>::template load<false>(row + e + u * STEP);
+        for (int u = 0; u < DT_UNROLL; ++u) v[u] = Pack<T, G>::template load<true>(row + e + u * STEP);
         add(v);
     }
     if (e - static_cast<int>(threadIdx.x) * G < end) {      // what is left of the part: -infinity beyond it
@@ -118,18 +120,21 @@ __global__ __launch_bounds__(DT_THREADS) void distill_stats_kernel(const MuonDis
     if (blockIdx.x == 0) *a.counter = 0;
 }
 
-// A wave for each token: its parts joined, its list, its loss.  The workgroup that is done last adds up the losses.
-__global__ __launch_bounds__(DT_THREADS) void distill_finish_kernel(const MuonDistill a, int parts) {
-    __shared__ float sums[DT_WAVES];
-    __shared__ int counts[DT_WAVES];
+// A wave for each token: its parts joined, its list, its loss.  The workgroup that is done last adds up the losses.  (At most 256
+// workgroups: with one for every four tokens, 2048 of them at one counter took 96 us.)
+constexpr int DF_THREADS = 1024, DF_WAVES = DF_THREADS / 64, DF_GROUPS = 256;
+static int finish_groups(int64_t tokens) { return static_cast<int>(tokens < DF_WAVES * DF_GROUPS ? (tokens + DF_WAVES - 1) / DF_WAVES : DF_GROUPS); }
+__global__ __launch_bounds__(DF_THREADS) void distill_finish_kernel(const MuonDistill a, int parts) {
+    __shared__ float sums[DF_WAVES];
+    __shared__ int counts[DF_WAVES];
     __shared__ bool last;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * DT_WAVES + wave;
     const float c = LOG2E / a.temperature;
     const auto larger = [](float x, float y) { return fmaxf(x, y); };
-    float loss = 0.f;
-    bool on = false;
-    if (t < a.tokens) {
+    float total = 0.f;
+    int taking = 0;
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * DF_WAVES + wave; t < a.tokens; t += static_cast<int64_t>(gridDim.x) * DF_WAVES) {
+        float loss = 0.f;
         // the list: whether anything is there, its maximum and sum
         bool some = false;
         float most = -__builtin_inff();
@@ -141,7 +146,7 @@ __global__ __launch_bounds__(DT_THREADS) void distill_finish_kernel(const MuonDi
                     most = fmaxf(most, v);
                 }
             }
-        on = __ballot(some) != 0;
+        const bool on = __ballot(some) != 0;
         float tm = -__builtin_inff(), tl = 0.f, m = 0.f, l = 0.f;
         if (on) {
             tm = RunningSum::reference(group_reduce<64>(most, larger));     // (a list of nothing but NaN has a number here all the same)
@@ -172,17 +177,19 @@ __global__ __launch_bounds__(DT_THREADS) void distill_finish_kernel(const MuonDi
             a.losses[t] = loss;
             reinterpret_cast<f32x4v*>(a.stats)[t] = f32x4v{m, l, tm, tl};
         }
+        total += loss;
+        taking += on;
     }
     if (lane == 0) {
-        sums[wave] = loss;
-        counts[wave] = on;
+        sums[wave] = total;
+        counts[wave] = taking;
     }
     __syncthreads();
     float* const left = a.partials + 2 * a.tokens * parts;           // {sum, tokens} of each workgroup
     if (threadIdx.x == 0) {
         float s = 0.f;
         int n = 0;
-        for (int w = 0; w < DT_WAVES; ++w) {
+        for (int w = 0; w < DF_WAVES; ++w) {
             s += sums[w];
             n += counts[w];
         }
@@ -194,7 +201,7 @@ __global__ __launch_bounds__(DT_THREADS) void distill_finish_kernel(const MuonDi
     if (!last) return;
     float s = 0.f;
     int n = 0;
-    for (unsigned g = threadIdx.x; g < gridDim.x; g += DT_THREADS) {
+    for (unsigned g = threadIdx.x; g < gridDim.x; g += DF_THREADS) {
         s += __hip_atomic_load(&left[2 * g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         n += __float_as_int(__hip_atomic_load(&left[2 * g + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
     }
@@ -206,7 +213,7 @@ __global__ __launch_bounds__(DT_THREADS) void distill_finish_kernel(const MuonDi
     }
     __syncthreads();
     if (threadIdx.x > 0) return;
-    for (int w = 1; w < DT_WAVES; ++w) {
+    for (int w = 1; w < DF_WAVES; ++w) {
         s += sums[w];
         n += counts[w];
     }
@@ -215,7 +222,8 @@ __global__ __launch_bounds__(DT_THREADS) void distill_finish_kernel(const MuonDi
     if (a.loss) *a.loss = a.reduction == MUON_AMD_REDUCE_MEAN ? s / part : s;
 }
 
-constexpr int DB_CHUNK_PACKS = 16;                          // packs of a thread in a workgroup's share of a row
+// Packs of a thread in a workgroup's share of a row: one round of loads (8192 x 128256 bf16, both passes: 1140 us; 8 packs 1158, 16 packs 1176).
+constexpr int DB_CHUNK_PACKS = DT_UNROLL;
 template <typename T>
 __global__ __launch_bounds__(DT_THREADS) void distill_backward_kernel(const MuonDistill a, int parts) {
     constexpr int G = pack_of<T>, STEP = DT_THREADS * G, LENGTH = STEP * DB_CHUNK_PACKS;
@@ -248,16 +256,13 @@ __global__ __launch_bounds__(DT_THREADS) void distill_backward_kernel(const Muon
     };
     int e = begin + static_cast<int>(threadIdx.x) * G;
     if (begin + LENGTH <= end) {
+        Pack<T, G> v[DT_UNROLL];
 #pragma unroll
-        for (int round = 0; round < DB_CHUNK_PACKS / DT_UNROLL; ++round, e += DT_UNROLL * STEP) {
-            Pack<T, G> v[DT_UNROLL];
+        for (int u = 0; u < DT_UNROLL; ++u) v[u] = Pack<T, G>::template load<true>(row + e + u * STEP);
 #pragma unroll
-            for (int u = 0; u < DT_UNROLL; ++u) v[u] = Pack<T, G>::template load<false>(row + e + u * STEP);
-#pragma unroll
-            for (int u = 0; u < DT_UNROLL; ++u) put(v[u], e + u * STEP);
-        }
+        for (int u = 0; u < DT_UNROLL; ++u) put(v[u], e + u * STEP);
     } else {
-        for (; e < end; e += STEP) put(load_pack<T, G, false>(row, e, end), e);
+        for (; e < end; e += STEP) put(load_pack<T, G, true>(row, e, end), e);
     }
     // The teacher's entries go over what was written there: the barrier orders the two.  The first entry of an index
     // writes for all that have it.
@@ -313,7 +318,7 @@ int muon_amd_distill_max_top(void) { return DT_MAX_TOP; }
 
 int64_t muon_amd_distill_partials(int64_t tokens, int vocab, int dtype) {
     if (tokens <= 0 || vocab <= 0) return 0;
-    return 2 * tokens * distill_parts(tokens, vocab, dtype) + 2 * ((tokens + DT_WAVES - 1) / DT_WAVES);
+    return 2 * tokens * distill_parts(tokens, vocab, dtype) + 2 * finish_groups(tokens);
 }
 
 int muon_amd_distill(const MuonDistill* args, void* stream) {
@@ -326,7 +331,7 @@ int muon_amd_distill(const MuonDistill* args, void* stream) {
     if (a.dtype == MUON_AMD_SRC_BF16) hipLaunchKernelGGL(distill_stats_kernel<uint16_t>, grid, dim3(DT_THREADS), 0, st, a, parts, length);
     else hipLaunchKernelGGL(distill_stats_kernel<float>, grid, dim3(DT_THREADS), 0, st, a, parts, length);
     if (const int rc = check_launch("distill")) return rc;
-    hipLaunchKernelGGL(distill_finish_kernel, dim3(static_cast<unsigned>((a.tokens + DT_WAVES - 1) / DT_WAVES)), dim3(DT_THREADS), 0, st, a, parts);
+    hipLaunchKernelGGL(distill_finish_kernel, dim3(finish_groups(a.tokens)), dim3(DF_THREADS), 0, st, a, parts);
     return check_launch("distill");
 }
 
