@@ -6,6 +6,7 @@
 // makes the copies that other strides need and raises what there is to raise.  The kernels are reached through the
 // addresses of the C ABI's entry points (bind), so that another build of the library can stand behind them.
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -23,6 +24,7 @@
 #include <list>
 #include <optional>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/muon_amd.h"
@@ -92,6 +94,35 @@ variable_list once(variable_list grads, const char* message) {
     for (Tensor& g : grads)
         if (g.defined()) g = torch::autograd::DelayedError(message, 1)({g})[0];
     return grads;
+}
+
+// A backward pass that a HIP graph records joins, at its end, the streams on which the graph's leaves were first used.  Where an
+// autograd graph from before the capture keeps such a leaf's node alive and that was on the default stream, the capture is
+// broken and the process ends in the runtime: the call that would record the forward pass says so instead.
+void refuse_leaves_of_the_default_stream(std::initializer_list<const Tensor*> ts) {
+    if (!capturing()) return;
+    std::vector<torch::autograd::Node*> next;
+    std::unordered_set<torch::autograd::Node*> seen;
+    const auto add = [&](torch::autograd::Node* n) {
+        if (n && seen.insert(n).second) next.push_back(n);
+    };
+    std::vector<std::shared_ptr<torch::autograd::Node>> held;
+    for (const Tensor* t : ts)
+        if (t && t->defined() && t->requires_grad()) {
+            held.push_back(t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t));
+            add(held.back().get());
+        }
+    while (!next.empty()) {
+        torch::autograd::Node* const n = next.back();
+        next.pop_back();
+        if (dynamic_cast<torch::autograd::AccumulateGrad*>(n)) {
+            const auto stream = n->stream();
+            if (stream && *stream == c10::impl::VirtualGuardImpl(stream->device_type()).getDefaultStream(stream->device()))
+                throw LibraryError("an autograd graph that was recorded on the default stream holds a leaf of this call: release it (its loss, its outputs) before the "
+                                   "call is captured into a HIP graph");
+        }
+        for (const auto& edge : n->next_edges()) add(edge.function.get());
+    }
 }
 
 // ---- residual_norm -------------------------------------------------------------------------------------------
@@ -245,6 +276,7 @@ std::optional<std::tuple<Tensor, Tensor>> residual_norm(const Tensor& x, const T
     if (!residual_taken(x, block, post, pre, gate, scale, eps)) return std::nullopt;
     const py::gil_scoped_release released;
     if (any_requires_grad({&x, &block, &post, &pre, gate ? &*gate : nullptr, scale ? &*scale : nullptr})) {
+        refuse_leaves_of_the_default_stream({&x, &block, &post, &pre, gate ? &*gate : nullptr, scale ? &*scale : nullptr});
         const variable_list out = ResidualNorm::apply(x, block, post, pre, gate, scale, eps);
         return std::make_tuple(out[0], out[1]);
     }
@@ -384,6 +416,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>> route_topk(con
     const RouteScores by{scores, groups, kept, bias.value_or(Tensor())};
     const py::gil_scoped_release released;
     if (any_requires_grad({&logits})) {
+        refuse_leaves_of_the_default_stream({&logits});
         const variable_list out = RouteTopk::apply(logits, k, mask, normalize, by);
         return std::make_tuple(out[0], out[1], out[2], out[3], out[4]);
     }
@@ -515,6 +548,7 @@ std::optional<std::tuple<Tensor, Tensor>> linear_cross_entropy(const Tensor& hid
     if (reduction < 0 || any_tangent({&hidden, &weight})) return std::nullopt;
     const py::gil_scoped_release released;
     if (any_requires_grad({&hidden, &weight})) {
+        refuse_leaves_of_the_default_stream({&hidden, &weight});
         const variable_list out = LinearCrossEntropy::apply(hidden, weight, targets, reduction, ignore_index);
         return std::make_tuple(out[0], out[1]);
     }
@@ -619,7 +653,10 @@ std::optional<Tensor> distill_topk(const Tensor& logits, const Tensor& teacher, 
     // (a temperature whose reciprocal is no normal number would leave none)
     if (!(temperature >= 1e-30 && temperature <= 1e30) || reduction < 0 || any_tangent({&logits, &teacher}) || any_requires_grad({&teacher})) return std::nullopt;
     const py::gil_scoped_release released;
-    if (any_requires_grad({&logits})) return DistillTopk::apply(logits, teacher, indices, mask, reduction, temperature);
+    if (any_requires_grad({&logits})) {
+        refuse_leaves_of_the_default_stream({&logits});
+        return DistillTopk::apply(logits, teacher, indices, mask, reduction, temperature);
+    }
     DistillTensors t{logits, teacher, indices, mask.value_or(Tensor()), Tensor(), Tensor()};
     return distill_forward(t, reduction, temperature);
 }
