@@ -6,9 +6,17 @@
     clip_coefficient, AdamW(state_bits=8)     embedding, head, router, norms, gates and scales, clipped on the way
     clip_grad_norm_, SingleDeviceMuon         every matrix of the experts and of the token mixing (3-D: a batch of matrices)
 
+and, where asked for,
+
+    linear_cross_entropy      (--fused-head) the loss without the logits, with a z-loss of the head
+    distill_topk              (--distill 0.5) half of the loss from a teacher: the chain itself, which knows each token's four successors
+    route_topk(scores="sigmoid", bias=..., groups=...)       (--balanced) experts chosen by biased scores within groups; the biases follow the
+                              tokens per expert instead of a loss
+
 The data is a seeded random Markov chain over a small vocabulary, so nothing has to be downloaded.
 
     python examples/train_moe.py [--steps 200] [--width 256] [--layers 4] [--experts 8] [--top-k 2] [--state-bits 8]
+                                 [--fused-head] [--distill 0.5] [--balanced]
 """
 import argparse
 import os
@@ -21,14 +29,18 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import muon_amd  # noqa: E402
 
 VOCAB, LENGTH, BATCH = 128, 64, 16
+CHANCES = (0.55, 0.25, 0.15, 0.05)           # of a token's four successors
+BIAS_RATE, Z_LOSS = 1e-2, 1e-4
 
 
 class Block(nn.Module):
     """Mixes each token with the ones before it, then sends it through its experts."""
 
-    def __init__(self, width, experts, top_k):
+    def __init__(self, width, experts, top_k, balanced=False):
         super().__init__()
         self.top_k = top_k
+        self.balanced = balanced
+        self.register_buffer("bias", torch.zeros(experts))
         self.mix = nn.Parameter(torch.randn(2 * width, width) * (2 * width) ** -0.5)
         self.router = nn.Parameter(torch.randn(width, experts) * width ** -0.5)
         self.up = nn.Parameter(torch.randn(experts, width, 2 * width) * width ** -0.5)
@@ -42,7 +54,15 @@ class Block(nn.Module):
         """stream: the residual stream, fp32; y: its norm, bf16.  -> both after this block, and the router's losses."""
         before = torch.cat([torch.zeros_like(y[:, :1]), y[:, :-1]], 1)
         tokens = torch.cat([y, before], -1).flatten(0, 1) @ self.mix.bfloat16()
-        routing = muon_amd.route_topk(tokens @ self.router.bfloat16(), self.top_k)
+        logits = tokens @ self.router.bfloat16()
+        if self.balanced:
+            groups = max(g for g in (1, 2, 4) if self.bias.numel() % g == 0 and self.bias.numel() // g >= self.top_k)
+            routing = muon_amd.route_topk(logits, self.top_k, scores="sigmoid", bias=self.bias, groups=groups, groups_kept=(groups + 1) // 2)
+            with torch.no_grad():                                # experts with few tokens are lifted, those with many lowered
+                load = routing.counts.float()
+                self.bias += BIAS_RATE * torch.sign(load.mean() - load)
+        else:
+            routing = muon_amd.route_topk(logits, self.top_k)
         out = torch.zeros_like(tokens)
         for e in range(self.up.size(0)):
             token, choice = torch.where(routing.indices == e)
@@ -54,11 +74,11 @@ class Block(nn.Module):
 
 
 class Model(nn.Module):
-    def __init__(self, width, layers, experts, top_k):
+    def __init__(self, width, layers, experts, top_k, balanced=False):
         super().__init__()
         self.embedding = nn.Parameter(torch.randn(VOCAB, width))
         self.head = nn.Parameter(torch.zeros(width, VOCAB))
-        self.blocks = nn.ModuleList(Block(width, experts, top_k) for _ in range(layers))
+        self.blocks = nn.ModuleList(Block(width, experts, top_k, balanced) for _ in range(layers))
 
     def forward(self, ids):
         stream = self.embedding[ids]
@@ -67,7 +87,10 @@ class Model(nn.Module):
         for block in self.blocks:
             stream, y, b, lse = block(stream, y)
             balance, z = balance + b, z + lse
-        return (y @ self.head.bfloat16()).float(), balance / len(self.blocks), z / len(self.blocks)
+        return y, balance / len(self.blocks), z / len(self.blocks)
+
+    def logits(self, y):
+        return (y @ self.head.bfloat16()).float()
 
 
 def batches(device, seed=0):
@@ -77,16 +100,22 @@ def batches(device, seed=0):
     while True:
         ids = torch.randint(VOCAB, (BATCH, 1), generator=gen)
         for _ in range(LENGTH):
-            pick = torch.multinomial(torch.tensor([0.55, 0.25, 0.15, 0.05]), BATCH, replacement=True, generator=gen)
+            pick = torch.multinomial(torch.tensor(CHANCES), BATCH, replacement=True, generator=gen)
             ids = torch.cat([ids, successors[ids[:, -1], pick][:, None]], 1)
         yield ids.to(device)
 
 
-def train(steps=200, width=256, layers=4, experts=8, top_k=2, state_bits=8, seed=0, report=None):
+def teacher(ids, seed=0):
+    """What the chain behind `batches` expects after each token: logits of its four successors, and which they are."""
+    successors = torch.randint(VOCAB, (VOCAB, 4), generator=torch.Generator().manual_seed(seed)).to(ids.device)
+    return torch.tensor(CHANCES, device=ids.device).log().expand(*ids.shape, 4), successors[ids]
+
+
+def train(steps=200, width=256, layers=4, experts=8, top_k=2, state_bits=8, seed=0, report=None, fused_head=False, distill=0.0, balanced=False):
     """-> the losses of all steps (next-token cross entropy in nats)."""
     torch.manual_seed(seed)
     device = torch.device("cuda", torch.cuda.current_device())
-    model = Model(width, layers, experts, top_k).to(device)
+    model = Model(width, layers, experts, top_k, balanced).to(device)
     matrices = [p for b in model.blocks for p in (b.mix, b.up, b.down)]
     ids_of_matrices = {id(p) for p in matrices}
     others = [p for p in model.parameters() if id(p) not in ids_of_matrices]
@@ -94,9 +123,15 @@ def train(steps=200, width=256, layers=4, experts=8, top_k=2, state_bits=8, seed
     adamw = muon_amd.AdamW(others, lr=3e-3, betas=(0.9, 0.95), weight_decay=0.01, state_bits=state_bits)
     losses = []
     for step, ids in zip(range(steps), batches(device, seed)):
-        logits, balance, z = model(ids[:, :-1])
-        loss = nn.functional.cross_entropy(logits.flatten(0, 1), ids[:, 1:].flatten())
-        (loss + 0.01 * balance + 0.001 * z).backward()
+        y, balance, z = model(ids[:, :-1])
+        if fused_head:
+            loss, lse = muon_amd.linear_cross_entropy(y, model.head.t().bfloat16(), ids[:, 1:])
+            objective = loss + Z_LOSS * lse.square().mean()
+        else:
+            loss = objective = nn.functional.cross_entropy(model.logits(y).flatten(0, 1), ids[:, 1:].flatten())
+        if distill:
+            objective = (1 - distill) * objective + distill * muon_amd.distill_topk(model.logits(y), *teacher(ids[:, :-1], seed))
+        (objective + (0.0 if balanced else 0.01) * balance + 0.001 * z).backward()
         muon_amd.clip_grad_norm_(matrices, 1.0)
         norm, coefficient = muon_amd.clip_coefficient(others, 1.0)
         muon.step()
@@ -118,5 +153,8 @@ if __name__ == "__main__":
     ap.add_argument("--experts", type=int, default=8)
     ap.add_argument("--top-k", type=int, default=2)
     ap.add_argument("--state-bits", type=int, default=8, choices=(8, 32))
+    ap.add_argument("--fused-head", action="store_true")
+    ap.add_argument("--distill", type=float, default=0.0)
+    ap.add_argument("--balanced", action="store_true")
     a = ap.parse_args()
-    train(a.steps, a.width, a.layers, a.experts, a.top_k, a.state_bits, report=20)
+    train(a.steps, a.width, a.layers, a.experts, a.top_k, a.state_bits, report=20, fused_head=a.fused_head, distill=a.distill, balanced=a.balanced)
