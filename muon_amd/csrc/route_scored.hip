@@ -410,6 +410,7 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
             part += on;
         }
     }
+    wave_order();                                // (what a lane has left in memory is read by others of its wave)
     if (__ballot(later)) {
         const int whole = threadIdx.x & 63;
         for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS + sub - slot; first < a.tokens; first += step) {
