@@ -175,7 +175,7 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const Hea
     extern __shared__ __align__(16) uint16_t lds[];
     const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint16_t*)lds));
     const int count = *a.count;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WGN, wn = wave % WGN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WGN;
     const int rows = PRODUCT == HEAD_DWEIGHT ? a.rows : count;
     const int row_tiles = (rows + Cfg::BT - 1) / Cfg::BT, tiles = row_tiles * a.col_tiles;
     const int id = static_cast<int>(blockIdx.x), splits = PRODUCT == HEAD_DHIDDEN ? *a.splits : 1;
@@ -183,6 +183,13 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const Hea
     const int place = place_of(id, tiles * splits), split = place / tiles;
     const TileAt tile = tile_at(place - split * tiles, row_tiles, a.col_tiles);
     const int i0 = tile.row * Cfg::BT, j0 = tile.col * Cfg::BT;
+    // A tile at the end of the rows or columns may have nothing in its second half: the waves there fetch their share of the operands and keep
+    // the barriers, but leave the matrix pipes to the others.  Waves w and w + 4 share a SIMD: where columns are empty the second
+    // row of waves is turned by two, so that every SIMD has one wave of either kind.
+    const int cols = PRODUCT == HEAD_STATS || PRODUCT == HEAD_GRAD ? a.vocab - a.vocab_begin : a.cols;
+    const bool narrow = cols - j0 <= Cfg::BT / 2, low = rows - i0 <= Cfg::BT / 2;
+    const int wn = WGN == 4 && narrow ? (wave % WGN) ^ (wm * 2) : wave % WGN;
+    const bool empty = (narrow && wn * WN >= Cfg::BT / 2) || (low && wm * WM >= Cfg::BT / 2);
     // k-blocks of this share
     const int all = PRODUCT == HEAD_DWEIGHT ? (count + BK - 1) / BK : a.kblocks;
     const int k0 = static_cast<int>(static_cast<int64_t>(all) * split / splits), nk = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - k0;
@@ -252,8 +259,6 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const Hea
             else sp_.issue(jj % DPH, dk[1], ddst[1] + (jj % DPH) * NW * 1024);
             __builtin_amdgcn_sched_barrier(0);
         };
-        load(0, 0, 1, 0);
-        wait_both<0>(af[0], bf[0]);
         int sp = 0, sq = 1, kb = 0;
         const auto block = [&](auto more) __attribute__((always_inline)) {
             constexpr int MORE = decltype(more)::value;
@@ -304,12 +309,46 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const Hea
             sp = spn;
             sq = sqn;
         };
-        for (; kb < nk - RING; ++kb) block(std::integral_constant<int, RING>{});
-        if (nk - kb == 2) {
-            block(std::integral_constant<int, 1>{});
-            ++kb;
+        if (empty) {
+            const auto pass = [&](auto more) __attribute__((always_inline)) {
+                constexpr int MORE = decltype(more)::value;
+                if (kb > 0) {
+#pragma unroll
+                    for (int jj = DPK; jj < 2 * DPH; ++jj)
+                        if (MORE == RING || (MORE == RING - 1 && jj < DPH)) transfer(jj);
+                }
+                if (MORE > 0) {
+                    NS_WAIT_VMCNT((MORE == RING ? NHALF - 4 : MORE > 0 ? 2 * MORE - 2 : 0) * DPH);
+                    __builtin_amdgcn_s_barrier();
+                    const int h0 = 2 * kb + NHALF;
+                    ddst[0] = dst0 + sp * HALF_BYTES;
+                    ddst[1] = dst0 + sq * HALF_BYTES;
+                    dk[0] = h0 >> 1;
+                    dk[1] = (h0 + 1) >> 1;
+                }
+                if (MORE == RING) {
+#pragma unroll
+                    for (int jj = 0; jj < DPK; ++jj) transfer(jj);
+                }
+                sp = sp + 2 >= NHALF ? sp + 2 - NHALF : sp + 2;
+                sq = sq + 2 >= NHALF ? sq + 2 - NHALF : sq + 2;
+            };
+            for (; kb < nk - RING; ++kb) pass(std::integral_constant<int, RING>{});
+            if (nk - kb == 2) {
+                pass(std::integral_constant<int, 1>{});
+                ++kb;
+            }
+            pass(std::integral_constant<int, 0>{});
+        } else {
+            load(0, 0, 1, 0);
+            wait_both<0>(af[0], bf[0]);
+            for (; kb < nk - RING; ++kb) block(std::integral_constant<int, RING>{});
+            if (nk - kb == 2) {
+                block(std::integral_constant<int, 1>{});
+                ++kb;
+            }
+            block(std::integral_constant<int, 0>{});
         }
-        block(std::integral_constant<int, 0>{});
         __syncthreads();            // every wave is done with the ring
     }
 
