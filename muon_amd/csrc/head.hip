@@ -625,21 +625,19 @@ __global__ __launch_bounds__(HO_THREADS) void head_order_kernel(const MuonHeadLo
     }
 }
 
-// The shares that the k-blocks of e W are cut into.  A launch takes as many rounds of workgroups as it has tiles for every CU, and a tile
-// as long as its share and about six k-blocks more (its prologue and epilogue): the number of shares with the least of that.
-// (4096 x 32000 x 2048: 504 -> 438 us against a fixed 4; 5003 x 50257 x 1600, a third ignored: 658 -> 534.)
-constexpr int HD_SPLITS = 12;
-__device__ __forceinline__ int splits_for(int64_t count, int ld, int kblocks, int most) {
-    const int tiles = static_cast<int>((count + 255) / 256) * ((ld + 255) / 256);
-    int best = 1, least = 0x7fffffff;
-    for (int s = 1; s <= most; ++s) {
-        const int cost = (tiles * s + HD_CUS - 1) / HD_CUS * ((kblocks + s - 1) / s + 6);
-        if (cost < least) {
-            least = cost;
-            best = s;
-        }
+// The shares that the k-blocks of e W are cut into, formed by a wave.  A launch takes as many rounds of workgroups as it has tiles for the
+// places on the GPU, a tile as long as its share and about six k-blocks more (its prologue and epilogue), and each share's sums
+// are written and read once (in the time of a k-block 5 MB are): the number of shares with the least of that.  (4096 x 32000 x 2048:
+// 504 -> 438 us against a fixed 4; 5003 x 50257 x 1600, a third ignored: 658 -> 534.)
+constexpr int HD_SPLITS = 128;
+__device__ __forceinline__ int splits_for(int64_t count, int ld, int kblocks, int most, int tile) {
+    const int tiles = static_cast<int>((count + tile - 1) / tile) * ((ld + tile - 1) / tile), places = tile == 256 ? HD_CUS : 2 * HD_CUS;
+    uint64_t least = ~0ull;
+    for (int s = 1 + static_cast<int>(threadIdx.x & 63); s <= most; s += 64) {
+        const int64_t cost = static_cast<int64_t>((tiles * s + places - 1) / places) * ((kblocks + s - 1) / s + 6) + s * count * ld / 625000;
+        least = min(least, static_cast<uint64_t>(cost) << 8 | s);
     }
-    return best;
+    return static_cast<int>(group_reduce<64>(least, [](uint64_t u, uint64_t v) { return min(u, v); }) & 255);
 }
 
 // The tokens' common factor g of a mean or sum, without its power of two: e is formed and rounded without it, and the products are
@@ -653,13 +651,16 @@ __device__ __forceinline__ float common_factor(const MuonHeadLoss& a) {
 
 // The hidden states of the rows, in bf16 rows of `ld` elements with zeros beyond the width, up to a whole tile of rows; backward their
 // coefficients too.  A wave for each row.
-__global__ __launch_bounds__(256) void head_gather_kernel(const MuonHeadLoss a, uint16_t* rows, int ld, f32x4v* coef, float* scale, int kblocks, int most_splits) {
+__global__ __launch_bounds__(256) void head_gather_kernel(const MuonHeadLoss a, uint16_t* rows, int ld, f32x4v* coef, float* scale, int kblocks, int most_splits, int tile) {
     const int lane = threadIdx.x & 63;
     const float factor = coef ? common_factor(a) : 1.f;
     const int64_t count = a.order[a.tokens];
-    if (coef && blockIdx.x == 0 && threadIdx.x == 0) {
-        scale[0] = factor;
-        reinterpret_cast<int32_t*>(scale)[1] = splits_for(count, ld, kblocks, most_splits);
+    if (coef && blockIdx.x == 0 && threadIdx.x < 64) {
+        const int splits = splits_for(count, ld, kblocks, most_splits, tile);
+        if (threadIdx.x == 0) {
+            scale[0] = factor;
+            reinterpret_cast<int32_t*>(scale)[1] = splits;
+        }
     }
     const int64_t padded = (count + HD_TILE - 1) / HD_TILE * HD_TILE;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < padded; r += static_cast<int64_t>(gridDim.x) * 4) {
@@ -798,31 +799,56 @@ __global__ __launch_bounds__(HJ_THREADS) void head_join_kernel(const MuonHeadLos
     *a.loss = a.reduction == MUON_AMD_REDUCE_MEAN ? total / *a.part : total;
 }
 
-// Adds the shares of the hidden states' gradient and writes it to the tokens; zeros for those that take no part.  A wave for each row.
+// Adds the shares of the hidden states' gradient and writes it to the tokens; zeros for those that take no part.  A wave takes 512 channels
+// of a row; where there are many shares (and few rows), the four waves of a workgroup share them.
+constexpr int HH_MANY = 8;
 __global__ __launch_bounds__(256) void head_dhidden_kernel(const MuonHeadLoss a, const float* part, int64_t stride, int ld, const float* scale) {
-    const int lane = threadIdx.x & 63, shares = reinterpret_cast<const int32_t*>(scale)[1];
+    __shared__ float sums[3][64][9];                         // (a place more, so that lanes fall on different banks)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, shares = reinterpret_cast<const int32_t*>(scale)[1], segments = (a.width + 511) / 512;
+    const bool many = shares >= HH_MANY;
     const float factor = scale[0];
-    const int64_t count = a.order[a.tokens];
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < a.tokens; r += static_cast<int64_t>(gridDim.x) * 4) {
-        const int at = a.order[r];
+    const int64_t count = a.order[a.tokens], items = a.tokens * segments;
+    const int first = many ? wave : 0, step = many ? 4 : 1;
+    for (int64_t item = many ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + wave; item < items; item += many ? gridDim.x : static_cast<int64_t>(gridDim.x) * 4) {
+        const int64_t r = item / segments;
+        const int e = static_cast<int>(item % segments) * 512 + lane * 8, at = a.order[r];
         const bool on = at >= 0;
-        uint16_t* const out = static_cast<uint16_t*>(a.dhidden) + static_cast<int64_t>(on ? at : ~at) * a.width;
-        for (int e = lane * 8; e < a.width; e += 512) {
-            float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (on && r < count)
-                for (int s = 0; s < shares; ++s) {
-                    const float* const p = part + s * stride + r * ld + e;
-                    const f32x4v lo = load_as<true, f32x4v>(p), hi = load_as<true, f32x4v>(p + 4);
+        float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (on && r < count && e < a.width) {
+            const float* const p = part + r * ld + e;
+            const auto add = [&](auto together, int s) __attribute__((always_inline)) {
+                constexpr int K = decltype(together)::value;
+                f32x4v v[K][2];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        sum[i] += lo[i];
-                        sum[4 + i] += hi[i];
-                    }
+                for (int k = 0; k < K; ++k) {
+                    v[k][0] = load_as<true, f32x4v>(p + (s + k * step) * stride);
+                    v[k][1] = load_as<true, f32x4v>(p + (s + k * step) * stride + 4);
                 }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] *= factor;
-            store_pack<uint16_t, 8, false>(out, e, a.width, Pack<uint16_t, 8>::of(sum));
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum[i] += v[k][i / 4][i % 4];
+            };
+            int s = first;
+            for (; s + 3 * step < shares; s += 4 * step) add(std::integral_constant<int, 4>{}, s);
+            for (; s < shares; s += step) add(std::integral_constant<int, 1>{}, s);
         }
+        if (many) {
+            if (wave > 0)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sums[wave - 1][lane][i] = sum[i];
+            __syncthreads();
+            if (wave == 0)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i] += sums[0][lane][i] + (sums[1][lane][i] + sums[2][lane][i]);
+            __syncthreads();
+            if (wave > 0) continue;
+        }
+        if (e >= a.width) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] *= factor;
+        uint16_t* const out = static_cast<uint16_t*>(a.dhidden) + static_cast<int64_t>(on ? at : ~at) * a.width;
+        store_pack<uint16_t, 8, false>(out, e, a.width, Pack<uint16_t, 8>::of(sum));
     }
 }
 
@@ -841,7 +867,7 @@ struct HeadPlan {
     int64_t rows, ld;              // padded rows and width
     int tile, col_tiles;           // of the statistics
     int64_t piece;                 // columns of e
-    int pieces, splits;
+    int pieces, splits, dh_tile;
     // offsets in the workspace, in bytes
     int64_t hidden, weight, stats, logit, left, coef, scale, e, part, bytes;
 };
@@ -877,7 +903,9 @@ static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
         p.piece = up((v + p.pieces - 1) / p.pieces, 256);
         p.pieces = static_cast<int>((v + p.piece - 1) / p.piece);
         p.e = take(p.rows * p.piece * 2);
-        // at most so many shares (the tokens that take part decide, on the device): of 8 k-blocks or more each, in half a GiB or one share
+        // at most so many shares (the tokens that take part decide, on the device): of 8 k-blocks or more each, in half a GiB or one share.  Tiles of
+        // 128 x 128 where those of 256 x 256 are few.
+        p.dh_tile = (p.rows / 256) * ((p.ld + 255) / 256) >= 64 ? 256 : 128;
         int64_t most_splits = HD_SPLITS;
         if (most_splits > p.piece / BK / 8) most_splits = p.piece / BK / 8;
         if (most_splits > HD_PIECE_BYTES / 2 / (p.rows * p.ld * 4)) most_splits = HD_PIECE_BYTES / 2 / (p.rows * p.ld * 4);
@@ -939,7 +967,7 @@ int raise_head_limits() {
 static int gather(const MuonHeadLoss& a, const HeadPlan& p, char* ws, f32x4v* coef, const uint16_t** w, int64_t* ld, hipStream_t s) {
     const int64_t blocks = p.rows / 4 < 4096 ? p.rows / 4 : 4096;
     hipLaunchKernelGGL(head_gather_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, reinterpret_cast<uint16_t*>(ws + p.hidden), static_cast<int>(p.ld), coef,
-                       reinterpret_cast<float*>(ws + p.scale), static_cast<int>(p.piece / BK), p.splits);
+                       reinterpret_cast<float*>(ws + p.scale), static_cast<int>(p.piece / BK), p.splits, p.dh_tile);
     if (const int rc = check_launch("linear_cross_entropy: rows")) return rc;
     *w = static_cast<const uint16_t*>(a.weight);
     *ld = a.ld_weight;
@@ -1067,8 +1095,8 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
             h.ldq = ldw;
             h.end_q = ((size - 1) * ldw + p.ld - 8) * 2;
             h.col_limit = static_cast<int>(p.ld);
-            h.row_tiles = static_cast<int>(p.rows / 256);
-            h.col_tiles = static_cast<int>(up(p.ld, 256) / 256);
+            h.row_tiles = static_cast<int>(p.rows / p.dh_tile);
+            h.col_tiles = static_cast<int>(up(p.ld, p.dh_tile) / p.dh_tile);
             h.splits = splits;
             h.most_splits = p.splits;
             h.cols = static_cast<int>(p.ld);
@@ -1077,7 +1105,7 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
             h.add = i > 0;
             h.part_stride = p.rows * p.ld;
             h.ld_out = p.ld;
-            if (const int rc = launch_product<HeadLarge, HEAD_DHIDDEN>(h, s)) return rc;
+            if (const int rc = launch_product<HEAD_DHIDDEN>(h, p.dh_tile == 256, s)) return rc;
         }
         if (a.dweight) {
             HeadGemm h{};
@@ -1101,7 +1129,7 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
         }
     }
     if (a.dhidden) {
-        const int64_t blocks = (a.tokens + 3) / 4 < 8192 ? (a.tokens + 3) / 4 : 8192;
+        const int64_t items = a.tokens * ((a.width + 511) / 512), blocks = items < 8192 ? items : 8192;
         hipLaunchKernelGGL(head_dhidden_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, part, p.rows * p.ld, static_cast<int>(p.ld),
                            reinterpret_cast<const float*>(ws + p.scale));
         return check_launch("head_loss_backward: hidden");
