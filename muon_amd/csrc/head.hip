@@ -867,10 +867,17 @@ struct HeadPlan {
     int64_t rows, ld;              // padded rows and width
     int tile, col_tiles;           // of the statistics
     int64_t piece;                 // columns of e
-    int pieces, splits, dh_tile;
+    int pieces, splits, dh_tile, dw_tile;
     // offsets in the workspace, in bytes
     int64_t hidden, weight, stats, logit, left, coef, scale, e, part, bytes;
 };
+
+// Whether the products of tokens with the vocabulary take less time in 256 x 256 tiles, one to a CU, than in 128 x 128 tiles, two to a CU: a round
+// of the latter does half the work, and takes a little more than half the time.
+static bool fewer_rounds(int64_t tokens, int64_t vocab) {
+    const auto rounds = [&](int64_t tile, int64_t places) { return ((tokens + tile - 1) / tile * ((vocab + tile - 1) / tile) + places - 1) / places; };
+    return 100 * rounds(256, HD_CUS) <= 62 * rounds(128, 2 * HD_CUS);
+}
 
 static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
     HeadPlan p{};
@@ -880,7 +887,7 @@ static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
     p.rows = up(n, HD_TILE);
     // (whether W can be read as it is goes by its address too: a plan without one leaves room for the copy)
     p.padded = !p.few && (d % BK != 0 || a.ld_weight % 8 != 0 || reinterpret_cast<uintptr_t>(a.weight) % 16 != 0 || !a.weight);
-    p.large = (p.rows / 256) * up(v, 256) / 256 >= 512;
+    p.large = fewer_rounds(n, v);
     p.tile = p.few ? HF_VOCAB : p.large ? 256 : 128;
     p.col_tiles = static_cast<int>(up(v, p.tile) / p.tile);
     int64_t at = 0;
@@ -905,6 +912,8 @@ static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
         p.e = take(p.rows * p.piece * 2);
         // at most so many shares (the tokens that take part decide, on the device): of 8 k-blocks or more each, in half a GiB or one share.  Tiles of
         // 128 x 128 where those of 256 x 256 are few.
+        // (two k-blocks of 128 x 128 tiles keep a CU busier than a few of a large one: 130 x 100000 x 768 243 -> 234 us, 1000 x 50257 x 2048 948 us and 963)
+        p.dw_tile = p.rows > 512 ? 256 : 128;
         p.dh_tile = (p.rows / 256) * ((p.ld + 255) / 256) >= 64 ? 256 : 128;
         int64_t most_splits = HD_SPLITS;
         if (most_splits > p.piece / BK / 8) most_splits = p.piece / BK / 8;
@@ -1119,13 +1128,13 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
             h.end_q = (p.rows * p.ld - 8) * 2;
             h.col_limit = static_cast<int>(p.ld);
             h.rows = size;
-            h.row_tiles = static_cast<int>(up(size, 256) / 256);
-            h.col_tiles = static_cast<int>(up(a.width, 256) / 256);
+            h.row_tiles = static_cast<int>(up(size, p.dw_tile) / p.dw_tile);
+            h.col_tiles = static_cast<int>(up(a.width, p.dw_tile) / p.dw_tile);
             h.cols = a.width;
             h.scale = reinterpret_cast<const float*>(ws + p.scale);
             h.out = static_cast<uint16_t*>(a.dweight) + static_cast<int64_t>(begin) * a.width;
             h.ld_out = a.width;
-            if (const int rc = launch_product<HeadLarge, HEAD_DWEIGHT>(h, s)) return rc;
+            if (const int rc = launch_product<HEAD_DWEIGHT>(h, p.dw_tile == 256, s)) return rc;
         }
     }
     if (a.dhidden) {
