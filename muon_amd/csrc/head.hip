@@ -13,7 +13,7 @@
 //
 // Tokens that are ignored leave the products: a first launch numbers those that take part, and their hidden states are copied
 // to consecutive rows (zeros up to whole tiles).  The products take the tokens' number from the device; workgroups beyond it end
-// at once.  Up to 64 tokens forward (evaluation, single tokens) the matrix is streamed once through registers instead.
+// at once.  Few tokens forward (evaluation, single tokens): the matrix is streamed once through registers instead.
 //
 // The products bound everything: matrix instructions at 256 x 256 tiles of 8 waves, k-blocks of 64 in an LDS ring filled by
 // buffer_load ... lds a block and a half ahead, as in ns_gemm.hip.
@@ -882,11 +882,14 @@ static bool fewer_rounds(int64_t tokens, int64_t vocab) {
 static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
     HeadPlan p{};
     const int64_t n = a.tokens, d = a.width, v = a.vocab;
-    p.few = !backward && n <= HD_FEW;
     p.ld = up(d, BK);
     p.rows = up(n, HD_TILE);
-    // (whether W can be read as it is goes by its address too: a plan without one leaves room for the copy)
-    p.padded = !p.few && (d % BK != 0 || a.ld_weight % 8 != 0 || reinterpret_cast<uintptr_t>(a.weight) % 16 != 0 || !a.weight);
+    p.padded = d % BK != 0 || a.ld_weight % 8 != 0 || reinterpret_cast<uintptr_t>(a.weight) % 16 != 0;
+    // Streamed: up to 32 tokens; up to 64 where the tiles would need a copy of W or W is small (64 x 50257 x 768: streamed 36.4 us, by tiles 26.7;
+    // 64 x 128256 x 4096: 330 and 249; 33 x 8000 x 512: 12.7 and 16.5; 48 x 100000 x 1000, W copied: 60 and 133; 32 x 128256 x 4096: 233
+    // and 248).
+    p.few = !backward && (n <= HD_FEW / 2 || (n <= HD_FEW && (p.padded || v * d < (1 << 24))));
+    p.padded = p.padded && !p.few;
     p.large = fewer_rounds(n, v);
     p.tile = p.few ? HF_VOCAB : p.large ? 256 : 128;
     p.col_tiles = static_cast<int>(up(v, p.tile) / p.tile);

@@ -107,6 +107,13 @@ def test_few_tokens(tokens, width):
 
 
 @gpu
+@pytest.mark.parametrize("tokens", [31, 32, 33, 64])
+def test_few_tokens_of_a_large_matrix(tokens):
+    check(*make(tokens, 33000, 512, seed=tokens, ignored=0.2))   # (between the two ways that few tokens go)
+    check(*make(tokens, 33000, 520, seed=tokens, ignored=0.2), reduction="none")
+
+
+@gpu
 @pytest.mark.parametrize("tokens", [65, 127, 128, 129, 255, 256, 257, 511, 700])
 def test_tokens(tokens):
     check(*make(tokens, 1111, 128, seed=tokens, ignored=0.2))
