@@ -135,41 +135,55 @@ __global__ __launch_bounds__(DF_THREADS) void distill_finish_kernel(const MuonDi
     int taking = 0;
     for (int64_t t = static_cast<int64_t>(blockIdx.x) * DF_WAVES + wave; t < a.tokens; t += static_cast<int64_t>(gridDim.x) * DF_WAVES) {
         float loss = 0.f;
+        // All that the token has to be read for is requested together: each lane's entry of the list (more than 64 are read again below), the
+        // student's logit there, a part's sums.
+        const bool open = !a.mask || a.mask[t];
+        const f32x2_t* const p = reinterpret_cast<const f32x2_t*>(a.partials) + t * parts;
+        const f32x2_t first = lane < parts ? p[lane] : f32x2_t{-__builtin_inff(), 0.f};
+        const auto entry = [&](int k, float& v, float& x) {
+            const int i = open && k < a.top ? index_of(a, t, k) : -1;
+            v = k < a.top ? teacher_of(a, t * a.ld_teacher + k) : -__builtin_inff();
+            const int64_t at = t * a.ld_logits + (i >= 0 ? i : 0);
+            x = i < 0 ? 0.f : a.dtype == MUON_AMD_SRC_BF16 ? element<uint16_t>(a.logits, at) : element<float>(a.logits, at);
+            if (i < 0) v = -__builtin_inff();
+        };
+        float v0, x0;
+        entry(lane, v0, x0);
         // the list: whether anything is there, its maximum and sum
-        bool some = false;
-        float most = -__builtin_inff();
-        if (!a.mask || a.mask[t])
-            for (int k = lane; k < a.top; k += 64) {
-                const float v = teacher_of(a, t * a.ld_teacher + k);
-                if (index_of(a, t, k) >= 0 && v != -__builtin_inff()) {
-                    some = true;
-                    most = fmaxf(most, v);
-                }
-            }
+        bool some = v0 != -__builtin_inff();
+        float most = fmaxf(v0, -__builtin_inff());
+        for (int k = lane + 64; k < a.top; k += 64) {
+            float v, x;
+            entry(k, v, x);
+            some |= v != -__builtin_inff();
+            most = fmaxf(most, v);
+        }
         const bool on = __ballot(some) != 0;
         float tm = -__builtin_inff(), tl = 0.f, m = 0.f, l = 0.f;
         if (on) {
             tm = RunningSum::reference(group_reduce<64>(most, larger));     // (a list of nothing but NaN has a number here all the same)
-            float s = 0.f;
-            for (int k = lane; k < a.top; k += 64) {
-                const float v = teacher_of(a, t * a.ld_teacher + k);
-                if (index_of(a, t, k) >= 0) s += RunningSum::power(v, tm, c);
+            float s = RunningSum::power(v0, tm, c);
+            for (int k = lane + 64; k < a.top; k += 64) {
+                float v, x;
+                entry(k, v, x);
+                s += RunningSum::power(v, tm, c);
             }
             tl = __log2f(group_sum<64>(s));
             RunningSum r;
-            const f32x2_t* const p = reinterpret_cast<const f32x2_t*>(a.partials) + t * parts;
-            for (int i = lane; i < parts; i += 64) r.join(p[i][0], p[i][1], c);
+            r.join(first[0], first[1], c);
+            for (int i = lane + 64; i < parts; i += 64) r.join(p[i][0], p[i][1], c);
             m = group_reduce<64>(r.m, larger);
             l = __log2f(group_sum<64>(r.s * RunningSum::power(r.m, RunningSum::reference(m), c)));
             m = RunningSum::reference(m);
-            for (int k = lane; k < a.top; k += 64) {
-                const int i = index_of(a, t, k);
-                const float y = (teacher_of(a, t * a.ld_teacher + k) - tm) * c - tl;           // log2 q
-                if (i < 0 || y == -__builtin_inff()) continue;
-                const int64_t at = t * a.ld_logits + i;
-                const float x = a.dtype == MUON_AMD_SRC_BF16 ? element<uint16_t>(a.logits, at) : element<float>(a.logits, at);
-                const float q = __builtin_amdgcn_exp2f(y);
-                if (q != 0.f) loss = fmaf(q, y - ((x - m) * c - l), loss);
+            const auto term = [&](float v, float x) {
+                const float y = (v - tm) * c - tl, q = __builtin_amdgcn_exp2f(y);             // log2 q, q
+                if (v != -__builtin_inff() && q != 0.f) loss = fmaf(q, y - ((x - m) * c - l), loss);
+            };
+            term(v0, x0);
+            for (int k = lane + 64; k < a.top; k += 64) {
+                float v, x;
+                entry(k, v, x);
+                term(v, x);
             }
             loss = group_sum<64>(loss) * (LN2 * a.temperature * a.temperature);
         }
