@@ -650,8 +650,8 @@ std::optional<Tensor> distill_topk(const Tensor& logits, const Tensor& teacher, 
         teacher.size(-1) > api.max_top)
         return std::nullopt;
     if (mask && (mask->scalar_type() != at::kBool || mask->device() != device || mask->sizes() != rows(logits))) return std::nullopt;
-    // (a temperature whose reciprocal is no normal number would leave none)
-    if (!(temperature >= 1e-30 && temperature <= 1e30) || reduction < 0 || any_tangent({&logits, &teacher}) || any_requires_grad({&teacher})) return std::nullopt;
+    // (its square and reciprocal are to be normal numbers)
+    if (!(temperature >= 1e-15 && temperature <= 1e15) || reduction < 0 || any_tangent({&logits, &teacher}) || any_requires_grad({&teacher})) return std::nullopt;
     const py::gil_scoped_release released;
     if (any_requires_grad({&logits})) {
         refuse_leaves_of_the_default_stream({&logits});

@@ -45,8 +45,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     out.  Any other target outside of 0 .. V - 1 gives a loss that is not a number, and such gradients.
 
     The products are of bf16 numbers with fp32 sums.  Backward forms the logits again in pieces of the vocabulary, rounds their gradient to
-    bf16 once, and returns both gradients in bf16; it takes 1 GiB of workspace, or more where 131072 tokens are passed, and 4 D
-    bytes a token, up to four times.  V is at most 2^24, D 65536.  The same call gives the same bits."""
+    bf16 once, and returns both gradients in bf16.  There are at most 2^24 tokens and classes, 65536 channels.  The same call gives the same bits.
+    Workspaces: forward 8 bytes for 256 logits (128 where there are few), backward at most 1 GiB for the logits' gradient (4096 of its columns
+    where there are more than 131072 tokens) and half a GiB or 4 D bytes a token, whichever is more, for sums; both 2 D bytes a token, and a
+    copy of the matrix unless D is a multiple of 64 and its rows lie at multiples of 16 bytes."""
     if isinstance(ignore_index, int) and not isinstance(ignore_index, bool) and -1 << 63 <= ignore_index < 1 << 63:
         out = _lib.native().linear_cross_entropy(hidden, weight, targets, ignore_index, _reduction(reduction))
         if out is not None:
@@ -88,7 +90,7 @@ def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
         p = softmax(logits / T) over the vocabulary;  q = softmax(teacher_logits / T) over the token's list
         loss = T^2 sum_k q_k (log q_k - log p[teacher_indices_k])
 
-    as the mean over the tokens that take part (zero where none does), their "sum", or ("none") of each token, fp32.  Entries
+    as the mean over the tokens that take part (zero where none does), their "sum", or ("none") of each token, fp32; T from 1e-15 to 1e15.  Entries
     whose index is outside of the vocabulary (-1 by habit) or whose teacher logit is -infinity are not there; a token whose
     list has none, or whose `mask` (bool, the shape of logits without its last dimension) is false, takes no part: its loss and
     gradient are zero, whatever its logits hold.  An index that comes several times counts with the sum of its
@@ -124,8 +126,8 @@ def _refuse_distill(logits, teacher_logits, teacher_indices, temperature, mask, 
         require_gpu_tensor(mask, "mask")
         if mask.dtype != torch.bool or mask.shape != logits.shape[:-1] or mask.device != logits.device:
             raise ValueError(f"mask must be a bool tensor of shape {tuple(logits.shape[:-1])} on {logits.device}, got {mask.dtype} {tuple(mask.shape)}")
-    if not isinstance(temperature, (int, float)) or not 1e-30 <= temperature <= 1e30:
-        raise ValueError(f"temperature must be a number from 1e-30 to 1e30, got {temperature!r}")
+    if not isinstance(temperature, (int, float)) or not 1e-15 <= temperature <= 1e15:
+        raise ValueError(f"temperature must be a number from 1e-15 to 1e15, got {temperature!r}")
     _refuse_reduction(reduction)
     _no_tangent(logits, "logits")
     _no_tangent(teacher_logits, "teacher_logits")

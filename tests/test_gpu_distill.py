@@ -353,3 +353,46 @@ def test_refusals():
     assert lib.muon_amd_distill_backward(ctypes.byref(_lib.DistillArgs(**{**good, "tokens": 1 << 24, "vocab": 1 << 30})), None) == -1
     assert lib.muon_amd_distill(None, None) == -1 and lib.muon_amd_distill_backward(None, None) == -1
     assert lib.muon_amd_distill_partials(0, 8, 0) == 0 and lib.muon_amd_distill_partials(100, 8, 0) > 0
+
+
+@gpu
+def test_the_largest_temperature():
+    check(*make((5,), 1234, 6, F32), T=1e15)
+    check(*make((5,), 1234, 6, F32), T=1e15, reduction="none")
+
+
+@gpu
+def test_the_smallest_temperature():
+    # p and q have one entry each: a loss is T (max - x at the teacher's best), of a difference's rounding and those of 1 / T, log2(e), T ^ 2, ln 2
+    # and four products, twelve in all; the gradient is T g at the one and - T g at the other.
+    T = 1e-15
+    x, v, i, _ = make((5,), 1234, 6, F32)
+    leaf = x.to(DEV).requires_grad_()
+    losses = muon_amd.distill_topk(leaf, v.to(DEV), i.to(DEV), temperature=T, reduction="none")
+    grad, = torch.autograd.grad(losses.sum(), leaf)
+    at, top = i.gather(1, v.argmax(1, keepdim=True)), x.argmax(1, keepdim=True)
+    want = T * (x.double().gather(1, top) - x.double().gather(1, at))[:, 0]
+    assert ((losses.cpu().double() - want).abs() <= 12 * U * want).all()
+    one = torch.zeros(5, 1234, dtype=torch.float64)
+    expected = one.scatter(1, top, T) - one.scatter(1, at, T)
+    assert ((grad.cpu().double() - expected).abs() <= 12 * U * T).all()
+
+
+@gpu
+def test_refusals_of_temperatures():
+    x, v, i, _ = (t if t is None else t.to(DEV) for t in make((4,), 50, 3, F32))
+    for T in (1e-16, 1e16, 10 ** 20):
+        with pytest.raises(ValueError):
+            muon_amd.distill_topk(x, v, i, temperature=T)
+
+
+def test_refusals_beyond_a_launch():
+    import ctypes
+
+    from muon_amd import _lib
+    lib = _lib.load()
+    pointers = ("logits", "teacher", "indices", "losses", "part", "stats", "partials", "counter", "dloss", "dlogits")
+    good = dict({p: 4096 for p in pointers}, tokens=1 << 24, ld_logits=8, ld_teacher=2, ld_indices=2, vocab=8, top=2, index_bits=32, temperature=1.0)
+    for bad in ({}, dict(vocab=1 << 30), dict(tokens=1, temperature=1e-16), dict(tokens=1, temperature=1e16)):      # 2^24 workgroups of 256: 2^32 threads
+        for call in (lib.muon_amd_distill, lib.muon_amd_distill_backward):
+            assert call(ctypes.byref(_lib.DistillArgs(**{**good, **bad})), None) == -1
