@@ -123,15 +123,17 @@ __device__ __forceinline__ void put_choices(const MuonRoute& a, int64_t t, const
             return (d == d ? exp_of(d) : d) * per;
         }
     };
-    float chosen = 0.f;
-    for (int j = lane; j < a.k; j += L) {
+    const int own = lane < a.k ? picks[lane] : -1;
+    const float first = own >= 0 ? score_at(own) : 0.f;
+    float chosen = first;
+    for (int j = lane + L; j < a.k; j += L) {
         const int e = picks[j];
         if (e >= 0) chosen += score_at(e);
     }
     chosen = a.normalize ? group_sum<L>(chosen) : 1.f;
     for (int j = lane; j < a.k; j += L) {
         const int e = picks[j];
-        const float score = e >= 0 ? score_at(e) : 0.f;
+        const float score = j == lane ? first : e >= 0 ? score_at(e) : 0.f;
         a.indices[t * a.k + j] = e;
         a.weights[t * a.k + j] = chosen != 0.f ? score / chosen : 0.f;
         if (e >= 0) atomicAdd(&tokens[e], 1);
@@ -210,8 +212,8 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
             norm = 0.f;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float t = exp_with_nan(-fabsf(x[i])), u = __builtin_amdgcn_rcpf(1.f + t), e = x[i] >= 0.f ? __builtin_amdgcn_rcpf(t) : t;
-                s[i] = x[i] >= 0.f ? u : t * u;
+                const float e = exp_with_nan(x[i]);
+                s[i] = e * __builtin_amdgcn_rcpf(1.f + e);
                 total += e;
                 norm += s[i];
             }
@@ -245,20 +247,24 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
         constexpr float OFF = SIGMOID ? 8.f * RS_UNIT : 40.f * RS_UNIT, RELATIVE = SIGMOID ? 8.f * RS_UNIT : 128.f * RS_UNIT;
         const float off = bias ? OFF * (SIGMOID ? 1.f : per) : 0.f, relative = bias ? RS_UNIT : RELATIVE + RS_UNIT;
         // from here on what is chosen by; the token takes part if anything is available
-        float c[N];
-        bool some = false;
+        float c[N], most = -__builtin_inff();
 #pragma unroll
         for (int q = 0; q < N / 4; ++q) {
             const f32x4v b = *reinterpret_cast<const f32x4v*>(&biases[base + 4 * q]);
 #pragma unroll
             for (int i = 4 * q; i < 4 * q + 4; ++i) {
                 c[i] = x[i] == -__builtin_inff() ? -__builtin_inff() : s[i] + b[i % 4];
-                some |= c[i] != -__builtin_inff();
+                most = fmaxf(most, c[i]);
             }
         }
-        const bool on = group_reduce<L>(static_cast<int>(some), [](int u, int v) { return u | v; }) != 0;
+        if (biases_none || __ballot(total != total)) {               // (a maximum passes over what is no number)
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] = on ? fmaf(s[i], norm, acc[i]) : acc[i];
+            for (int i = 0; i < N; ++i) most = c[i] == c[i] ? most : 0.f;
+        }
+        const bool on = group_reduce<L>(most, most_of) != -__builtin_inff();
+        norm = on ? norm : 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = fmaf(s[i], norm, acc[i]);
         // (a row in which anything is no number is done again, where that is the largest value)
         bool close = total != total || biases_none, lane_in = true;
         uint64_t in_groups = 0;
