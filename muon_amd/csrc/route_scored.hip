@@ -6,13 +6,15 @@
 // with counts, balance and z loss as in route.hip, the balance loss over s / sum s.  The bias steers the choice alone.
 //
 // What is chosen goes by the order of the c as real numbers, so that it does not depend on how an exponential is rounded.  A row's c are formed in
-// fp32, and where two that decide something (neighbours among the k + 1 largest, the last group kept and the
+// fp32, and where two that decide something (neighbours among the k + 1 largest, the last of these and what is left out, the last group kept and the
 // best one left out) are nearer than what that may be off, the wave does the row again in 64 bits: 5 to 7 rows of 10000 (8 of 256 by
-// sigmoid in bf16, 6 of 160 by softmax in fp32).  Equal logits with equal biases are a tie, not a near one.
+// sigmoid in bf16, 6 of 160 by softmax in fp32).  Equal logits with equal biases are a tie, not a near one; a row of nothing else (a router
+// that starts at zero) is never done again.
 //
 // Layout as in route.hip: a row in the registers of L lanes, N elements each.  The two largest c of a group come from its lanes, or through LDS where
-// groups begin anywhere in a lane's elements.  Instructions bound it: 65536 tokens, 8 of 256 in 4 of 8 groups, sigmoid, bf16 66 us for 38 MB (with
-// 64-bit keys for the choice and the biases in registers 116); 30011 tokens, 6 of 160 in 3 of 8, softmax, fp32 39 us.
+// groups begin anywhere in a lane's elements.  Instructions bound it (the vector units are busy 95 % of the time): 65536 tokens, 8 of 256 in 4 of 8
+// groups, sigmoid, bf16 64 us for 38 MB (with 64-bit keys for the choice and the biases in registers 116), all logits equal likewise; 30011
+// tokens, 6 of 160 in 3 of 8, softmax, fp32 39 us.
 #include "route.h"
 
 namespace muon_amd {
@@ -40,7 +42,8 @@ __device__ __forceinline__ T wave_best(T v) {
     return group_reduce<64>(v, [](T x, T y) { return x > y ? x : y; });
 }
 
-// A row once more in 64 bits, by a whole wave: writes the k choices (-1 where there is none).  c: LDS of this wave for E doubles; best: for 64.
+// A row once more in 64 bits, by a whole wave: writes the k choices (-1 where there is none).  c: LDS of this wave for E doubles; best: for 64 (which
+// the choices may go over).
 template <typename T, bool SIGMOID>
 __device__ __forceinline__ void choose_again(const T* row, const float* bias, int experts, int k, int groups, int kept, double* c, double* best, int* picks) {
     const int lane = threadIdx.x & 63;
@@ -140,29 +143,43 @@ __device__ __forceinline__ void put_choices(const MuonRoute& a, int64_t t, const
     }
 }
 
+// The sum of v over the lanes before this one in its group of L.
+template <int L>
+__device__ __forceinline__ int sum_before(int v, int lane) {
+    int at = v;
+    const auto step = [&](int o, bool there) { at += there ? o : 0; };
+    if constexpr (L >= 2) step(moved<0x111>(at), L >= 16 || lane >= 1);          // row_shr:1 (zero at the start of 16 lanes)
+    if constexpr (L >= 4) step(moved<0x112>(at), L >= 16 || lane >= 2);
+    if constexpr (L >= 8) step(moved<0x114>(at), L >= 16 || lane >= 4);
+    if constexpr (L >= 16) step(moved<0x118>(at), true);
+    if constexpr (L >= 32) step(__shfl(at, (threadIdx.x & 32) | 15, 64), lane & 16);
+    if constexpr (L >= 64) step(__shfl(at, 31, 64), lane & 32);
+    return at - v;
+}
+
 template <typename T, int N, int L, bool SIGMOID>
 __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonRoute a, const float* bias, int groups, int kept) {
     constexpr int ROWS = RT_THREADS / L, WROWS = 64 / L;                      // rows of the workgroup, of a wave
     constexpr int PICKS = N * L < RT_MAX_K + 1 ? N * L : RT_MAX_K + 1, PG = N * L < RS_MAX_GROUPS ? N * L : RS_MAX_GROUPS;
-    constexpr int ROWC = N * L + N * L / 32;                                  // a row's c, a place more every 32: groups a power of two apart
-    constexpr int CFLOATS = WROWS * ROWC > 2 * N * L ? WROWS * ROWC : 2 * N * L, GFLOATS = 2 * WROWS * PG > 128 ? 2 * WROWS * PG : 128;
-    constexpr int LIST = N * L / 2;
-    __shared__ float sums[RT_WAVES][N * L];
+    constexpr int LIST = PICKS;                                               // (all `wanted`; the places of more take longer to count than a shorter list)
+    constexpr int SPREAD = (N * L + N * L / 32 + 1) / 2 * 2;                  // a row's c, a place more every 32: groups a power of two apart
+    constexpr int ROWC = SPREAD > 2 * LIST ? SPREAD : 2 * LIST;               // that, or its list
+    constexpr int CFLOATS = WROWS * ROWC > 2 * N * L ? WROWS * ROWC : 2 * N * L;
+    constexpr int ROWG = 2 * (PG > PICKS ? PG : PICKS), GFLOATS = WROWS * ROWG > 128 ? WROWS * ROWG : 128;     // a row's groups, then its choices
     __shared__ int tokens[N * L];
     __shared__ __align__(16) float biases[N * L];
     __shared__ float squares[RT_WAVES];
     __shared__ int parts[RT_WAVES];
     __shared__ __align__(8) float by_expert[RT_WAVES][CFLOATS];
     __shared__ __align__(8) float by_group[RT_WAVES][GFLOATS];
-    __shared__ int pick_at[RT_WAVES][WROWS][PICKS];
-    __shared__ float pick_c[RT_WAVES][WROWS][PICKS];
     const int lane = threadIdx.x % L, sub = threadIdx.x / L, first_of_lane = lane * N, E = a.experts, wave = threadIdx.x >> 6, slot = (threadIdx.x & 63) / L;
     const int size = E / groups, wanted = a.k < E ? a.k + 1 : a.k;           // (one more than is chosen: what the last one is near to)
     float* const row_c = by_expert[wave] + slot * ROWC;
-    float* const row_g = by_group[wave] + slot * 2 * PG;                      // scores of the groups, what each may be off by
-    int* const row_at = pick_at[wave][slot];
-    float* const row_pick = pick_c[wave][slot];
+    float* const row_g = by_group[wave] + slot * ROWG;                        // scores of the groups, what each may be off by
+    int* const row_at = reinterpret_cast<int*>(row_g);                        // once the groups are known: the choices and their c
+    float* const row_pick = row_g + PICKS;
     const auto most_of = [](float u, float v) { return fmaxf(u, v); };
+    const auto sum_of = [](int u, int v) { return u + v; };
     for (int e = threadIdx.x; e < N * L; e += RT_THREADS) {
         tokens[e] = 0;
         biases[e] = bias && e < E ? bias[e] : 0.f;
@@ -181,9 +198,14 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
     }
     float square = 0.f;
     int part = 0;
-    bool later = false, biases_none = false;
-    for (int e = 0; e < N; ++e) biases_none |= biases[first_of_lane + e] != biases[first_of_lane + e];
+    bool later = false, biases_none = false, biases_flat = true;             // (flat: one number for all experts)
+    for (int e = 0; e < N; ++e) {
+        const float b = biases[first_of_lane + e];
+        biases_none |= b != b;
+        biases_flat &= first_of_lane + e >= E || b == biases[0];
+    }
     biases_none = __ballot(biases_none) != 0;
+    biases_flat = __ballot(!biases_flat) == 0;
     const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
     for (int64_t t = static_cast<int64_t>(blockIdx.x) * ROWS + sub; t - sub < a.tokens; t += step) {
         // (opaque copies: what follows from them for each of N elements is formed where it is used, not kept in N registers each)
@@ -202,10 +224,20 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
         }
         // logsumexp, scores.  Where the largest logit (of every row of the wave) is not far from zero, a sigmoid's exponential serves both: what
         // is lost of logits far below it is nothing beside its own.
-        float top = -__builtin_inff(), total = 0.f, norm = 1.f;
+        float top = -__builtin_inff(), low = __builtin_inff(), total = 0.f, norm = 1.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);
+        for (int i = 0; i < N; ++i) {
+            top = fmaxf(top, x[i]);
+            low = fminf(low, x[i]);
+        }
+        const bool gaps = __ballot(low == -__builtin_inff()) != 0;             // logits that are not available
+        if (gaps) {
+            low = __builtin_inff();
+#pragma unroll
+            for (int i = 0; i < N; ++i) low = fminf(low, x[i] == -__builtin_inff() ? __builtin_inff() : x[i]);
+        }
         top = group_reduce<L>(top, most_of);
+        const bool flat = biases_flat && -group_reduce<L>(-low, most_of) == top;
         if (top == -__builtin_inff()) top = 0.f;
         if (SIGMOID && !__ballot(!(fabsf(top) <= 40.f))) {
             top = 0.f;
@@ -253,10 +285,15 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
             const f32x4v b = *reinterpret_cast<const f32x4v*>(&biases[base + 4 * q]);
 #pragma unroll
             for (int i = 4 * q; i < 4 * q + 4; ++i) {
-                c[i] = x[i] == -__builtin_inff() ? -__builtin_inff() : s[i] + b[i % 4];
-                most = fmaxf(most, c[i]);
+                c[i] = s[i] + b[i % 4];
             }
         }
+        if (gaps) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) c[i] = x[i] == -__builtin_inff() ? -__builtin_inff() : c[i];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) most = fmaxf(most, c[i]);
         if (biases_none || __ballot(total != total)) {               // (a maximum passes over what is no number)
 #pragma unroll
             for (int i = 0; i < N; ++i) most = c[i] == c[i] ? most : 0.f;
@@ -266,7 +303,7 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = fmaf(s[i], norm, acc[i]);
         // (a row in which anything is no number is done again, where that is the largest value)
-        bool close = total != total || biases_none, lane_in = true;
+        bool again = total != total || biases_none, close = false, lane_in = true;
         uint64_t in_groups = 0;
         if (kept < groups) {
             // the two largest c of each group: of a lane's elements where they are of one group, else through all of them in LDS
@@ -285,6 +322,7 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
                 for (int i = 0; i < N; ++i) row_c[base + base / 32 + i] = c[i];      // (a lane's elements lie within 32)
             }
             wave_order();
+            bool uneven = false;                                               // (a row of equal logits: not one score for all groups)
             for (int g = lane; g < groups; g += L) {
                 float first = -__builtin_inff(), second = -__builtin_inff();
                 if (whole) {
@@ -301,6 +339,7 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
                     }
                 }
                 const bool one = second == -__builtin_inff();
+                uneven |= one && size > 1 && first != -__builtin_inff();
                 row_g[g] = one ? first : first + second;
                 row_g[PG + g] = 2.f * off + 2.f * relative * (fabsf(first) + (one ? 0.f : fabsf(second)));
             }
@@ -325,6 +364,7 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
             low = -group_reduce<L>(-low, most_of);
             high = group_reduce<L>(high, most_of);
             close |= low <= high;
+            again |= uneven && low <= high;
             if (whole) {
                 lane_in = in_groups >> (group_of[0] & 255) & 1;
             } else {
@@ -357,49 +397,98 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
         int listed = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) listed += key[i] >= best;
-        int at = listed;                                     // of this lane and those before it
-#pragma unroll
-        for (int d = 1; d < L; d <<= 1) {
-            const int o = __shfl_up(at, d, L);
-            at += lane >= d ? o : 0;
-        }
-        at -= listed;
-        listed = group_reduce<L>(listed, [](int u, int v) { return u + v; });
+        const int at = sum_before<L>(listed, lane);
+        listed = group_reduce<L>(listed, sum_of);
         uint32_t* const list = reinterpret_cast<uint32_t*>(row_c);               // {value, index}, LIST of them
+        uint32_t* entry = list + 2 * at;
+        const auto put = [&](int i) {
+            *reinterpret_cast<u32x2v*>(entry) = u32x2v{key[i], static_cast<uint32_t>(base + i)};
+            entry += 2;
+        };
+        const bool cut = __ballot(listed > LIST) != 0;
         wave_order();
+        if (!cut) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (key[i] >= best && at < LIST) {
-                list[2 * at] = key[i];
-                list[2 * at + 1] = base + i;
-                ++at;
-            }
-        wave_order();
-        for (int j = lane; j < wanted; j += L) row_at[j] = -1;
-        wave_order();
-        if (listed <= LIST) {
-            for (int q = lane; q < listed; q += L) {
-                const uint32_t value = list[2 * q], index = list[2 * q + 1];
-                int before = 0;
-                for (int o = 0; o < listed; ++o) {
-                    const uint32_t other = list[2 * o];
-                    before += other > value || (other == value && list[2 * o + 1] < index);
-                }
-                if (before < wanted) {
-                    row_at[before] = index;
-                    row_pick[before] = value_of(value);
-                }
-            }
+            for (int i = 0; i < N; ++i)
+                if (key[i] >= best) put(i);
         } else {
-            close = true;                        // (many equal values: the way that needs no list)
+            // A row of the wave has more equal values than the list holds.  The largest value that `wanted` elements reach (all that are
+            // available, where these are fewer): those above it are less than `wanted`, and of those that are equal to it the first ones by index go
+            // into the list, `wanted` in all at most.
+            int above, equal;
+            uint32_t value = 0;
+            bool found = false;
+            for (int j = 0; j < wanted && __ballot(!found); ++j) {
+                uint32_t m = ORDERED_MINUS_INF - value;
+#pragma unroll
+                for (int i = 0; i < N; ++i) m = max(m, key[i] - value);
+                m = group_reduce<L>(m, [](uint32_t u, uint32_t v) { return max(u, v); });
+                value += found || value == ORDERED_MINUS_INF ? 0u : m;
+                int reach = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) reach += key[i] >= value;
+                found = group_reduce<L>(reach, sum_of) >= wanted;
+            }
+            best = max(value, ORDERED_MINUS_INF + 1);
+            above = 0, equal = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                above += key[i] > best;
+                equal += key[i] == best;
+            }
+            const int need = wanted - group_reduce<L>(above, sum_of);
+            int place = sum_before<L>(equal, lane);
+            above += min(max(need - place, 0), equal);
+            entry = list + 2 * sum_before<L>(above, lane);
+            listed = group_reduce<L>(above, sum_of);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (key[i] > best || (key[i] == best && place < need)) put(i);
+                place += key[i] == best;
+            }
         }
         wave_order();
-        for (int j = lane + 1; j < wanted; j += L) {
-            const int at = row_at[j], prev = row_at[j - 1];
-            const float c = row_pick[j], before = row_pick[j - 1];
-            if (at < 0 || !(before - c <= 2.f * off + 2.f * relative * (fabsf(c) + fabsf(before)))) continue;
-            if (!(logit_of(row, at) == logit_of(row, prev) && (!bias || bias[at] == bias[prev]))) close = true;
+        for (int q = lane; q < listed; q += L) {
+            const uint32_t value = list[2 * q], index = list[2 * q + 1];
+            int before = 0;
+            for (int o = 0; o < listed; ++o) {
+                const uint32_t other = list[2 * o];
+                before += other > value || (other == value && list[2 * o + 1] < index);
+            }
+            if (before < wanted) {
+                row_at[before] = index;
+                row_pick[before] = value_of(value);
+            }
         }
+        for (int j = listed + lane; j < wanted; j += L) row_at[j] = -1;
+        wave_order();
+        // Whether two scores are nearer than what they may be off, and not a tie: neighbours in the order, and the last one with those that are
+        // not in it, where there are ties (as large as it, or the next smaller ones).
+        const auto near = [&](float c, int at, float o, int other) {
+            if (!(fabsf(o - c) <= 2.f * off + 2.f * relative * (fabsf(c) + fabsf(o)))) return false;
+            return !(logit_of(row, at) == logit_of(row, other) && (!bias || bias[at] == bias[other]));
+        };
+        if (!flat) {
+            for (int j = lane + 1; j < wanted; j += L) {
+                const int at = row_at[j];
+                if (at >= 0) close |= near(row_pick[j], at, row_pick[j - 1], row_at[j - 1]);
+            }
+            const int last = row_at[wanted - 1];
+            const float least = row_pick[wanted - 1];
+            if (listed > wanted)
+#pragma unroll 1
+                for (int q = lane; q < listed; q += L) {
+                    const float c = value_of(list[2 * q]);
+                    const int index = static_cast<int>(list[2 * q + 1]);
+                    if (c <= least && index != last) close |= near(c, index, least, last);
+                }
+            if (cut && last >= 0) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (key[i] <= best && key[i] > ORDERED_MINUS_INF && base + i != last) close |= near(value_of(key[i]), base + i, least, last);
+            }
+        }
+        close = again || (close && !flat);
         close = group_reduce<L>(static_cast<int>(close), [](int u, int v) { return u | v; }) != 0;
         if (t >= a.tokens) continue;
         if (on && close) {                       // (the rows that are done again come after the loop, out of its registers' way)
@@ -427,8 +516,8 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
                 const int64_t t = first + __builtin_ctzll(again);
                 const T* const row = row_of<T>(a, t);
                 choose_again<T, SIGMOID>(row, bias, E, a.k, groups, kept, reinterpret_cast<double*>(by_expert[wave]),
-                                         reinterpret_cast<double*>(by_group[wave]), pick_at[wave][0]);
-                put_choices<T, 64, SIGMOID>(a, t, row, a.lse[t], expf(-a.lse_rest[t]), pick_at[wave][0], tokens, whole);
+                                         reinterpret_cast<double*>(by_group[wave]), reinterpret_cast<int*>(by_group[wave]));
+                put_choices<T, 64, SIGMOID>(a, t, row, a.lse[t], expf(-a.lse_rest[t]), reinterpret_cast<int*>(by_group[wave]), tokens, whole);
                 wave_order();
             }
         }
@@ -437,7 +526,7 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         acc[i] = sum_of_groups<L>(acc[i]);
-        if ((threadIdx.x & 63) < L) sums[threadIdx.x >> 6][first_of_lane + i] = acc[i];
+        if ((threadIdx.x & 63) < L) by_expert[wave][first_of_lane + i] = acc[i];
     }
     square = group_sum<64>(square);
     part = group_reduce<64>(part, [](int u, int v) { return u + v; });
@@ -450,7 +539,7 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
     for (int e = threadIdx.x; e < E; e += RT_THREADS) {
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < RT_WAVES; ++w) sum += sums[w][e];
+        for (int w = 0; w < RT_WAVES; ++w) sum += by_expert[w][e];
         out[2 * e] = sum;
         out[2 * e + 1] = __int_as_float(tokens[e]);
     }

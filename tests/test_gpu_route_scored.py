@@ -359,3 +359,42 @@ def test_refusals():
     assert lib.muon_amd_route_scored_backward(ctypes.byref(_lib.RouteArgs(**{**good, "dlogits": None})), 1, None) == -1
     assert lib.muon_amd_route_scored(None, 1, None, 1, 1, None) == -1 and lib.muon_amd_route_scored_backward(None, 1, None) == -1
     assert lib.muon_amd_route_max_groups() == 64
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scores,values", [("sigmoid", (18.0, 18.25, 19.0, 20.0)), ("softmax", (0.0, -2.0 ** -28, -2.0 ** -27, -2.0 ** -26))])
+@pytest.mark.parametrize("experts", [8, 16, 40, 64, 100, 256, 320, 1000])
+def test_equal_logits_beside_near_ones(experts, scores, values, dtype):
+    """Scores that are one number in 32 bits, of logits of which several are equal and others are not: the equal ones are no reason to stop looking."""
+    g = torch.Generator().manual_seed(experts)
+    for k in sorted({1, 2, min(8, experts // 2), min(32, experts)}):
+        logits, mask, dw, bias = make((41, experts), k, dtype, seed=k)
+        near = torch.rand(41, experts, generator=g) < (torch.arange(41)[:, None] + 1) / 41            # from a few of them to all
+        pick = torch.tensor(values)[torch.randint(len(values), (41, experts), generator=g)]
+        logits = torch.where(near, pick, logits.float() - 12).to(dtype)
+        check(logits, mask, dw, None, k, scores)
+        # (groups by softmax: 1 + e^-2a is larger than 2 e^-a by a^2, at a = 2^-28 half of 2^-56 of the sum, which 64 bits do not hold)
+        if scores == "sigmoid" and experts % 8 == 0 and k <= experts // 8 * 3:
+            check(logits, mask, dw, None, k, scores, groups=8, kept=3)
+    row = torch.full((1, experts), -30.0)
+    row[0, :3] = torch.tensor([values[1], values[1], values[0] if scores == "softmax" else values[2]])
+    r, _ = check(row.to(dtype), None, torch.ones(1, 1), None, 1, scores)
+    assert r.indices.item() == 2
+
+
+@gpu
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,k,groups,kept", [(8, 2, 1, 1), (8, 4, 2, 1), (8, 8, 1, 1), (60, 6, 5, 2), (160, 6, 8, 3), (256, 8, 8, 4), (256, 32, 8, 4), (1024, 32, 16, 2)])
+def test_rows_of_equal_logits(experts, k, groups, kept, scores):
+    for dtype in (F32, BF16):
+        logits, mask, dw, bias = make((37, experts), k, dtype, seed=k, masked=True)
+        logits[:20] = 0.0
+        logits[20:30] = logits[20:30, :1]
+        logits[3, ::3] = -INF
+        logits[4, 1:] = -INF
+        logits[5, 1:experts // groups] = -INF
+        logits[25, -1] += 0.5
+        logits[26, experts // 2:] -= 0.5
+        for b in (None, torch.zeros(experts), torch.full((experts,), 0.25), bias, torch.where(bias > 0.1, -INF, 0.0)):
+            check(logits, mask, dw, b, k, scores, groups, kept)
