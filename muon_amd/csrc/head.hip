@@ -624,6 +624,54 @@ __global__ __launch_bounds__(HO_THREADS) void head_order_kernel(const MuonHeadLo
     }
 }
 
+// The same for few tokens, and their hidden states' copy with it: every workgroup counts all of them, and a wave takes one (64 x 50257 x 768:
+// 27.4 -> 25.0 us against a launch for each).
+constexpr int HO_FEW = 1024, HO_EACH = 4, HO_WAVES = 4;
+__global__ __launch_bounds__(HO_WAVES * 64) void head_order_few_kernel(const MuonHeadLoss a, uint16_t* rows, int ld, int64_t padded) {
+    __shared__ int counted[HO_WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tokens = static_cast<int>(a.tokens), first = blockIdx.x * HO_WAVES;
+    int n = 0;                                               // those that take part, and in the upper half those before this workgroup's
+#pragma unroll
+    for (int i = 0; i < HO_EACH; ++i) {
+        const int t = i * HO_WAVES * 64 + threadIdx.x;
+        if (t < tokens && target_of(a, t) != a.ignore_index) n += t < first ? 0x10001 : 1;
+    }
+    static_assert(HO_EACH * HO_WAVES * 64 == HO_FEW, "all tokens are counted");
+    const int t = first + wave;
+    const int64_t target = t < tokens ? target_of(a, t) : a.ignore_index;
+    const uint64_t here = __ballot(lane < HO_WAVES && first + lane < tokens && target_of(a, first + lane) != a.ignore_index);
+    n = group_reduce<64>(n, [](int u, int v) { return u + v; });
+    if (lane == 0) counted[wave] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < HO_WAVES; ++w) n += counted[w];
+    const int count = n & 0xffff, before = (n >> 16) + __builtin_popcountll(here & ((1ull << wave) - 1));
+    const bool on = target != a.ignore_index;
+    if (t < tokens) {
+        const int row = on ? before : count + (t - before);
+        if (lane == 0) {
+            a.order[row] = on ? t : ~t;
+            a.rows[row] = on ? target_in(a, target) : -1;
+            if (!on) {
+                a.losses[t] = 0.f;
+                a.lse[t] = 0.f;
+            }
+        }
+        if (on) {
+            const uint16_t* const from = static_cast<const uint16_t*>(a.hidden) + t * a.ld_hidden;
+            for (int e = lane * 8; e < ld; e += 512) load_pack<uint16_t, 8, false>(from, e, a.width).template store<false>(rows + static_cast<int64_t>(row) * ld + e);
+        }
+    }
+    if (t >= count && t < padded)
+        for (int e = lane * 8; e < ld; e += 512) Pack<uint16_t, 8>::zero().template store<false>(rows + static_cast<int64_t>(t) * ld + e);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        a.order[tokens] = count;
+        *a.part = static_cast<float>(count > 0 ? count : 1);
+        *a.counter = 0;
+    }
+}
+
 // The shares that the k-blocks of e W are cut into, formed by a wave.  A launch takes as many rounds of workgroups as it has tiles for the
 // places on the GPU, a tile as long as its share and about six k-blocks more (its prologue and epilogue), and each share's sums
 // are written and read once (in the time of a k-block 5 MB are): the number of shares with the least of that.  (4096 x 32000 x 2048:
@@ -884,9 +932,9 @@ static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
     p.ld = up(d, BK);
     p.rows = up(n, HD_TILE);
     p.padded = d % BK != 0 || a.ld_weight % 8 != 0 || reinterpret_cast<uintptr_t>(a.weight) % 16 != 0;
-    // Streamed: up to 32 tokens; up to 64 where the tiles would need a copy of W or W is small (64 x 50257 x 768: streamed 36.4 us, by tiles 26.7;
-    // 64 x 128256 x 4096: 330 and 249; 33 x 8000 x 512: 12.7 and 16.5; 48 x 100000 x 1000, W copied: 60 and 133; 32 x 128256 x 4096: 233
-    // and 248).
+    // Streamed: up to 32 tokens; up to 64 where the tiles would need a copy of W or W is small (64 x 50257 x 768: streamed 36.4 us, by tiles 25.0;
+    // 64 x 128256 x 4096: 330 and 249; 33 x 8000 x 512: 13.1 and 18.6; 48 x 100000 x 1000, W copied: 60 and 131; 32 x 128256 x 4096: 233
+    // and 246).
     p.few = !backward && (n <= HD_FEW / 2 || (n <= HD_FEW && (p.padded || v * d < (1 << 24))));
     p.padded = p.padded && !p.few;
     p.large = fewer_rounds(n, v);
@@ -974,11 +1022,20 @@ int raise_head_limits() {
     return rc == MUON_AMD_OK ? raise_head_limits_of<HeadSmall>() : rc;
 }
 
-// The copies that the products read; W is then (w, ld).
+// The copies that the products read; W is then (w, ld).  Forward (no coefficients) numbers the tokens too.
 static int gather(const MuonHeadLoss& a, const HeadPlan& p, char* ws, f32x4v* coef, const uint16_t** w, int64_t* ld, hipStream_t s) {
     const int64_t blocks = p.rows / 4 < 4096 ? p.rows / 4 : 4096;
-    hipLaunchKernelGGL(head_gather_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, reinterpret_cast<uint16_t*>(ws + p.hidden), static_cast<int>(p.ld), coef,
-                       reinterpret_cast<float*>(ws + p.scale), static_cast<int>(p.piece / BK), p.splits, p.dh_tile);
+    uint16_t* const rows = reinterpret_cast<uint16_t*>(ws + p.hidden);
+    if (!coef && a.tokens <= HO_FEW) {
+        hipLaunchKernelGGL(head_order_few_kernel, dim3(static_cast<unsigned>(p.rows / HO_WAVES)), dim3(HO_WAVES * 64), 0, s, a, rows, static_cast<int>(p.ld), p.rows);
+    } else {
+        if (!coef) {
+            hipLaunchKernelGGL(head_order_kernel, dim3(1), dim3(HO_THREADS), 0, s, a);
+            if (const int rc = check_launch("head_loss: order")) return rc;
+        }
+        hipLaunchKernelGGL(head_gather_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, rows, static_cast<int>(p.ld), coef,
+                           reinterpret_cast<float*>(ws + p.scale), static_cast<int>(p.piece / BK), p.splits, p.dh_tile);
+    }
     if (const int rc = check_launch("linear_cross_entropy: rows")) return rc;
     *w = static_cast<const uint16_t*>(a.weight);
     *ld = a.ld_weight;
@@ -1032,8 +1089,6 @@ int muon_amd_head_loss(const MuonHeadLoss* args, void* stream) {
         if (const int rc = check_launch("head_loss: few")) return rc;
         return join(head_join_kernel<true>);
     } else {
-        hipLaunchKernelGGL(head_order_kernel, dim3(1), dim3(HO_THREADS), 0, s, a);
-        if (const int rc = check_launch("head_loss: order")) return rc;
         HeadGemm g{};
         if (const int rc = gather(a, p, ws, nullptr, &g.Q, &g.ldq, s)) return rc;
         g.P = reinterpret_cast<const uint16_t*>(ws + p.hidden);

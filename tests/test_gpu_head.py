@@ -434,3 +434,10 @@ def test_refusals():
     for backward in (0, 1):
         assert lib.muon_amd_head_loss_workspace(ctypes.byref(_lib.HeadLossArgs(**good)), backward) > 0
         assert lib.muon_amd_head_loss_workspace(None, backward) == 0
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [1020, 1023, 1024, 1025])
+def test_around_a_thousand_tokens(tokens):
+    check(*make(tokens, 500, 72, seed=tokens, ignored=0.4))      # (between the two ways that tokens are numbered)
+    check(*make(tokens, 500, 64, seed=tokens), z=False)
