@@ -291,16 +291,30 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
 #pragma unroll
             for (int i = 0; i < 4; ++i) u[4 * q + i] = v[i];
         }
+        if (SIGMOID && !__ballot(!(lse >= 0.f && lse <= 33.f))) {
+            // One exponential serves both: no logit is too large for it, and where it loses bits for being small, so does p.
+            const float whole = exp_of(-lse), per = fmaf(-rest, whole, whole);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            p[i] = exp_of(x[i] - lse - rest);      // (zero where the token takes no part: x is -infinity)
-            if constexpr (SIGMOID) {
-                s[i] = sigmoid_of(x[i], rest_of[i]);
+            for (int i = 0; i < N; ++i) {
+                const float e = exp_of(x[i]);
+                rest_of[i] = __builtin_amdgcn_rcpf(1.f + e);
+                s[i] = e * rest_of[i];
+                p[i] = e * per;
                 norm += s[i];
                 dot = fmaf(s[i], g[i], dot);
-            } else {
-                dot = fmaf(p[i], g[i], dot);
-                if (!a.normalize) dot += u[i];     // p dw: what comes through the probabilities themselves
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                p[i] = exp_of(x[i] - lse - rest);  // (zero where the token takes no part: x is -infinity)
+                if constexpr (SIGMOID) {
+                    s[i] = sigmoid_of(x[i], rest_of[i]);
+                    norm += s[i];
+                    dot = fmaf(s[i], g[i], dot);
+                } else {
+                    dot = fmaf(p[i], g[i], dot);
+                    if (!a.normalize) dot += u[i]; // p dw: what comes through the probabilities themselves
+                }
             }
         }
         dot = group_sum<L>(dot);
