@@ -284,7 +284,12 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
         wave_order();
         float x[N], p[N], u[N], dot = 0.f;
         [[maybe_unused]] float s[SIGMOID ? N : 1], rest_of[SIGMOID ? N : 1], norm = 0.f;
-        packs.get(base, E, on, x);
+        packs.get(base, E, x);
+        const int limit = on ? E - base : 0;
+        if (__ballot(limit < N)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = i < limit ? x[i] : -__builtin_inff();
+        }
 #pragma unroll
         for (int q = 0; q < N / 4; ++q) {
             const f32x4v v = extra[sub][q * L + lane];
@@ -321,9 +326,9 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
         if constexpr (SIGMOID) {
             norm = group_sum<L>(norm);
             norm = norm != 0.f ? 1.f / norm : 0.f;
-            dot *= norm;
+            dot = dot * norm * norm;
         }
-        const float all = on ? fmaf(cz, lse, -dot) : 0.f;
+        [[maybe_unused]] const float all = on ? fmaf(cz, lse, -dot) : 0.f, zed = cz * lse;
         wave_order();
         if (a.dweights) {
             if (mine >= 0) *slot(mine) = 0.f;
@@ -339,14 +344,11 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
 #pragma unroll
             for (int i = 0; i < G; ++i) {
                 const int k = G * q + i;
-                if constexpr (SIGMOID) {
-                    const float from = s[k] * rest_of[k] * (norm * (g[k] - dot)) + u[k] * rest_of[k];
-                    d[i] = on ? fmaf(p[k], cz * lse, from) : 0.f;
-                } else {
-                    d[i] = fmaf(p[k], g[k] + all, u[k]);
-                }
+                if constexpr (SIGMOID) d[i] = fmaf(p[k], zed, rest_of[k] * fmaf(s[k], fmaf(g[k], norm, -dot), u[k]));
+                else d[i] = fmaf(p[k], g[k] + all, u[k]);
             }
-            store_pack<T, G, false>(static_cast<T*>(a.dlogits) + t * E, base + G * q, E, Pack<T, G>::of(d));
+            const Pack<T, G> v = Pack<T, G>::of(d);
+            store_pack<T, G, false>(static_cast<T*>(a.dlogits) + t * E, base + G * q, E, !SIGMOID || on ? v : Pack<T, G>::zero());
         }
     }
 }
