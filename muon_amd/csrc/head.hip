@@ -74,6 +74,7 @@ struct HeadCfg {
     static constexpr int HALF_BYTES = BT * ROW_BYTES, DPH = BT / 8 / NW, RING = (NHALF - 1) / 2;
     static constexpr size_t LDS_BYTES = static_cast<size_t>(NHALF) * HALF_BYTES;
     static_assert(WN == 64, "an epilogue's strip is 64 columns");
+    static_assert(2 * HALF_BYTES >= WGN * BT * 8, "what the statistics' epilogue leaves");
     static_assert(RING == 2 && NHALF % 2 == 1, "one copy of the k-block for each of the last two");
     static_assert(LDS_BYTES * MINB <= 163840, "LDS of a CU");
 };
@@ -987,16 +988,19 @@ static int check_head(const MuonHeadLoss* a, const char* what) {
     return MUON_AMD_OK;
 }
 
+// `most` k-blocks in a workgroup: where these are few, the ring is as long as they need, and more workgroups share a CU (their prologues and
+// epilogues are all there is; dW of 2 tokens, 32000 x 4096: 78 -> 70 us, of 20 tokens, 50257 x 768: 23.6 -> 21.0).
 template <typename Cfg, int PRODUCT>
-static int launch_product(const HeadGemm& g, hipStream_t s) {
+static int launch_product(const HeadGemm& g, int64_t most, hipStream_t s) {
     const int64_t grid = static_cast<int64_t>(g.row_tiles) * g.col_tiles * (g.most_splits > 0 ? g.most_splits : 1);
     MUON_REQUIRE(grid > 0 && grid <= 0xffffffffll / Cfg::NT, "linear_cross_entropy: %lld tiles", static_cast<long long>(grid));
-    hipLaunchKernelGGL((head_gemm_kernel<Cfg, PRODUCT>), dim3(static_cast<unsigned>(grid)), dim3(Cfg::NT), Cfg::LDS_BYTES, s, g);
+    hipLaunchKernelGGL((head_gemm_kernel<Cfg, PRODUCT>), dim3(static_cast<unsigned>(grid)), dim3(Cfg::NT),
+                       2 * most < Cfg::NHALF ? static_cast<size_t>(2 * most) * Cfg::HALF_BYTES : Cfg::LDS_BYTES, s, g);
     return check_launch("linear_cross_entropy");
 }
 template <int PRODUCT>
-static int launch_product(const HeadGemm& g, bool large, hipStream_t s) {
-    return large ? launch_product<HeadLarge, PRODUCT>(g, s) : launch_product<HeadSmall, PRODUCT>(g, s);
+static int launch_product(const HeadGemm& g, bool large, int64_t most, hipStream_t s) {
+    return large ? launch_product<HeadLarge, PRODUCT>(g, most, s) : launch_product<HeadSmall, PRODUCT>(g, most, s);
 }
 
 template <typename Cfg, int PRODUCT>
@@ -1104,7 +1108,7 @@ int muon_amd_head_loss(const MuonHeadLoss* args, void* stream) {
         g.stats = stats;
         g.ld_stats = p.rows;
         g.target_logit = logit;
-        if (const int rc = launch_product<HEAD_STATS>(g, p.large, s)) return rc;
+        if (const int rc = launch_product<HEAD_STATS>(g, p.large, g.kblocks, s)) return rc;
     }
     return join(head_join_kernel<false>);
 }
@@ -1150,7 +1154,7 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
         g.coef = coef;
         g.out = e;
         g.ld_out = p.piece;
-        if (const int rc = launch_product<HEAD_GRAD>(g, p.large, s)) return rc;
+        if (const int rc = launch_product<HEAD_GRAD>(g, p.large, g.kblocks, s)) return rc;
         if (a.dhidden) {
             HeadGemm h{};
             h.count = g.count;
@@ -1171,7 +1175,7 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
             h.add = i > 0;
             h.part_stride = p.rows * p.ld;
             h.ld_out = p.ld;
-            if (const int rc = launch_product<HEAD_DHIDDEN>(h, p.dh_tile == 256, s)) return rc;
+            if (const int rc = launch_product<HEAD_DHIDDEN>(h, p.dh_tile == 256, h.kblocks, s)) return rc;
         }
         if (a.dweight) {
             HeadGemm h{};
@@ -1191,7 +1195,7 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
             h.scale = reinterpret_cast<const float*>(ws + p.scale);
             h.out = static_cast<uint16_t*>(a.dweight) + static_cast<int64_t>(begin) * a.width;
             h.ld_out = a.width;
-            if (const int rc = launch_product<HEAD_DWEIGHT>(h, p.dw_tile == 256, s)) return rc;
+            if (const int rc = launch_product<HEAD_DWEIGHT>(h, p.dw_tile == 256, up(a.tokens, BK) / BK, s)) return rc;
         }
     }
     if (a.dhidden) {
