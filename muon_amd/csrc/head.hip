@@ -74,7 +74,7 @@ struct HeadCfg {
     static constexpr int HALF_BYTES = BT * ROW_BYTES, DPH = BT / 8 / NW, RING = (NHALF - 1) / 2;
     static constexpr size_t LDS_BYTES = static_cast<size_t>(NHALF) * HALF_BYTES;
     static_assert(WN == 64, "an epilogue's strip is 64 columns");
-    static_assert(2 * HALF_BYTES >= WGN * BT * 8, "what the statistics' epilogue leaves");
+    static_assert(2 * HALF_BYTES >= WGN * BT * 8 && 2 * HALF_BYTES >= NW * 4096, "what the epilogues leave in LDS");
     static_assert(RING == 2 && NHALF % 2 == 1, "one copy of the k-block for each of the last two");
     static_assert(LDS_BYTES * MINB <= 163840, "LDS of a CU");
 };
@@ -428,6 +428,9 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const Hea
                 }
         }
     } else {
+        // 32 rows at a time go through LDS, so that a store's lanes take 128 bytes of each of 8 rows (a piece of a row at another place in each
+        // of 8 rows: other banks).  (dW of 2 tokens, 32000 x 4096: 70 -> 58 us; of 500 tokens, 50257 x 1024: 78 -> 71.)
+        u32x4* const strip = reinterpret_cast<u32x4*>(lds) + wave * 256;
         const float scale = PRODUCT == HEAD_DWEIGHT ? *a.scale : 1.f;
 #pragma unroll
         for (int x = 0; x < TM; ++x) {
@@ -467,11 +470,17 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const Hea
                 for (int q = 0; q < 4; q += 2) {
                     const auto u = __builtin_amdgcn_permlane32_swap(po[2 * q], po[2 * q + 2], false, false);
                     const auto w = __builtin_amdgcn_permlane32_swap(po[2 * q + 1], po[2 * q + 3], false, false);
-                    const Pack<uint16_t, 8> v = {{u[0], w[0], u[1], w[1]}};
-                    const int col = col0 + y * 32 + (q + g) * 8;
-                    if (PRODUCT == HEAD_GRAD || row < rows) store_pack<uint16_t, 8, false>(a.out + row * a.ld_out, col, a.cols, v);
+                    strip[lr * 8 + ((y * 4 + q + g) ^ (lr & 7))] = u32x4{u[0], w[0], u[1], w[1]};
                 }
             }
+            wave_order();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = i * 8 + lane_e / 8, to = row0 + x * 32 + at;
+                const u32x4 v = strip[at * 8 + ((lane_e & 7) ^ (at & 7))];
+                if (PRODUCT == HEAD_GRAD || to < rows) store_pack<uint16_t, 8, false>(a.out + to * a.ld_out, col0 + (lane_e & 7) * 8, a.cols, Pack<uint16_t, 8>{v});
+            }
+            wave_order();
         }
     }
 }

@@ -60,6 +60,12 @@ __device__ __forceinline__ float group_sum(float v) {
     return group_reduce<L>(v, [](float a, float b) { return a + b; });
 }
 
+// What lanes of a wave left in LDS is there for its other lanes (whose accesses are in order), for the compiler too.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // e^d for d at most 0: 2^(d log2 e) by the target's instruction, with what the product lost put back, so
 // about two units off over the whole range.  Not a number gives zero like -infinity: what a row with such a logit, or with
 // +infinity, returns then follows from its sum of zero (1 / 0 times 0) or from its lse, neither of which is a number.

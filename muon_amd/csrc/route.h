@@ -79,12 +79,6 @@ struct RowPacks {
     }
 };
 
-// What lanes of a wave left in LDS is there for its other lanes (whose accesses are in order), for the compiler too.
-__device__ __forceinline__ void wave_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // Joins what `groups` workgroups of a forward launch left (route.hip).
 int launch_route_join(const MuonRoute& a, int groups, hipStream_t stream);
 
