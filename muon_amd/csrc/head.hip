@@ -488,37 +488,43 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const Hea
 // ---------------------------------------------------------------------------------------------
 // Few tokens: W streamed through registers
 // ---------------------------------------------------------------------------------------------
-// A workgroup takes 64 rows of W, its four waves every fourth block of 64 channels: fragments of 16 rows x 32 channels straight from
-// memory (a 128-byte line of a row is two of them), against those of up to 64 tokens, which the caches hold.  The waves'
-// sums are added in LDS.  W's bytes bound it.
+// A workgroup takes 64 rows of W, its four waves every fourth block of 64 channels, against up to 64 tokens, which the caches hold.  A wave's loads
+// take whole lines of 128 bytes of 8 rows each, a block ahead; through LDS (of its own, so there is nothing to wait for) they become the
+// fragments of 16 rows x 32 channels.  Workgroups begin at different blocks, as rows that lie a power of two apart would otherwise all be read from
+// the same memory channels at a time.  The waves' sums are added in LDS.  W's bytes bound it (128256 x 4096 not in a cache, one token: 207 -> 186 us
+// against fragments straight from memory, every workgroup from the first block on; 32 tokens: 233 -> 184; 32000 x 2048, one token: 33.4 -> 31.0); beyond
+// 32 tokens so do the hidden states' fragments, as many bytes again from the L2 (64 tokens: 214).
 constexpr int HF_THREADS = 256, HF_VOCAB = 64;
 typedef float f32x4a __attribute__((ext_vector_type(4)));
 template <bool TAIL>
-__device__ __forceinline__ bf16x8 few_chunk(const uint16_t* row, int k, int width) {
-    if constexpr (!TAIL) return __builtin_bit_cast(bf16x8, Pack<uint16_t, 8>::load<false>(row + k).v);
-    else return __builtin_bit_cast(bf16x8, load_pack<uint16_t, 8, false>(row, k, width).v);
+__device__ __forceinline__ u32x4 few_chunk(const uint16_t* row, int k, int width) {
+    if constexpr (!TAIL) return Pack<uint16_t, 8>::load<false>(row + k).v;
+    else return load_pack<uint16_t, 8, false>(row, k, width).v;
 }
 template <int NT>
-__global__ __launch_bounds__(HF_THREADS, NT == 4 ? 4 : 1) void head_few_kernel(const uint16_t* hidden, int64_t ld_hidden, const uint16_t* weight, int64_t ld_weight, int tokens,
+__global__ __launch_bounds__(HF_THREADS, NT == 4 ? 2 : NT == 2 ? 3 : 4) void head_few_kernel(const uint16_t* hidden, int64_t ld_hidden, const uint16_t* weight, int64_t ld_weight, int tokens,
                                                               int width, int vocab, const void* targets, int target_bits, f32x2_t* stats, int64_t ld_stats,
                                                               float* target_logit, int32_t* counter) {
-    typedef uint32_t words __attribute__((ext_vector_type(4)));
     // a row's columns exchanged by its number, four at a time: the lanes of a token's 16 then write to different banks
     constexpr int WAVES = NT == 4 ? 2 : 4;       // whose sums lie in LDS at once (what four of them take for 64 tokens would leave two workgroups a CU)
-    __shared__ __align__(16) float sums[WAVES][16 * NT][HF_VOCAB];
+    constexpr int TILE = HF_VOCAB * 8;           // 16-byte pieces of a wave's block
+    typedef float Sums[16 * NT][HF_VOCAB];
+    __shared__ u32x4 pieces[4 * TILE];           // the waves' blocks, then their sums
+    static_assert(sizeof(pieces) >= WAVES * sizeof(Sums), "the waves' sums");
+    Sums* const sums = reinterpret_cast<Sums*>(pieces);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kq = (lane >> 4) * 8;
     const int v0 = blockIdx.x * HF_VOCAB;
-    const uint16_t* wrow[4];
+    const uint16_t* wrow[8];
     const uint16_t* hrow[NT];
 #pragma unroll
-    for (int f = 0; f < 4; ++f) wrow[f] = weight + min(v0 + 16 * f + r, vocab - 1) * ld_weight;
+    for (int i = 0; i < 8; ++i) wrow[i] = weight + min(v0 + 8 * i + (lane >> 3), vocab - 1) * ld_weight + (lane & 7) * 8;
 #pragma unroll
-    for (int f = 0; f < NT; ++f) hrow[f] = hidden + min(16 * f + r, tokens - 1) * ld_hidden;
+    for (int f = 0; f < NT; ++f) hrow[f] = hidden + min(16 * f + r, tokens - 1) * ld_hidden + kq;
     if (blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;       // (of the launch that joins)
-    // each lane's token's target, where it is a row of W (requested before the rows: a load for each token at the end took a third of the time)
+    // the target of the token that the thread has in the end, where it is a row of W (requested before the rows: at the end it is waited for)
     int target = -1;
-    if (lane < tokens) {
-        const int64_t at = target_bits == 64 ? static_cast<const int64_t*>(targets)[lane] : static_cast<const int32_t*>(targets)[lane];
+    if (const int t = threadIdx.x / (HF_THREADS / (16 * NT)); t < tokens) {
+        const int64_t at = target_bits == 64 ? static_cast<const int64_t*>(targets)[t] : static_cast<const int32_t*>(targets)[t];
         if (at >= 0 && at < vocab) target = static_cast<int>(at);
     }
     f32x4a acc[4][NT];
@@ -526,35 +532,53 @@ __global__ __launch_bounds__(HF_THREADS, NT == 4 ? 4 : 1) void head_few_kernel(c
     for (int f = 0; f < 4; ++f)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[f][t] = f32x4a{0.f, 0.f, 0.f, 0.f};
-    // S steps of 32 channels at a time: as many loads as the registers leave in flight
-    constexpr int S = NT == 4 ? 1 : 2;
-    const auto steps = [&](auto tail, int k) __attribute__((always_inline)) {
+    u32x4 next[8], next_h[2][NT];
+    const auto fetch = [&](auto tail, int k) __attribute__((always_inline)) {
         constexpr bool TAIL = decltype(tail)::value;
-        bf16x8 w[S][4], h[S][NT];
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
+        for (int i = 0; i < 8; ++i) next[i] = few_chunk<TAIL>(wrow[i], k, width - (lane & 7) * 8);
 #pragma unroll
-            for (int f = 0; f < 4; ++f) w[s][f] = few_chunk<TAIL>(wrow[f], k + 32 * s + kq, width);
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) h[s][t] = few_chunk<TAIL>(hrow[t], k + 32 * s + kq, width);
-        }
-#pragma unroll
-        for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int f = 0; f < 4; ++f)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) acc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[s][f], h[s][t], acc[f][t], 0, 0, 0);
+            for (int t = 0; t < NT; ++t) next_h[s][t] = few_chunk<TAIL>(hrow[t], k + 32 * s, width - kq);
     };
-    const int whole = width / 64;
-    if constexpr (S == 2) {
-#pragma unroll 2
-        for (int b = wave; b < whole; b += 4) steps(std::false_type{}, b * 64);
-    } else {
+    // (piece c of row v lies at c ^ (v / 2 % 8) of the row's eight: sixteen rows next to each other are on all banks)
+    u32x4* const tile = pieces + wave * TILE;
+    const int to = (lane >> 3) * 8 + ((lane & 7) ^ (lane >> 4)), from = r * 8 + ((lane >> 4) ^ (r >> 1));
+    const auto multiply = [&](auto more, int k) __attribute__((always_inline)) {
+        u32x4 h[2][NT];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) tile[64 * i + (to ^ (i & 1) * 4)] = next[i];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) h[s][t] = next_h[s][t];
+        if constexpr (decltype(more)::value) fetch(std::false_type{}, k);
+        wave_order();
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                const bf16x8 w = __builtin_bit_cast(bf16x8, tile[128 * f + (from ^ s * 4)]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, __builtin_bit_cast(bf16x8, h[s][t]), acc[f][t], 0, 0, 0);
+            }
+        wave_order();
+    };
+    const int whole = width / 64, turn = whole > 0 ? blockIdx.x % whole : 0;
+    const auto block = [&](int b) { return (b + turn < whole ? b + turn : b + turn - whole) * 64; };
+    if (wave < whole) {
+        fetch(std::false_type{}, block(wave));
+        int b = wave;
 #pragma unroll 1
-        for (int i = 2 * wave; i < 2 * whole; i += i % 2 ? 7 : 1) steps(std::false_type{}, i * 32);
+        for (; b + 4 < whole; b += 4) multiply(std::true_type{}, block(b + 4));
+        multiply(std::false_type{}, 0);
     }
-    if (width % 64 && wave == whole % 4)
-        for (int k = whole * 64; k < width; k += 32 * S) steps(std::true_type{}, k);
+    if (width % 64 && wave == whole % 4) {
+        fetch(std::true_type{}, whole * 64);
+        multiply(std::false_type{}, 0);
+    }
+    __syncthreads();                             // every wave is done with its block
     // a lane holds rows 4 (lane / 16) .. + 3 of W for token lane % 16
     const auto slot = [&](int f, int t) { return reinterpret_cast<f32x4a*>(&sums[wave % WAVES][16 * t + r][(16 * f + 4 * (lane >> 4)) ^ (r << 2)]); };
     if (wave >= 4 - WAVES) {
@@ -571,17 +595,28 @@ __global__ __launch_bounds__(HF_THREADS, NT == 4 ? 4 : 1) void head_few_kernel(c
             for (int t = 0; t < NT; ++t) *slot(f, t) += acc[f][t];
     }
     __syncthreads();
-    for (int t = wave; t < tokens; t += 4) {
-        const int v = v0 + lane;
-        const int at = lane ^ ((t & 15) << 2);
-        float x = sums[0][t][at] + sums[1][t][at];
-        if constexpr (WAVES == 4) x += sums[2][t][at] + sums[3][t][at];
-        if (v >= vocab) x = -__builtin_inff();
-        if (v == __builtin_amdgcn_readlane(target, t)) target_logit[t] = x;
-        const float m = group_reduce<64>(x, [](float p, float q) { return fmaxf(p, q); });
-        const float s = group_sum<64>(__builtin_amdgcn_exp2f((x - (m == -__builtin_inff() ? 0.f : m)) * LOG2E));
-        if (lane == 0) stats[blockIdx.x * ld_stats + t] = f32x2_t{m, s};
+    // as many threads to each token as there are: maximum and sum of the token's columns here, and its target where that is one of them
+    constexpr int P = HF_THREADS / (16 * NT), C = HF_VOCAB / P;
+    const int t = threadIdx.x / P, part = threadIdx.x % P, turned = (t & 15) << 2;
+    float x[C], m = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < C / 4; ++j) {
+        const int col = part * C + 4 * j;
+        f32x4a v = *reinterpret_cast<const f32x4a*>(&sums[0][t][col ^ turned]) + *reinterpret_cast<const f32x4a*>(&sums[1][t][col ^ turned]);
+        if constexpr (WAVES == 4) v += *reinterpret_cast<const f32x4a*>(&sums[2][t][col ^ turned]) + *reinterpret_cast<const f32x4a*>(&sums[3][t][col ^ turned]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[4 * j + i] = v0 + col + i < vocab ? v[i] : -__builtin_inff();
+            m = fmaxf(m, x[4 * j + i]);
+            if (target == v0 + col + i) target_logit[t] = v[i];
+        }
     }
+    m = group_reduce<P>(m, [](float u, float v) { return fmaxf(u, v); });
+    const float ref = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < C; ++i) sum += __builtin_amdgcn_exp2f((x[i] - ref) * LOG2E);
+    sum = group_sum<P>(sum);
+    if (part == 0 && t < tokens) stats[blockIdx.x * ld_stats + t] = f32x2_t{m, sum};
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -942,10 +977,10 @@ static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
     p.ld = up(d, BK);
     p.rows = up(n, HD_TILE);
     p.padded = d % BK != 0 || a.ld_weight % 8 != 0 || reinterpret_cast<uintptr_t>(a.weight) % 16 != 0;
-    // Streamed: up to 32 tokens; up to 64 where the tiles would need a copy of W or W is small (64 x 50257 x 768: streamed 36.4 us, by tiles 25.0;
-    // 64 x 128256 x 4096: 330 and 249; 33 x 8000 x 512: 13.1 and 18.6; 48 x 100000 x 1000, W copied: 60 and 131; 32 x 128256 x 4096: 233
-    // and 246).
-    p.few = !backward && (n <= HD_FEW / 2 || (n <= HD_FEW && (p.padded || v * d < (1 << 24))));
+    // Streamed: up to 32 tokens (32 x 128256 x 4096: streamed 184 us, by tiles 244); up to 64 where the tiles would need a copy of W, or W is small, or its
+    // rows are long (64 x 32000 x 2048: 37 and 48; 64 x 20000 x 1024: 22 and 28; 64 x 50257 x 768, W in the last cache: 26.7 and 24.3; 64 x 8000 x
+    // 512: 15.2 and 18.4; 48 x 100000 x 1000, W copied: 74 and 132).
+    p.few = !backward && (n <= HD_FEW / 2 || (n <= HD_FEW && (p.padded || d >= 1024 || v * d < (1 << 24))));
     p.padded = p.padded && !p.few;
     p.large = fewer_rounds(n, v);
     p.tile = p.few ? HF_VOCAB : p.large ? 256 : 128;

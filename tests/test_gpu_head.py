@@ -441,3 +441,10 @@ def test_refusals():
 def test_around_a_thousand_tokens(tokens):
     check(*make(tokens, 500, 72, seed=tokens, ignored=0.4))      # (between the two ways that tokens are numbered)
     check(*make(tokens, 500, 64, seed=tokens), z=False)
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [1, 16, 17, 32, 33, 48, 64])
+@pytest.mark.parametrize("vocab,width", [(1, 64), (65, 1216), (200, 1990), (640, 4160), (7, 130)])
+def test_streamed_matrices(tokens, vocab, width):
+    check(*make(tokens, vocab, width, seed=tokens + vocab, ignored=0.3))         # (blocks of 64 channels: one, numbers that are no multiple of the waves', part of one)
