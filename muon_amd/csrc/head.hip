@@ -6,7 +6,7 @@
 //
 // Forward is one matrix product whose epilogue leaves the maximum and the sum of exponentials of each row of its tile, 8 bytes for
 // 256 logits, joined by a second launch.  Backward goes through the vocabulary in pieces: the logits of a piece are formed again
-// (the same product, so the same bits), e is written once in bf16 (rounding each term of sums over the
+// (the same product; the same bits too, but where few tokens were streamed forward), e is written once in bf16 (rounding each term of sums over the
 // vocabulary or the tokens by at most 2^-8 of itself, as the sums are rounded when they are written), and two products follow, whose second operand (and for
 // dW the first one too) lies k-major and is read through transposing LDS reads, so nothing is written twice.  8 N V D operations
 // instead of the 6 N V D of a backward pass that keeps N V logits.  8192 x 128256 x 4096: 6.6 ms forward, 6.9 + 6.8 + 7.4 ms backward (1235 to 1310
@@ -132,11 +132,13 @@ __device__ __forceinline__ void wait_both(A& a, B& b) {
 }
 
 // An operand's half-stages: where a lane's pieces lie from the tile's base, and how the base moves from k-block to k-block.
-template <typename Cfg, bool K>
+// TURN: the k-blocks are taken from number `turn` on, and from the first one after the last of `blocks`.
+template <typename Cfg, bool K, bool TURN>
 struct Source {
     uint32_t off[Cfg::DPH];
     uint64_t base;                 // (wave-uniform)
     int64_t step, end;
+    int turn, blocks;
     // first: the tile's first row (k-major: column); limit: columns of a k-major row that may be read
     __device__ __forceinline__ void set(const uint16_t* p, int64_t ld, int64_t end_bytes, int first, int limit, int k0, int lane, int wave) {
         constexpr int ROWK = Cfg::BT * 2;
@@ -159,6 +161,7 @@ struct Source {
     }
     // Piece j of k-block kb.
     __device__ __forceinline__ void issue(int j, int kb, uint32_t lds_addr) const {
+        if constexpr (TURN) kb = kb + turn < blocks ? kb + turn : kb + turn - blocks;
         const int64_t moved = kb * step, left = end - moved;
         const uint64_t b = base + moved;
         const u32x4 rsrc = {static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
@@ -167,7 +170,10 @@ struct Source {
     }
 };
 
-template <typename Cfg, int PRODUCT>
+// TURN: for one row of tiles.  W is then read once, and its rows may lie a power of two apart: workgroups begin at different k-blocks, so
+// that they read from different memory channels (128 x 128256 x 4096 forward, not in a cache: 250 -> 205 us, both passes 1199 -> 1110; with more rows of tiles those
+// that are worked on together share what they read).
+template <typename Cfg, int PRODUCT, bool TURN>
 __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const HeadGemm a) {
     constexpr int NW = Cfg::NW, WGN = Cfg::WGN, WM = Cfg::WM, WN = Cfg::WN, TM = Cfg::TM, TN = Cfg::TN, NHALF = Cfg::NHALF;
     constexpr int HALF_BYTES = Cfg::HALF_BYTES, DPH = Cfg::DPH, RING = Cfg::RING, ROWK = Cfg::BT * 2;
@@ -203,10 +209,14 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::MINB) void head_gemm_kernel(const Hea
             for (int i = 0; i < 16; ++i) acc[x][y][i] = 0.f;
 
     if (nk > 0) {
-        Source<Cfg, PK> sp_;
-        Source<Cfg, QK> sq_;
+        Source<Cfg, PK, TURN> sp_;
+        Source<Cfg, QK, TURN> sq_;
         sp_.set(a.P, a.ldp, a.end_p, i0, a.row_limit, k0 * BK, lane, wave);
         sq_.set(a.Q, a.ldq, a.end_q, j0, a.col_limit, k0 * BK, lane, wave);
+        if constexpr (TURN) {
+            sp_.turn = sq_.turn = (a.vocab_begin / Cfg::BT + tile.col) % nk;
+            sp_.blocks = sq_.blocks = nk;
+        }
         const uint32_t dst0 = lds_base + wave * 1024;
 #pragma unroll
         for (int h = 0; h < NHALF; ++h)
@@ -1034,22 +1044,28 @@ static int check_head(const MuonHeadLoss* a, const char* what) {
 
 // `most` k-blocks in a workgroup: where these are few, the ring is as long as they need, and more workgroups share a CU (their prologues and
 // epilogues are all there is; dW of 2 tokens, 32000 x 4096: 78 -> 70 us, of 20 tokens, 50257 x 768: 23.6 -> 21.0).
-template <typename Cfg, int PRODUCT>
+template <typename Cfg, int PRODUCT, bool TURN>
 static int launch_product(const HeadGemm& g, int64_t most, hipStream_t s) {
     const int64_t grid = static_cast<int64_t>(g.row_tiles) * g.col_tiles * (g.most_splits > 0 ? g.most_splits : 1);
     MUON_REQUIRE(grid > 0 && grid <= 0xffffffffll / Cfg::NT, "linear_cross_entropy: %lld tiles", static_cast<long long>(grid));
-    hipLaunchKernelGGL((head_gemm_kernel<Cfg, PRODUCT>), dim3(static_cast<unsigned>(grid)), dim3(Cfg::NT),
+    hipLaunchKernelGGL((head_gemm_kernel<Cfg, PRODUCT, TURN>), dim3(static_cast<unsigned>(grid)), dim3(Cfg::NT),
                        2 * most < Cfg::NHALF ? static_cast<size_t>(2 * most) * Cfg::HALF_BYTES : Cfg::LDS_BYTES, s, g);
     return check_launch("linear_cross_entropy");
 }
+template <typename Cfg, int PRODUCT>
+static int launch_product(const HeadGemm& g, int64_t tokens, int64_t most, hipStream_t s) {
+    if constexpr (PRODUCT == HEAD_STATS || PRODUCT == HEAD_GRAD)
+        if (tokens <= Cfg::BT) return launch_product<Cfg, PRODUCT, true>(g, most, s);
+    return launch_product<Cfg, PRODUCT, false>(g, most, s);
+}
 template <int PRODUCT>
-static int launch_product(const HeadGemm& g, bool large, int64_t most, hipStream_t s) {
-    return large ? launch_product<HeadLarge, PRODUCT>(g, most, s) : launch_product<HeadSmall, PRODUCT>(g, most, s);
+static int launch_product(const HeadGemm& g, bool large, int64_t tokens, int64_t most, hipStream_t s) {
+    return large ? launch_product<HeadLarge, PRODUCT>(g, tokens, most, s) : launch_product<HeadSmall, PRODUCT>(g, tokens, most, s);
 }
 
-template <typename Cfg, int PRODUCT>
+template <typename Cfg, int PRODUCT, bool TURN = false>
 static int raise_head_limit() {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(head_gemm_kernel<Cfg, PRODUCT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(head_gemm_kernel<Cfg, PRODUCT, TURN>), hipFuncAttributeMaxDynamicSharedMemorySize,
                             static_cast<int>(Cfg::LDS_BYTES)) != hipSuccess) {
         (void)hipGetLastError();
         set_error("linear_cross_entropy: cannot raise dynamic LDS to %zu bytes", Cfg::LDS_BYTES);
@@ -1063,6 +1079,8 @@ static int raise_head_limits_of() {
     if (rc == MUON_AMD_OK) rc = raise_head_limit<Cfg, HEAD_GRAD>();
     if (rc == MUON_AMD_OK) rc = raise_head_limit<Cfg, HEAD_DHIDDEN>();
     if (rc == MUON_AMD_OK) rc = raise_head_limit<Cfg, HEAD_DWEIGHT>();
+    if (rc == MUON_AMD_OK) rc = raise_head_limit<Cfg, HEAD_STATS, true>();
+    if (rc == MUON_AMD_OK) rc = raise_head_limit<Cfg, HEAD_GRAD, true>();
     return rc;
 }
 int raise_head_limits() {
@@ -1152,7 +1170,7 @@ int muon_amd_head_loss(const MuonHeadLoss* args, void* stream) {
         g.stats = stats;
         g.ld_stats = p.rows;
         g.target_logit = logit;
-        if (const int rc = launch_product<HEAD_STATS>(g, p.large, g.kblocks, s)) return rc;
+        if (const int rc = launch_product<HEAD_STATS>(g, p.large, a.tokens, g.kblocks, s)) return rc;
     }
     return join(head_join_kernel<false>);
 }
@@ -1198,7 +1216,7 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
         g.coef = coef;
         g.out = e;
         g.ld_out = p.piece;
-        if (const int rc = launch_product<HEAD_GRAD>(g, p.large, g.kblocks, s)) return rc;
+        if (const int rc = launch_product<HEAD_GRAD>(g, p.large, a.tokens, g.kblocks, s)) return rc;
         if (a.dhidden) {
             HeadGemm h{};
             h.count = g.count;
@@ -1219,7 +1237,7 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
             h.add = i > 0;
             h.part_stride = p.rows * p.ld;
             h.ld_out = p.ld;
-            if (const int rc = launch_product<HEAD_DHIDDEN>(h, p.dh_tile == 256, h.kblocks, s)) return rc;
+            if (const int rc = launch_product<HEAD_DHIDDEN>(h, p.dh_tile == 256, a.tokens, h.kblocks, s)) return rc;
         }
         if (a.dweight) {
             HeadGemm h{};
@@ -1239,7 +1257,7 @@ int muon_amd_head_loss_backward(const MuonHeadLoss* args, void* stream) {
             h.scale = reinterpret_cast<const float*>(ws + p.scale);
             h.out = static_cast<uint16_t*>(a.dweight) + static_cast<int64_t>(begin) * a.width;
             h.ld_out = a.width;
-            if (const int rc = launch_product<HEAD_DWEIGHT>(h, p.dw_tile == 256, up(a.tokens, BK) / BK, s)) return rc;
+            if (const int rc = launch_product<HEAD_DWEIGHT>(h, p.dw_tile == 256, a.tokens, up(a.tokens, BK) / BK, s)) return rc;
         }
     }
     if (a.dhidden) {
