@@ -286,7 +286,7 @@ std::optional<std::tuple<Tensor, Tensor>> residual_norm(const Tensor& x, const T
 
 // ---- route_topk ------------------------------------------------------------------------------------------------
 struct RouteOut {
-    Tensor weights, indices, counts, balance, z, part, lse;
+    Tensor weights, indices, counts, balance, z, lse;
 };
 
 MuonRoute route_args(const Tensor& logits, const Tensor& mask, const RouteOut& o, bool normalize, std::vector<Tensor>& keep) {
@@ -305,9 +305,9 @@ MuonRoute route_args(const Tensor& logits, const Tensor& mask, const RouteOut& o
     a.weights = o.weights.data_ptr<float>();
     a.indices = o.indices.data_ptr<int32_t>();
     a.counts = o.counts.data_ptr<int32_t>();
-    a.part = o.part.data_ptr<float>();
     a.lse = o.lse.data_ptr<float>();
     a.lse_rest = a.lse + a.tokens;
+    a.part = a.lse_rest + a.tokens;
     a.k = static_cast<int32_t>(o.weights.size(-1));
     a.normalize = normalize;
     return a;
@@ -338,8 +338,7 @@ RouteOut route_forward(const Tensor& logits, int64_t k, const Tensor& mask, bool
     o.counts = at::empty({experts}, i32);
     o.balance = at::empty({}, f32);
     o.z = at::empty({}, f32);
-    o.part = at::empty({}, f32);
-    o.lse = at::empty({2, tokens}, f32);              // and what rounding it left out
+    o.lse = at::empty({2 * tokens + 1}, f32);         // and what rounding it left out, and the tokens that take part
     const Tensor partials = at::empty({api.route_partials(tokens, static_cast<int>(experts))}, f32);
     std::vector<Tensor> keep;
     keep.reserve(2);
@@ -367,14 +366,14 @@ struct RouteTopk : torch::autograd::Function<RouteTopk> {
         ctx->set_materialize_grads(false);
         ctx->saved_data["scores"] = by.scores;
         ctx->saved_data["normalize"] = normalize;
-        ctx->save_for_backward({logits, m, o.weights, o.indices, o.counts, o.part, o.lse});
+        ctx->save_for_backward({logits, m, o.weights, o.indices, o.counts, o.lse});
         ctx->mark_non_differentiable({o.indices, o.counts});
         return {o.weights, o.indices, o.counts, o.balance, o.z};
     }
     static variable_list backward(AutogradContext* ctx, variable_list douts) {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor& logits = saved[0];
-        const RouteOut o{saved[2], saved[3], saved[4], Tensor(), Tensor(), saved[5], saved[6]};
+        const RouteOut o{saved[2], saved[3], saved[4], Tensor(), Tensor(), saved[5]};
         Tensor dlogits = at::empty(logits.sizes(), logits.options());
         if (o.lse.defined()) {
             std::vector<Tensor> keep;
@@ -429,7 +428,7 @@ int bits_of(const Tensor& t) { return t.scalar_type() == at::kLong ? 64 : 32; }
 
 // ---- linear_cross_entropy ----------------------------------------------------------------------------------------
 struct HeadTensors {
-    Tensor hidden, weight, targets, part, order, rows, stats;
+    Tensor hidden, weight, targets, kept;       // the last one: order, rows, stats, part and counter (4 tokens + 3 words)
 };
 constexpr int64_t HEAD_MAX_DISTANCE = int64_t(1) << 21;          // between rows of the matrix
 
@@ -447,11 +446,12 @@ MuonHeadLoss head_args(const HeadTensors& t, int64_t reduction, int64_t ignore_i
     a.hidden = h.data_ptr();
     a.weight = w.data_ptr();
     a.targets = hold(t.targets.contiguous()).data_ptr();
-    a.part = t.part.data_ptr<float>();
-    a.order = t.order.data_ptr<int32_t>();
-    a.rows = t.rows.data_ptr<int32_t>();
-    a.stats = t.stats.data_ptr<float>();
     a.tokens = h.size(0);
+    a.order = t.kept.data_ptr<int32_t>();
+    a.rows = a.order + a.tokens + 1;
+    a.stats = reinterpret_cast<float*>(a.rows + a.tokens);
+    a.part = a.stats + 2 * a.tokens;
+    a.counter = reinterpret_cast<int32_t*>(a.part + 1);
     a.ld_hidden = h.stride(0);
     a.ld_weight = w.stride(0);
     a.ignore_index = ignore_index;
@@ -470,22 +470,18 @@ Tensor head_workspace(MuonHeadLoss& a, bool backward, const Tensor& like) {
 
 // (loss, lse); `t` gets what backward needs.
 std::tuple<Tensor, Tensor> head_forward(HeadTensors& t, int64_t reduction, int64_t ignore_index) {
-    const auto f32 = t.hidden.options().dtype(at::kFloat), i32 = t.hidden.options().dtype(at::kInt);
+    const auto f32 = t.hidden.options().dtype(at::kFloat);
     const auto shape = t.targets.sizes();
     const int64_t tokens = t.targets.numel();
     Tensor lse = at::empty(shape, f32);
     if (tokens == 0) return {reduction ? at::zeros({}, f32) : at::zeros(shape, f32), lse};
-    const Tensor losses = at::empty(shape, f32), loss = reduction ? at::empty({}, f32) : Tensor(), counter = at::empty({}, i32);
-    t.part = at::empty({}, f32);
-    t.order = at::empty({tokens + 1}, i32);
-    t.rows = at::empty({tokens}, i32);
-    t.stats = at::empty({tokens, 2}, f32);
+    const Tensor losses = at::empty(shape, f32), loss = reduction ? at::empty({}, f32) : Tensor();
+    t.kept = at::empty({4 * tokens + 3}, t.hidden.options().dtype(at::kInt));
     std::vector<Tensor> keep;
     MuonHeadLoss a = head_args(t, reduction, ignore_index, keep);
     a.losses = losses.data_ptr<float>();
     a.lse = lse.data_ptr<float>();
     a.loss = reduction ? loss.data_ptr<float>() : nullptr;
-    a.counter = counter.data_ptr<int32_t>();
     const Tensor ws = head_workspace(a, false, t.hidden);
     const c10::DeviceGuard guard(t.hidden.device());
     check(api.head_loss(&a, current_stream(t.hidden.device())), "linear_cross_entropy");
@@ -495,18 +491,18 @@ std::tuple<Tensor, Tensor> head_forward(HeadTensors& t, int64_t reduction, int64
 struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t reduction,
                                  int64_t ignore_index) {
-        HeadTensors t{hidden, weight, targets, Tensor(), Tensor(), Tensor(), Tensor()};
+        HeadTensors t{hidden, weight, targets, Tensor()};
         auto [loss, lse] = head_forward(t, reduction, ignore_index);
         ctx->set_materialize_grads(false);
         ctx->saved_data["reduction"] = reduction;
         ctx->saved_data["ignore_index"] = ignore_index;
-        ctx->save_for_backward({t.hidden, t.weight, t.targets, t.part, t.order, t.rows, t.stats});
+        ctx->save_for_backward({t.hidden, t.weight, t.targets, t.kept});
         return {loss, lse};
     }
     static variable_list backward(AutogradContext* ctx, variable_list douts) {
         const variable_list saved = ctx->get_saved_variables();
-        const HeadTensors t{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], saved[6]};
-        const bool nothing = !t.order.defined() || (!douts[0].defined() && !douts[1].defined());
+        const HeadTensors t{saved[0], saved[1], saved[2], saved[3]};
+        const bool nothing = !t.kept.defined() || (!douts[0].defined() && !douts[1].defined());
         const auto gradient = [&](size_t edge, const Tensor& of) {
             if (!ctx->needs_input_grad(edge)) return Tensor();
             return nothing ? at::zeros(of.sizes(), of.options()) : at::empty(of.sizes(), of.options());
@@ -552,13 +548,13 @@ std::optional<std::tuple<Tensor, Tensor>> linear_cross_entropy(const Tensor& hid
         const variable_list out = LinearCrossEntropy::apply(hidden, weight, targets, reduction, ignore_index);
         return std::make_tuple(out[0], out[1]);
     }
-    HeadTensors t{hidden, weight, targets, Tensor(), Tensor(), Tensor(), Tensor()};
+    HeadTensors t{hidden, weight, targets, Tensor()};
     return head_forward(t, reduction, ignore_index);
 }
 
 // ---- distill_topk ------------------------------------------------------------------------------------------------
 struct DistillTensors {
-    Tensor logits, teacher, indices, mask, part, stats;         // (the mask may be undefined)
+    Tensor logits, teacher, indices, mask, stats;               // (the mask may be undefined; behind the statistics lie the tokens that take part)
 };
 MuonDistill distill_args(const DistillTensors& t, int64_t reduction, double temperature, std::vector<Tensor>& keep) {
     const auto hold = [&](Tensor r) -> const Tensor& {
@@ -574,9 +570,9 @@ MuonDistill distill_args(const DistillTensors& t, int64_t reduction, double temp
     a.teacher = v.data_ptr();
     a.indices = i.data_ptr();
     a.mask = t.mask.defined() ? static_cast<const uint8_t*>(hold(t.mask.contiguous()).data_ptr()) : nullptr;
-    a.part = t.part.data_ptr<float>();
-    a.stats = t.stats.data_ptr<float>();
     a.tokens = x.size(0);
+    a.stats = t.stats.data_ptr<float>();
+    a.part = a.stats + 4 * a.tokens;
     a.ld_logits = x.stride(0);
     a.ld_teacher = v.stride(0);
     a.ld_indices = i.stride(0);
@@ -597,8 +593,7 @@ Tensor distill_forward(DistillTensors& t, int64_t reduction, double temperature)
     const int64_t vocab = t.logits.size(-1), tokens = t.logits.numel() / vocab;
     if (tokens == 0) return reduction ? at::zeros({}, f32) : at::zeros(shape, f32);
     Tensor losses = at::empty(shape, f32), loss = reduction ? at::empty({}, f32) : Tensor();
-    t.part = at::empty({}, f32);
-    t.stats = at::empty({tokens, 4}, f32);
+    t.stats = at::empty({4 * tokens + 1}, f32);
     const Tensor partials = at::empty({api.distill_partials(tokens, static_cast<int>(vocab), dtype_of(t.logits)) + 1}, f32);
     std::vector<Tensor> keep;
     MuonDistill a = distill_args(t, reduction, temperature, keep);
@@ -614,16 +609,16 @@ Tensor distill_forward(DistillTensors& t, int64_t reduction, double temperature)
 struct DistillTopk : torch::autograd::Function<DistillTopk> {
     static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& indices, const std::optional<Tensor>& mask,
                           int64_t reduction, double temperature) {
-        DistillTensors t{logits, teacher, indices, mask.value_or(Tensor()), Tensor(), Tensor()};
+        DistillTensors t{logits, teacher, indices, mask.value_or(Tensor()), Tensor()};
         const Tensor loss = distill_forward(t, reduction, temperature);
         ctx->saved_data["reduction"] = reduction;
         ctx->saved_data["temperature"] = temperature;
-        ctx->save_for_backward({t.logits, t.teacher, t.indices, t.mask, t.part, t.stats});
+        ctx->save_for_backward({t.logits, t.teacher, t.indices, t.mask, t.stats});
         return loss;
     }
     static variable_list backward(AutogradContext* ctx, variable_list douts) {
         const variable_list saved = ctx->get_saved_variables();
-        const DistillTensors t{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5]};
+        const DistillTensors t{saved[0], saved[1], saved[2], saved[3], saved[4]};
         Tensor dlogits = at::empty(t.logits.sizes(), t.logits.options());
         if (t.stats.defined()) {
             std::vector<Tensor> keep;
@@ -657,7 +652,7 @@ std::optional<Tensor> distill_topk(const Tensor& logits, const Tensor& teacher, 
         refuse_leaves_of_the_default_stream({&logits});
         return DistillTopk::apply(logits, teacher, indices, mask, reduction, temperature);
     }
-    DistillTensors t{logits, teacher, indices, mask.value_or(Tensor()), Tensor(), Tensor()};
+    DistillTensors t{logits, teacher, indices, mask.value_or(Tensor()), Tensor()};
     return distill_forward(t, reduction, temperature);
 }
 
