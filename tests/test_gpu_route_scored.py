@@ -398,3 +398,21 @@ def test_rows_of_equal_logits(experts, k, groups, kept, scores):
         logits[26, experts // 2:] -= 0.5
         for b in (None, torch.zeros(experts), torch.full((experts,), 0.25), bias, torch.where(bias > 0.1, -INF, 0.0)):
             check(logits, mask, dw, b, k, scores, groups, kept)
+
+
+@gpu
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_offsets_beyond_32_bits(scores):
+    tokens, experts = 2 ** 31 // 256 + 5, 256
+    logits = torch.zeros(tokens, experts, dtype=BF16, device=DEV)
+    tail, _, dw, bias = make((999, experts), 8, BF16, seed=1)
+    logits[-999:] = tail.to(DEV)
+    leaf, alone = logits.requires_grad_(), tail.to(DEV).requires_grad_()
+    r, s = (muon_amd.route_topk(t, 8, scores=scores, bias=bias.to(DEV), groups=8, groups_kept=4) for t in (leaf, alone))
+    assert torch.equal(r.indices[-999:], s.indices) and torch.equal(r.weights[-999:], s.weights)
+    assert int(r.counts.sum()) == 8 * tokens
+    give = torch.zeros(tokens, 8, device=DEV)
+    give[-999:] = dw.to(DEV)
+    got, = torch.autograd.grad(r.weights, leaf, give)
+    want, = torch.autograd.grad(s.weights, alone, dw.to(DEV))
+    assert torch.equal(got[-999:], want) and not got[:-999].any()
