@@ -1017,8 +1017,11 @@ static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
         p.e = take(p.rows * p.piece * 2);
         // at most so many shares (the tokens that take part decide, on the device): of 8 k-blocks or more each, in half a GiB or one share.  Tiles of
         // 128 x 128 where those of 256 x 256 are few.
-        // (two k-blocks of 128 x 128 tiles keep a CU busier than a few of a large one: 130 x 100000 x 768 243 -> 234 us, 1000 x 50257 x 2048 948 us and 963)
-        p.dw_tile = p.rows > 512 ? 256 : 128;
+        // (dW: a few k-blocks of two 128 x 128 tiles keep a CU busier than those of a large one, 130 x 100000 x 768 234 and 243 us, but where tiles are
+        // many their prologues add up: 65 x 128256 x 4096 617 us by large ones and 711, 250 x 128256 x 4096 736 and 867, 1000 x 50257 x 2048 948 and 963;
+        // a single k-block has four small tiles to a CU: 2 x 32000 x 4096 151 and 146)
+        const int64_t large_tiles = (up(v, 256) / 256) * (up(d, 256) / 256);
+        p.dw_tile = p.rows > 512 || (n > BK && large_tiles >= 8 * HD_CUS) ? 256 : 128;
         p.dh_tile = (p.rows / 256) * ((p.ld + 255) / 256) >= 64 ? 256 : 128;
         int64_t most_splits = HD_SPLITS;
         if (most_splits > p.piece / BK / 8) most_splits = p.piece / BK / 8;

@@ -448,3 +448,8 @@ def test_around_a_thousand_tokens(tokens):
 @pytest.mark.parametrize("vocab,width", [(1, 64), (65, 1216), (200, 1990), (640, 4160), (7, 130)])
 def test_streamed_matrices(tokens, vocab, width):
     check(*make(tokens, vocab, width, seed=tokens + vocab, ignored=0.3))         # (blocks of 64 channels: one, numbers that are no multiple of the waves', part of one)
+
+
+@gpu
+def test_few_tokens_and_large_tiles_of_the_matrix():
+    check(*make(70, 66000, 2050, seed=1, ignored=0.2))           # (the matrix's gradient in tiles that are many for a k-block or two)
