@@ -9,7 +9,7 @@
 // (the same product; the same bits too, but where few tokens were streamed forward), e is written once in bf16 (rounding each term of sums over the
 // vocabulary or the tokens by at most 2^-8 of itself, as the sums are rounded when they are written), and two products follow, whose second operand (and for
 // dW the first one too) lies k-major and is read through transposing LDS reads, so nothing is written twice.  8 N V D operations
-// instead of the 6 N V D of a backward pass that keeps N V logits.  8192 x 128256 x 4096: 6.6 ms forward, 6.9 + 6.8 + 7.4 ms backward (1235 to 1310
+// instead of the 6 N V D of a backward pass that keeps N V logits.  8192 x 128256 x 4096: 6.4 ms forward, 6.6 + 6.4 + 6.9 ms backward (1254 to 1354
 // TFLOP/s; a library's product of that size 1377).
 //
 // Tokens that are ignored leave the products: a first launch numbers those that take part, and their hidden states are copied

@@ -13,8 +13,8 @@
 //
 // Layout as in route.hip: a row in the registers of L lanes, N elements each.  The two largest c of a group come from its lanes, or through LDS where
 // groups begin anywhere in a lane's elements.  Instructions bound it (the vector units are busy 95 % of the time): 65536 tokens, 8 of 256 in 4 of 8
-// groups, sigmoid, bf16 64 us for 38 MB (with 64-bit keys for the choice and the biases in registers 116), all logits equal likewise; 30011
-// tokens, 6 of 160 in 3 of 8, softmax, fp32 39 us.
+// groups, sigmoid, bf16 61 us for 38 MB (with 64-bit keys for the choice and the biases in registers 116), all logits equal likewise; 30011
+// tokens, 6 of 160 in 3 of 8, softmax, fp32 41 us.
 #include "route.h"
 
 namespace muon_amd {
