@@ -51,7 +51,68 @@ __device__ __forceinline__ int index_of(const MuonDistill& a, int64_t t, int k) 
     return i >= 0 && i < a.vocab ? static_cast<int>(i) : -1;
 }
 
-// Part `blockIdx.x % parts` of a token's logits: its maximum and sum.
+// A token's list, by a wave.  What a lane has of it in the first place (an entry and the student's logit there; more than 64 are read again
+// below) is requested when it is made, and used in finish().
+struct TokenList {
+    float v0, x0;
+    bool open;
+    __device__ __forceinline__ void entry(const MuonDistill& a, int64_t t, int k, float& v, float& x) const {
+        const int i = open && k < a.top ? index_of(a, t, k) : -1;
+        v = k < a.top ? teacher_of(a, t * a.ld_teacher + k) : -__builtin_inff();
+        const int64_t at = t * a.ld_logits + (i >= 0 ? i : 0);
+        x = i < 0 ? 0.f : a.dtype == MUON_AMD_SRC_BF16 ? element<uint16_t>(a.logits, at) : element<float>(a.logits, at);
+        if (i < 0) v = -__builtin_inff();
+    }
+    __device__ __forceinline__ TokenList(const MuonDistill& a, int64_t t) : open(!a.mask || a.mask[t]) { entry(a, t, threadIdx.x & 63, v0, x0); }
+    // The token's loss and statistics, with the maximum and sum of its logits in `r` (of each lane: joined here).  Whether it takes part.
+    __device__ __forceinline__ bool finish(const MuonDistill& a, int64_t t, float c, const RunningSum& r, float& loss) const {
+        const auto larger = [](float x, float y) { return fmaxf(x, y); };
+        const int lane = threadIdx.x & 63;
+        // the list: whether anything is there, its maximum and sum
+        bool some = v0 != -__builtin_inff();
+        float most = fmaxf(v0, -__builtin_inff());
+        for (int k = lane + 64; k < a.top; k += 64) {
+            float v, x;
+            entry(a, t, k, v, x);
+            some |= v != -__builtin_inff();
+            most = fmaxf(most, v);
+        }
+        const bool on = __ballot(some) != 0;
+        float tm = -__builtin_inff(), tl = 0.f, m = 0.f, l = 0.f;
+        loss = 0.f;
+        if (on) {
+            tm = RunningSum::reference(group_reduce<64>(most, larger));     // (a list of nothing but NaN has a number here all the same)
+            float s = RunningSum::power(v0, tm, c);
+            for (int k = lane + 64; k < a.top; k += 64) {
+                float v, x;
+                entry(a, t, k, v, x);
+                s += RunningSum::power(v, tm, c);
+            }
+            tl = __log2f(group_sum<64>(s));
+            m = group_reduce<64>(r.m, larger);
+            l = __log2f(group_sum<64>(r.s * RunningSum::power(r.m, RunningSum::reference(m), c)));
+            m = RunningSum::reference(m);
+            const auto term = [&](float v, float x) {
+                const float y = (v - tm) * c - tl, q = __builtin_amdgcn_exp2f(y);             // log2 q, q
+                if (v != -__builtin_inff() && q != 0.f) loss = fmaf(q, y - ((x - m) * c - l), loss);
+            };
+            term(v0, x0);
+            for (int k = lane + 64; k < a.top; k += 64) {
+                float v, x;
+                entry(a, t, k, v, x);
+                term(v, x);
+            }
+            loss = group_sum<64>(loss) * (LN2 * a.temperature * a.temperature);
+        }
+        if (lane == 0) {
+            a.losses[t] = loss;
+            reinterpret_cast<f32x4v*>(a.stats)[t] = f32x4v{m, l, tm, tl};
+        }
+        return on;
+    }
+};
+
+// Part `blockIdx.x % parts` of a token's logits: its maximum and sum.  The only part has the list too, which is in the cache by then.
 template <typename T>
 __global__ __launch_bounds__(DT_THREADS) void distill_stats_kernel(const MuonDistill a, int parts, int length) {
     constexpr int G = pack_of<T>;
@@ -113,86 +174,54 @@ __global__ __launch_bounds__(DT_THREADS) void distill_stats_kernel(const MuonDis
         sum[threadIdx.x >> 6] = s;
     }
     __syncthreads();
-    if (threadIdx.x > 0) return;
-    RunningSum all;
-    for (int w = 0; w < DT_WAVES; ++w) all.join(top[w], sum[w], c);
-    reinterpret_cast<f32x2_t*>(a.partials)[blockIdx.x] = f32x2_t{all.m, all.s};
-    if (blockIdx.x == 0) *a.counter = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.counter = 0;
+    if (threadIdx.x >= 64) return;
+    if (parts == 1) {
+        const int lane = threadIdx.x;
+        RunningSum mine;
+        if (lane < DT_WAVES) mine.m = top[lane], mine.s = sum[lane];
+        float loss;
+        TokenList(a, t).finish(a, t, c, mine, loss);
+    } else if (threadIdx.x == 0) {
+        RunningSum all;
+        for (int w = 0; w < DT_WAVES; ++w) all.join(top[w], sum[w], c);
+        reinterpret_cast<f32x2_t*>(a.partials)[blockIdx.x] = f32x2_t{all.m, all.s};
+    }
 }
 
-// A wave for each token: its parts joined, its list, its loss.  The workgroup that is done last adds up the losses.  (At most 256
-// workgroups: with one for every four tokens, 2048 of them at one counter took 96 us.)
+// The workgroup that is done last adds up the losses.  LISTS: a wave for each token, its parts joined, its list, its loss; else these are there, and
+// a thread for each token only adds.  (At most 256 workgroups: with one for every four tokens, 2048 of them at one counter took 96 us.)
 constexpr int DF_THREADS = 1024, DF_WAVES = DF_THREADS / 64, DF_GROUPS = 256;
-static int finish_groups(int64_t tokens) { return static_cast<int>(tokens < DF_WAVES * DF_GROUPS ? (tokens + DF_WAVES - 1) / DF_WAVES : DF_GROUPS); }
+static int finish_groups(int64_t tokens, int each) { return static_cast<int>(tokens < each * DF_GROUPS ? (tokens + each - 1) / each : DF_GROUPS); }
+template <bool LISTS>
 __global__ __launch_bounds__(DF_THREADS) void distill_finish_kernel(const MuonDistill a, int parts) {
     __shared__ float sums[DF_WAVES];
     __shared__ int counts[DF_WAVES];
     __shared__ bool last;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const float c = LOG2E / a.temperature;
-    const auto larger = [](float x, float y) { return fmaxf(x, y); };
     float total = 0.f;
     int taking = 0;
-    for (int64_t t = static_cast<int64_t>(blockIdx.x) * DF_WAVES + wave; t < a.tokens; t += static_cast<int64_t>(gridDim.x) * DF_WAVES) {
-        float loss = 0.f;
-        // All that the token has to be read for is requested together: each lane's entry of the list (more than 64 are read again below), the
-        // student's logit there, a part's sums.
-        const bool open = !a.mask || a.mask[t];
-        const f32x2_t* const p = reinterpret_cast<const f32x2_t*>(a.partials) + t * parts;
-        const f32x2_t first = lane < parts ? p[lane] : f32x2_t{-__builtin_inff(), 0.f};
-        const auto entry = [&](int k, float& v, float& x) {
-            const int i = open && k < a.top ? index_of(a, t, k) : -1;
-            v = k < a.top ? teacher_of(a, t * a.ld_teacher + k) : -__builtin_inff();
-            const int64_t at = t * a.ld_logits + (i >= 0 ? i : 0);
-            x = i < 0 ? 0.f : a.dtype == MUON_AMD_SRC_BF16 ? element<uint16_t>(a.logits, at) : element<float>(a.logits, at);
-            if (i < 0) v = -__builtin_inff();
-        };
-        float v0, x0;
-        entry(lane, v0, x0);
-        // the list: whether anything is there, its maximum and sum
-        bool some = v0 != -__builtin_inff();
-        float most = fmaxf(v0, -__builtin_inff());
-        for (int k = lane + 64; k < a.top; k += 64) {
-            float v, x;
-            entry(k, v, x);
-            some |= v != -__builtin_inff();
-            most = fmaxf(most, v);
-        }
-        const bool on = __ballot(some) != 0;
-        float tm = -__builtin_inff(), tl = 0.f, m = 0.f, l = 0.f;
-        if (on) {
-            tm = RunningSum::reference(group_reduce<64>(most, larger));     // (a list of nothing but NaN has a number here all the same)
-            float s = RunningSum::power(v0, tm, c);
-            for (int k = lane + 64; k < a.top; k += 64) {
-                float v, x;
-                entry(k, v, x);
-                s += RunningSum::power(v, tm, c);
-            }
-            tl = __log2f(group_sum<64>(s));
+    if constexpr (LISTS) {
+        const float c = LOG2E / a.temperature;
+        for (int64_t t = static_cast<int64_t>(blockIdx.x) * DF_WAVES + wave; t < a.tokens; t += static_cast<int64_t>(gridDim.x) * DF_WAVES) {
+            // All that the token has to be read for is requested together: each lane's entry of the list, the student's logit there, a part's sums.
+            const f32x2_t* const p = reinterpret_cast<const f32x2_t*>(a.partials) + t * parts;
+            const f32x2_t first = lane < parts ? p[lane] : f32x2_t{-__builtin_inff(), 0.f};
+            const TokenList list(a, t);
             RunningSum r;
             r.join(first[0], first[1], c);
             for (int i = lane + 64; i < parts; i += 64) r.join(p[i][0], p[i][1], c);
-            m = group_reduce<64>(r.m, larger);
-            l = __log2f(group_sum<64>(r.s * RunningSum::power(r.m, RunningSum::reference(m), c)));
-            m = RunningSum::reference(m);
-            const auto term = [&](float v, float x) {
-                const float y = (v - tm) * c - tl, q = __builtin_amdgcn_exp2f(y);             // log2 q, q
-                if (v != -__builtin_inff() && q != 0.f) loss = fmaf(q, y - ((x - m) * c - l), loss);
-            };
-            term(v0, x0);
-            for (int k = lane + 64; k < a.top; k += 64) {
-                float v, x;
-                entry(k, v, x);
-                term(v, x);
-            }
-            loss = group_sum<64>(loss) * (LN2 * a.temperature * a.temperature);
+            float loss;
+            taking += list.finish(a, t, c, r, loss);
+            total += loss;
         }
-        if (lane == 0) {
-            a.losses[t] = loss;
-            reinterpret_cast<f32x4v*>(a.stats)[t] = f32x4v{m, l, tm, tl};
+    } else {
+        for (int64_t t = static_cast<int64_t>(blockIdx.x) * DF_THREADS + threadIdx.x; t < a.tokens; t += static_cast<int64_t>(gridDim.x) * DF_THREADS) {
+            total += a.losses[t];
+            taking += reinterpret_cast<const f32x4v*>(a.stats)[t][2] != -__builtin_inff();
         }
-        total += loss;
-        taking += on;
+        total = group_sum<64>(total);
+        taking = group_reduce<64>(taking, [](int u, int v) { return u + v; });
     }
     if (lane == 0) {
         sums[wave] = total;
@@ -338,7 +367,7 @@ int muon_amd_distill_max_top(void) { return DT_MAX_TOP; }
 
 int64_t muon_amd_distill_partials(int64_t tokens, int vocab, int dtype) {
     if (tokens <= 0 || vocab <= 0) return 0;
-    return 2 * tokens * distill_parts(tokens, vocab, dtype) + 2 * finish_groups(tokens);
+    return 2 * tokens * distill_parts(tokens, vocab, dtype) + 2 * DF_GROUPS;
 }
 
 int muon_amd_distill(const MuonDistill* args, void* stream) {
@@ -352,7 +381,8 @@ int muon_amd_distill(const MuonDistill* args, void* stream) {
     if (a.dtype == MUON_AMD_SRC_BF16) hipLaunchKernelGGL(distill_stats_kernel<uint16_t>, grid, dim3(DT_THREADS), 0, st, a, parts, length);
     else hipLaunchKernelGGL(distill_stats_kernel<float>, grid, dim3(DT_THREADS), 0, st, a, parts, length);
     if (const int rc = check_launch("distill")) return rc;
-    hipLaunchKernelGGL(distill_finish_kernel, dim3(finish_groups(a.tokens)), dim3(DF_THREADS), 0, st, a, parts);
+    if (parts > 1) hipLaunchKernelGGL(distill_finish_kernel<true>, dim3(finish_groups(a.tokens, DF_WAVES)), dim3(DF_THREADS), 0, st, a, parts);
+    else hipLaunchKernelGGL(distill_finish_kernel<false>, dim3(finish_groups(a.tokens, DF_THREADS)), dim3(DF_THREADS), 0, st, a, parts);
     return check_launch("distill");
 }
 
