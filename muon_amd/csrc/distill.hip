@@ -54,8 +54,9 @@ __device__ __forceinline__ int index_of(const MuonDistill& a, int64_t t, int k) 
 // A token's list, by a wave.  What a lane has of it in the first place (an entry and the student's logit there; more than 64 are read again
 // below) is requested when it is made, and used in finish().
 struct TokenList {
-    float v0, x0;
-    bool open;
+    float v0 = 0.f, x0 = 0.f;
+    bool open = false;
+    __device__ __forceinline__ TokenList() {}
     __device__ __forceinline__ void entry(const MuonDistill& a, int64_t t, int k, float& v, float& x) const {
         const int i = open && k < a.top ? index_of(a, t, k) : -1;
         v = k < a.top ? teacher_of(a, t * a.ld_teacher + k) : -__builtin_inff();
@@ -122,6 +123,8 @@ __global__ __launch_bounds__(DT_THREADS) void distill_stats_kernel(const MuonDis
     const int part = blockIdx.x % parts, begin = part * length, end = min(begin + length, a.vocab);
     const T* const row = static_cast<const T*>(a.logits) + t * a.ld_logits;
     RunningSum r;
+    TokenList list;
+    if (parts == 1 && threadIdx.x < 64) list = TokenList(a, t);
     const auto add = [&](const Pack<T, G>(&v)[DT_UNROLL]) {
         float most = -__builtin_inff();
 #pragma unroll
@@ -181,7 +184,7 @@ __global__ __launch_bounds__(DT_THREADS) void distill_stats_kernel(const MuonDis
         RunningSum mine;
         if (lane < DT_WAVES) mine.m = top[lane], mine.s = sum[lane];
         float loss;
-        TokenList(a, t).finish(a, t, c, mine, loss);
+        list.finish(a, t, c, mine, loss);
     } else if (threadIdx.x == 0) {
         RunningSum all;
         for (int w = 0; w < DT_WAVES; ++w) all.join(top[w], sum[w], c);
