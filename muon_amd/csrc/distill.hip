@@ -13,7 +13,8 @@
 // however far from zero these are (with x c - m c in one instruction, a row at 1e30 is lost in the rounding of m c).  Rows are shared by several workgroups where
 // there are few of them, and joined in the order of their parts.  Loads and stores of the rows carry the non-temporal hint: nothing is read again
 // while it is in a cache, but for what fits the last one (8192 x 128256 bf16, both passes: 1140 -> 1021 us, 6.2 TB/s of the 6.3 GB; 4096 x
-// 32000: 155.6 -> 154.2, with plain loads backward 149.4).  Of 8192 x 128256 forward takes 311 us (6.8 TB/s), the lists 16, backward 686 (6.1 TB/s).
+// 32000: 155.6 -> 154.2, with plain loads backward 149.4).  Of 8192 x 128256 forward takes 317 us (6.6 TB/s), the
+// losses' sum 5, backward 689 (6.1 TB/s).
 #include "lanes.h"
 
 namespace muon_amd {
@@ -113,7 +114,8 @@ struct TokenList {
     }
 };
 
-// Part `blockIdx.x % parts` of a token's logits: its maximum and sum.  The only part has the list too, which is in the cache by then.
+// Part `blockIdx.x % parts` of a token's logits: its maximum and sum.  The only part of a token has its list too (a launch for the lists
+// took 13 us for 4096 x 64; the whole call 154.5 -> 148.4 us, requested ahead of the row 146.9).
 template <typename T>
 __global__ __launch_bounds__(DT_THREADS) void distill_stats_kernel(const MuonDistill a, int parts, int length) {
     constexpr int G = pack_of<T>;
