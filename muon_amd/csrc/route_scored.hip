@@ -112,13 +112,18 @@ __device__ __forceinline__ void choose_again(const T* row, const float* bias, in
     }
 }
 
-// The weights and indices of a row by L lanes: scores of the choices, formed again from their logits (softmax: e^(l - top) per).
+// The weights and indices of a row by L lanes: scores of the choices, formed again from their logits (softmax: e^(l - top) per).  Weights that add up to
+// one go by the ratios of scores, which are there where the scores themselves are below the smallest number: where one of the chosen is so far down, the
+// row's scores are formed relative to e^m, m its largest chosen logit (or 0, for a sigmoid above that), e^(l - m) or e^(l - m) / (1 + e^l).
 constexpr int LATER = -2;                        // first index of a row that is to be done again
+constexpr float FAR_DOWN = -80.f;                // (e^-87 is the smallest normal number)
 template <typename T, int L, bool SIGMOID>
 __device__ __forceinline__ void put_choices(const MuonRoute& a, int64_t t, const T* row, float top, float per, const int* picks, int* tokens, int lane) {
+    bool relative = false;
     const auto score_at = [&](int e) {
         const float l = logit_of(row, e);
         if constexpr (SIGMOID) {
+            if (relative) return exp_with_nan(l - top) * __builtin_amdgcn_rcpf(1.f + exp_of(l));
             float rest;
             return sigmoid_of(l, rest);
         } else {
@@ -127,6 +132,22 @@ __device__ __forceinline__ void put_choices(const MuonRoute& a, int64_t t, const
         }
     };
     const int own = lane < a.k ? picks[lane] : -1;
+    if (a.normalize) {
+        const auto down = [&](int e) { return e >= 0 && logit_of(row, e) - (SIGMOID ? 0.f : top) < FAR_DOWN; };
+        bool far = down(own);
+        for (int j = lane + L; j < a.k; j += L) far |= down(picks[j]);
+        if (__ballot(far)) {
+            const auto most_of = [](float u, float v) { return fmaxf(u, v); };
+            float most = own >= 0 ? logit_of(row, own) : -__builtin_inff();
+            for (int j = lane + L; j < a.k; j += L)
+                if (picks[j] >= 0) most = fmaxf(most, logit_of(row, picks[j]));
+            most = group_reduce<L>(most, most_of);
+            far = group_reduce<L>(far ? 1.f : 0.f, most_of) != 0.f;
+            relative = far && (!SIGMOID || most <= 0.f);
+            top = relative ? most : top;
+            per = relative ? 1.f : per;
+        }
+    }
     const float first = own >= 0 ? score_at(own) : 0.f;
     float chosen = first;
     for (int j = lane + L; j < a.k; j += L) {
