@@ -116,7 +116,7 @@ __device__ __forceinline__ void choose_again(const T* row, const float* bias, in
 // one go by the ratios of scores, which are there where the scores themselves are below the smallest number: where one of the chosen is so far down, the
 // row's scores are formed relative to e^m, m its largest chosen logit (or 0, for a sigmoid above that), e^(l - m) or e^(l - m) / (1 + e^l).
 constexpr int LATER = -2;                        // first index of a row that is to be done again
-constexpr float FAR_DOWN = -80.f;                // (e^-87 is the smallest normal number)
+constexpr float FAR_DOWN = 0x1p-116f;            // (2^-126 is the smallest normal number)
 template <typename T, int L, bool SIGMOID>
 __device__ __forceinline__ void put_choices(const MuonRoute& a, int64_t t, const T* row, float top, float per, const int* picks, int* tokens, int lane) {
     bool relative = false;
@@ -132,27 +132,30 @@ __device__ __forceinline__ void put_choices(const MuonRoute& a, int64_t t, const
         }
     };
     const int own = lane < a.k ? picks[lane] : -1;
-    if (a.normalize) {
-        const auto down = [&](int e) { return e >= 0 && logit_of(row, e) - (SIGMOID ? 0.f : top) < FAR_DOWN; };
-        bool far = down(own);
-        for (int j = lane + L; j < a.k; j += L) far |= down(picks[j]);
-        if (__ballot(far)) {
-            const auto most_of = [](float u, float v) { return fmaxf(u, v); };
-            float most = own >= 0 ? logit_of(row, own) : -__builtin_inff();
-            for (int j = lane + L; j < a.k; j += L)
-                if (picks[j] >= 0) most = fmaxf(most, logit_of(row, picks[j]));
-            most = group_reduce<L>(most, most_of);
-            far = group_reduce<L>(far ? 1.f : 0.f, most_of) != 0.f;
-            relative = far && (!SIGMOID || most <= 0.f);
-            top = relative ? most : top;
-            per = relative ? 1.f : per;
-        }
-    }
-    const float first = own >= 0 ? score_at(own) : 0.f;
-    float chosen = first;
-    for (int j = lane + L; j < a.k; j += L) {
-        const int e = picks[j];
-        if (e >= 0) chosen += score_at(e);
+    float first, chosen;
+    bool far = false;
+    const auto add_up = [&] {
+        first = own >= 0 ? score_at(own) : 0.f;
+        chosen = first;
+        far |= own >= 0 && first < FAR_DOWN;
+        for (int j = lane + L; j < a.k; j += L)
+            if (const int e = picks[j]; e >= 0) {
+                const float s = score_at(e);
+                far |= s < FAR_DOWN;
+                chosen += s;
+            }
+    };
+    add_up();
+    if (a.normalize && __ballot(far)) {
+        const auto most_of = [](float u, float v) { return fmaxf(u, v); };
+        float most = own >= 0 ? logit_of(row, own) : -__builtin_inff();
+        for (int j = lane + L; j < a.k; j += L)
+            if (picks[j] >= 0) most = fmaxf(most, logit_of(row, picks[j]));
+        most = group_reduce<L>(most, most_of);
+        relative = group_reduce<L>(far ? 1.f : 0.f, most_of) != 0.f && (!SIGMOID || most <= 0.f);
+        top = relative ? most : top;
+        per = relative ? 1.f : per;
+        add_up();
     }
     chosen = a.normalize ? group_sum<L>(chosen) : 1.f;
     for (int j = lane; j < a.k; j += L) {
