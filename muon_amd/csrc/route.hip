@@ -314,6 +314,7 @@ __global__ __launch_bounds__(RB_THREADS) void route_backward_kernel(const MuonRo
                 p[i] = exp_of(x[i] - lse - rest);  // (zero where the token takes no part: x is -infinity)
                 if constexpr (SIGMOID) {
                     s[i] = sigmoid_of(x[i], rest_of[i]);
+                    if (lse < 0.f) s[i] = p[i] * rest_of[i];       // s / e^lse: the row's norm takes it out, and it does not vanish with s
                     norm += s[i];
                     dot = fmaf(s[i], g[i], dot);
                 } else {

@@ -324,6 +324,12 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
             for (int i = 0; i < N; ++i) most = c[i] == c[i] ? most : 0.f;
         }
         const bool on = group_reduce<L>(most, most_of) != -__builtin_inff();
+        // (shares of sigmoids so small are the probabilities, to 2^-57, and do not vanish with them; such rows have gone the second way above)
+        if (const bool small = top < -40.f; SIGMOID && __ballot(small)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] = small ? exp_with_nan(x[i] - top) : s[i];
+            norm = small ? per : norm;
+        }
         norm = on ? norm : 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = fmaf(s[i], norm, acc[i]);

@@ -1,5 +1,5 @@
 """Routing by scores near and below the smallest number of 32 bits, against the formulas in 64 bits (GPU): the weights of a token's choices are ratios
-of their scores, which are ordinary numbers where the scores are not.  Bounds as in test_gpu_route_scored.py, for
+of their scores, and its shares of the balance loss ratios too, which are ordinary numbers where the scores are not.  Bounds as in test_gpu_route_scored.py, for
 every row; the balance loss has E 2^-126 more: E sum_e (counts_e / n k) (mean share_e), where the factors of the shares add up to one, and a share below 2^-126 may
 be zero (an expert that has a token's whole probability and none of its choices leaves a balance loss of e^-200: there is no such number in 32 bits)."""
 import pytest
@@ -30,6 +30,34 @@ def check(logits, mask, dw, bias, k, scores, groups=1, kept=1, normalize=True, c
 
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("experts,k,groups,kept", [(8, 2, 1, 1), (16, 4, 4, 2), (48, 6, 6, 3), (64, 32, 1, 1), (256, 8, 8, 4), (1024, 32, 16, 5)])
+def test_sigmoids_that_vanish(experts, k, groups, kept, normalize, dtype):
+    """All of a token's sigmoids at e^-60 to e^-300, between tokens of ordinary ones."""
+    logits, mask, dw, bias = make((120, experts), k, dtype, seed=experts, masked=True)
+    logits[::2] = (logits[::2].float() * 3 - torch.linspace(60, 300, 60)[:, None]).to(dtype)
+    for b in (None, torch.zeros(experts)):
+        r, _ = check(logits, mask, dw, b, k, "sigmoid", groups, kept, normalize)
+        if normalize:                                            # k numbers of 32 bits that add up to one
+            assert ((r.weights.sum(1) - 1).abs()[mask.to(DEV)] <= 3 * k * U).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("experts,k", [(8, 4), (64, 8), (256, 32)])
+def test_choices_far_below_the_first(experts, k, dtype):
+    """A token's choices reach from an ordinary score to ones that vanish, and to weights that do not (from -20 to -100: e^-80)."""
+    g = torch.Generator().manual_seed(k)
+    logits = torch.full((64, experts), -150.0)
+    logits[:, :k] = -torch.linspace(0, 80, k) - torch.linspace(-30, 30, 64)[:, None] + torch.rand(64, k, generator=g)
+    logits = logits[:, torch.randperm(experts, generator=g)].to(dtype)
+    dw = torch.randn(64, k, generator=g)
+    for scores in ("sigmoid", "softmax"):
+        check(logits, None, dw, None, k, scores)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("below", [80, 88, 95, 200])
 @pytest.mark.parametrize("experts,k,groups,kept", [(8, 2, 1, 1), (32, 4, 4, 2), (64, 32, 1, 1), (256, 8, 8, 4)])
 def test_an_expert_that_is_not_available_far_above_the_others(experts, k, groups, kept, below, dtype):
@@ -42,3 +70,17 @@ def test_an_expert_that_is_not_available_far_above_the_others(experts, k, groups
         r, _ = check(logits, mask, dw, b, k, "softmax", groups, kept)
         assert ((r.weights.sum(1) - 1).abs()[mask.to(DEV)] <= 3 * k * U).all()
         check(logits, mask, dw, b, k, "softmax", groups, kept, normalize=False)
+
+
+@gpu
+def test_a_row_that_is_no_number_far_down():
+    """NaN and infinities among choices far down stay what they are in other rows: no number for the row, nothing for its neighbours."""
+    logits, _, dw, _ = make((64, 16), 4, F32, std=30.0)
+    logits -= 100
+    clean, _ = check(logits, None, dw, None, 4, "sigmoid")
+    logits[7, 2] = float("nan")
+    logits[9, 5] = INF
+    r = muon_amd.route_topk(logits.to(DEV), 4, scores="sigmoid")
+    rest = torch.tensor([i for i in range(64) if i not in (7, 9)])
+    assert torch.equal(r.weights[rest], clean.weights[rest]) and torch.equal(r.indices[rest], clean.indices[rest])
+    assert torch.isnan(r.weights[7]).any() and r.weights[9, 0] == 1 and r.indices[9, 0] == 5
