@@ -300,9 +300,9 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
             for (int i = 0; i < N; ++i) s[i] *= per;
         }
         // What a c may be off by, beside its own rounding: of scores up to 1 or the row's largest probability, or without a bias relative to itself
-        // (softmax: that includes the rounding of differences of logits).
+        // (softmax: that includes the rounding of differences of logits) and, where it is below the smallest normal number, by that.
         constexpr float OFF = SIGMOID ? 8.f * RS_UNIT : 40.f * RS_UNIT, RELATIVE = SIGMOID ? 8.f * RS_UNIT : 128.f * RS_UNIT;
-        const float off = bias ? OFF * (SIGMOID ? 1.f : per) : 0.f, relative = bias ? RS_UNIT : RELATIVE + RS_UNIT;
+        const float off = bias ? OFF * (SIGMOID ? 1.f : per) : 0x1p-124f, relative = bias ? RS_UNIT : RELATIVE + RS_UNIT;
         // from here on what is chosen by; the token takes part if anything is available
         float c[N], most = -__builtin_inff();
 #pragma unroll

@@ -84,3 +84,18 @@ def test_a_row_that_is_no_number_far_down():
     rest = torch.tensor([i for i in range(64) if i not in (7, 9)])
     assert torch.equal(r.weights[rest], clean.weights[rest]) and torch.equal(r.indices[rest], clean.indices[rest])
     assert torch.isnan(r.weights[7]).any() and r.weights[9, 0] == 1 and r.indices[9, 0] == 5
+
+
+@gpu
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,kept", [(8, 4, 2), (16, 4, 2), (60, 10, 5), (64, 8, 4), (256, 32, 16)])
+def test_groups_at_the_smallest_number(experts, groups, kept, scores):
+    """Groups whose scores are sums of numbers on both sides of 2^-126, where the smaller ones are flushed: chosen as in 64 bits."""
+    g = torch.Generator().manual_seed(experts)
+    logits = -85.5 - 6.5 * torch.rand(3000, experts, generator=g)
+    if scores == "softmax":
+        logits = logits - logits.amax(1, keepdim=True) - 85.5 - torch.rand(3000, 1, generator=g)
+        logits[:, 0] = 0.0
+    dw = torch.randn(3000, 1, generator=g)
+    for k in (1, kept):
+        check(logits, None, dw.expand(3000, k), None, k, scores, groups, kept)
