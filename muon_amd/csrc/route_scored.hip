@@ -301,6 +301,9 @@ __global__ __launch_bounds__(RT_THREADS, 4) void route_scored_kernel(const MuonR
         }
         // What a c may be off by, beside its own rounding: of scores up to 1 or the row's largest probability, or without a bias relative to itself
         // (softmax: that includes the rounding of differences of logits) and, where it is below the smallest normal number, by that.
+        // The 0.22 |d| units of an exponential (lanes.h) need no room there.  They take every argument d as d (1 - 1.34e-8), which keeps the order of
+        // scores; two sums of two that are equal have arguments whose means, weighted by the terms, are within ln 2 of each other (the mean is ln S minus the
+        // entropy of the terms' shares), so that the sums move apart by 0.16 units (sigmoids near one: by less); and beside a bias they are 0.22 |d| e^d, at most 0.08.
         constexpr float OFF = SIGMOID ? 8.f * RS_UNIT : 40.f * RS_UNIT, RELATIVE = SIGMOID ? 8.f * RS_UNIT : 128.f * RS_UNIT;
         const float off = bias ? OFF * (SIGMOID ? 1.f : per) : 0x1p-124f, relative = bias ? RS_UNIT : RELATIVE + RS_UNIT;
         // from here on what is chosen by; the token takes part if anything is available
