@@ -280,7 +280,7 @@ typedef struct MuonDistill {
     int64_t tokens, ld_logits, ld_teacher, ld_indices, ld_dloss;
     int32_t vocab, top, dtype, teacher_dtype, index_bits, reduction;
     float temperature;
-    int32_t reserved;
+    int32_t differentiable;      /* forward: not zero where a backward call follows: what that would refuse is refused at once */
 } MuonDistill;
 
 /* One matrix of the AOL rescaling step of the 4-iteration variant (muon.py:776-785), in the

@@ -102,7 +102,7 @@ class DistillArgs(ctypes.Structure):
                                                 "dloss", "dlogits")] +
                 [(n, ctypes.c_int64) for n in ("tokens", "ld_logits", "ld_teacher", "ld_indices", "ld_dloss")] +
                 [(n, ctypes.c_int32) for n in ("vocab", "top", "dtype", "teacher_dtype", "index_bits", "reduction")] +
-                [("temperature", ctypes.c_float), ("reserved", ctypes.c_int32)])
+                [("temperature", ctypes.c_float), ("differentiable", ctypes.c_int32)])
 
 
 _c_int = ctypes.c_int

@@ -344,11 +344,16 @@ static int check_distill_grid(int64_t groups, const MuonDistill& a, const char* 
     MUON_REQUIRE(groups <= 0xffffffffll / DT_THREADS, "%s: %lld tokens of %d logits are more than a launch holds", what, static_cast<long long>(a.tokens), a.vocab);
     return MUON_AMD_OK;
 }
+// Workgroups to a token's gradient.
+static int64_t backward_parts(const MuonDistill& a) {
+    const int64_t length = DT_THREADS * DB_CHUNK_PACKS * (a.dtype == MUON_AMD_SRC_BF16 ? 8 : 4);
+    return (a.vocab + length - 1) / length;
+}
 static int part_length(int vocab, int parts) { return ((vocab + parts - 1) / parts + 7) / 8 * 8; }
 
 static int check_distill(const MuonDistill* a, const char* what) {
     MUON_REQUIRE(a, "%s: null arguments", what);
-    MUON_REQUIRE(a->tokens > 0 && a->tokens <= (int64_t(1) << 24) && a->vocab > 0 && a->vocab <= (1 << 30), "%s: tokens=%lld vocab=%d", what,
+    MUON_REQUIRE(a->tokens > 0 && a->tokens < (int64_t(1) << 24) && a->vocab > 0 && a->vocab <= (1 << 30), "%s: tokens=%lld vocab=%d", what,
                  static_cast<long long>(a->tokens), a->vocab);
     MUON_REQUIRE(a->top > 0 && a->top <= DT_MAX_TOP, "%s: top=%d (at most %d)", what, a->top, DT_MAX_TOP);
     MUON_REQUIRE(a->logits && a->teacher && a->indices && a->stats && a->part, "%s: null pointer", what);
@@ -382,6 +387,8 @@ int muon_amd_distill(const MuonDistill* args, void* stream) {
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const int parts = distill_parts(a.tokens, a.vocab, a.dtype), length = part_length(a.vocab, parts);
     if (const int rc = check_distill_grid(a.tokens * parts, a, "distill")) return rc;
+    if (a.differentiable)
+        if (const int rc = check_distill_grid(a.tokens * backward_parts(a), a, "distill, whose gradient is wanted")) return rc;
     const dim3 grid(static_cast<unsigned>(a.tokens * parts));
     if (a.dtype == MUON_AMD_SRC_BF16) hipLaunchKernelGGL(distill_stats_kernel<uint16_t>, grid, dim3(DT_THREADS), 0, st, a, parts, length);
     else hipLaunchKernelGGL(distill_stats_kernel<float>, grid, dim3(DT_THREADS), 0, st, a, parts, length);
@@ -396,8 +403,7 @@ int muon_amd_distill_backward(const MuonDistill* args, void* stream) {
     const MuonDistill a = *args;
     MUON_REQUIRE(a.dloss && a.dlogits, "distill_backward: null gradient");
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int64_t length = DT_THREADS * DB_CHUNK_PACKS * (a.dtype == MUON_AMD_SRC_BF16 ? 8 : 4);
-    const int64_t parts = (a.vocab + length - 1) / length;
+    const int64_t parts = backward_parts(a);
     if (const int rc = check_distill_grid(a.tokens * parts, a, "distill_backward")) return rc;
     const dim3 grid(static_cast<unsigned>(a.tokens * parts));
     if (a.dtype == MUON_AMD_SRC_BF16) hipLaunchKernelGGL(distill_backward_kernel<uint16_t>, grid, dim3(DT_THREADS), 0, st, a, static_cast<int>(parts));

@@ -587,7 +587,7 @@ MuonDistill distill_args(const DistillTensors& t, int64_t reduction, double temp
 }
 
 // The loss; `t` gets what backward needs.
-Tensor distill_forward(DistillTensors& t, int64_t reduction, double temperature) {
+Tensor distill_forward(DistillTensors& t, int64_t reduction, double temperature, bool differentiable) {
     const auto f32 = t.logits.options().dtype(at::kFloat);
     const auto shape = t.logits.sizes().slice(0, t.logits.dim() - 1);
     const int64_t vocab = t.logits.size(-1), tokens = t.logits.numel() / vocab;
@@ -601,6 +601,7 @@ Tensor distill_forward(DistillTensors& t, int64_t reduction, double temperature)
     a.loss = reduction ? loss.data_ptr<float>() : nullptr;
     a.partials = partials.data_ptr<float>();
     a.counter = reinterpret_cast<int32_t*>(a.partials + partials.numel() - 1);
+    a.differentiable = differentiable;
     const c10::DeviceGuard guard(t.logits.device());
     check(api.distill(&a, current_stream(t.logits.device())), "distill");
     return reduction ? loss : losses;
@@ -610,7 +611,7 @@ struct DistillTopk : torch::autograd::Function<DistillTopk> {
     static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& indices, const std::optional<Tensor>& mask,
                           int64_t reduction, double temperature) {
         DistillTensors t{logits, teacher, indices, mask.value_or(Tensor()), Tensor()};
-        const Tensor loss = distill_forward(t, reduction, temperature);
+        const Tensor loss = distill_forward(t, reduction, temperature, true);
         ctx->saved_data["reduction"] = reduction;
         ctx->saved_data["temperature"] = temperature;
         ctx->save_for_backward({t.logits, t.teacher, t.indices, t.mask, t.stats});
@@ -641,7 +642,7 @@ std::optional<Tensor> distill_topk(const Tensor& logits, const Tensor& teacher, 
     const auto rows = [&](const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); };
     if (!taken(logits) || !taken(teacher) || !whole_numbers(indices) || teacher.device() != device || indices.device() != device) return std::nullopt;
     if (logits.dim() < 1 || teacher.dim() != logits.dim() || indices.sizes() != teacher.sizes() || rows(teacher) != rows(logits)) return std::nullopt;
-    if (logits.size(-1) < 1 || logits.size(-1) > (int64_t(1) << 30) || logits.numel() / logits.size(-1) > (int64_t(1) << 24) || teacher.size(-1) < 1 ||
+    if (logits.size(-1) < 1 || logits.size(-1) > (int64_t(1) << 30) || logits.numel() / logits.size(-1) >= (int64_t(1) << 24) || teacher.size(-1) < 1 ||
         teacher.size(-1) > api.max_top)
         return std::nullopt;
     if (mask && (mask->scalar_type() != at::kBool || mask->device() != device || mask->sizes() != rows(logits))) return std::nullopt;
@@ -653,7 +654,7 @@ std::optional<Tensor> distill_topk(const Tensor& logits, const Tensor& teacher, 
         return DistillTopk::apply(logits, teacher, indices, mask, reduction, temperature);
     }
     DistillTensors t{logits, teacher, indices, mask.value_or(Tensor()), Tensor()};
-    return distill_forward(t, reduction, temperature);
+    return distill_forward(t, reduction, temperature, false);
 }
 
 // ---- addresses of an optimizer's tensors -------------------------------------------------------------------------

@@ -94,7 +94,8 @@ def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     whose index is outside of the vocabulary (-1 by habit) or whose teacher logit is -infinity are not there; a token whose
     list has none, or whose `mask` (bool, the shape of logits without its last dimension) is false, takes no part: its loss and
     gradient are zero, whatever its logits hold.  An index that comes several times counts with the sum of its
-    q.  The gradient flows to logits alone.  At most 1024 entries a token.  Sums are fp32 in a fixed order."""
+    q.  The gradient flows to logits alone.  At most 1024 entries a token, fewer than 2^24 tokens; where
+    a gradient is wanted, fewer than 2^24 pieces of 16 KiB that the tokens' logits take (a row takes whole ones).  Sums are fp32 in a fixed order."""
     if isinstance(temperature, (int, float)):
         out = _lib.native().distill_topk(logits, teacher_logits, teacher_indices, float(temperature), mask, _reduction(reduction))
         if out is not None:
@@ -120,8 +121,8 @@ def _refuse_distill(logits, teacher_logits, teacher_indices, temperature, mask, 
         raise ValueError(f"teacher_logits must be {tuple(logits.shape[:-1])} lists of 1 to {limit} entries, got {tuple(teacher_logits.shape)}")
     if teacher_indices.shape != teacher_logits.shape:
         raise ValueError(f"teacher_indices must have the shape of teacher_logits, {tuple(teacher_logits.shape)}, got {tuple(teacher_indices.shape)}")
-    if logits.numel() // logits.size(-1) > 1 << 24:
-        raise ValueError(f"{logits.numel() // logits.size(-1)} tokens: at most 2^24 are taken")
+    if logits.numel() // logits.size(-1) >= 1 << 24:
+        raise ValueError(f"{logits.numel() // logits.size(-1)} tokens: fewer than 2^24 are taken")
     if mask is not None:
         require_gpu_tensor(mask, "mask")
         if mask.dtype != torch.bool or mask.shape != logits.shape[:-1] or mask.device != logits.device:
