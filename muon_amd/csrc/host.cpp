@@ -98,7 +98,8 @@ variable_list once(variable_list grads, const char* message) {
 
 // A backward pass that a HIP graph records joins, at its end, the streams on which the graph's leaves were first used.  Where an
 // autograd graph from before the capture keeps such a leaf's node alive and that was on the default stream, the capture is
-// broken and the process ends in the runtime: the call that would record the forward pass says so instead.
+// broken and the process ends in the runtime: the call that would record the forward pass says so instead.  Whether a backward
+// pass follows is not known there: a forward pass alone, which would do no harm, is recorded with gradients off.
 void refuse_leaves_of_the_default_stream(std::initializer_list<const Tensor*> ts) {
     if (!capturing()) return;
     std::vector<torch::autograd::Node*> next;
@@ -119,7 +120,7 @@ void refuse_leaves_of_the_default_stream(std::initializer_list<const Tensor*> ts
             const auto stream = n->stream();
             if (stream && *stream == c10::impl::VirtualGuardImpl(stream->device_type()).getDefaultStream(stream->device()))
                 throw LibraryError("an autograd graph that was recorded on the default stream holds a leaf of this call: release it (its loss, its outputs) before the "
-                                   "call is captured into a HIP graph");
+                                   "call is captured into a HIP graph, or capture a forward pass alone under torch.no_grad()");
         }
         for (const auto& edge : n->next_edges()) add(edge.function.get());
     }
