@@ -125,7 +125,9 @@ def train(steps=200, width=256, layers=4, experts=8, top_k=2, state_bits=8, seed
     for step, ids in zip(range(steps), batches(device, seed)):
         y, balance, z = model(ids[:, :-1])
         if fused_head:
-            loss, lse = muon_amd.linear_cross_entropy(y, model.head.t().bfloat16(), ids[:, 1:])
+            # (in row-major memory: a transposed matrix would be copied by both passes)
+            head = model.head.t().to(torch.bfloat16, memory_format=torch.contiguous_format)
+            loss, lse = muon_amd.linear_cross_entropy(y, head, ids[:, 1:])
             objective = loss + Z_LOSS * lse.square().mean()
         else:
             loss = objective = nn.functional.cross_entropy(model.logits(y).flatten(0, 1), ids[:, 1:].flatten())
