@@ -988,8 +988,11 @@ static HeadPlan head_plan(const MuonHeadLoss& a, bool backward) {
     p.rows = up(n, HD_TILE);
     p.padded = d % BK != 0 || a.ld_weight % 8 != 0 || reinterpret_cast<uintptr_t>(a.weight) % 16 != 0;
     // Streamed: up to 32 tokens (32 x 128256 x 4096: streamed 184 us, by tiles 244); up to 64 where the tiles would need a copy of W, or W is small, or its
-    // rows are long (64 x 32000 x 2048: 37 and 48; 64 x 20000 x 1024: 22 and 28; 64 x 50257 x 768, W in the last cache: 26.7 and 24.3; 64 x 8000 x
-    // 512: 15.2 and 18.4; 48 x 100000 x 1000, W copied: 74 and 132).
+    // rows are long.  W not in a cache, streamed and by tiles, on the side of the streams: 64 x 32000 x 2048 37 and 44 us, 40 x 128256 x 1024 58 and 62, 64 x
+    // 20000 x 1024 21.0 and 26.5, 64 x 8000 x 512 15.2 and 18.4, 48 x 100000 x 1000 (copied) 74 and 132; of the tiles: 64 x 200000 x 128 38 and 31, 64 x
+    // 262144 x 256 57 and 45, 64 x 128256 x 512 43.7 and 39.7, 64 x 128256 x 960 65 and 62, 64 x 50257 x 768 30.4 and 30.2 (in the last cache 26.6 and 24.6).
+    // Shorter rows and more tokens are for the tiles, and whole rounds of them; near the border either may lose a tenth (48 x 100000 x 896 47 and 54, 33 x
+    // 50257 x 768 27 and 30, 40 x 128256 x 512 39.5 both).
     p.few = !backward && (n <= HD_FEW / 2 || (n <= HD_FEW && (p.padded || d >= 1024 || v * d < (1 << 24))));
     p.padded = p.padded && !p.few;
     p.large = fewer_rounds(n, v);

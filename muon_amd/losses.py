@@ -45,10 +45,11 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     out.  Any other target outside of 0 .. V - 1 gives a loss that is not a number, and such gradients.
 
     The products are of bf16 numbers with fp32 sums.  Backward forms the logits again in pieces of the vocabulary, rounds their gradient to
-    bf16 once, and returns both gradients in bf16.  There are at most 2^24 tokens and classes, 65536 channels.  The same call gives the same bits.
+    bf16 once, and returns both gradients in bf16.  There are at most 2^24 tokens and classes, 65536 channels, and fewer than 2^39 logits (in whole
+    tiles of 256 x 256).  Infinities in the matrix may leave gradients that are no numbers (zero times infinity).  The same call gives the same bits.
     Workspaces: forward 8 bytes for 256 logits (128 where there are few), backward at most 1 GiB for the logits' gradient (4096 of its columns
-    where there are more than 131072 tokens) and half a GiB or 4 D bytes a token, whichever is more, for sums; both 2 D bytes a token, and a
-    copy of the matrix unless D is a multiple of 64 and its rows lie at multiples of 16 bytes."""
+    where there are more than 131072 tokens) and half a GiB or 4 D bytes a token, whichever is more, for sums; both 2 D bytes a token, a
+    copy of the matrix unless D is a multiple of 64 and its rows lie at multiples of 16 bytes, and one before that unless its channels lie next to each other."""
     if isinstance(ignore_index, int) and not isinstance(ignore_index, bool) and -1 << 63 <= ignore_index < 1 << 63:
         out = _lib.native().linear_cross_entropy(hidden, weight, targets, ignore_index, _reduction(reduction))
         if out is not None:
