@@ -12,10 +12,10 @@
 // s = sum 2^((x - m) c); m and log2(s) are kept apart for backward, so that probabilities go by differences of logits
 // however far from zero these are (with x c - m c in one instruction, a row at 1e30 is lost in the rounding of m c).  Rows are shared by several workgroups where
 // there are few of them, and joined in the order of their parts.  Loads and stores of the rows carry the non-temporal hint: nothing is read again
-// while it is in a cache, but for what fits the last one (8192 x 128256 bf16, both passes: 1140 -> 1021 us, 6.2 TB/s of the 6.3 GB).  Backward
-// has them for every size, though logits that are about as large as the last cache, and that nothing has pushed out since forward read them, come faster by plain ones (4096 x 32000,
-// 262 MB, repeated: 147 us and 140; 8192 x 128256: 1007 and 1067): what else runs between the two passes of a training step decides, and is not known here.  Of 8192 x 128256 forward takes 317 us (6.6 TB/s), the
-// losses' sum 5, backward 689 (6.1 TB/s).
+// while it is in a cache, but for what fits the last one (8192 x 128256 bf16, both passes: 1140 -> 1021 us, 6.2 TB/s of the
+// 6.3 GB).  Backward has them for every size, though logits about as large as the last cache come faster by plain loads where nothing has pushed them out
+// since forward read them (4096 x 32000, 262 MB, repeated: 147 us and 140; 8192 x 128256: 1007 and 1067): what runs between the two passes of a training
+// step decides that, and is not known here.  Of 8192 x 128256 forward takes 317 us (6.6 TB/s), the losses' sum 5, backward 689 (6.1 TB/s).
 #include "lanes.h"
 
 namespace muon_amd {

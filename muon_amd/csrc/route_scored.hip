@@ -8,15 +8,14 @@
 // What is chosen goes by the order of the c as real numbers, so that it does not depend on how an exponential is rounded.  A row's c are formed in
 // fp32, and where two that decide something (neighbours among the k + 1 largest, the last of these and what is left out, the last group kept and the
 // best one left out) are nearer than what that may be off, the wave does the row again in 64 bits: 5 to 7 rows of 10000 (8 of 256 by
-// sigmoid in bf16, 6 of 160 by softmax in fp32, logits of a spread of 1.5).  Where sigmoids without a bias saturate, that is every row, one after the other: forward over
-// 65536 x 256 in 4 of 8 groups takes 62 us at a spread of 1.5, 235 (fp32: 262) at 5, 310 from 12 on; a bias tells them apart again (62 to 82).  Equal logits with equal biases are a tie, not a near one; a row of nothing else (a router
-// that starts at zero) is never done again.
+// sigmoid in bf16, 6 of 160 by softmax in fp32, logits of a spread of 1.5).  Where sigmoids saturate and no bias tells them apart, that is every
+// row, one after the other in its wave: forward over 65536 x 256 in 4 of 8 groups takes 62 us at a spread of 1.5, 235 (fp32: 262) at 5, 310 from 12 on;
+// with random biases 62 to 82.  Equal logits with equal biases are a tie, not a near one; a row of nothing else (a router that starts at zero) is never done again.
 //
 // Layout as in route.hip: a row in the registers of L lanes, N elements each.  The two largest c of a group come from its lanes, or through LDS where
 // groups begin anywhere in a lane's elements.  Instructions bound it (85 for each logit; the vector units issue in 85 % of the cycles in which their CU
-// has work): 65536 tokens, 8 of 256 in 4 of 8
-// groups, sigmoid, bf16 61 us for 38 MB (with 64-bit keys for the choice and the biases in registers 116), all logits equal likewise; 30011
-// tokens, 6 of 160 in 3 of 8, softmax, fp32 41 us.
+// has work): 65536 tokens, 8 of 256 in 4 of 8 groups, sigmoid, bf16 61 us for 38 MB (with 64-bit keys for the choice and the biases in registers
+// 116), all logits equal likewise; 30011 tokens, 6 of 160 in 3 of 8, softmax, fp32 41 us.
 #include "route.h"
 
 namespace muon_amd {
