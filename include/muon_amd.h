@@ -593,7 +593,8 @@ int     muon_amd_head_loss_backward(const MuonHeadLoss* args_host, void* stream)
 /* ---- distillation from a teacher's top logits -------------------------------------------------- */
 /* Per token: T^2 sum_k q_k (log q_k - log p_{i_k}) with p = softmax(logits / T), q = softmax(teacher / T) over the token's list.
  * Entries whose index is outside of the vocabulary or whose logit is -infinity are not there; a token without any takes no
- * part.  Backward reads what forward wrote.                                                        */
+ * part.  Backward reads what forward wrote.  Fewer than 2^24 tokens; backward, fewer than 2^24 pieces of 16 KiB, of which a
+ * row takes whole ones.                                                                            */
 size_t  muon_amd_sizeof_distill(void);
 int     muon_amd_distill_max_top(void);
 int64_t muon_amd_distill_partials(int64_t tokens, int vocab, int dtype);
